@@ -44,7 +44,9 @@ enum { NVFP4_POLICY_DERIVED_DIV8 = 0, NVFP4_POLICY_RESIDUAL_AMAX = 1, NVFP4_POLI
 /* operand orientation (reference: tune_swap_ab, src/api.hpp:84-104) */
 enum { NVFP4_ORIENT_NORMAL = 0, NVFP4_ORIENT_SWAP_AB = 1 };
 /* weight input dtypes of nvfp4_quantize_weight */
-enum { NVFP4_DTYPE_BF16 = 0, NVFP4_DTYPE_F32 = 1 };
+enum { NVFP4_DTYPE_BF16 = 0, NVFP4_DTYPE_F32 = 1, NVFP4_DTYPE_F16 = 2 /* not a weight type: rows, logits and products below */ };
+/* router scores of nvfp4_route_tokens */
+enum { NVFP4_SCORES_SOFTMAX = 0, NVFP4_SCORES_SIGMOID = 1 };
 
 /* Text of the calling thread's last error ("" if none).  Never NULL. */
 NVFP4_API const char* nvfp4_last_error(void);
@@ -325,6 +327,42 @@ NVFP4_API int nvfp4_plan_one_rank(const int64_t* ids, int64_t n, int num_experts
                                   int64_t* dst_row, int32_t* device_status, void* stream);
 NVFP4_API int nvfp4_peer_barrier(const int64_t* flag_peers, int rank, int world, int slot, int64_t epoch,
                                  int64_t budget_cycles, int32_t* device_status, void* stream);
+
+/* ---- Operators around the grouped GEMM of a mixture-of-experts layer --------------------------------------------------------
+ * Routing, rows sorted by expert and back, with the gradients of all three.  `dtype` is an NVFP4_DTYPE_* code; strides are in
+ * elements, the last dimension is contiguous.  No counterparts in the reference project, which begins at rows that are grouped already.
+ *
+ * nvfp4_route_tokens: the k largest logits of every row of (tokens, experts), in descending order, equal ones by their index, and a
+ *   weight for each: the row's softmax or sigmoid score, divided by the sum of the chosen ones with `renormalize`.  A logit of -inf
+ *   is an expert that is not to be had; where fewer than k others are left the remaining ids are -1 and their weights 0.  A NaN
+ *   counts as the largest value and makes the weights NaN.  ids, weights (tokens, k), contiguous.  experts in [1, 1024],
+ *   k in [1, min(32, experts)].
+ * nvfp4_route_tokens_backward: dlogits (tokens, experts), contiguous, of the logits' type, from the gradient `dweights` (tokens, k) FP32
+ *   of the weights; ids as the forward call gave them. */
+NVFP4_API int nvfp4_route_tokens(const void* logits, int64_t ld_elems, int dtype, int64_t tokens, int experts, int k, int scores,
+                                 int renormalize, int64_t* ids, float* weights, void* stream);
+NVFP4_API int nvfp4_route_tokens_backward(const void* logits, int64_t ld_elems, int dtype, int64_t tokens, int experts, int k, int scores,
+                                          int renormalize, const int64_t* ids, const float* dweights, void* dlogits, void* stream);
+
+/* nvfp4_sort_tokens: token rows x (tokens, hidden) into the contiguous layout of nvfp4_grouped_gemm_contiguous.  Pair p = token * k + choice
+ *   goes to a row of expert ids[p]'s group; groups lie in the order of the experts, each starts on a multiple of `alignment`, and a
+ *   group's pairs keep their order.  M, the rows of the buffer, is what the host can bound without the routing:
+ *     M = (n + min(experts, n) * (alignment - 1)) / alignment * alignment,   n = tokens * k.
+ *   Writes rows (M, hidden), zero where there is no pair; place[p], the pair's row, -1 for an id outside [0, experts); source[r],
+ *   the row's pair, -1 for none; m_indices[r], the expert whose group holds the row, -1 behind the last group.
+ *   experts in [1, 1024], M < 2^31.  Any hidden; rows whose bytes, start and strides are multiples of 16 move fastest.
+ * nvfp4_unsort_tokens: y[t] = sum over j < k of w[t, j] * rows[place[t, j]] (FP32, ascending j, rounded once; w NULL: 1), y (tokens, hidden)
+ *   contiguous.  place outside [0, M) contributes nothing.  With w NULL it is the gradient of nvfp4_sort_tokens, too.
+ * nvfp4_unsort_tokens_backward: drows (M, hidden) contiguous = w[t, j] * dy[t] at place[t, j], zero at rows whose source is -1;
+ *   dw[t, j] = <dy[t], rows[place[t, j]]> in FP32.  Either may be NULL, and rows with dw NULL.  place and source as nvfp4_sort_tokens
+ *   gives them. */
+NVFP4_API int nvfp4_sort_tokens(const void* x, int64_t ldx_elems, int dtype, int64_t tokens, int k, int hidden, const int64_t* ids, int experts,
+                                int alignment, int64_t M, void* rows, int64_t* place, int32_t* source, int32_t* m_indices, void* stream);
+NVFP4_API int nvfp4_unsort_tokens(const void* rows, int64_t ld_elems, int dtype, int64_t M, const int64_t* place, const float* w, int64_t tokens,
+                                  int k, int hidden, void* y, void* stream);
+NVFP4_API int nvfp4_unsort_tokens_backward(const void* dy, int64_t ldy_elems, const void* rows, int64_t ld_elems, int dtype, int64_t M,
+                                           const int64_t* place, const int32_t* source, const float* w, int64_t tokens, int k, int hidden,
+                                           void* drows, float* dw, void* stream);
 
 /* Test hook: Algorithm 1 exactly as the GEMM's transform warps run it (same device
  * code, same shared-memory layouts), with the codes copied out instead of being fed to

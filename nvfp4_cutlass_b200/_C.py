@@ -46,7 +46,8 @@ EXPORTS = ("nvfp4_last_error", "nvfp4_version", "nvfp4_get_num_sms", "nvfp4_set_
            "nvfp4_grouped_gemm_masked_quantized", "nvfp4_grouped_gemm_masked_quantized_swiglu", "nvfp4_grouped_gemm_masked_quantized_rows", "nvfp4_expert_mlp_few_rows", "nvfp4_combine_rows_peer", "nvfp4_expert_histogram",
            "nvfp4_grouped_gemm_swiglu_contiguous", "nvfp4_grouped_gemm_masked", "nvfp4_load_checkpoint_weights",
            "nvfp4_read_status", "nvfp4_debug_split_workspace", "nvfp4_debug_wait_timeout", "nvfp4_debug_quantize_weight_expired", "nvfp4_plan_peer_masked", "nvfp4_plan_one_rank",
-           "nvfp4_peer_barrier")
+           "nvfp4_peer_barrier", "nvfp4_route_tokens", "nvfp4_route_tokens_backward", "nvfp4_sort_tokens", "nvfp4_unsort_tokens",
+           "nvfp4_unsort_tokens_backward")
 
 
 def library_path() -> str:
@@ -97,6 +98,11 @@ def lib() -> ctypes.CDLL:
         L.nvfp4_debug_mma_peak.argtypes = [i32, ctypes.POINTER(ctypes.c_double), vp]
         L.nvfp4_debug_mma_peak_pair.argtypes = [i32, ctypes.POINTER(ctypes.c_double), vp]
         L.nvfp4_debug_mma_pattern.argtypes = [i32, i32, i32, i32, i32, ctypes.POINTER(ctypes.c_double), vp]
+        L.nvfp4_route_tokens.argtypes = [vp, i64, i32, i64, i32, i32, i32, i32, vp, vp, vp]
+        L.nvfp4_route_tokens_backward.argtypes = [vp, i64, i32, i64, i32, i32, i32, i32, vp, vp, vp, vp]
+        L.nvfp4_sort_tokens.argtypes = [vp, i64, i32, i64, i32, i32, vp, i32, i32, i64, vp, vp, vp, vp, vp]
+        L.nvfp4_unsort_tokens.argtypes = [vp, i64, i32, i64, vp, vp, i64, i32, i32, vp, vp]
+        L.nvfp4_unsort_tokens_backward.argtypes = [vp, i64, vp, i64, i32, i64, vp, vp, vp, i64, i32, i32, vp, vp, vp]
         _contiguous_call = _bind(L)
         _lib = L                                     # last: another thread that finds it set makes its call at once
     return _lib
@@ -687,6 +693,106 @@ def combine_rows_peer(peers: torch.Tensor, rows_ld_elems: int, src_rank: torch.T
                                              tokens, k, hidden, y.data_ptr(), y.stride(0), peers.numel(), rows_cap, int(sm_budget),
                                              1 if bulk else 0, status.data_ptr() if status is not None else None, _stream()))
     return y
+
+
+# ---- operators around the grouped GEMM: routing, rows sorted by expert and back (tokens.py puts the gradients on top) ----
+
+DTYPE_CODES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+SCORE_CODES = {"softmax": 0, "sigmoid": 1}
+
+
+def _matrix(t, name: str) -> int:
+    """Row stride of a 2-D CUDA tensor of a known type with contiguous rows."""
+    _require(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.dtype in DTYPE_CODES,
+             f"{name} is a 2-D BF16, FP16 or FP32 CUDA tensor")
+    rows, columns = t.shape
+    _require(columns <= 1 or t.stride(1) == 1, f"{name} is contiguous along its last dimension")
+    if rows <= 1:
+        return max(columns, 1)
+    _require(t.stride(0) >= columns, f"the rows of {name} do not overlap")
+    return t.stride(0)
+
+
+def route_tokens(logits: torch.Tensor, k: int, scores: str, renormalize: bool):
+    """(ids int64, weights float32), both (tokens, k); see nvfp4_route_tokens in the header."""
+    ld = _matrix(logits, "logits")
+    (tokens, experts), dev = logits.shape, logits.device
+    _require(1 <= experts <= 1024 and 1 <= k <= min(32, experts), f"experts ({experts}) in [1, 1024], k ({k}) in [1, min(32, experts)]")
+    _require(scores in SCORE_CODES, "scores is 'softmax' or 'sigmoid'")
+    ids = torch.empty(tokens, k, dtype=torch.int64, device=dev)
+    weights = torch.empty(tokens, k, dtype=torch.float32, device=dev)
+    with _on(dev):
+        _check(lib().nvfp4_route_tokens(logits.data_ptr(), ld, DTYPE_CODES[logits.dtype], tokens, experts, k, SCORE_CODES[scores],
+                                        1 if renormalize else 0, ids.data_ptr(), weights.data_ptr(), _stream()))
+    return ids, weights
+
+
+def route_tokens_backward(logits: torch.Tensor, ids: torch.Tensor, dweights: torch.Tensor, scores: str, renormalize: bool) -> torch.Tensor:
+    ld = _matrix(logits, "logits")
+    (tokens, experts), k = logits.shape, ids.shape[1]
+    dweights = dweights.to(torch.float32).contiguous()
+    dlogits = torch.empty(tokens, experts, dtype=logits.dtype, device=logits.device)
+    with _on(_one_device(logits, ids, dweights)):
+        _check(lib().nvfp4_route_tokens_backward(logits.data_ptr(), ld, DTYPE_CODES[logits.dtype], tokens, experts, k, SCORE_CODES[scores],
+                                                 1 if renormalize else 0, ids.data_ptr(), dweights.data_ptr(), dlogits.data_ptr(), _stream()))
+    return dlogits
+
+
+def sorted_rows(pairs: int, num_experts: int, alignment: int) -> int:
+    """Rows of the buffer that sort_tokens fills: a bound on the padded groups that needs no routing."""
+    return (pairs + min(num_experts, pairs) * (alignment - 1)) // alignment * alignment
+
+
+def sort_tokens(x: torch.Tensor, ids: torch.Tensor, num_experts: int, alignment: int):
+    """(rows (M, hidden), place int64 like ids, source int32 (M,), m_indices int32 (M,)); see nvfp4_sort_tokens in the header."""
+    ldx = _matrix(x, "x")
+    _require(isinstance(ids, torch.Tensor) and ids.dtype == torch.int64 and ids.dim() == 2 and ids.shape[0] == x.shape[0] and ids.shape[1] >= 1,
+             "ids is int64 with one row per token and at least one column")
+    _require(1 <= num_experts <= 1024, f"num_experts ({num_experts}) in [1, 1024]")
+    _require(1 <= alignment <= 1 << 20, f"alignment ({alignment}) in [1, 2^20]")
+    (tokens, hidden), k, dev = x.shape, ids.shape[1], _one_device(x, ids)
+    _require(hidden >= 1, "x has at least one column")
+    m = sorted_rows(tokens * k, num_experts, alignment)
+    _require(m < 1 << 31, f"{m} rows do not fit 31 bits")
+    ids = ids.contiguous()
+    rows = torch.empty(m, hidden, dtype=x.dtype, device=dev)
+    place = torch.empty(tokens, k, dtype=torch.int64, device=dev)
+    source = torch.empty(m, dtype=torch.int32, device=dev)
+    m_indices = torch.empty(m, dtype=torch.int32, device=dev)
+    with _on(dev):
+        _check(lib().nvfp4_sort_tokens(x.data_ptr(), ldx, DTYPE_CODES[x.dtype], tokens, k, hidden, ids.data_ptr(), num_experts, alignment, m,
+                                       rows.data_ptr(), place.data_ptr(), source.data_ptr(), m_indices.data_ptr(), _stream()))
+    return rows, place, source, m_indices
+
+
+def unsort_tokens(rows: torch.Tensor, place: torch.Tensor, weights) -> torch.Tensor:
+    """y[t] = sum_j weights[t, j] * rows[place[t, j]] (weights None: 1), of the rows' type."""
+    ld = _matrix(rows, "rows")
+    _require(place.dtype == torch.int64 and place.dim() == 2 and place.shape[1] >= 1 and place.is_contiguous(), "place is contiguous int64 (tokens, k)")
+    _require(weights is None or (weights.dtype == torch.float32 and weights.shape == place.shape and weights.is_contiguous()),
+             "weights are contiguous float32, one for every place")
+    (m, hidden), (tokens, k), dev = rows.shape, place.shape, _one_device(rows, place, weights)
+    _require(hidden >= 1, "rows have at least one column")
+    y = torch.empty(tokens, hidden, dtype=rows.dtype, device=dev)
+    with _on(dev):
+        _check(lib().nvfp4_unsort_tokens(rows.data_ptr(), ld, DTYPE_CODES[rows.dtype], m, place.data_ptr(),
+                                         weights.data_ptr() if weights is not None else None, tokens, k, hidden, y.data_ptr(), _stream()))
+    return y
+
+
+def unsort_tokens_backward(dy: torch.Tensor, rows, place: torch.Tensor, source: torch.Tensor, weights, want_rows: bool, want_weights: bool):
+    """(drows, dweights), None where not wanted."""
+    ldy, m = _matrix(dy, "dy"), source.numel()
+    (tokens, hidden), k, dev = dy.shape, place.shape[1], _one_device(dy, rows, place, source, weights)
+    ld = _matrix(rows, "rows") if want_weights else hidden
+    drows = torch.empty(m, hidden, dtype=dy.dtype, device=dev) if want_rows else None
+    dweights = torch.empty(tokens, k, dtype=torch.float32, device=dev) if want_weights else None
+    with _on(dev):
+        _check(lib().nvfp4_unsort_tokens_backward(dy.data_ptr(), ldy, rows.data_ptr() if want_weights else None, ld, DTYPE_CODES[dy.dtype], m,
+                                                  place.data_ptr(), source.data_ptr(), weights.data_ptr() if weights is not None else None, tokens,
+                                                  k, hidden, drows.data_ptr() if want_rows else None,
+                                                  dweights.data_ptr() if want_weights else None, _stream()))
+    return drows, dweights
 
 
 def debug_decompose(a: torch.Tensor, scale_policy: str = "derived_div8"):

@@ -754,6 +754,105 @@ int nvfp4_combine_rows_peer(const int64_t* peers, int64_t rows_ld_elems, const i
                                     device_status, static_cast<cudaStream_t>(stream));
 }
 
+// ---- operators around the grouped GEMM --------------------------------------------------------------------------
+
+static bool known_dtype(int dtype) { return dtype == NVFP4_DTYPE_BF16 || dtype == NVFP4_DTYPE_F16 || dtype == NVFP4_DTYPE_F32; }
+static bool on_elements(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == NVFP4_DTYPE_F32 ? 3u : 1u)) == 0; }
+
+static int check_route(int64_t ld, int dtype, int64_t tokens, int experts, int k, int scores)
+{
+    NVFP4_REQUIRE(known_dtype(dtype), "unknown type code %d", dtype);
+    NVFP4_REQUIRE(experts >= 1 && experts <= 1024 && k >= 1 && k <= 32 && k <= experts,
+                  "experts (%d) must be in [1, 1024] and k (%d) in [1, min(32, experts)]", experts, k);
+    NVFP4_REQUIRE(scores == NVFP4_SCORES_SOFTMAX || scores == NVFP4_SCORES_SIGMOID, "unknown score function %d", scores);
+    NVFP4_REQUIRE(tokens >= 0 && tokens <= INT_MAX && ld >= experts, "bad number of tokens or row stride (tokens=%lld, ld=%lld)",
+                  static_cast<long long>(tokens), static_cast<long long>(ld));
+    return NVFP4_OK;
+}
+
+int nvfp4_route_tokens(const void* logits, int64_t ld_elems, int dtype, int64_t tokens, int experts, int k, int scores, int renormalize,
+                       int64_t* ids, float* weights, void* stream)
+{
+    host::clear_error();
+    if (int rc = check_route(ld_elems, dtype, tokens, experts, k, scores)) return rc;
+    if (tokens == 0) return NVFP4_OK;
+    NVFP4_REQUIRE(logits && ids && weights, "null pointer argument");
+    NVFP4_REQUIRE(on_elements(logits, dtype), "logits are not aligned to their type");
+    return launch_route(logits, ld_elems, dtype, tokens, experts, k, scores == NVFP4_SCORES_SIGMOID, renormalize != 0, ids, weights,
+                        static_cast<cudaStream_t>(stream));
+}
+
+int nvfp4_route_tokens_backward(const void* logits, int64_t ld_elems, int dtype, int64_t tokens, int experts, int k, int scores, int renormalize,
+                                const int64_t* ids, const float* dweights, void* dlogits, void* stream)
+{
+    host::clear_error();
+    if (int rc = check_route(ld_elems, dtype, tokens, experts, k, scores)) return rc;
+    if (tokens == 0) return NVFP4_OK;
+    NVFP4_REQUIRE(logits && ids && dweights && dlogits, "null pointer argument");
+    NVFP4_REQUIRE(on_elements(logits, dtype) && on_elements(dlogits, dtype), "logits are not aligned to their type");
+    return launch_route_backward(logits, ld_elems, dtype, tokens, experts, k, scores == NVFP4_SCORES_SIGMOID, renormalize != 0, ids, dweights,
+                                 dlogits, static_cast<cudaStream_t>(stream));
+}
+
+static int check_token_rows(int dtype, int64_t M, int64_t tokens, int k, int hidden, int64_t ld)
+{
+    NVFP4_REQUIRE(known_dtype(dtype), "unknown type code %d", dtype);
+    NVFP4_REQUIRE(tokens >= 0 && k >= 1 && hidden >= 1 && hidden <= (1 << 28), "bad sizes (tokens=%lld, k=%d, hidden=%d)",
+                  static_cast<long long>(tokens), k, hidden);
+    NVFP4_REQUIRE(tokens <= INT_MAX / k, "too many (token, choice) pairs (tokens=%lld, k=%d)", static_cast<long long>(tokens), k);
+    NVFP4_REQUIRE(M >= 0 && M <= INT_MAX, "number of rows (%lld) outside [0, 2^31)", static_cast<long long>(M));
+    NVFP4_REQUIRE(ld >= hidden, "row stride (%lld) smaller than the row (%d)", static_cast<long long>(ld), hidden);
+    return NVFP4_OK;
+}
+
+int nvfp4_sort_tokens(const void* x, int64_t ldx_elems, int dtype, int64_t tokens, int k, int hidden, const int64_t* ids, int experts, int alignment,
+                      int64_t M, void* rows, int64_t* place, int32_t* source, int32_t* m_indices, void* stream)
+{
+    host::clear_error();
+    if (int rc = check_token_rows(dtype, M, tokens, k, hidden, ldx_elems)) return rc;
+    NVFP4_REQUIRE(experts >= 1 && experts <= 1024 && alignment >= 1 && alignment <= (1 << 20), "experts (%d) must be in [1, 1024], alignment (%d) in [1, 2^20]",
+                  experts, alignment);
+    const int64_t n = tokens * k, want = (n + (experts < n ? experts : n) * (alignment - 1)) / alignment * alignment;
+    NVFP4_REQUIRE(M == want, "M is %lld for these sizes (got %lld)", static_cast<long long>(want), static_cast<long long>(M));
+    if (tokens == 0) return NVFP4_OK;
+    NVFP4_REQUIRE(x && ids && rows && place && source && m_indices, "null pointer argument");
+    NVFP4_REQUIRE(on_elements(x, dtype) && on_elements(rows, dtype), "rows are not aligned to their type");
+    const int64_t size = dtype == NVFP4_DTYPE_F32 ? 4 : 2;
+    host::DeviceInfo* dev;
+    if (int rc = host::device_info(-1, &dev)) return rc;
+    return launch_sort_tokens(x, ldx_elems * size, tokens, k, hidden * size, ids, experts, alignment, M, rows, place, source, m_indices, dev->hw_sms,
+                              static_cast<cudaStream_t>(stream));
+}
+
+int nvfp4_unsort_tokens(const void* rows, int64_t ld_elems, int dtype, int64_t M, const int64_t* place, const float* w, int64_t tokens, int k,
+                        int hidden, void* y, void* stream)
+{
+    host::clear_error();
+    if (int rc = check_token_rows(dtype, M, tokens, k, hidden, ld_elems)) return rc;
+    if (tokens == 0) return NVFP4_OK;
+    NVFP4_REQUIRE((rows || M == 0) && place && y, "null pointer argument");
+    NVFP4_REQUIRE(on_elements(rows, dtype) && on_elements(y, dtype), "rows are not aligned to their type");
+    host::DeviceInfo* dev;
+    if (int rc = host::device_info(-1, &dev)) return rc;
+    return launch_unsort_tokens(rows, ld_elems, dtype, M, place, w, tokens, k, hidden, y, dev->hw_sms, static_cast<cudaStream_t>(stream));
+}
+
+int nvfp4_unsort_tokens_backward(const void* dy, int64_t ldy_elems, const void* rows, int64_t ld_elems, int dtype, int64_t M, const int64_t* place,
+                                 const int32_t* source, const float* w, int64_t tokens, int k, int hidden, void* drows, float* dw, void* stream)
+{
+    host::clear_error();
+    if (int rc = check_token_rows(dtype, M, tokens, k, hidden, ld_elems)) return rc;
+    NVFP4_REQUIRE(ldy_elems >= hidden, "row stride (%lld) smaller than the row (%d)", static_cast<long long>(ldy_elems), hidden);
+    NVFP4_REQUIRE(tokens + (M + 7) / 8 <= INT_MAX, "too many tokens and rows");
+    if ((drows == nullptr && dw == nullptr) || (tokens == 0 && M == 0)) return NVFP4_OK;
+    NVFP4_REQUIRE(tokens == 0 || (dy && place), "null pointer argument");
+    NVFP4_REQUIRE(dw == nullptr || rows != nullptr || M == 0, "the weights' gradient needs the rows");
+    NVFP4_REQUIRE(drows == nullptr || source != nullptr || M == 0, "the rows' gradient needs their sources");
+    NVFP4_REQUIRE(on_elements(dy, dtype) && on_elements(rows, dtype) && on_elements(drows, dtype), "rows are not aligned to their type");
+    return launch_unsort_tokens_backward(dy, ldy_elems, rows, ld_elems, dtype, M, place, source, w, tokens, k, hidden, drows, dw,
+                                         static_cast<cudaStream_t>(stream));
+}
+
 int nvfp4_debug_decompose(const void* a, int64_t lda_elems, int M, int K, int scale_policy, void* q0, void* q1,
                           void* s0, void* s1, void* stream)
 {

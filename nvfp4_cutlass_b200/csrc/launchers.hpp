@@ -56,6 +56,18 @@ int launch_combine_rows_peer(const int64_t* peers, int64_t rows_ld_elems, const 
                              const float* w, int64_t tokens, int k, int hidden, void* y, int64_t y_ld_elems, int world,
                              int64_t rows_cap, int num_sms, bool bulk, int32_t* status, cudaStream_t stream);
 
+int launch_route(const void* logits, int64_t ld, int dtype, int64_t tokens, int experts, int k, bool sigmoid, bool renormalize, int64_t* ids,
+                 float* weights, cudaStream_t stream);
+int launch_route_backward(const void* logits, int64_t ld, int dtype, int64_t tokens, int experts, int k, bool sigmoid, bool renormalize,
+                          const int64_t* ids, const float* grad, void* dlogits, cudaStream_t stream);
+int launch_sort_tokens(const void* x, int64_t ldx_bytes, int64_t tokens, int k, int64_t row_bytes, const int64_t* ids, int experts, int alignment,
+                       int64_t m, void* rows, int64_t* place, int32_t* source, int32_t* m_indices, int num_sms, cudaStream_t stream);
+int launch_unsort_tokens(const void* rows, int64_t ld, int dtype, int64_t m, const int64_t* place, const float* w, int64_t tokens, int k, int hidden,
+                         void* y, int num_sms, cudaStream_t stream);
+int launch_unsort_tokens_backward(const void* dy, int64_t ldy, const void* rows, int64_t ld, int dtype, int64_t m, const int64_t* place,
+                                  const int32_t* source, const float* w, int64_t tokens, int k, int hidden, void* drows, float* dw,
+                                  cudaStream_t stream);
+
 int launch_gemm_swap(const void* a, int64_t lda, const void* b, const void* sfb, const float* gw, void* d,
                      int64_t ldd, const int32_t* m_indices, int M, int N, int K, int E, bool residual,
                      int token_tile, int block_k, int policy, bool pdl, int num_sms, int32_t* status, cudaStream_t stream);

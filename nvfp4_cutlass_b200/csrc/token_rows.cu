@@ -1,0 +1,594 @@
+// Token rows sorted by expert into the grouped GEMM's contiguous layout, and back with the routing weights applied; both with gradients.
+//
+// Forward there: a stable counting sort of the n = tokens * k (token, choice) pairs.  Expert e's rows start on a multiple of the
+// alignment behind the padded rows of the experts before it, its pairs in their order; the buffer has the rows that the host
+// can bound without knowing the routing (sorted_rows), rows without a pair are zero, and nothing comes back to the host.
+//   pass A   every warp counts its run of pairs per expert: __match_any_sync finds the lanes of one expert, one of them counts them
+//   scan     over a block's warps per expert, over blocks, over experts (padded sizes)
+//   pass B   every warp walks its run again and hands out rows from its counters
+// No atomics: the order does not depend on timing.
+// Up to kOneKernelPairs pairs every block of a single kernel works the whole plan out for itself (a few thousand cycles, less than a
+// launch) and then takes its share of the buffer's rows; above, a kernel counts chunks of pairs, one hands out rows and one moves the
+// rows, each launched while its predecessor drains.  All of it is bound by the bytes of the buffer that is written.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "host_common.hpp"
+#include "launchers.hpp"
+#include "ptx.cuh"
+
+namespace nvfp4 {
+namespace {
+
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr uint32_t kAll = 0xffffffffu;
+constexpr int kMaxExperts = 1024;                    // two per thread in the scans; 64 KB of counters
+constexpr int64_t kOneKernelPairs = 4096;
+
+// Shared memory of a block that plans, in words: per-warp counters, then per expert first row, rows, first sorted pair.
+__host__ __device__ constexpr size_t plan_words(int experts) { return static_cast<size_t>(experts) * (kWarps + 3) + 1 + 2 * kWarps; }
+
+struct Plan {
+    uint32_t* table;       // [kWarps][experts] pairs of an expert in a warp's run, then: in lower warps' runs
+    uint32_t* start;       // [experts + 1] first row of the expert's group; last: end of all groups
+    uint32_t* count;       // [experts] rows with a pair
+    uint32_t* first;       // [experts] pairs of lower experts
+    uint32_t* scratch;     // [2 * kWarps]
+    __device__ Plan(uint32_t* smem, int experts)
+        : table(smem), start(table + kWarps * experts), count(start + experts + 1), first(count + experts), scratch(first + experts)
+    {
+    }
+};
+
+// The lanes' experts for pairs p0 + lane, -1 for pairs behind `hi` and ids out of range.
+__device__ __forceinline__ int expert_of(const int64_t* __restrict__ ids, int64_t p, int64_t hi, int experts)
+{
+    if (p >= hi) return -1;
+    const int64_t e = ids[p];
+    return e >= 0 && e < experts ? static_cast<int>(e) : -1;
+}
+
+// A warp's run of the pairs [lo, hi) that the block handles, in whole groups of 32.
+__device__ __forceinline__ void my_run(int64_t lo, int64_t hi, int64_t& from, int64_t& to)
+{
+    const int64_t groups = (hi - lo + 31) / 32, each = (groups + kWarps - 1) / kWarps, warp = threadIdx.x >> 5;
+    from = min(lo + warp * each * 32, hi);
+    to = min(from + each * 32, hi);
+}
+
+__device__ __forceinline__ void clear_table(const Plan& s, int experts)
+{
+    for (int i = threadIdx.x; i < kWarps * experts; i += kThreads) s.table[i] = 0;
+    __syncthreads();
+}
+
+// Pass A over [lo, hi); afterwards table holds, per warp, what lower warps have of an expert, and total(e) is called with the block's sum.
+template <typename Total>
+__device__ __forceinline__ void count_pairs(const int64_t* __restrict__ ids, int64_t lo, int64_t hi, int experts, const Plan& s, Total&& total)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t from, to;
+    my_run(lo, hi, from, to);
+    for (int64_t p0 = from; p0 < to; p0 += 32) {
+        const int e = expert_of(ids, p0 + lane, to, experts);
+        const unsigned same = __match_any_sync(kAll, e);
+        if (e >= 0 && lane == __ffs(same) - 1) s.table[warp * experts + e] += __popc(same);
+        __syncwarp();
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += kThreads) {
+        uint32_t sum = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const uint32_t c = s.table[w * experts + e];
+            s.table[w * experts + e] = sum;
+            sum += c;
+        }
+        total(e, sum);
+    }
+    __syncthreads();
+}
+
+// Pass B: row(e, rank) for every pair of [lo, hi) in its order, rank among the block's pairs of expert e; row(-1, 0) for a pair without.
+template <typename Row>
+__device__ __forceinline__ void hand_out(const int64_t* __restrict__ ids, int64_t lo, int64_t hi, int experts, const Plan& s, Row&& row)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t from, to;
+    my_run(lo, hi, from, to);
+    for (int64_t p0 = from; p0 < to; p0 += 32) {
+        const int64_t p = p0 + lane;
+        const int e = expert_of(ids, p, to, experts);
+        const unsigned same = __match_any_sync(kAll, e);
+        const int leader = __ffs(same) - 1;
+        uint32_t base = 0;
+        if (e >= 0 && lane == leader) {
+            base = s.table[warp * experts + e];
+            s.table[warp * experts + e] = base + __popc(same);
+        }
+        base = __shfl_sync(kAll, base, leader);
+        if (p < to) row(p, e, base + __popc(same & ((1u << lane) - 1u)));
+        __syncwarp();
+    }
+}
+
+// start and first from count, by all threads of the block.
+__device__ __forceinline__ void scan_experts(int experts, uint32_t alignment, const Plan& s)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e0 = 2 * threadIdx.x;
+    uint32_t c[2], a[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        c[i] = e0 + i < experts ? s.count[e0 + i] : 0u;
+        a[i] = (c[i] + alignment - 1) / alignment * alignment;
+    }
+    uint32_t rows = a[0] + a[1], pairs = c[0] + c[1];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t r = __shfl_up_sync(kAll, rows, d), q = __shfl_up_sync(kAll, pairs, d);
+        if (lane >= d) { rows += r; pairs += q; }
+    }
+    if (lane == 31) { s.scratch[warp] = rows; s.scratch[kWarps + warp] = pairs; }
+    __syncthreads();
+    uint32_t rows_before = rows - a[0] - a[1], pairs_before = pairs - c[0] - c[1];
+    for (int w = 0; w < warp; ++w) { rows_before += s.scratch[w]; pairs_before += s.scratch[kWarps + w]; }
+    if (e0 < experts) { s.start[e0] = rows_before; s.first[e0] = pairs_before; }
+    if (e0 + 1 < experts) { s.start[e0 + 1] = rows_before + a[0]; s.first[e0 + 1] = pairs_before + c[0]; }
+    if (e0 < experts && e0 + 2 >= experts) s.start[experts] = rows_before + a[0] + a[1];
+    __syncthreads();
+}
+
+// Expert whose group holds a row; `experts` behind the last group.  Empty groups share their start with the next one.
+__device__ __forceinline__ int group_of(const uint32_t* start, int experts, uint32_t row)
+{
+    int lo = 0, hi = experts + 1;                    // start[lo] <= row < start[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (start[mid] <= row) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Rows move as words W of 16, 4 or 2 bytes: the widest that both buffers' starts, strides and the row's length are multiples of.
+// A warp's piece of a row: kPieceWords words a lane.
+constexpr int kPieceWords = 4;
+
+template <typename W>
+__global__ void __launch_bounds__(kThreads)
+sort_one_kernel(const W* __restrict__ x, int64_t ldx, const int64_t* __restrict__ ids, int64_t n, int k, int experts, uint32_t alignment, uint32_t m,
+                uint32_t row_words, W* __restrict__ rows, int64_t* __restrict__ place, int32_t* __restrict__ source, int32_t* __restrict__ m_indices)
+{
+    extern __shared__ uint32_t smem[];
+    const Plan s(smem, experts);
+    uint16_t* order = reinterpret_cast<uint16_t*>(smem + plan_words(experts));      // pairs in the order of the experts
+    ptx::grid_dependency_wait();
+    clear_table(s, experts);
+    count_pairs(ids, 0, n, experts, s, [&](int e, uint32_t sum) { s.count[e] = sum; });
+    scan_experts(experts, alignment, s);
+    hand_out(ids, 0, n, experts, s, [&](int64_t p, int e, uint32_t rank) {
+        if (e >= 0) order[s.first[e] + rank] = static_cast<uint16_t>(p);
+        if (blockIdx.x == 0) place[p] = e >= 0 ? static_cast<int64_t>(s.start[e]) + rank : -1;
+    });
+    __syncthreads();
+    const uint32_t lane = threadIdx.x & 31, pieces = (row_words + 32 * kPieceWords - 1) / (32 * kPieceWords);
+    const uint64_t units = static_cast<uint64_t>(m) * pieces;
+    // consecutive units to different blocks
+    for (uint64_t unit = static_cast<uint64_t>(threadIdx.x >> 5) * gridDim.x + blockIdx.x; unit < units; unit += static_cast<uint64_t>(gridDim.x) * kWarps) {
+        const uint32_t r = static_cast<uint32_t>(unit / pieces), piece = static_cast<uint32_t>(unit % pieces);
+        const int e = group_of(s.start, experts, r);
+        const bool live = e < experts && r - s.start[e] < s.count[e];
+        const uint32_t pair = live ? order[s.first[e] + (r - s.start[e])] : 0u;
+        if (piece == 0 && lane == 0) {
+            source[r] = live ? static_cast<int32_t>(pair) : -1;
+            m_indices[r] = e < experts ? e : -1;
+        }
+        const W* from = x + static_cast<int64_t>(pair / k) * ldx;
+        W* to = rows + static_cast<int64_t>(r) * row_words;
+        W v[kPieceWords];
+        const uint32_t c0 = piece * 32 * kPieceWords + lane;
+#pragma unroll
+        for (int i = 0; i < kPieceWords; ++i) {
+            v[i] = W{};
+            if (live && c0 + i * 32 < row_words) v[i] = __ldg(from + c0 + i * 32);
+        }
+#pragma unroll
+        for (int i = 0; i < kPieceWords; ++i)
+            if (c0 + i * 32 < row_words) to[c0 + i * 32] = v[i];
+    }
+}
+
+__global__ void __launch_bounds__(kThreads)
+sort_count_kernel(const int64_t* __restrict__ ids, int64_t n, int64_t chunk, int experts, uint32_t* __restrict__ counts)
+{
+    extern __shared__ uint32_t smem[];
+    const Plan s(smem, experts);
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
+    clear_table(s, experts);
+    const int64_t lo = blockIdx.x * chunk, hi = min(lo + chunk, n);
+    count_pairs(ids, lo, hi, experts, s, [&](int e, uint32_t sum) { counts[static_cast<int64_t>(blockIdx.x) * experts + e] = sum; });
+}
+
+// groups: [experts + 1] first rows, [experts] rows with a pair; written by block 0.
+__global__ void __launch_bounds__(kThreads)
+sort_place_kernel(const int64_t* __restrict__ ids, int64_t n, int64_t chunk, int experts, uint32_t alignment, const uint32_t* __restrict__ counts,
+                  uint32_t* __restrict__ groups, int64_t* __restrict__ place, int32_t* __restrict__ source)
+{
+    extern __shared__ uint32_t smem[];
+    const Plan s(smem, experts);
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
+    // column sums of the chunks' counts, all of them and those before this block's; the warps' table is free until pass A and
+    // takes the partial sums: slice i of the threads adds every slices-th chunk
+    const int width = experts < kThreads ? (experts + 31) / 32 * 32 : kThreads, slices = kThreads / width;      // slices <= kWarps
+    const int slice = threadIdx.x / width, column = threadIdx.x % width;
+    uint32_t all[2] = {0, 0}, before[2] = {0, 0};
+    for (int i = 0; i < 2; ++i) {
+        const int e = column + i * width;
+        if (e >= experts || slice >= slices) continue;
+        for (unsigned c = slice; c < gridDim.x; c += slices) {
+            const uint32_t v = counts[static_cast<int64_t>(c) * experts + e];
+            all[i] += v;
+            if (c < blockIdx.x) before[i] += v;
+        }
+    }
+    auto add_up = [&](const uint32_t (&part)[2], auto&& store) {
+        for (int i = 0; i < 2; ++i)
+            if (column + i * width < experts && slice < slices) s.table[slice * experts + column + i * width] = part[i];
+        __syncthreads();
+        for (int e = threadIdx.x; e < experts; e += kThreads) {
+            uint32_t sum = 0;
+            for (int j = 0; j < slices; ++j) sum += s.table[j * experts + e];
+            store(e, sum);
+        }
+        __syncthreads();
+    };
+    add_up(all, [&](int e, uint32_t sum) { s.count[e] = sum; });
+    scan_experts(experts, alignment, s);
+    if (blockIdx.x == 0) {
+        for (int e = threadIdx.x; e <= experts; e += kThreads) groups[e] = s.start[e];
+        for (int e = threadIdx.x; e < experts; e += kThreads) groups[experts + 1 + e] = s.count[e];
+    }
+    add_up(before, [&](int e, uint32_t sum) { s.first[e] = s.start[e] + sum; });      // from here on: first row of this chunk's pairs
+    clear_table(s, experts);
+    const int64_t lo = blockIdx.x * chunk, hi = min(lo + chunk, n);
+    count_pairs(ids, lo, hi, experts, s, [](int, uint32_t) {});
+    hand_out(ids, lo, hi, experts, s, [&](int64_t p, int e, uint32_t rank) {
+        const int64_t r = e >= 0 ? static_cast<int64_t>(s.first[e]) + rank : -1;
+        place[p] = r;
+        if (r >= 0) source[r] = static_cast<int32_t>(p);
+    });
+}
+
+// Every token's row is read once and written k times (unit: a piece of a token); behind the tokens come the rows eight at a time: the
+// ones without a pair are zeroed, and all get their expert.
+constexpr uint32_t kRowsPerUnit = 8;
+template <typename W>
+__global__ void __launch_bounds__(kThreads)
+sort_move_kernel(const W* __restrict__ x, int64_t ldx, uint32_t tokens, int k, int experts, uint32_t m, uint32_t row_words,
+                 const uint32_t* __restrict__ groups, const int64_t* __restrict__ place, W* __restrict__ rows, int32_t* __restrict__ source,
+                 int32_t* __restrict__ m_indices)
+{
+    const uint32_t lane = threadIdx.x & 31, pieces = (row_words + 32 * kPieceWords - 1) / (32 * kPieceWords);
+    const uint64_t token_units = static_cast<uint64_t>(tokens) * pieces, units = token_units + (m + kRowsPerUnit - 1) / kRowsPerUnit;
+    ptx::grid_dependency_wait();
+    for (uint64_t unit = static_cast<uint64_t>(threadIdx.x >> 5) * gridDim.x + blockIdx.x; unit < units; unit += static_cast<uint64_t>(gridDim.x) * kWarps) {
+        if (unit < token_units) {
+            const uint32_t t = static_cast<uint32_t>(unit / pieces), c0 = static_cast<uint32_t>(unit % pieces) * 32 * kPieceWords + lane;
+            const W* from = x + static_cast<int64_t>(t) * ldx;
+            W v[kPieceWords];
+#pragma unroll
+            for (int i = 0; i < kPieceWords; ++i)
+                if (c0 + i * 32 < row_words) v[i] = __ldg(from + c0 + i * 32);
+            for (int j0 = 0; j0 < k; j0 += 32) {
+                const int64_t mine = j0 + static_cast<int>(lane) < k ? place[static_cast<int64_t>(t) * k + j0 + lane] : -1;
+                const int here = min(32, k - j0);
+                for (int j = 0; j < here; ++j) {
+                    const int64_t r = __shfl_sync(kAll, mine, j);
+                    if (r < 0) continue;
+                    W* to = rows + r * row_words;
+#pragma unroll
+                    for (int i = 0; i < kPieceWords; ++i)
+                        if (c0 + i * 32 < row_words) to[c0 + i * 32] = v[i];
+                }
+            }
+            continue;
+        }
+        const uint32_t r0 = static_cast<uint32_t>(unit - token_units) * kRowsPerUnit;
+        bool pad = false;
+        if (lane < kRowsPerUnit && r0 + lane < m) {
+            const uint32_t r = r0 + lane;
+            const int e = group_of(groups, experts, r);
+            pad = e >= experts || r - groups[e] >= groups[experts + 1 + e];
+            m_indices[r] = e < experts ? e : -1;
+            if (pad) source[r] = -1;
+        }
+        for (unsigned todo = __ballot_sync(kAll, pad); todo != 0; todo &= todo - 1) {
+            W* to = rows + static_cast<int64_t>(r0 + __ffs(todo) - 1) * row_words;
+            for (uint32_t c = lane; c < row_words; c += 32) to[c] = W{};
+        }
+    }
+}
+
+// ---- back: y[t] = sum_j w[t, j] * rows[place[t, j]] ------------------------------------------------------------------------------------
+
+// kN elements of T as one access
+template <typename T, int kN>
+struct alignas(sizeof(T) * kN) Pack {
+    T v[kN];
+};
+template <typename P>
+__device__ __forceinline__ P load_pack(const P* at)
+{
+    if constexpr (sizeof(P) == 16) {
+        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(at));
+        return *reinterpret_cast<const P*>(&raw);
+    } else {
+        return *at;
+    }
+}
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ void from_float(float v, float& out) { out = v; }
+__device__ __forceinline__ void from_float(float v, __nv_bfloat16& out) { out = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void from_float(float v, __half& out) { out = __float2half_rn(v); }
+
+// A warp takes a piece of a token, kPer packs a lane; the rows of up to four choices are under way together.  FP32, ascending j.
+// The gradient of the sort is the same sum without weights.
+constexpr int kPer = 2, kFlight = 4;
+template <typename T, int kN>
+__global__ void __launch_bounds__(256)
+unsort_kernel(const Pack<T, kN>* __restrict__ rows, int64_t ld, const int64_t* __restrict__ place, const float* __restrict__ w, uint32_t tokens,
+              int k, int64_t m, uint32_t row_packs, Pack<T, kN>* __restrict__ y)
+{
+    const uint32_t lane = threadIdx.x & 31, pieces = (row_packs + 32 * kPer - 1) / (32 * kPer);
+    const uint64_t units = static_cast<uint64_t>(tokens) * pieces;
+    ptx::grid_dependency_wait();
+    for (uint64_t unit = static_cast<uint64_t>(threadIdx.x >> 5) * gridDim.x + blockIdx.x; unit < units; unit += static_cast<uint64_t>(gridDim.x) * 8) {
+        const uint32_t t = static_cast<uint32_t>(unit / pieces), c0 = static_cast<uint32_t>(unit % pieces) * 32 * kPer + lane;
+        float acc[kPer][kN];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+#pragma unroll
+            for (int q = 0; q < kN; ++q) acc[i][q] = 0.0f;
+        for (int j0 = 0; j0 < k; j0 += 32) {
+            int64_t mine = -1;
+            float weight = 1.0f;
+            if (j0 + static_cast<int>(lane) < k) {
+                mine = place[static_cast<int64_t>(t) * k + j0 + lane];
+                if (mine >= m) mine = -1;
+                if (w != nullptr) weight = w[static_cast<int64_t>(t) * k + j0 + lane];
+            }
+            const int here = min(32, k - j0);
+            for (int j1 = 0; j1 < here; j1 += kFlight) {
+                Pack<T, kN> v[kFlight][kPer];
+                bool live[kFlight];
+                float wj[kFlight];
+#pragma unroll
+                for (int u = 0; u < kFlight; ++u) {
+                    const int64_t r = __shfl_sync(kAll, mine, (j1 + u) & 31);
+                    wj[u] = __shfl_sync(kAll, weight, (j1 + u) & 31);
+                    live[u] = j1 + u < here && r >= 0;
+                    if (live[u]) {
+#pragma unroll
+                        for (int i = 0; i < kPer; ++i)
+                            if (c0 + i * 32 < row_packs) v[u][i] = load_pack(rows + r * ld + c0 + i * 32);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < kFlight; ++u) {
+                    if (!live[u]) continue;
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i)
+#pragma unroll
+                        for (int q = 0; q < kN; ++q) acc[i][q] = fmaf(wj[u], to_float(v[u][i].v[q]), acc[i][q]);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (c0 + i * 32 >= row_packs) continue;
+            Pack<T, kN> o;
+#pragma unroll
+            for (int q = 0; q < kN; ++q) from_float(acc[i][q], o.v[q]);
+            y[static_cast<int64_t>(t) * row_packs + c0 + i * 32] = o;
+        }
+    }
+}
+
+// Gradients of that sum: drows[place[t, j]] = w[t, j] * dy[t], zero for rows without a pair, dw[t, j] = <dy[t], rows[place[t, j]]>.
+// A block takes a token: dy is read once for every group of eight choices (from L1 after the first), every row of `rows` once, every
+// row of `drows` is written once.  A token's dot products stay inside its block and are added in a fixed order.  Behind the
+// tokens: blocks that zero the rows whose source is -1.  drows or dw may be NULL; rows is read for dw alone.
+constexpr int kBackThreads = 256, kBackWarps = kBackThreads / 32, kGroup = 8;
+template <typename T, int kN>
+__global__ void __launch_bounds__(kBackThreads)
+unsort_backward_kernel(const Pack<T, kN>* __restrict__ dy, int64_t ldy, const Pack<T, kN>* __restrict__ rows, int64_t ld,
+                       const int64_t* __restrict__ place, const int32_t* __restrict__ source, const float* __restrict__ w, uint32_t tokens, int k,
+                       int64_t m, uint32_t row_packs, Pack<T, kN>* __restrict__ drows, float* __restrict__ dw)
+{
+    __shared__ float part[kBackWarps][kGroup];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    ptx::grid_dependency_wait();
+    if (blockIdx.x >= tokens) {                                              // a warp per row
+        const int64_t r = static_cast<int64_t>(blockIdx.x - tokens) * kBackWarps + warp;
+        if (r >= m || source[r] >= 0) return;
+        for (uint32_t c = lane; c < row_packs; c += 32) drows[r * row_packs + c] = Pack<T, kN>{};
+        return;
+    }
+    const int64_t t = blockIdx.x;
+    for (int j0 = 0; j0 < k; j0 += kGroup) {
+        int64_t r[kGroup];
+        float wj[kGroup], dot[kGroup];
+#pragma unroll
+        for (int u = 0; u < kGroup; ++u) {
+            r[u] = j0 + u < k ? place[t * k + j0 + u] : -1;
+            if (r[u] >= m) r[u] = -1;
+            wj[u] = w != nullptr && j0 + u < k ? w[t * k + j0 + u] : 1.0f;
+            dot[u] = 0.0f;
+        }
+        for (uint32_t c = threadIdx.x; c < row_packs; c += kBackThreads) {
+            const Pack<T, kN> g = load_pack(dy + t * ldy + c);
+            float gf[kN];
+#pragma unroll
+            for (int q = 0; q < kN; ++q) gf[q] = to_float(g.v[q]);
+            if (dw != nullptr) {
+                Pack<T, kN> v[kGroup];
+#pragma unroll
+                for (int u = 0; u < kGroup; ++u)
+                    if (r[u] >= 0) v[u] = load_pack(rows + r[u] * ld + c);
+#pragma unroll
+                for (int u = 0; u < kGroup; ++u) {
+                    if (r[u] < 0) continue;
+#pragma unroll
+                    for (int q = 0; q < kN; ++q) dot[u] = fmaf(gf[q], to_float(v[u].v[q]), dot[u]);
+                }
+            }
+            if (drows != nullptr) {
+#pragma unroll
+                for (int u = 0; u < kGroup; ++u) {
+                    if (r[u] < 0) continue;
+                    Pack<T, kN> o;
+#pragma unroll
+                    for (int q = 0; q < kN; ++q) from_float(wj[u] * gf[q], o.v[q]);
+                    drows[r[u] * row_packs + c] = o;
+                }
+            }
+        }
+        if (dw == nullptr) continue;
+#pragma unroll
+        for (int u = 0; u < kGroup; ++u) {
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) dot[u] += __shfl_xor_sync(kAll, dot[u], d);
+            if (lane == 0) part[warp][u] = dot[u];
+        }
+        __syncthreads();
+        if (threadIdx.x < kGroup && j0 + static_cast<int>(threadIdx.x) < k) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kBackWarps; ++i) sum += part[i][threadIdx.x];
+            dw[t * k + j0 + threadIdx.x] = sum;
+        }
+        __syncthreads();
+    }
+}
+
+// Calls f(T*, elements of a 16-byte pack or 1) for a type code.
+template <typename F>
+int with_pack(int dtype, bool wide, F&& f)
+{
+    auto packs = [&](auto* type) {
+        constexpr int kN = 16 / static_cast<int>(sizeof(*type));
+        return wide ? f(type, std::integral_constant<int, kN>{}) : f(type, std::integral_constant<int, 1>{});
+    };
+    switch (dtype) {
+        case NVFP4_DTYPE_BF16: return packs(static_cast<__nv_bfloat16*>(nullptr));
+        case NVFP4_DTYPE_F16: return packs(static_cast<__half*>(nullptr));
+        default: return packs(static_cast<float*>(nullptr));
+    }
+}
+
+size_t elem_bytes(int dtype) { return dtype == NVFP4_DTYPE_F32 ? 4 : 2; }
+
+// Blocks of `warps` warps for so many units, at most `per_sm` to an SM.
+unsigned blocks_for(uint64_t units, int warps, int num_sms, int per_sm)
+{
+    const uint64_t most = static_cast<uint64_t>(num_sms) * per_sm, want = (units + warps - 1) / warps;
+    // few units: one warp's worth to a block rather than one block's worth to an SM
+    const uint64_t spread = units < static_cast<uint64_t>(num_sms) ? units : (want < static_cast<uint64_t>(num_sms) ? num_sms : want);
+    return static_cast<unsigned>(spread < most ? spread : most);
+}
+
+template <typename W>
+int sort_with(const void* x, int64_t ldx_bytes, int64_t tokens, int k, int64_t row_bytes, const int64_t* ids, int experts, int alignment, int64_t m,
+              void* rows, int64_t* place, int32_t* source, int32_t* m_indices, int num_sms, cudaStream_t stream)
+{
+    const int64_t n = tokens * k, ldx = ldx_bytes / static_cast<int64_t>(sizeof(W));
+    const uint32_t row_words = static_cast<uint32_t>(row_bytes / static_cast<int64_t>(sizeof(W)));
+    const uint64_t pieces = (row_words + 32 * kPieceWords - 1) / (32 * kPieceWords);
+    const size_t plan_bytes = plan_words(experts) * sizeof(uint32_t);
+    int dev = 0;
+    NVFP4_CUDA_CHECK(cudaGetDevice(&dev));
+    constexpr size_t kMostSmem = plan_words(kMaxExperts) * sizeof(uint32_t) + kOneKernelPairs * sizeof(uint16_t);
+    static bool attr_set[host::kMaxDevices] = {};
+    if (!attr_set[dev]) {
+        NVFP4_CUDA_CHECK(cudaFuncSetAttribute(sort_one_kernel<W>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostSmem)));
+        NVFP4_CUDA_CHECK(cudaFuncSetAttribute(sort_count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostSmem)));
+        NVFP4_CUDA_CHECK(cudaFuncSetAttribute(sort_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostSmem)));
+        attr_set[dev] = true;
+    }
+    if (n <= kOneKernelPairs)
+        return host::launch_kernel(sort_one_kernel<W>, dim3(blocks_for(static_cast<uint64_t>(m) * pieces, kWarps, num_sms, 2)), dim3(kThreads),
+                                   plan_bytes + static_cast<size_t>(n) * sizeof(uint16_t), stream, true, static_cast<const W*>(x), ldx, ids, n, k,
+                                   experts, static_cast<uint32_t>(alignment), static_cast<uint32_t>(m), row_words, static_cast<W*>(rows), place, source,
+                                   m_indices);
+    int64_t chunk = (n + num_sms - 1) / num_sms;
+    chunk = (chunk + kThreads - 1) / kThreads * kThreads;
+    const unsigned blocks = static_cast<unsigned>((n + chunk - 1) / chunk);
+    cudaMemPool_t pool;
+    if (int rc = host::workspace_pool(dev, &pool)) return rc;
+    uint32_t* counts = nullptr;
+    const size_t count_words = static_cast<size_t>(blocks) * experts;
+    NVFP4_CUDA_CHECK(cudaMallocFromPoolAsync(reinterpret_cast<void**>(&counts), (count_words + 2 * experts + 1) * sizeof(uint32_t), pool, stream));
+    uint32_t* groups = counts + count_words;
+    int rc = host::launch_kernel(sort_count_kernel, dim3(blocks), dim3(kThreads), plan_bytes, stream, true, ids, n, chunk, experts, counts);
+    if (rc == NVFP4_OK)
+        rc = host::launch_kernel(sort_place_kernel, dim3(blocks), dim3(kThreads), plan_bytes, stream, true, ids, n, chunk, experts,
+                                 static_cast<uint32_t>(alignment), counts, groups, place, source);
+    if (rc == NVFP4_OK)
+        rc = host::launch_kernel(sort_move_kernel<W>,
+                                 dim3(blocks_for(static_cast<uint64_t>(tokens) * pieces + (m + kRowsPerUnit - 1) / kRowsPerUnit, kWarps, num_sms, 4)),
+                                 dim3(kThreads), 0, stream, true, static_cast<const W*>(x), ldx, static_cast<uint32_t>(tokens), k, experts,
+                                 static_cast<uint32_t>(m), row_words, groups, place, static_cast<W*>(rows), source, m_indices);
+    cudaFreeAsync(counts, stream);
+    return rc;
+}
+
+}  // namespace
+
+int launch_sort_tokens(const void* x, int64_t ldx_bytes, int64_t tokens, int k, int64_t row_bytes, const int64_t* ids, int experts, int alignment,
+                       int64_t m, void* rows, int64_t* place, int32_t* source, int32_t* m_indices, int num_sms, cudaStream_t stream)
+{
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(rows) | static_cast<uintptr_t>(ldx_bytes | row_bytes);
+    auto with = (bits & 15u) == 0 ? sort_with<uint4> : (bits & 3u) == 0 ? sort_with<uint32_t> : sort_with<uint16_t>;
+    return with(x, ldx_bytes, tokens, k, row_bytes, ids, experts, alignment, m, rows, place, source, m_indices, num_sms, stream);
+}
+
+int launch_unsort_tokens(const void* rows, int64_t ld, int dtype, int64_t m, const int64_t* place, const float* w, int64_t tokens, int k, int hidden,
+                         void* y, int num_sms, cudaStream_t stream)
+{
+    const size_t size = elem_bytes(dtype);
+    const bool wide = ((reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(y) | static_cast<uintptr_t>(ld * size) | hidden * size) & 15u) == 0;
+    return with_pack(dtype, wide, [&](auto* type, auto n) {
+        using T = std::remove_pointer_t<decltype(type)>;
+        constexpr int kN = decltype(n)::value;
+        const uint32_t packs = static_cast<uint32_t>(hidden / kN);
+        const uint64_t units = static_cast<uint64_t>(tokens) * ((packs + 32 * kPer - 1) / (32 * kPer));
+        return host::launch_kernel(unsort_kernel<T, kN>, dim3(blocks_for(units, 8, num_sms, 8)), dim3(256), 0, stream, true,
+                                   static_cast<const Pack<T, kN>*>(rows), ld / kN, place, w, static_cast<uint32_t>(tokens), k, m, packs,
+                                   static_cast<Pack<T, kN>*>(y));
+    });
+}
+
+int launch_unsort_tokens_backward(const void* dy, int64_t ldy, const void* rows, int64_t ld, int dtype, int64_t m, const int64_t* place,
+                                  const int32_t* source, const float* w, int64_t tokens, int k, int hidden, void* drows, float* dw,
+                                  cudaStream_t stream)
+{
+    const size_t size = elem_bytes(dtype);
+    const bool wide = ((reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(drows) |
+                        static_cast<uintptr_t>(ldy * size) | static_cast<uintptr_t>(ld * size) | hidden * size) & 15u) == 0;
+    return with_pack(dtype, wide, [&](auto* type, auto n) {
+        using T = std::remove_pointer_t<decltype(type)>;
+        constexpr int kN = decltype(n)::value;
+        const int64_t zeroing = drows != nullptr ? (m + kBackWarps - 1) / kBackWarps : 0;
+        return host::launch_kernel(unsort_backward_kernel<T, kN>, dim3(static_cast<unsigned>(tokens + zeroing)), dim3(kBackThreads), 0, stream, true,
+                                   static_cast<const Pack<T, kN>*>(dy), ldy / kN, static_cast<const Pack<T, kN>*>(rows), ld / kN, place, source, w,
+                                   static_cast<uint32_t>(tokens), k, m, static_cast<uint32_t>(hidden / kN), static_cast<Pack<T, kN>*>(drows), dw);
+    });
+}
+
+}  // namespace nvfp4
