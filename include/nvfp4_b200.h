@@ -47,6 +47,9 @@ enum { NVFP4_ORIENT_NORMAL = 0, NVFP4_ORIENT_SWAP_AB = 1 };
 enum { NVFP4_DTYPE_BF16 = 0, NVFP4_DTYPE_F32 = 1, NVFP4_DTYPE_F16 = 2 /* not a weight type: rows, logits and products below */ };
 /* router scores of nvfp4_route_tokens */
 enum { NVFP4_SCORES_SOFTMAX = 0, NVFP4_SCORES_SIGMOID = 1 };
+/* activations of nvfp4_linear; GELU is z Phi(z), GELU_TANH its form with tanh */
+enum { NVFP4_ACTIVATION_NONE = 0, NVFP4_ACTIVATION_RELU = 1, NVFP4_ACTIVATION_GELU = 2, NVFP4_ACTIVATION_GELU_TANH = 3,
+       NVFP4_ACTIVATION_SILU = 4 };
 
 /* Text of the calling thread's last error ("" if none).  Never NULL. */
 NVFP4_API const char* nvfp4_last_error(void);
@@ -363,6 +366,27 @@ NVFP4_API int nvfp4_unsort_tokens(const void* rows, int64_t ld_elems, int dtype,
 NVFP4_API int nvfp4_unsort_tokens_backward(const void* dy, int64_t ldy_elems, const void* rows, int64_t ld_elems, int dtype, int64_t M,
                                            const int64_t* place, const int32_t* source, const float* w, int64_t tokens, int k, int hidden,
                                            void* drows, float* dw, void* stream);
+
+/* Dense products on the tensor cores, operands BF16 or FP16 (`dtype`), FP32 sums rounded once.  x, w, z, dz and what else is an operand:
+ * 16-byte-aligned starts, row strides that are multiples of 8 elements; K >= 1, K % 8 == 0.  M and N are any; outputs, bias
+ * and residual have any alignment and stride.
+ * nvfp4_linear: d[M,N] = activation(x[M,K] w[N,K]^T + bias[N]) + residual[M,N].  d and residual have out_dtype, `dtype` or
+ *   NVFP4_DTYPE_F32; bias (of type `dtype`) and residual may be NULL.  z (may be NULL) receives what the activation is applied to, rounded to
+ *   `dtype`, for the backward pass.
+ * nvfp4_linear_dz: dz[M,N] = dd * activation'(z), rounded to `dtype` for the products below, and db[N], the sums of its columns taken before
+ *   that rounding.  dd has out_dtype, any alignment and stride; z is not read for NVFP4_ACTIVATION_NONE.  z and dz have row strides of
+ *   N rounded up to 8 at least, and the elements behind column N of dz are overwritten.  dz or db may be NULL.
+ * nvfp4_linear_dx: dx[M,K] = dz w.      nvfp4_linear_dw: dw[N,K] = dz^T x.      Rounded to `dtype`.
+ * device_status (may be NULL) receives bit 0 if a bounded wait expired.  No counterparts in the reference project. */
+NVFP4_API int nvfp4_linear(const void* x, int64_t ldx_elems, const void* w, int64_t ldw_elems, const void* bias, const void* residual,
+                           int64_t ldr_elems, void* d, int64_t ldd_elems, void* z, int64_t ldz_elems, int M, int N, int K, int dtype,
+                           int out_dtype, int activation, int32_t* device_status, void* stream);
+NVFP4_API int nvfp4_linear_dz(const void* dd, int64_t ldd_elems, const void* z, int64_t ldz_elems, void* dz, int64_t lddz_elems, void* db, int M,
+                              int N, int dtype, int out_dtype, int activation, void* stream);
+NVFP4_API int nvfp4_linear_dx(const void* dz, int64_t lddz_elems, const void* w, int64_t ldw_elems, void* dx, int64_t lddx_elems, int M, int N,
+                              int K, int dtype, int32_t* device_status, void* stream);
+NVFP4_API int nvfp4_linear_dw(const void* dz, int64_t lddz_elems, const void* x, int64_t ldx_elems, void* dw, int64_t lddw_elems, int M, int N,
+                              int K, int dtype, int32_t* device_status, void* stream);
 
 /* Test hook: Algorithm 1 exactly as the GEMM's transform warps run it (same device
  * code, same shared-memory layouts), with the codes copied out instead of being fed to

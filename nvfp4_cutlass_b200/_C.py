@@ -47,7 +47,7 @@ EXPORTS = ("nvfp4_last_error", "nvfp4_version", "nvfp4_get_num_sms", "nvfp4_set_
            "nvfp4_grouped_gemm_swiglu_contiguous", "nvfp4_grouped_gemm_masked", "nvfp4_load_checkpoint_weights",
            "nvfp4_read_status", "nvfp4_debug_split_workspace", "nvfp4_debug_wait_timeout", "nvfp4_debug_quantize_weight_expired", "nvfp4_plan_peer_masked", "nvfp4_plan_one_rank",
            "nvfp4_peer_barrier", "nvfp4_route_tokens", "nvfp4_route_tokens_backward", "nvfp4_sort_tokens", "nvfp4_unsort_tokens",
-           "nvfp4_unsort_tokens_backward")
+           "nvfp4_unsort_tokens_backward", "nvfp4_linear", "nvfp4_linear_dz", "nvfp4_linear_dx", "nvfp4_linear_dw")
 
 
 def library_path() -> str:
@@ -103,6 +103,10 @@ def lib() -> ctypes.CDLL:
         L.nvfp4_sort_tokens.argtypes = [vp, i64, i32, i64, i32, i32, vp, i32, i32, i64, vp, vp, vp, vp, vp]
         L.nvfp4_unsort_tokens.argtypes = [vp, i64, i32, i64, vp, vp, i64, i32, i32, vp, vp]
         L.nvfp4_unsort_tokens_backward.argtypes = [vp, i64, vp, i64, i32, i64, vp, vp, vp, i64, i32, i32, vp, vp, vp]
+        L.nvfp4_linear.argtypes = [vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, i32, i32, vp, vp]
+        L.nvfp4_linear_dz.argtypes = [vp, i64, vp, i64, vp, i64, vp, i32, i32, i32, i32, i32, vp]
+        L.nvfp4_linear_dx.argtypes = [vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp]
+        L.nvfp4_linear_dw.argtypes = [vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp]
         _contiguous_call = _bind(L)
         _lib = L                                     # last: another thread that finds it set makes its call at once
     return _lib
@@ -706,8 +710,10 @@ def _matrix(t, name: str) -> int:
     _require(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.dtype in DTYPE_CODES,
              f"{name} is a 2-D BF16, FP16 or FP32 CUDA tensor")
     rows, columns = t.shape
+    if rows == 0:                                        # strides say nothing
+        return max(columns, 1)
     _require(columns <= 1 or t.stride(1) == 1, f"{name} is contiguous along its last dimension")
-    if rows <= 1:
+    if rows == 1:
         return max(columns, 1)
     _require(t.stride(0) >= columns, f"the rows of {name} do not overlap")
     return t.stride(0)
@@ -793,6 +799,80 @@ def unsort_tokens_backward(dy: torch.Tensor, rows, place: torch.Tensor, source: 
                                                   k, hidden, drows.data_ptr() if want_rows else None,
                                                   dweights.data_ptr() if want_weights else None, _stream()))
     return drows, dweights
+
+
+# ---- dense products (dense.py puts the gradients on top) ----
+
+ACTIVATION_CODES = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+def _operand(t, name: str) -> int:
+    """Row stride of an operand of the dense products."""
+    ld = _matrix(t, name)
+    _require(t.dtype != torch.float32, f"{name} is BF16 or FP16")
+    _require(ld % 8 == 0 and t.data_ptr() % 16 == 0, f"{name} starts on 16 bytes, its row stride is a multiple of 8 elements")
+    return ld
+
+
+def _padded(rows: int, columns: int, like: torch.Tensor) -> torch.Tensor:
+    """(rows, columns) whose row stride is a multiple of 8."""
+    return torch.empty(rows, (columns + 7) // 8 * 8, dtype=like.dtype, device=like.device)[:, :columns]
+
+
+def linear(x: torch.Tensor, w: torch.Tensor, bias, residual, activation: str, out_dtype, keep: bool = False, device_status=None):
+    """(d, z): d = activation(x w^T + bias) + residual, z what the activation is applied to, None without `keep`; see nvfp4_linear."""
+    ldx, ldw = _operand(x, "x"), _operand(w, "w")
+    (m, k), n, dev = x.shape, w.shape[0], _one_device(x, w, bias, residual, device_status)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    _require(w.dtype == x.dtype and w.shape[1] == k, "x (M, K) and w (N, K) are of one type and one K")
+    _require(k >= 8 and k % 8 == 0, f"K ({k}) is a positive multiple of 8")
+    _require(activation in ACTIVATION_CODES, f"activation is one of {', '.join(ACTIVATION_CODES)}")
+    _require(out_dtype in (x.dtype, torch.float32), "out_dtype is the type of x or float32")
+    _require(bias is None or (bias.dtype == x.dtype and bias.shape == (n,) and (bias.is_contiguous())), "bias is (N,), contiguous, of the type of x")
+    _require(residual is None or (residual.dtype == out_dtype and residual.shape == (m, n)), "residual is (M, N), of the output's type")
+    ldr = _matrix(residual, "residual") if residual is not None else 0
+    d = torch.empty(m, n, dtype=out_dtype, device=dev)
+    z = _padded(m, n, x) if keep else None
+    with _on(dev):
+        _check(lib().nvfp4_linear(x.data_ptr(), ldx, w.data_ptr(), ldw, bias.data_ptr() if bias is not None else None,
+                                  residual.data_ptr() if residual is not None else None, ldr, d.data_ptr(), n,
+                                  z.data_ptr() if keep else None, z.stride(0) if keep else 0, m, n, k, DTYPE_CODES[x.dtype],
+                                  DTYPE_CODES[out_dtype], ACTIVATION_CODES[activation],
+                                  device_status.data_ptr() if device_status is not None else None, _stream()))
+    return d, z
+
+
+def linear_backward(dd: torch.Tensor, x, w, z, dtype: torch.dtype, activation: str, want_x: bool, want_w: bool, want_bias: bool, device_status=None):
+    """(dx, dw, db) of `linear`, None where not wanted; dd contiguous along its rows."""
+    ldd, (m, n) = _matrix(dd, "dd"), dd.shape
+    dev = _one_device(dd, x, w, z, device_status)
+    like = torch.empty(0, dtype=dtype, device=dev)
+    status = device_status.data_ptr() if device_status is not None else None
+    code = DTYPE_CODES[dtype]
+    k = x.shape[1] if x is not None else w.shape[1] if w is not None else 0
+    products = want_x or want_w
+    # without an activation the incoming gradient is dz itself, where it can be an operand
+    as_it_is = activation == "none" and dd.dtype == dtype and ldd % 8 == 0 and dd.data_ptr() % 16 == 0
+    dz = dd if as_it_is else _padded(m, n, like) if products else None
+    db = torch.empty(n, dtype=dtype, device=dev) if want_bias else None
+    dx = torch.empty(m, k, dtype=dtype, device=dev) if want_x else None
+    dw = torch.empty(n, k, dtype=dtype, device=dev) if want_w else None
+    if m == 0 or n == 0:                                 # sums over nothing
+        for t in (dx, dw, db):
+            if t is not None:
+                t.zero_()
+        return dx, dw, db
+    ldz = dz.stride(0) if products and m > 1 else (n + 7) // 8 * 8
+    with _on(dev):
+        if want_bias or (products and not as_it_is):
+            _check(lib().nvfp4_linear_dz(dd.data_ptr(), ldd, z.data_ptr() if z is not None else None, z.stride(0) if z is not None else 0,
+                                         None if as_it_is or not products else dz.data_ptr(), ldz, db.data_ptr() if want_bias else None, m, n,
+                                         code, DTYPE_CODES[dd.dtype], ACTIVATION_CODES[activation], _stream()))
+        if want_x:
+            _check(lib().nvfp4_linear_dx(dz.data_ptr(), ldz, w.data_ptr(), _operand(w, "w"), dx.data_ptr(), k, m, n, k, code, status, _stream()))
+        if want_w:
+            _check(lib().nvfp4_linear_dw(dz.data_ptr(), ldz, x.data_ptr(), _operand(x, "x"), dw.data_ptr(), k, m, n, k, code, status, _stream()))
+    return dx, dw, db
 
 
 def debug_decompose(a: torch.Tensor, scale_policy: str = "derived_div8"):

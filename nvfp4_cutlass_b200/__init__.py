@@ -10,6 +10,7 @@ from . import _C, layout
 from ._C import get_num_sms, m_grouped_bf16_dual_nvfp4_gemm_contiguous, set_num_sms
 from ._C import m_grouped_bf16_dual_nvfp4_gemm_masked
 from .layout import dequantize_weight_nvfp4, load_checkpoint_weights_nvfp4, make_m_indices, quantize_weight_nvfp4
+from .dense import linear
 from .tokens import TokenOrder, route_tokens, sort_tokens, unsort_tokens
 
 __all__ = [
@@ -23,6 +24,7 @@ __all__ = [
     "sort_tokens",
     "unsort_tokens",
     "TokenOrder",
+    "linear",
     "layout",
     "get_num_sms",
     "set_num_sms",

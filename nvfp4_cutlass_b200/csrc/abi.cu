@@ -853,6 +853,102 @@ int nvfp4_unsort_tokens_backward(const void* dy, int64_t ldy_elems, const void* 
                                          static_cast<cudaStream_t>(stream));
 }
 
+// An operand of the dense products.
+static int check_operand(const char* name, const void* p, int64_t ld, int64_t columns)
+{
+    NVFP4_REQUIRE(p != nullptr, "null pointer argument (%s)", name);
+    NVFP4_REQUIRE((reinterpret_cast<uintptr_t>(p) & 15u) == 0, "%s must be 16-byte aligned", name);
+    NVFP4_REQUIRE(ld >= columns && ld % 8 == 0 && ld < (1ll << 38), "row stride of %s (%lld) must cover the row and be a multiple of 8 elements", name,
+                  static_cast<long long>(ld));
+    return NVFP4_OK;
+}
+static int check_linear(int M, int N, int K, int dtype)
+{
+    NVFP4_REQUIRE(dtype == NVFP4_DTYPE_BF16 || dtype == NVFP4_DTYPE_F16, "operands are BF16 or FP16 (type code %d)", dtype);
+    NVFP4_REQUIRE(M >= 0 && N >= 0 && K >= 8 && K % 8 == 0, "M and N must not be negative, K must be a positive multiple of 8 (M=%d, N=%d, K=%d)", M, N, K);
+    return NVFP4_OK;
+}
+static int tensor_core_device(host::DeviceInfo** dev)
+{
+    if (int rc = host::device_info(-1, dev)) return rc;
+    if ((*dev)->cc_major != 10) return host::fail(NVFP4_E_UNSUPPORTED, "needs an sm_100 GPU, found sm_%d%d", (*dev)->cc_major, (*dev)->cc_minor);
+    return NVFP4_OK;
+}
+
+int nvfp4_linear(const void* x, int64_t ldx_elems, const void* w, int64_t ldw_elems, const void* bias, const void* residual, int64_t ldr_elems, void* d,
+                 int64_t ldd_elems, void* z, int64_t ldz_elems, int M, int N, int K, int dtype, int out_dtype, int activation, int32_t* device_status,
+                 void* stream)
+{
+    host::clear_error();
+    if (int rc = check_linear(M, N, K, dtype)) return rc;
+    NVFP4_REQUIRE(out_dtype == dtype || out_dtype == NVFP4_DTYPE_F32, "the output has the operands' type or FP32 (type codes %d, %d)", out_dtype, dtype);
+    NVFP4_REQUIRE(activation >= NVFP4_ACTIVATION_NONE && activation <= NVFP4_ACTIVATION_SILU, "unknown activation %d", activation);
+    if (M == 0 || N == 0) return NVFP4_OK;
+    if (int rc = check_operand("x", x, ldx_elems, K)) return rc;
+    if (int rc = check_operand("w", w, ldw_elems, K)) return rc;
+    NVFP4_REQUIRE(d != nullptr && ldd_elems >= N && (residual == nullptr || ldr_elems >= N) && (z == nullptr || ldz_elems >= N),
+                  "null output, or row strides smaller than the row");
+    NVFP4_REQUIRE(on_elements(d, out_dtype) && on_elements(residual, out_dtype) && on_elements(bias, dtype) && on_elements(z, dtype),
+                  "output, bias or residual is not aligned to its type");
+    host::DeviceInfo* dev;
+    if (int rc = tensor_core_device(&dev)) return rc;
+    return launch_linear(x, ldx_elems, w, ldw_elems, bias, residual, ldr_elems, d, ldd_elems, z, ldz_elems, M, N, K, dtype == NVFP4_DTYPE_BF16,
+                         out_dtype == NVFP4_DTYPE_F32, activation, device_status, dev->num_sms, static_cast<cudaStream_t>(stream));
+}
+
+int nvfp4_linear_dz(const void* dd, int64_t ldd_elems, const void* z, int64_t ldz_elems, void* dz, int64_t lddz_elems, void* db, int M, int N, int dtype,
+                    int out_dtype, int activation, void* stream)
+{
+    host::clear_error();
+    if (int rc = check_linear(M, N, 8, dtype)) return rc;
+    NVFP4_REQUIRE(out_dtype == dtype || out_dtype == NVFP4_DTYPE_F32, "the output has the operands' type or FP32 (type codes %d, %d)", out_dtype, dtype);
+    NVFP4_REQUIRE(activation >= NVFP4_ACTIVATION_NONE && activation <= NVFP4_ACTIVATION_SILU, "unknown activation %d", activation);
+    if (M == 0 || N == 0 || (dz == nullptr && db == nullptr)) return NVFP4_OK;
+    const int64_t padded = (static_cast<int64_t>(N) + 7) / 8 * 8;
+    NVFP4_REQUIRE(dd != nullptr && ldd_elems >= N && on_elements(dd, out_dtype), "dd is null, not aligned to its type, or its rows overlap");
+    NVFP4_REQUIRE(on_elements(db, dtype), "db is not aligned to its type");
+    if (activation != NVFP4_ACTIVATION_NONE)
+        if (int rc = check_operand("z", z, ldz_elems, padded)) return rc;
+    if (dz != nullptr)
+        if (int rc = check_operand("dz", dz, lddz_elems, padded)) return rc;
+    host::DeviceInfo* dev;
+    if (int rc = tensor_core_device(&dev)) return rc;
+    return launch_linear_dz(dd, ldd_elems, out_dtype == NVFP4_DTYPE_F32, z, ldz_elems, dz, lddz_elems, db, M, N, dtype == NVFP4_DTYPE_BF16, activation,
+                            dev->hw_sms, static_cast<cudaStream_t>(stream));
+}
+
+int nvfp4_linear_dx(const void* dz, int64_t lddz_elems, const void* w, int64_t ldw_elems, void* dx, int64_t lddx_elems, int M, int N, int K, int dtype,
+                    int32_t* device_status, void* stream)
+{
+    host::clear_error();
+    if (int rc = check_linear(M, N, K, dtype)) return rc;
+    NVFP4_REQUIRE(N >= 1, "an empty contraction (N=%d)", N);
+    if (M == 0) return NVFP4_OK;
+    if (int rc = check_operand("dz", dz, lddz_elems, N)) return rc;
+    if (int rc = check_operand("w", w, ldw_elems, K)) return rc;
+    NVFP4_REQUIRE(dx != nullptr && lddx_elems >= K && on_elements(dx, dtype), "dx is null, not aligned to its type, or its rows overlap");
+    host::DeviceInfo* dev;
+    if (int rc = tensor_core_device(&dev)) return rc;
+    return launch_linear_dx(dz, lddz_elems, w, ldw_elems, dx, lddx_elems, M, N, K, dtype == NVFP4_DTYPE_BF16, device_status, dev->num_sms,
+                            static_cast<cudaStream_t>(stream));
+}
+
+int nvfp4_linear_dw(const void* dz, int64_t lddz_elems, const void* x, int64_t ldx_elems, void* dw, int64_t lddw_elems, int M, int N, int K, int dtype,
+                    int32_t* device_status, void* stream)
+{
+    host::clear_error();
+    if (int rc = check_linear(M, N, K, dtype)) return rc;
+    NVFP4_REQUIRE(M >= 1, "an empty contraction (M=%d)", M);
+    if (N == 0) return NVFP4_OK;
+    if (int rc = check_operand("dz", dz, lddz_elems, N)) return rc;
+    if (int rc = check_operand("x", x, ldx_elems, K)) return rc;
+    NVFP4_REQUIRE(dw != nullptr && lddw_elems >= K && on_elements(dw, dtype), "dw is null, not aligned to its type, or its rows overlap");
+    host::DeviceInfo* dev;
+    if (int rc = tensor_core_device(&dev)) return rc;
+    return launch_linear_dw(dz, lddz_elems, x, ldx_elems, dw, lddw_elems, M, N, K, dtype == NVFP4_DTYPE_BF16, device_status, dev->num_sms,
+                            static_cast<cudaStream_t>(stream));
+}
+
 int nvfp4_debug_decompose(const void* a, int64_t lda_elems, int M, int K, int scale_policy, void* q0, void* q1,
                           void* s0, void* s1, void* stream)
 {

@@ -68,6 +68,15 @@ int launch_unsort_tokens_backward(const void* dy, int64_t ldy, const void* rows,
                                   const int32_t* source, const float* w, int64_t tokens, int k, int hidden, void* drows, float* dw,
                                   cudaStream_t stream);
 
+int launch_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual, int64_t ldr, void* d, int64_t ldd,
+                  void* z, int64_t ldz, int M, int N, int K, bool bf16, bool out32, int activation, int32_t* status, int num_sms, cudaStream_t stream);
+int launch_linear_dz(const void* dd, int64_t ldd, bool dd32, const void* z, int64_t ldz, void* dz, int64_t lddz, void* db, int M, int N, bool bf16,
+                     int activation, int num_sms, cudaStream_t stream);
+int launch_linear_dx(const void* dz, int64_t lddz, const void* w, int64_t ldw, void* dx, int64_t lddx, int M, int N, int K, bool bf16, int32_t* status,
+                     int num_sms, cudaStream_t stream);
+int launch_linear_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, void* dw, int64_t lddw, int M, int N, int K, bool bf16, int32_t* status,
+                     int num_sms, cudaStream_t stream);
+
 int launch_gemm_swap(const void* a, int64_t lda, const void* b, const void* sfb, const float* gw, void* d,
                      int64_t ldd, const int32_t* m_indices, int M, int N, int K, int E, bool residual,
                      int token_tile, int block_k, int policy, bool pdl, int num_sms, int32_t* status, cudaStream_t stream);

@@ -1,0 +1,718 @@
+// Dense products with bias, activation and residual in the epilogue, BF16 or FP16 operands on the tensor cores, and their gradients.
+//
+//   d = activation(x w^T + bias) + residual                x (M, K), w (N, K)
+//   dz = dd * activation'(z)      dx = dz w      dw = dz^T x      db = sum over rows of dz
+//
+// Each product is D[r, c] = sum_k A[r, k] B[c, k] with an operand's memory running along k (K-major: x and w in the forward product) or
+// along its own rows (MN-major: w in dx, both in dw); TMA brings 64 of k either way and the instruction descriptor says which, so
+// nothing is transposed in memory.  Two kernels:
+//   product_kernel       one 128 x BN tile to a CTA; up to eight CTAs of a cluster share the contraction of a tile where there are few
+//                        tiles, and add their partial sums through distributed shared memory in a fixed order
+//   product_pair_kernel  persistent CTA pairs, 256 x 256 tiles, two accumulators in turn: the epilogue of a tile runs under the
+//                        products of the next
+// Sums are FP32 in tensor memory from the first product to the epilogue, which rounds once.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "gemm_common.cuh"
+#include "host_common.hpp"
+#include "launchers.hpp"
+
+namespace nvfp4 {
+namespace {
+
+using gemm::Ring;
+
+constexpr uint32_t BM = 128, BK = 64;                // rows of A to a CTA; contraction of a ring position (one 128-byte row of either operand)
+constexpr uint32_t kRowBytes = BK * 2;
+constexpr uint32_t kSlotA = BM * kRowBytes;
+constexpr uint32_t kBlockMn = 64 * kRowBytes;        // an MN-major box: 64 rows of the operand x 64 of k
+constexpr uint32_t kAll = 0xffffffffu;
+constexpr uint32_t kMaxDepth = 8;
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+// ---- activations -----------------------------------------------------------------------------------------------------
+// gelu(z) = z Phi(z); its tanh form 0.5 z (1 + tanh u), u = c (z + 0.044715 z^3), is z / (1 + exp(-2 u)): neither loses the digits of
+// small values to a sum near zero.
+constexpr float kGeluC = 0.7978845608028654f;        // sqrt(2 / pi)
+template <int kAct>
+__device__ __forceinline__ float activate(float z)
+{
+    if constexpr (kAct == NVFP4_ACTIVATION_RELU) return z > 0.0f || z != z ? z : 0.0f;
+    else if constexpr (kAct == NVFP4_ACTIVATION_GELU) return z * normcdff(z);
+    else if constexpr (kAct == NVFP4_ACTIVATION_GELU_TANH) return z / (1.0f + expf(-2.0f * kGeluC * z * fmaf(0.044715f * z, z, 1.0f)));
+    else if constexpr (kAct == NVFP4_ACTIVATION_SILU) return z / (1.0f + expf(-z));
+    else return z;
+}
+template <int kAct>
+__device__ __forceinline__ float slope(float z)
+{
+    if constexpr (kAct == NVFP4_ACTIVATION_NONE) return 1.0f;
+    if (z != z) return z;
+    if constexpr (kAct == NVFP4_ACTIVATION_RELU) return z > 0.0f ? 1.0f : 0.0f;
+    z = fminf(fmaxf(z, -40.0f), 40.0f);              // constant to FP32 beyond: no infinity times zero
+    if constexpr (kAct == NVFP4_ACTIVATION_GELU) return fmaf(z, 0.3989422804014327f * expf(-0.5f * z * z), normcdff(z));
+    const float u2 = kAct == NVFP4_ACTIVATION_SILU ? z : 2.0f * kGeluC * z * fmaf(0.044715f * z, z, 1.0f);
+    const float du2 = kAct == NVFP4_ACTIVATION_SILU ? 1.0f : 2.0f * kGeluC * fmaf(3.0f * 0.044715f * z, z, 1.0f);
+    const float e = expf(-fabsf(u2)), near = 1.0f / (1.0f + e), far = e * near;           // of sigmoid(u2) and 1 - sigmoid(u2) the larger, the smaller
+    return fmaf(z * du2, near * far, u2 >= 0.0f ? near : far);
+}
+// Calls f(std::integral_constant<int, activation>) for a code: one switch around a loop of elements.
+template <typename F>
+__device__ __forceinline__ void with_activation(int code, F&& f)
+{
+    switch (code) {
+        case NVFP4_ACTIVATION_RELU: return f(std::integral_constant<int, NVFP4_ACTIVATION_RELU>{});
+        case NVFP4_ACTIVATION_GELU: return f(std::integral_constant<int, NVFP4_ACTIVATION_GELU>{});
+        case NVFP4_ACTIVATION_GELU_TANH: return f(std::integral_constant<int, NVFP4_ACTIVATION_GELU_TANH>{});
+        case NVFP4_ACTIVATION_SILU: return f(std::integral_constant<int, NVFP4_ACTIVATION_SILU>{});
+        default: return f(std::integral_constant<int, NVFP4_ACTIVATION_NONE>{});
+    }
+}
+
+// ---- epilogue --------------------------------------------------------------------------------------------------------
+
+struct Epilogue {
+    void* d; int64_t ldd;                            // (rows, cols), of the operands' type or FP32
+    void* z; int64_t ldz;                            // what the activation is applied to, for the backward pass, or NULL
+    const void* bias;                                // (cols) or NULL
+    const void* residual; int64_t ldr;               // of d's type, or NULL
+    uint32_t rows, cols;
+    int activation;
+    bool out32;
+};
+
+// Up to kN accumulators of a lane: output column `col`, rows row0 + i, i < count.  The lanes of a warp hold neighbouring columns, so that
+// every access of the warp is one run of an output row, whatever its alignment.
+template <typename T, uint32_t kN>
+__device__ __forceinline__ void finish(float (&v)[kN], uint32_t row0, uint32_t count, uint32_t col, const Epilogue& e)
+{
+    const uint32_t rows = row0 < e.rows && col < e.cols ? min(count, e.rows - row0) : 0u;
+    float r[kN];
+    if (e.residual != nullptr) {
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i) {
+            r[i] = 0.0f;
+            const int64_t at = static_cast<int64_t>(row0 + i) * e.ldr + col;
+            if (i < rows) r[i] = e.out32 ? static_cast<const float*>(e.residual)[at] : to_float(static_cast<const T*>(e.residual)[at]);
+        }
+    }
+    if (e.bias != nullptr) {
+        const float b = col < e.cols ? to_float(static_cast<const T*>(e.bias)[col]) : 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i) v[i] += b;
+    }
+    if (e.z != nullptr) {
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i)
+            if (i < rows) static_cast<T*>(e.z)[static_cast<int64_t>(row0 + i) * e.ldz + col] = from_float<T>(v[i]);
+    }
+    if (e.activation != NVFP4_ACTIVATION_NONE)
+        with_activation(e.activation, [&](auto act) {
+#pragma unroll
+            for (uint32_t i = 0; i < kN; ++i) v[i] = activate<decltype(act)::value>(v[i]);
+        });
+    if (e.residual != nullptr) {
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i) v[i] += r[i];
+    }
+    if (e.out32) {
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i)
+            if (i < rows) static_cast<float*>(e.d)[static_cast<int64_t>(row0 + i) * e.ldd + col] = v[i];
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i)
+            if (i < rows) static_cast<T*>(e.d)[static_cast<int64_t>(row0 + i) * e.ldd + col] = from_float<T>(v[i]);
+    }
+}
+
+// 32 x 32 values, lane l holding row l: afterwards lane l holds column l.  Five butterfly steps.
+__device__ __forceinline__ void transpose(float (&v)[32], uint32_t lane)
+{
+#pragma unroll
+    for (uint32_t s = 16; s > 0; s >>= 1) {
+        const bool up = (lane & s) != 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 32; ++i) {
+            if ((i & s) != 0) continue;
+            const float got = __shfl_xor_sync(kAll, up ? v[i] : v[i | s], s);
+            if (up) v[i] = got;
+            else v[i | s] = got;
+        }
+    }
+}
+
+template <uint32_t kN>
+__device__ __forceinline__ void load_accumulators(uint32_t taddr, float (&v)[kN])
+{
+    uint32_t raw[kN];
+    if constexpr (kN == 32) ptx::tmem_ld_32x32b_x32(taddr, raw);
+    else ptx::tmem_ld_32x32b_x16(taddr, raw);
+    ptx::tmem_ld_wait();
+#pragma unroll
+    for (uint32_t i = 0; i < kN; ++i) v[i] = __uint_as_float(raw[i]);
+}
+
+// ---- operands --------------------------------------------------------------------------------------------------------
+
+// The tile of an operand's rows [row0, row0 + kRows) x contraction [64 kb, 64 kb + 64) into shared memory.  What lies outside of the
+// tensor arrives as zeros.  load(dst, inner, outer) is the TMA load of one box.
+template <uint32_t kRows, typename Load>
+__device__ __forceinline__ void load_tile(uint8_t* dst, bool mn_major, uint32_t row0, uint32_t kb, Load&& load)
+{
+    if (!mn_major) {
+        load(dst, kb * BK, row0);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < (kRows + 63) / 64; ++i) load(dst + i * kBlockMn, row0 + i * 64, kb * BK);
+    }
+}
+// Descriptor of the 16 of k at step `step` of a tile
+__device__ __forceinline__ uint64_t operand_desc(uint32_t tile, bool mn_major, uint32_t step)
+{
+    return mn_major ? ptx::make_smem_desc_mn(tile + step * 16 * kRowBytes, kBlockMn, 8 * kRowBytes)
+                    : ptx::make_smem_desc(tile + step * 32, 8 * kRowBytes, ptx::kSwizzle128B);
+}
+
+struct Product {
+    uint32_t tiles_a, tiles_b, k_blocks;
+    uint32_t splits_log2, depth;                     // product_kernel: CTAs to a tile, ring positions
+    bool a_mn, b_mn;
+    int32_t* status;
+};
+
+// ---- one tile to a CTA or cluster --------------------------------------------------------------------------------------
+
+constexpr int kTileThreads = 192;                    // warp 0: TMA, warp 1: products, warps 2-5: epilogue
+constexpr uint32_t tile_stage(uint32_t bn) { return kSlotA + bn * kRowBytes; }
+constexpr uint32_t tile_smem(uint32_t bn, uint32_t depth, bool split)
+{
+    return 1024 + depth * tile_stage(bn) + (split ? bn * BM * 4 : 0) + (2 * kMaxDepth + 1) * 8 + 16;
+}
+
+// kSwap: A is the weight and the output's columns lie on the tensor memory's lanes; else A is x and a warp's 32 x 32 accumulators are
+// transposed first.
+template <typename T, uint32_t BN, bool kSwap>
+__global__ void __launch_bounds__(kTileThreads, 2)
+product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Product p, const Epilogue e)
+{
+    constexpr uint32_t kChunk = BN < 32 ? BN : 32, kStage = tile_stage(BN);
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (smem - ptx::smem_u32(smem_raw));
+    const uint32_t splits = 1u << p.splits_log2, depth = p.depth;
+    float* partial = reinterpret_cast<float*>(gen + depth * kStage);          // [splits][BN / splits][BM], from each CTA of the cluster
+    uint64_t* full = reinterpret_cast<uint64_t*>(gen + depth * kStage + (splits > 1 ? BN * BM * 4 : 0));
+    uint64_t* drained = full + kMaxDepth;
+    uint64_t* tmem_full = drained + kMaxDepth;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_full + 1);
+    volatile uint32_t* abort_flag = tmem_slot + 1;
+
+    const uint32_t warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const uint32_t rank = blockIdx.x & (splits - 1), tile = blockIdx.x >> p.splits_log2;
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < depth; ++i) { ptx::mbar_init(full + i, 1); ptx::mbar_init(drained + i, 1); }
+        ptx::mbar_init(tmem_full, 1);
+        *abort_flag = 0;
+        ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&tm_a);
+        ptx::prefetch_tensormap(&tm_b);
+    }
+    if (warp == 1) ptx::tmem_alloc<BN < 32 ? 32 : BN>(tmem_slot);
+    ptx::tcgen05_fence_before_sync();
+    if (splits > 1) ptx::cluster_sync();             // every CTA of the cluster runs before anybody writes into its shared memory
+    else __syncthreads();
+    ptx::tcgen05_fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    ptx::grid_dependency_wait();
+
+    uint32_t a_blk, b_blk;
+    gemm::tile_coords(tile, p.tiles_a, p.tiles_b, 8, a_blk, b_blk);
+    const uint32_t a0 = a_blk * BM, b0 = b_blk * BN;
+    const uint32_t kb0 = static_cast<uint32_t>(static_cast<uint64_t>(p.k_blocks) * rank >> p.splits_log2);
+    const uint32_t kb1 = static_cast<uint32_t>(static_cast<uint64_t>(p.k_blocks) * (rank + 1) >> p.splits_log2);
+    bool ok = true;
+    auto give_up = [&] {
+        *abort_flag = 1;
+        if (p.status != nullptr) atomicOr(p.status, 1);
+        ok = false;
+    };
+    auto next = [&](Ring& r) {
+        if (++r.slot == depth) { r.slot = 0; r.phase ^= 1; }
+    };
+    if (warp == 0) {
+        const uint32_t issue = ptx::elect_one();
+        Ring r;
+        for (uint32_t kb = kb0; kb < kb1; ++kb) {
+            if (!ptx::all_lanes(ptx::mbar_wait_impl(drained + r.slot, r.phase ^ 1, abort_flag))) { give_up(); break; }
+            uint8_t* to = gen + r.slot * kStage;
+            uint64_t* bar = full + r.slot;
+            ptx::mbar_arrive_expect_tx(bar, kStage, issue);
+            load_tile<BM>(to, p.a_mn, a0, kb, [&](uint8_t* dst, uint32_t c0, uint32_t c1) { ptx::tma_load_2d(dst, &tm_a, bar, c0, c1, issue); });
+            load_tile<BN>(to + kSlotA, p.b_mn, b0, kb, [&](uint8_t* dst, uint32_t c0, uint32_t c1) { ptx::tma_load_2d(dst, &tm_b, bar, c0, c1, issue); });
+            next(r);
+        }
+        ptx::grid_launch_dependents();
+        // the last commits arrive before the block may leave
+        for (uint32_t i = 0; ok && i < depth; ++i) {
+            if (!ptx::all_lanes(ptx::mbar_wait_impl(drained + r.slot, r.phase ^ 1, abort_flag))) give_up();
+            next(r);
+        }
+    } else if (warp == 1) {
+        const uint32_t issue = ptx::elect_one();
+        const uint32_t idesc = ptx::make_idesc_f16(BM, BN, std::is_same<T, __nv_bfloat16>::value, p.a_mn, p.b_mn);
+        Ring r;
+        for (uint32_t kb = kb0; kb < kb1; ++kb) {
+            if (!ptx::all_lanes(ptx::mbar_wait_impl(full + r.slot, r.phase, abort_flag))) { give_up(); break; }
+            ptx::tcgen05_fence_after_sync();
+            const uint32_t at = smem + r.slot * kStage;
+#pragma unroll
+            for (uint32_t s = 0; s < BK / 16; ++s)
+                ptx::tcgen05_mma_f16(tmem, operand_desc(at, p.a_mn, s), operand_desc(at + kSlotA, p.b_mn, s), idesc, (kb != kb0) | s, issue);
+            ptx::tcgen05_commit(drained + r.slot, issue);
+            next(r);
+        }
+        if (ok) ptx::tcgen05_commit(tmem_full, issue);
+    } else {
+        if (!ptx::all_lanes(ptx::mbar_wait_relaxed(tmem_full, 0, abort_flag, 20))) give_up();
+        ptx::tcgen05_fence_after_sync();
+    }
+
+    // epilogue: warp's quadrant of the lanes, 128 rows of A in all
+    const uint32_t quad = warp & 3, row = quad * 32 + lane;
+    const uint32_t taddr = tmem + ((quad * 32) << 16);
+    const uint32_t live = kSwap ? min(BN, e.rows - b0) : BN;                  // columns of the tile that anybody wants
+    auto give = [&](float (&v)[kChunk], uint32_t column, uint32_t count) {    // columns [column, column + count) of the tile
+        if constexpr (kSwap) {
+            finish<T>(v, b0 + column, count, a0 + row, e);
+        } else {
+            transpose(v, lane);
+            finish<T>(v, a0 + quad * 32, 32, b0 + column + lane, e);
+        }
+    };
+    if (splits > 1) {
+        const uint32_t width_log2 = __popc(BN - 1) - p.splits_log2, width = 1u << width_log2;          // columns that a CTA finishes
+        if (warp >= 2 && ok) {
+#pragma unroll 1
+            for (uint32_t c0 = 0; c0 < BN; c0 += kChunk) {
+                if (c0 >= live) break;
+                float v[kChunk];
+                load_accumulators(taddr + c0, v);
+#pragma unroll
+                for (uint32_t i = 0; i < kChunk; ++i) {
+                    const uint32_t c = c0 + i;
+                    if (c < live)
+                        ptx::st_cluster_f32(ptx::map_to_cta(ptx::smem_u32(partial + ((rank << width_log2) + (c & (width - 1))) * BM + row), c >> width_log2), v[i]);
+                }
+            }
+        }
+        ptx::cluster_sync();                         // partial sums have arrived; nobody touches another CTA's memory from here on
+        if (warp >= 2 && ok) {
+#pragma unroll 1
+            for (uint32_t c0 = 0; c0 < width; c0 += kChunk) {
+                const uint32_t first = rank * width + c0;
+                if (first >= live) break;
+                const uint32_t count = min(min(width - c0, kChunk), live - first);
+                float v[kChunk];
+#pragma unroll
+                for (uint32_t i = 0; i < kChunk; ++i) {
+                    v[i] = 0.0f;
+                    if (i < count)
+                        for (uint32_t s = 0; s < splits; ++s) v[i] += partial[((s << width_log2) + c0 + i) * BM + row];
+                }
+                give(v, first, count);
+            }
+        }
+    } else if (warp >= 2 && ok) {
+#pragma unroll 1
+        for (uint32_t c0 = 0; c0 < BN; c0 += kChunk) {
+            if (c0 >= live || (!kSwap && b0 + c0 >= e.cols)) break;
+            float v[kChunk];
+            load_accumulators(taddr + c0, v);
+            give(v, c0, kChunk);
+        }
+    }
+    ptx::tcgen05_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        ptx::tcgen05_fence_after_sync();
+        ptx::tmem_dealloc<BN < 32 ? 32 : BN>(tmem);
+    }
+}
+
+// ---- persistent CTA pairs ----------------------------------------------------------------------------------------------
+
+constexpr int kPairThreads = 384;                    // warp 0: TMA, warp 1: products (even CTA), warps 4-11: epilogue
+constexpr uint32_t kPairDepth = 6, kPairStage = 2 * kSlotA, kPairBN = 256, kPairEpiWarps = 8;
+constexpr uint32_t kPairSmem = 1024 + kPairDepth * kPairStage + (2 * kPairDepth + 4) * 8 + 16;
+
+template <typename T>
+__global__ void __launch_bounds__(kPairThreads, 1)
+product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Product p, const Epilogue e)
+{
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (smem - ptx::smem_u32(smem_raw));
+    uint64_t* full = reinterpret_cast<uint64_t*>(gen + kPairDepth * kPairStage);       // even CTA: both CTAs' operands have landed
+    uint64_t* drained = full + kPairDepth;           // each CTA: the products that read a ring position are done
+    uint64_t* tmem_full = drained + kPairDepth;      // each CTA, per accumulator: complete
+    uint64_t* tmem_empty = tmem_full + 2;            // even CTA, per accumulator: read by the epilogue warps of both
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
+    volatile uint32_t* abort_flag = tmem_slot + 1;
+
+    const uint32_t warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const uint32_t rank = ptx::cluster_cta_rank(), pair_id = ptx::cluster_id_x(), num_pairs = ptx::num_clusters_x();
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < kPairDepth; ++i) { ptx::mbar_init(full + i, 1); ptx::mbar_init(drained + i, 1); }
+        for (uint32_t i = 0; i < 2; ++i) { ptx::mbar_init(tmem_full + i, 1); ptx::mbar_init(tmem_empty + i, 2 * kPairEpiWarps); }
+        *abort_flag = 0;
+        ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&tm_a);
+        ptx::prefetch_tensormap(&tm_b);
+    }
+    if (warp == 1) ptx::tmem_alloc_pair<512>(tmem_slot);
+    ptx::tcgen05_fence_before_sync();
+    ptx::cluster_sync();
+    ptx::tcgen05_fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    ptx::grid_dependency_wait();
+
+    const uint32_t tiles = p.tiles_a * p.tiles_b;
+    bool ok = true;
+    auto give_up = [&] {
+        *abort_flag = 1;
+        if (p.status != nullptr) atomicOr(p.status, 1);
+        ok = false;
+    };
+    if (warp == 0) {
+        const uint32_t issue = ptx::elect_one();
+        const uint32_t full_even = ptx::map_to_cta(ptx::smem_u32(full), 0);
+        Ring r;
+        for (uint32_t tile = pair_id; ok && tile < tiles; tile += num_pairs) {
+            uint32_t a_blk, b_blk;
+            gemm::tile_coords(tile, p.tiles_a, p.tiles_b, 8, a_blk, b_blk);
+            const uint32_t a0 = (a_blk * 2 + rank) * BM, b0 = b_blk * kPairBN + rank * (kPairBN / 2);
+            for (uint32_t kb = 0; kb < p.k_blocks; ++kb) {
+                if (!ptx::all_lanes(ptx::mbar_wait_impl(drained + r.slot, r.phase ^ 1, abort_flag))) { give_up(); break; }
+                // the even CTA announces the bytes of both; the odd CTA's complete on its barrier
+                if (rank == 0) ptx::mbar_arrive_expect_tx(full + r.slot, 2 * kPairStage, issue);
+                uint8_t* to = gen + r.slot * kPairStage;
+                const uint32_t bar = full_even + r.slot * 8;
+                load_tile<BM>(to, p.a_mn, a0, kb, [&](uint8_t* dst, uint32_t c0, uint32_t c1) { ptx::tma_load_2d_pair(dst, &tm_a, bar, c0, c1, issue); });
+                load_tile<BM>(to + kSlotA, p.b_mn, b0, kb, [&](uint8_t* dst, uint32_t c0, uint32_t c1) { ptx::tma_load_2d_pair(dst, &tm_b, bar, c0, c1, issue); });
+                r.advance<kPairDepth>();
+            }
+        }
+        ptx::grid_launch_dependents();
+        if (ok && !gemm::drain_ring<kPairDepth>(r, [&](uint32_t i, uint32_t parity) {
+                return ptx::all_lanes(ptx::mbar_wait_impl(drained + i, parity, abort_flag)); })) give_up();
+    } else if (warp == 1) {
+        if (rank == 0) {
+            const uint32_t issue = ptx::elect_one();
+            const uint32_t idesc = ptx::make_idesc_f16(2 * BM, kPairBN, std::is_same<T, __nv_bfloat16>::value, p.a_mn, p.b_mn);
+            constexpr uint16_t kBoth = 3;
+            Ring r;
+            uint32_t n = 0;
+            for (uint32_t tile = pair_id; ok && tile < tiles; tile += num_pairs, ++n) {
+                const uint32_t acc = n & 1;
+                if (!ptx::all_lanes(ptx::mbar_wait_impl(tmem_empty + acc, ((n >> 1) & 1) ^ 1, abort_flag))) { give_up(); break; }
+                ptx::tcgen05_fence_after_sync();
+                for (uint32_t kb = 0; kb < p.k_blocks; ++kb) {
+                    if (!ptx::all_lanes(ptx::mbar_wait_impl(full + r.slot, r.phase, abort_flag))) { give_up(); break; }
+                    ptx::tcgen05_fence_after_sync();
+                    const uint32_t at = smem + r.slot * kPairStage;
+#pragma unroll
+                    for (uint32_t s = 0; s < BK / 16; ++s)
+                        ptx::tcgen05_mma_f16_pair(tmem + acc * kPairBN, operand_desc(at, p.a_mn, s), operand_desc(at + kSlotA, p.b_mn, s), idesc, kb | s, issue);
+                    ptx::tcgen05_commit_pair(drained + r.slot, kBoth, issue);
+                    r.advance<kPairDepth>();
+                }
+                if (ok) ptx::tcgen05_commit_pair(tmem_full + acc, kBoth, issue);
+            }
+        }
+    } else if (warp >= 4) {
+        const uint32_t quad = warp & 3, half = (warp - 4) >> 2;               // its lanes; columns [128 half, 128 half + 128) of the tile
+        const uint32_t tmem_empty_even = ptx::map_to_cta(ptx::smem_u32(tmem_empty), 0);
+        uint32_t n = 0;
+        for (uint32_t tile = pair_id; ok && tile < tiles; tile += num_pairs, ++n) {
+            const uint32_t acc = n & 1;
+            uint32_t a_blk, b_blk;
+            gemm::tile_coords(tile, p.tiles_a, p.tiles_b, 8, a_blk, b_blk);
+            const uint32_t row0 = (a_blk * 2 + rank) * BM + quad * 32, col0 = b_blk * kPairBN + half * 128;
+            if (!ptx::all_lanes(ptx::mbar_wait_relaxed(tmem_full + acc, (n >> 1) & 1, abort_flag, 50))) { give_up(); break; }
+            ptx::tcgen05_fence_after_sync();
+            const uint32_t taddr = tmem + ((quad * 32) << 16) + acc * kPairBN + half * 128;
+#pragma unroll 1
+            for (uint32_t c = 0; c < 128; c += 32) {
+                float v[32];
+                load_accumulators(taddr + c, v);
+                if (c == 96) {                                               // everything of this warp's is in registers
+                    ptx::tcgen05_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive_remote(tmem_empty_even + acc * 8);
+                }
+                if (row0 < e.rows && col0 + c < e.cols) {
+                    transpose(v, lane);
+                    finish<T>(v, row0, 32, col0 + c + lane, e);
+                }
+            }
+        }
+    }
+    // neither CTA leaves, or gives up its tensor memory, while the other can still signal it or read its operands
+    ptx::tcgen05_fence_before_sync();
+    ptx::cluster_sync();
+    if (warp == 1) {
+        ptx::tcgen05_fence_after_sync();
+        ptx::tmem_dealloc_pair<512>(tmem);
+    }
+}
+
+// ---- host: which kernel, which tiles -----------------------------------------------------------------------------------
+
+template <typename T>
+constexpr CUtensorMapDataType kMapType = std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+
+// Map of an operand with `rows` rows over a contraction of `k`; box: `tile` rows x 64, or 64 x 64 where memory runs along the rows.
+template <typename T>
+int operand_map(CUtensorMap* map, const void* base, int64_t ld, bool mn_major, uint64_t rows, uint64_t k, uint32_t tile)
+{
+    return host::encode_tensor_map_2d(map, kMapType<T>, 2, base, mn_major ? rows : k, mn_major ? k : rows, static_cast<uint64_t>(ld) * 2, BK,
+                                      mn_major ? 64 : tile, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+struct Operands {
+    const void* a; int64_t lda; bool a_mn; uint32_t rows_a;
+    const void* b; int64_t ldb; bool b_mn; uint32_t rows_b;
+    uint32_t k;
+    int32_t* status;
+};
+
+template <typename T, uint32_t BN, bool kSwap>
+int launch_tiles(const Operands& o, const Epilogue& e, uint32_t splits_log2, int num_sms, cudaStream_t stream)
+{
+    CUtensorMap tm_a, tm_b;
+    if (int rc = operand_map<T>(&tm_a, o.a, o.lda, o.a_mn, o.rows_a, o.k, BM)) return rc;
+    if (int rc = operand_map<T>(&tm_b, o.b, o.ldb, o.b_mn, o.rows_b, o.k, BN)) return rc;
+    Product p{};
+    p.tiles_a = (o.rows_a + BM - 1) / BM;
+    p.tiles_b = (o.rows_b + BN - 1) / BN;
+    p.k_blocks = (o.k + BK - 1) / BK;
+    p.splits_log2 = splits_log2;
+    p.a_mn = o.a_mn;
+    p.b_mn = o.b_mn;
+    p.status = o.status;
+    const uint64_t ctas = static_cast<uint64_t>(p.tiles_a) * p.tiles_b << splits_log2;
+    // one CTA to an SM: its ring may fill the shared memory; more: two share it
+    const uint32_t budget = ctas <= static_cast<uint64_t>(num_sms) ? 200 * 1024 : 112 * 1024;
+    p.depth = kMaxDepth;
+    while (p.depth > 2 && tile_smem(BN, p.depth, splits_log2 != 0) > budget) --p.depth;
+    int dev = 0;
+    NVFP4_CUDA_CHECK(cudaGetDevice(&dev));
+    static bool attr_set[host::kMaxDevices] = {};
+    if (!attr_set[dev]) {
+        NVFP4_CUDA_CHECK(cudaFuncSetAttribute(product_kernel<T, BN, kSwap>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+        attr_set[dev] = true;
+    }
+    NVFP4_REQUIRE(ctas <= INT32_MAX, "too many tiles (%llu)", static_cast<unsigned long long>(ctas));
+    return host::launch_kernel_cluster(product_kernel<T, BN, kSwap>, dim3(static_cast<unsigned>(ctas)), dim3(kTileThreads),
+                                       tile_smem(BN, p.depth, splits_log2 != 0), stream, true, 1u << splits_log2, tm_a, tm_b, p, e);
+}
+
+template <typename T>
+int launch_pairs(const Operands& o, const Epilogue& e, int num_sms, cudaStream_t stream)
+{
+    CUtensorMap tm_a, tm_b;
+    if (int rc = operand_map<T>(&tm_a, o.a, o.lda, o.a_mn, o.rows_a, o.k, BM)) return rc;
+    if (int rc = operand_map<T>(&tm_b, o.b, o.ldb, o.b_mn, o.rows_b, o.k, BM)) return rc;
+    Product p{};
+    p.tiles_a = (o.rows_a + 2 * BM - 1) / (2 * BM);
+    p.tiles_b = (o.rows_b + kPairBN - 1) / kPairBN;
+    p.k_blocks = (o.k + BK - 1) / BK;
+    p.a_mn = o.a_mn;
+    p.b_mn = o.b_mn;
+    p.status = o.status;
+    int dev = 0;
+    NVFP4_CUDA_CHECK(cudaGetDevice(&dev));
+    static bool attr_set[host::kMaxDevices] = {};
+    if (!attr_set[dev]) {
+        NVFP4_CUDA_CHECK(cudaFuncSetAttribute(product_pair_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+        attr_set[dev] = true;
+    }
+    const uint64_t tiles = static_cast<uint64_t>(p.tiles_a) * p.tiles_b, pairs = static_cast<uint64_t>(num_sms / 2);
+    NVFP4_REQUIRE(tiles <= INT32_MAX, "too many tiles (%llu)", static_cast<unsigned long long>(tiles));
+    return host::launch_kernel_cluster(product_pair_kernel<T>, dim3(static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs))), dim3(kPairThreads),
+                                       kPairSmem, stream, true, 2u, tm_a, tm_b, p, e);
+}
+
+// D of (rows_a, rows_b) = (e.rows, e.cols).
+template <typename T>
+int launch_product(const Operands& o, const Epilogue& e, int num_sms, cudaStream_t stream)
+{
+    const uint32_t k_blocks = (o.k + BK - 1) / BK;
+    auto splits_for = [&](uint64_t tiles, uint32_t most_log2) {
+        uint32_t s = 0;
+        while (s < most_log2 && (tiles << (s + 1)) <= static_cast<uint64_t>(num_sms) && k_blocks >> (s + 1) >= 4) ++s;
+        return s;
+    };
+    // a few rows: the weight's rows on the tensor memory's lanes, as many tokens to a tile as there are
+    if (o.rows_a <= 128 && !o.a_mn && !o.b_mn) {
+        const Operands s{o.b, o.ldb, false, o.rows_b, o.a, o.lda, false, o.rows_a, o.k, o.status};
+        const uint32_t splits = splits_for((o.rows_b + BM - 1) / BM, 3);
+        if (o.rows_a <= 16) return launch_tiles<T, 16, true>(s, e, splits, num_sms, stream);
+        if (o.rows_a <= 32) return launch_tiles<T, 32, true>(s, e, splits, num_sms, stream);
+        if (o.rows_a <= 64) return launch_tiles<T, 64, true>(s, e, splits, num_sms, stream);
+        return launch_tiles<T, 128, true>(s, e, splits, num_sms, stream);
+    }
+    const uint64_t pair_tiles = static_cast<uint64_t>((o.rows_a + 255) / 256) * ((o.rows_b + 255) / 256);
+    if (pair_tiles * 2 >= static_cast<uint64_t>(num_sms / 2) && o.rows_b > 128) return launch_pairs<T>(o, e, num_sms, stream);
+    const uint64_t tiles_128 = static_cast<uint64_t>((o.rows_a + 127) / 128) * ((o.rows_b + 127) / 128);
+    if (o.rows_b <= 64) return launch_tiles<T, 64, false>(o, e, splits_for((o.rows_a + 127) / 128, 1), num_sms, stream);
+    return launch_tiles<T, 128, false>(o, e, splits_for(tiles_128, 2), num_sms, stream);
+}
+
+// ---- dz and the bias' gradient -----------------------------------------------------------------------------------------
+
+// dz = dd * activation'(z), rounded once for the tensor cores, and per block of rows the sums of its columns before that rounding.
+// A thread takes eight columns (16 bytes of z and dz, whose rows are padded to that) of every eighth row of its block's; a block 256
+// columns.  One pass over dd and z, bound by their bytes.
+constexpr int kGradThreads = 256, kGradColumns = 256, kGradRowLanes = 8;
+template <typename T, typename D>
+__global__ void __launch_bounds__(kGradThreads)
+linear_dz_kernel(const D* __restrict__ dd, int64_t ldd, bool wide, const T* __restrict__ z, int64_t ldz, T* __restrict__ dz, int64_t lddz, uint32_t rows,
+                 uint32_t cols, uint32_t rows_each, int activation, float* __restrict__ sums)
+{
+    __shared__ float part[kGradRowLanes][kGradColumns];
+    const uint32_t group = threadIdx.x % 32, row_lane = threadIdx.x / 32;
+    const uint32_t col0 = blockIdx.x * kGradColumns + group * 8;
+    const uint32_t first = blockIdx.y * rows_each, last = min(rows, first + rows_each);
+    ptx::grid_dependency_wait();
+    float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    with_activation(activation, [&](auto act) {
+        if (col0 >= cols) return;
+        const uint32_t here = min(8u, cols - col0);
+        for (uint32_t r = first + row_lane; r < last; r += kGradRowLanes) {
+            const D* from = dd + static_cast<int64_t>(r) * ldd + col0;
+            alignas(16) D g[8];
+            if (wide) {
+#pragma unroll
+                for (uint32_t i = 0; i < sizeof(g) / 16; ++i) reinterpret_cast<uint4*>(g)[i] = __ldg(reinterpret_cast<const uint4*>(from) + i);
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) g[i] = i < here ? from[i] : from_float<D>(0.0f);
+            }
+            alignas(16) T pre[8];
+            if constexpr (decltype(act)::value != NVFP4_ACTIVATION_NONE)
+                *reinterpret_cast<uint4*>(pre) = __ldg(reinterpret_cast<const uint4*>(z + static_cast<int64_t>(r) * ldz + col0));
+            alignas(16) T out[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                float v = to_float(g[i]);
+                if constexpr (decltype(act)::value != NVFP4_ACTIVATION_NONE) v *= slope<decltype(act)::value>(to_float(pre[i]));
+                sum[i] += v;
+                out[i] = from_float<T>(v);
+            }
+            if (dz != nullptr) *reinterpret_cast<uint4*>(dz + static_cast<int64_t>(r) * lddz + col0) = *reinterpret_cast<const uint4*>(out);
+        }
+    });
+    if (sums == nullptr) return;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) part[row_lane][group * 8 + i] = sum[i];
+    __syncthreads();
+    const uint32_t col = blockIdx.x * kGradColumns + threadIdx.x;
+    if (col >= cols) return;
+    float total = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < kGradRowLanes; ++i) total += part[i][threadIdx.x];
+    sums[static_cast<int64_t>(blockIdx.y) * cols + col] = total;
+}
+template <typename T>
+__global__ void __launch_bounds__(kGradThreads)
+linear_db_kernel(const float* __restrict__ sums, uint32_t blocks, uint32_t cols, T* __restrict__ db)
+{
+    const uint32_t col = blockIdx.x * kGradThreads + threadIdx.x;
+    ptx::grid_dependency_wait();
+    if (col >= cols) return;
+    float total = 0.0f;
+    for (uint32_t b = 0; b < blocks; ++b) total += sums[static_cast<int64_t>(b) * cols + col];
+    db[col] = from_float<T>(total);
+}
+
+template <typename T, typename D>
+int launch_dz(const void* dd, int64_t ldd, const void* z, int64_t ldz, void* dz, int64_t lddz, void* db, uint32_t rows, uint32_t cols, int activation,
+              int num_sms, cudaStream_t stream)
+{
+    const unsigned columns = (cols + kGradColumns - 1) / kGradColumns;
+    // about four blocks to an SM, at least eight rows to a block
+    uint32_t blocks = (static_cast<uint32_t>(num_sms) * 4 + columns - 1) / columns;
+    uint32_t rows_each = (rows + blocks - 1) / blocks;
+    rows_each = (rows_each + kGradRowLanes - 1) / kGradRowLanes * kGradRowLanes;
+    blocks = (rows + rows_each - 1) / rows_each;
+    const bool wide = ((reinterpret_cast<uintptr_t>(dd) | static_cast<uintptr_t>(ldd * sizeof(D))) & 15u) == 0 && cols % 8 == 0;
+    float* sums = nullptr;
+    if (db != nullptr) {
+        int dev = 0;
+        NVFP4_CUDA_CHECK(cudaGetDevice(&dev));
+        cudaMemPool_t pool;
+        if (int rc = host::workspace_pool(dev, &pool)) return rc;
+        NVFP4_CUDA_CHECK(cudaMallocFromPoolAsync(reinterpret_cast<void**>(&sums), static_cast<size_t>(blocks) * cols * sizeof(float), pool, stream));
+    }
+    int rc = host::launch_kernel(linear_dz_kernel<T, D>, dim3(columns, blocks), dim3(kGradThreads), 0, stream, true, static_cast<const D*>(dd), ldd, wide,
+                                 static_cast<const T*>(z), ldz, static_cast<T*>(dz), lddz, rows, cols, rows_each, activation, sums);
+    if (db != nullptr) {
+        if (rc == NVFP4_OK)
+            rc = host::launch_kernel(linear_db_kernel<T>, dim3((cols + kGradThreads - 1) / kGradThreads), dim3(kGradThreads), 0, stream, true, sums,
+                                     blocks, cols, static_cast<T*>(db));
+        cudaFreeAsync(sums, stream);
+    }
+    return rc;
+}
+
+}  // namespace
+
+int launch_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual, int64_t ldr, void* d, int64_t ldd,
+                  void* z, int64_t ldz, int M, int N, int K, bool bf16, bool out32, int activation, int32_t* status, int num_sms, cudaStream_t stream)
+{
+    const Operands o{x, ldx, false, static_cast<uint32_t>(M), w, ldw, false, static_cast<uint32_t>(N), static_cast<uint32_t>(K), status};
+    const Epilogue e{d, ldd, z, ldz, bias, residual, ldr, static_cast<uint32_t>(M), static_cast<uint32_t>(N), activation, out32};
+    return bf16 ? launch_product<__nv_bfloat16>(o, e, num_sms, stream) : launch_product<__half>(o, e, num_sms, stream);
+}
+
+int launch_linear_dz(const void* dd, int64_t ldd, bool dd32, const void* z, int64_t ldz, void* dz, int64_t lddz, void* db, int M, int N, bool bf16,
+                     int activation, int num_sms, cudaStream_t stream)
+{
+    const uint32_t m = static_cast<uint32_t>(M), n = static_cast<uint32_t>(N);
+    if (bf16)
+        return dd32 ? launch_dz<__nv_bfloat16, float>(dd, ldd, z, ldz, dz, lddz, db, m, n, activation, num_sms, stream)
+                    : launch_dz<__nv_bfloat16, __nv_bfloat16>(dd, ldd, z, ldz, dz, lddz, db, m, n, activation, num_sms, stream);
+    return dd32 ? launch_dz<__half, float>(dd, ldd, z, ldz, dz, lddz, db, m, n, activation, num_sms, stream)
+                : launch_dz<__half, __half>(dd, ldd, z, ldz, dz, lddz, db, m, n, activation, num_sms, stream);
+}
+
+int launch_linear_dx(const void* dz, int64_t lddz, const void* w, int64_t ldw, void* dx, int64_t lddx, int M, int N, int K, bool bf16, int32_t* status,
+                     int num_sms, cudaStream_t stream)
+{
+    const Operands o{dz, lddz, false, static_cast<uint32_t>(M), w, ldw, true, static_cast<uint32_t>(K), static_cast<uint32_t>(N), status};
+    const Epilogue e{dx, lddx, nullptr, 0, nullptr, nullptr, 0, static_cast<uint32_t>(M), static_cast<uint32_t>(K), NVFP4_ACTIVATION_NONE, false};
+    return bf16 ? launch_product<__nv_bfloat16>(o, e, num_sms, stream) : launch_product<__half>(o, e, num_sms, stream);
+}
+
+int launch_linear_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, void* dw, int64_t lddw, int M, int N, int K, bool bf16, int32_t* status,
+                     int num_sms, cudaStream_t stream)
+{
+    const Operands o{dz, lddz, true, static_cast<uint32_t>(N), x, ldx, true, static_cast<uint32_t>(K), static_cast<uint32_t>(M), status};
+    const Epilogue e{dw, lddw, nullptr, 0, nullptr, nullptr, 0, static_cast<uint32_t>(N), static_cast<uint32_t>(K), NVFP4_ACTIVATION_NONE, false};
+    return bf16 ? launch_product<__nv_bfloat16>(o, e, num_sms, stream) : launch_product<__half>(o, e, num_sms, stream);
+}
+
+}  // namespace nvfp4

@@ -270,6 +270,33 @@ NVFP4_DEVICE uint64_t make_smem_desc(uint32_t smem_addr, uint32_t stride_bytes, 
            (1ull << 46) | (swizzle << 61);
 }
 
+// D[tmem] (+)= A[smem] * B[smem], BF16 or FP16 operands, K = 16 per instruction, FP32 accumulators.
+NVFP4_DEVICE void tcgen05_mma_f16(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate, uint32_t issue = 1)
+{
+    asm volatile(
+        "{\n"
+        " .reg .pred p, q;\n"
+        " setp.ne.b32 p, %4, 0;\n"
+        " setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(tmem_d),
+        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(issue)
+        : "memory");
+}
+// Instruction descriptor of kind::f16 with FP32 accumulators; both operands have one type.
+//   [4,6) D format (1 = FP32)  [7,10) A format (0 = FP16, 1 = BF16)  [10,13) B format  [15] A major (1 = MN)  [16] B major
+//   [17,23) N >> 3  [24,29) M >> 4
+NVFP4_DEVICE constexpr uint32_t make_idesc_f16(uint32_t m, uint32_t n, bool bf16, bool a_mn, bool b_mn)
+{
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+// The matrix descriptor of an operand whose 128-byte rows run along M or N (MN-major, 128-byte swizzle): 8 rows of K are
+// stride_bytes from the next 8, 64 elements of M or N leading_bytes from the next 64.
+NVFP4_DEVICE uint64_t make_smem_desc_mn(uint32_t smem_addr, uint32_t leading_bytes, uint32_t stride_bytes)
+{
+    return make_smem_desc(smem_addr, stride_bytes, kSwizzle128B) | (static_cast<uint64_t>(leading_bytes >> 4) << 16);
+}
+
 // 32 lanes x 32 columns of 32-bit: thread i of the warp gets row (lane base + i), columns [c, c + 32).
 NVFP4_DEVICE void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)[32])
 {
@@ -438,6 +465,11 @@ NVFP4_DEVICE uint32_t map_to_cta(uint32_t smem_addr, uint32_t rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
     return r;
 }
+// One word into shared memory of a CTA of the cluster (address from map_to_cta).
+NVFP4_DEVICE void st_cluster_f32(uint32_t cluster_addr, float v)
+{
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+}
 NVFP4_DEVICE void cluster_sync()
 {
     __syncwarp();                                    // one lane may come from a role of its own
@@ -563,6 +595,19 @@ NVFP4_DEVICE void tcgen05_mma_nvf4_pair(uint32_t tmem_d, uint64_t desc_a, uint64
         " @q tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.block16 [%0], %1, %2, %3, [%4], [%5], p;\n"
         "}\n" ::"r"(tmem_d),
         "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sfa), "r"(tmem_sfb), "r"(accumulate), "r"(issue)
+        : "memory");
+}
+// tcgen05_mma_f16 over a CTA pair, operands and accumulators split between the two as above.
+NVFP4_DEVICE void tcgen05_mma_f16_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate, uint32_t issue = 1)
+{
+    asm volatile(
+        "{\n"
+        " .reg .pred p, q;\n"
+        " setp.ne.b32 p, %4, 0;\n"
+        " setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(tmem_d),
+        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(issue)
         : "memory");
 }
 // All earlier pair MMAs of this thread arrive, when they retire, on the barrier at this offset in the CTAs of

@@ -1,0 +1,52 @@
+"""Dense products around the expert layer: activation(x w^T + bias) + residual in one kernel, with gradients.
+
+The router's projection (FP32 logits out of BF16 rows), shared experts and the projections of an attention block: what a model keeps in
+BF16 or FP16 beside the quantised experts.  Operands are read where they lie, whichever way a product needs them; sums are FP32.  CUDA
+kernels of the library throughout; CPU tensors are refused.  The reference project has the grouped quantised product alone.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _C
+from .tokens import _differentiable
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, residual, activation, out_dtype, device_status):
+        want_x, want_w, want_bias, _ = ctx.needs_input_grad[:4]
+        keep = activation != "none" and (want_x or want_w or want_bias)
+        d, z = _C.linear(x, w, bias, residual, activation, out_dtype, keep, device_status)
+        ctx.save_for_backward(x if want_w else None, w if want_x else None, z)
+        ctx.form = (x.dtype, activation)
+        ctx.device_status = device_status
+        return d
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dd):
+        want_x, want_w, want_bias, want_residual = ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        if want_x or want_w or want_bias:
+            rows = dd if dd.stride(-1) == 1 and dd.stride(0) >= dd.shape[1] else dd.contiguous()
+            dx, dw, db = _C.linear_backward(rows, *ctx.saved_tensors, *ctx.form, want_x, want_w, want_bias, ctx.device_status)
+        return dx, dw, db, dd if want_residual else None, None, None, None
+
+
+def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, *,
+           activation: str = "none", out_dtype: Optional[torch.dtype] = None, device_status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """activation(x w^T + bias) + residual, (M, N).
+
+    ``x`` (M, K) and ``w`` (N, K) BF16 or FP16, of one type, contiguous along K, starting on 16 bytes and with row strides that are multiples
+    of 8 elements; K a multiple of 8, M and N any.  ``bias`` (N,) of that type.  ``residual`` (M, N) and the result have
+    ``out_dtype``: the operands' type, or float32.  ``activation``: none, relu, gelu, gelu_tanh or silu.  Sums, bias, activation and residual
+    are FP32, rounded once.  ``device_status``: int32 on the device that receives bit 0 should a bounded wait in the kernels expire.
+
+    Differentiable in x, w, bias and residual.  The backward pass keeps x w^T + bias rounded to the operands' type, and rounds the
+    gradient in front of the activation to it: the tensor cores take no wider operands."""
+    if not _differentiable(x, w, bias, residual):
+        return _C.linear(x, w, bias, residual, activation, out_dtype, device_status=device_status)[0]
+    return _Linear.apply(x, w, bias, residual, activation, out_dtype, device_status)

@@ -1,0 +1,340 @@
+"""Dense products with bias, activation and residual, and their gradients: against 64-bit formulas and differences, refusals, streams, graphs."""
+import math
+
+import pytest
+import torch
+
+from nvfp4_gemm import _C, linear, route_tokens, sort_tokens, unsort_tokens
+
+gpu = pytest.mark.gpu
+HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+ACTIVATIONS = ["none", "relu", "gelu", "gelu_tanh", "silu"]
+# Largest |slope| and |curvature| of the activations (those of gelu are 1.13 and 0.80, of silu 1.10 and 0.50)
+SLOPE, CURVATURE = 1.2, 0.9
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def act64(z, name):
+    if name == "relu":
+        return torch.where(z > 0, z, torch.zeros_like(z))
+    if name == "gelu":
+        return 0.5 * z * torch.special.erfc(-z * math.sqrt(0.5))
+    if name == "gelu_tanh":
+        return z * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))
+    return z * torch.sigmoid(z) if name == "silu" else z
+
+
+def sum_error(a, b):
+    """Bound on an FP32 sum of products: K roundings (2^-23 each: the tensor core may cut instead of rounding) of partial sums no
+    larger than the sum of magnitudes."""
+    return (a.double().abs() @ b.double().abs()) * (a.shape[1] + 4) * 2.0 ** -23
+
+
+def make(m, n, k, dtype, seed, out=None):
+    g = gen(seed)
+    x = torch.randn(m, k, generator=g).to(dtype)
+    w = (torch.randn(n, k, generator=g) * k ** -0.5).to(dtype)
+    return x, w, torch.randn(n, generator=g).to(dtype), torch.randn(m, n, generator=g).to(out or dtype)
+
+
+def check_forward(got, x, w, bias, residual, activation, out):
+    z = x.double() @ w.double().t()
+    if bias is not None:
+        z = z + bias.double()
+    want = act64(z, activation)
+    # activation: its argument's error times the slope, and a few steps of its own (exp, a division, products: 8 roundings)
+    error = SLOPE * (sum_error(x, w.t()) + z.abs() * 2.0 ** -23) + want.abs() * 8 * 2.0 ** -23
+    if residual is not None:
+        want = want + residual.double()
+        error = error + want.abs() * 2.0 ** -23
+    floor = 2.0 ** -25 if out == torch.float16 else 1e-40
+    assert got.dtype == out and got.shape == want.shape
+    worst = ((got.cpu().double() - want).abs() - (error + (want.abs() + error) * 1.01 * HALF_STEP[out] + floor)).max()
+    assert worst <= 0, float(worst)
+
+
+# ---- refusals --------------------------------------------------------------------------------------------------------
+
+
+def error_of(rc):
+    assert rc == 1
+    return _C.lib().nvfp4_last_error().decode()
+
+
+def call(x=1024, ldx=64, w=1024, ldw=64, bias=None, residual=None, ldr=0, d=1024, ldd=32, z=None, ldz=0, m=4, n=32, k=64, dtype=0, out=0, act=0):
+    return _C.lib().nvfp4_linear(x, ldx, w, ldw, bias, residual, ldr, d, ldd, z, ldz, m, n, k, dtype, out, act, None, None)
+
+
+@pytest.mark.parametrize("change, text", [
+    (dict(x=None), "null"), (dict(w=None), "null"), (dict(d=None), "null output"), (dict(x=1032), "16-byte"), (dict(w=1026), "16-byte"),
+    (dict(ldx=68), "multiple of 8"), (dict(ldx=56), "cover the row"), (dict(ldw=60), "multiple of 8"), (dict(k=60), "K must be"), (dict(k=0), "K must be"),
+    (dict(m=-1), "negative"), (dict(dtype=1), "BF16 or FP16"), (dict(dtype=3), "BF16 or FP16"), (dict(out=2), "operands' type"), (dict(act=5), "activation"),
+    (dict(act=-1), "activation"), (dict(ldd=31), "smaller than the row"), (dict(residual=1024, ldr=8), "smaller than the row"), (dict(d=1025), "aligned"),
+    (dict(bias=1025), "aligned"), (dict(out=1, d=1026), "aligned"), (dict(z=1024, ldz=31), "smaller than the row")])
+def test_products_refuse(change, text):
+    assert text in error_of(call(**change))
+
+
+def test_gradients_refuse():
+    lib = _C.lib()
+    assert "K must be" in error_of(lib.nvfp4_linear_dx(1024, 32, 1024, 64, 1024, 64, 4, 32, 60, 0, None, None))
+    assert "dz must" in error_of(lib.nvfp4_linear_dx(1026, 32, 1024, 64, 1024, 64, 4, 32, 64, 0, None, None))
+    assert "empty contraction" in error_of(lib.nvfp4_linear_dx(1024, 32, 1024, 64, 1024, 64, 4, 0, 64, 0, None, None))
+    assert "empty contraction" in error_of(lib.nvfp4_linear_dw(1024, 32, 1024, 64, 1024, 64, 0, 32, 64, 0, None, None))
+    assert "rows overlap" in error_of(lib.nvfp4_linear_dw(1024, 32, 1024, 64, 1024, 56, 4, 32, 64, 0, None, None))
+    assert "z" in error_of(lib.nvfp4_linear_dz(1024, 32, None, 32, 1024, 32, None, 4, 32, 0, 0, 4, None))
+    assert "stride of dz" in error_of(lib.nvfp4_linear_dz(1024, 33, 1024, 40, 1024, 32, None, 4, 33, 0, 0, 4, None))
+    assert "operands' type" in error_of(lib.nvfp4_linear_dz(1024, 32, 1024, 32, 1024, 32, None, 4, 32, 0, 2, 4, None))
+    assert lib.nvfp4_linear_dz(1024, 32, 1024, 32, None, 32, None, 4, 32, 0, 0, 4, None) == 0
+
+
+def test_empty_products_are_nothing():
+    assert call(m=0, x=None) == 0 and call(n=0, d=None) == 0
+
+
+def test_host_tensors_are_refused():
+    with pytest.raises(RuntimeError, match="x is a 2-D"):
+        linear(torch.zeros(2, 8), torch.zeros(2, 8))
+
+
+# ---- forward ---------------------------------------------------------------------------------------------------------
+
+# tokens to the tiles of the few-row form (16, 32, 64, 128), contractions that split over clusters or not, narrow, odd and wide outputs,
+# left-over pieces of every tile, enough tiles for the pairs
+SIZES = [(1, 1, 8), (1, 4096, 4096), (3, 25, 3768), (16, 128, 64), (17, 513, 2048), (33, 1411, 2048), (64, 96, 520), (65, 31, 72), (128, 1000, 1024),
+         (129, 64, 200), (300, 33, 1032), (257, 129, 8), (500, 256, 4096), (1000, 65, 136), (2049, 128, 4096), (777, 3001, 264), (4099, 2050, 72), (2500, 4104, 392)]
+
+
+@gpu
+@pytest.mark.parametrize("m, n, k", SIZES)
+def test_products_against_64_bits(m, n, k):
+    for i, dtype in enumerate((torch.bfloat16, torch.float16)):
+        x, w, bias, residual = make(m, n, k, dtype, m + n + k)
+        act = ACTIVATIONS[(m + i) % 5]
+        check_forward(linear(x.cuda(), w.cuda()), x, w, None, None, "none", dtype)
+        check_forward(linear(x.cuda(), w.cuda(), bias.cuda(), residual.cuda(), activation=act), x, w, bias, residual, act, dtype)
+        check_forward(linear(x.cuda(), w.cuda(), bias.cuda(), out_dtype=torch.float32, activation=act), x, w, bias, None, act, torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("m, n, k", [(5, 200, 512), (200, 200, 64), (3000, 1536, 128)])
+def test_every_activation(m, n, k, activation):
+    for dtype in (torch.bfloat16, torch.float16):
+        x, w, bias, residual = make(m, n, k, dtype, 7, torch.float32)
+        w = w * 3                                                          # far into both tails
+        check_forward(linear(x.cuda(), w.cuda(), bias.cuda(), residual.cuda(), activation=activation, out_dtype=torch.float32), x, w, bias, residual,
+                      activation, torch.float32)
+        check_forward(linear(x.cuda(), w.cuda(), None, residual.to(dtype).cuda(), activation=activation), x, w, None, residual.to(dtype), activation, dtype)
+
+
+@gpu
+def test_strided_operands_and_residuals():
+    for m, n, k in ((9, 77, 128), (300, 77, 128), (2600, 2056, 64)):
+        for dtype in (torch.bfloat16, torch.float16):
+            x, w, bias, residual = make(m, n, k, dtype, 3)
+            wide_x = torch.full((m, k + 24), float("nan"), dtype=dtype, device="cuda")
+            wide_w = torch.full((2 * n, k), float("nan"), dtype=dtype, device="cuda")
+            wide_r = torch.full((m, n + 5), float("nan"), dtype=dtype, device="cuda")
+            vx, vw, vr = wide_x[:, 8:8 + k], wide_w[::2], wide_r[:, 3:3 + n]
+            vx.copy_(x), vw.copy_(w), vr.copy_(residual)
+            vb = torch.full((n + 1,), float("nan"), dtype=dtype, device="cuda")[1:]
+            vb.copy_(bias)
+            check_forward(linear(vx, vw, vb, vr, activation="silu"), x, w, bias, residual, "silu", dtype)
+            for bad in (wide_x[:, 1:1 + k], wide_x[:, :k].t()[:k, :m] if m >= k else wide_x[:, 4:4 + k]):
+                with pytest.raises(RuntimeError):
+                    linear(bad, vw)
+
+
+@gpu
+def test_infinities_and_nan_stay_in_their_rows():
+    for m in (40, 400, 2600):
+        x, w, bias, residual = make(m, 2056, 64, torch.bfloat16, 5)
+        x[3, 0], x[7, 1], x[m - 1, 5] = float("inf"), float("nan"), -float("inf")
+        got = linear(x.cuda(), w.cuda(), bias.cuda(), residual.cuda(), activation="relu").cpu()
+        clean = torch.ones(m, dtype=torch.bool)
+        clean[[3, 7, m - 1]] = False
+        check_forward(got[clean], x[clean], w, bias, residual[clean], "relu", torch.bfloat16)
+        assert torch.isnan(got[7]).all()
+        inf = torch.where(w[:, 0] > 0, float("inf"), torch.where(w[:, 0] < 0, 0.0, float("nan")))
+        assert torch.equal((inf + residual[3].float()).to(torch.bfloat16), got[3])
+
+
+@gpu
+def test_python_refusals():
+    x, w = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(8, 64, dtype=torch.bfloat16, device="cuda")
+    for args, kw in (((x, w.half()), {}), ((x, w[:, :32]), {}), ((x.float(), w.float()), {}), ((x[:, :60], w[:, :60]), {}), ((x, w, torch.zeros(7).cuda().bfloat16()), {}),
+                     ((x, w, torch.zeros(8).cuda()), {}), ((x, w, None, x), {}), ((x, w), dict(activation="tanh")), ((x, w), dict(out_dtype=torch.float16)),
+                     ((x, w, None, torch.zeros(4, 8, device="cuda")), {}), ((x, w.cpu()), {})):
+        with pytest.raises(RuntimeError):
+            linear(*args, **kw)
+    assert linear(x[:0], w).shape == (0, 8) and linear(x, w[:0]).shape == (4, 0)
+
+
+# ---- backward --------------------------------------------------------------------------------------------------------
+
+TRAIN_SIZES = [(1, 1, 8), (1, 300, 64), (7, 33, 72), (130, 64, 200), (33, 1411, 520), (300, 129, 1032), (1000, 128, 2048), (513, 2050, 264), (2600, 2056, 3080)]
+
+
+@gpu
+@pytest.mark.parametrize("activation", ["none", "relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("m, n, k", TRAIN_SIZES)
+def test_gradients_against_the_formulas(m, n, k, activation):
+    for dtype, out in ((torch.bfloat16, None), (torch.float16, torch.float32)):
+        x, w, bias, residual = make(m, n, k, dtype, 11, out)
+        dd = torch.randn(m, n, generator=gen(12)).to(out or dtype)
+        leaves = [t.cuda().requires_grad_() for t in (x, w, bias, residual)]
+        y = linear(*leaves, activation=activation, out_dtype=out)
+        check_forward(y.detach(), x, w, bias, residual, activation, out or dtype)
+        dx, dw, db, dr = torch.autograd.grad(y, leaves, dd.cuda())
+        assert torch.equal(dr.cpu(), dd)
+        z = (x.double() @ w.double().t() + bias.double()).requires_grad_()
+        (dz,) = torch.autograd.grad(act64(z, activation), z, dd.double())
+        z = z.detach()
+        # z is kept rounded: half a step of it times the curvature; a sign that the forward sum's error can flip costs relu the whole slope
+        z_error = sum_error(x, w.t()) + z.abs() * (HALF_STEP[dtype] * 1.01 + 2.0 ** -23) + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+        if activation == "none":
+            dz_error = torch.zeros_like(z)
+        elif activation == "relu":
+            dz_error = torch.where(z.abs() <= sum_error(x, w.t()) + z.abs() * 2.0 ** -23 + (2.0 ** -24 if dtype == torch.float16 else 0.0), dd.double().abs(), 0.0)
+        else:
+            dz_error = dd.double().abs() * (CURVATURE * z_error + 16 * 2.0 ** -23)
+        tiny = 2.0 ** -25 if dtype == torch.float16 else 1e-40
+        db_error = dz_error.sum(dim=0) + dz.abs().sum(dim=0) * (m + 4) * 2.0 ** -24
+        assert (db.cpu().double() - dz.sum(dim=0)).abs().le(db_error + (dz.sum(dim=0).abs() + db_error) * 1.01 * HALF_STEP[dtype] + tiny).all()
+        rounded = dz_error + (dz.abs() + dz_error) * 1.01 * HALF_STEP[dtype] + tiny      # dz rounded for the tensor cores
+        for got, want, size in ((dx, dz @ w.double(), (dz.abs() + rounded) @ w.double().abs()), (dw, dz.t() @ x.double(), (dz.abs() + rounded).t() @ x.double().abs())):
+            other, terms = (w, n) if got is dx else (x, m)
+            spread = (rounded if got is dx else rounded.t()) @ other.double().abs()
+            error = spread + size * (terms + 4) * 2.0 ** -23
+            assert got.dtype == dtype
+            assert (got.cpu().double() - want).abs().le(error + (want.abs() + error) * 1.01 * HALF_STEP[dtype] + tiny).all()
+
+
+@gpu
+def test_gradients_against_differences():
+    m, n, k = 6, 10, 16
+    g = gen(2)
+    x, w = torch.randn(m, k, generator=g).half(), (torch.randn(n, k, generator=g) * 0.3).half()
+    bias, dd = torch.randn(n, generator=g).half(), torch.randn(m, n, generator=g)
+    for activation in ("gelu", "gelu_tanh", "silu"):
+        leaves = [t.cuda().requires_grad_() for t in (x, w, bias)]
+        grads = torch.autograd.grad(linear(*leaves, activation=activation, out_dtype=torch.float32), leaves, dd.cuda())
+        f = lambda a, b, c: float((act64(a @ b.t() + c, activation) * dd.double()).sum())
+        base = [x.double(), w.double(), bias.double()]
+        for which, grad in enumerate(grads):
+            for at in range(0, base[which].numel(), 7):
+                h = 1e-5
+                moved = []
+                for sign in (h, -h):
+                    args = [t.clone() for t in base]
+                    args[which].view(-1)[at] += sign
+                    moved.append(f(*args))
+                slope = (moved[0] - moved[1]) / (2 * h)
+                # z and dz rounded to FP16 (2^-11 each, values of a few) in sums of up to 16 terms, the result rounded once
+                assert abs(slope - float(grad.reshape(-1)[at])) < 16 * 4 * 2 * 2.0 ** -11
+
+
+@gpu
+def test_gradients_wanted_alone_strided_and_of_nothing():
+    m, n, k = 70, 33, 136
+    x, w, bias, residual = (t.cuda() for t in make(m, n, k, torch.bfloat16, 3))
+    full = [t.clone().requires_grad_() for t in (x, w, bias, residual)]
+    dd = torch.randn(m, n + 3, generator=gen(1)).bfloat16().cuda()[:, 1:1 + n]
+    want = torch.autograd.grad(linear(*full, activation="silu"), full, dd)
+    for i in range(4):
+        args = [x, w, bias, residual]
+        args[i] = args[i].clone().requires_grad_()
+        (got,) = torch.autograd.grad(linear(*args, activation="silu"), [args[i]], dd)
+        assert torch.equal(got, want[i]), i
+    # one value for every element: an expanded gradient, with and without an activation
+    for act in ("none", "silu"):
+        a = torch.autograd.grad(linear(*full, activation=act).sum(), full)
+        b = torch.autograd.grad(linear(*full, activation=act), full, torch.ones(m, n, dtype=torch.bfloat16, device="cuda"))
+        assert all(torch.equal(s, t) for s, t in zip(a, b))
+    empty = [t.clone().requires_grad_() for t in (x[:0], w, bias)]
+    dx, dw, db = torch.autograd.grad(linear(*empty, activation="gelu").sum(), empty)
+    assert dx.shape == (0, k) and (dw == 0).all() and (db == 0).all()
+
+
+# ---- streams, graphs, repeated calls ---------------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("m, n, k", [(1, 4096, 4096), (40, 520, 2048), (400, 200, 1024), (3000, 2056, 128)])
+def test_repeated_calls_streams_and_graphs_give_the_same_bits(m, n, k):
+    x, w, bias, residual = (t.cuda() for t in make(m, n, k, torch.bfloat16, 9))
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    want = linear(x, w, bias, residual, activation="gelu", device_status=status)
+    outs = [linear(x, w, bias, residual, activation="gelu", device_status=status) for _ in range(20)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        outs.append(linear(x, w, bias, residual, activation="gelu", device_status=status))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = linear(x, w, bias, residual, activation="gelu", device_status=status)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(want, o) for o in outs + [held])
+    x.copy_(torch.randn(m, k, generator=gen(10)))
+    graph.replay()
+    assert torch.equal(held, linear(x, w, bias, residual, activation="gelu"))
+    assert _C.read_status(status) == 0
+
+
+@gpu
+def test_a_captured_training_step():
+    x, w, bias, residual = (t.cuda() for t in make(200, 136, 264, torch.bfloat16, 4))
+    leaves = [t.requires_grad_() for t in (x, w, bias, residual)]
+    dd = torch.randn(200, 136, generator=gen(5)).bfloat16().cuda()
+    step = lambda: torch.autograd.grad(linear(*leaves, activation="gelu"), leaves, dd)
+    want = [t.clone() for t in step()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@gpu
+def test_router_sorted_experts_and_shared_expert_train_together():
+    """logits = linear -> route -> sort -> a dense expert per group -> back, plus a shared expert whose last product adds the routed
+    sum as its residual: the gradients of the whole against the same layer in 64 bits."""
+    tokens, experts, k, hidden, inter = 96, 4, 2, 64, 128
+    g = gen(8)
+    half = lambda *s, scale=1.0: (torch.randn(*s, generator=g) * scale).to(torch.float16)
+    x, gate = half(tokens, hidden), half(experts, hidden, scale=0.3)
+    expert_w = half(experts, hidden, hidden, scale=0.125)
+    w1, w2 = half(inter, hidden, scale=0.125), half(hidden, inter, scale=0.09)
+    dy = torch.randn(tokens, hidden, generator=g).to(torch.float16)
+
+    leaves = [t.cuda().requires_grad_() for t in (x, gate, expert_w, w1, w2)]
+    lx, lg, le, l1, l2 = leaves
+    ids, weights = route_tokens(linear(lx, lg, out_dtype=torch.float32), k)
+    rows, order = sort_tokens(lx, ids, experts, alignment=16)
+    bounds = [int((order.m_indices == e).sum()) for e in range(experts)] + [int((order.m_indices < 0).sum())]
+    outs = [linear(part, le[e]) if e < experts else part for e, part in enumerate(torch.split(rows, bounds))]
+    routed = unsort_tokens(torch.cat(outs), order, weights)
+    y = linear(linear(lx, l1, activation="silu"), l2, residual=routed)
+    got = torch.autograd.grad(y, leaves, dy.cuda())
+
+    exact = [t.double().requires_grad_() for t in (x, gate, expert_w, w1, w2)]
+    ex, eg, ee, e1, e2 = exact
+    probs = torch.softmax(ex @ eg.t(), dim=1)
+    top = ids.cpu()
+    wt = probs.gather(1, top)
+    wt = wt / wt.sum(dim=1, keepdim=True)
+    routed = sum(wt[:, j, None] * torch.einsum("th,toh->to", ex, ee[top[:, j]]) for j in range(k))
+    want_y = act64(ex @ e1.t(), "silu") @ e2.t() + routed
+    want = torch.autograd.grad(want_y, exact, dy.double())
+    # every value passes at most six roundings to FP16 on its way (rows, hidden products, dz, sums): relative to the largest of its kind
+    for a, b in zip([y.detach(), *got], [want_y.detach(), *want]):
+        assert (a.cpu().double() - b).abs().max() <= 6 * 2.0 ** -11 * 4 * b.abs().max()
