@@ -371,18 +371,20 @@ NVFP4_API int nvfp4_unsort_tokens_backward(const void* dy, int64_t ldy_elems, co
  * 16-byte-aligned starts, row strides that are multiples of 8 elements; K >= 1, K % 8 == 0.  M and N are any; outputs, bias
  * and residual have any alignment and stride.
  * nvfp4_linear: d[M,N] = activation(x[M,K] w[N,K]^T + bias[N]) + residual[M,N].  d and residual have out_dtype, `dtype` or
- *   NVFP4_DTYPE_F32; bias (of type `dtype`) and residual may be NULL.  z (may be NULL) receives what the activation is applied to, rounded to
- *   `dtype`, for the backward pass.
- * nvfp4_linear_dz: dz[M,N] = dd * activation'(z), rounded to `dtype` for the products below, and db[N], the sums of its columns taken before
- *   that rounding.  dd has out_dtype, any alignment and stride; z is not read for NVFP4_ACTIVATION_NONE.  z and dz have row strides of
- *   N rounded up to 8 at least, and the elements behind column N of dz are overwritten.  dz or db may be NULL.
+ *   NVFP4_DTYPE_F32; bias (of type `dtype`) and residual may be NULL.  slopes (may be NULL; not written for NVFP4_ACTIVATION_NONE) receives
+ *   activation'(x w^T + bias) for the backward pass, in multiples of 2^-14; -32768 stands for NaN.
+ * nvfp4_linear_dz: dz[M,N] = dd * slopes, rounded to `dtype` for the products below, and db[N], the sums of its columns taken before
+ *   that rounding.  dd has out_dtype, any alignment and stride; slopes NULL: 1.  slopes and dz start on 16 bytes and have row strides
+ *   that are multiples of 8, N rounded up to 8 at least; what lies behind column N of dz's rows up to there is overwritten.  dz or db
+ *   may be NULL.
  * nvfp4_linear_dx: dx[M,K] = dz w.      nvfp4_linear_dw: dw[N,K] = dz^T x.      Rounded to `dtype`.
+ * An FP32 output takes partial sums of 256 products out of the tensor cores and adds them as FP32; others stay in their accumulator.
  * device_status (may be NULL) receives bit 0 if a bounded wait expired.  No counterparts in the reference project. */
 NVFP4_API int nvfp4_linear(const void* x, int64_t ldx_elems, const void* w, int64_t ldw_elems, const void* bias, const void* residual,
-                           int64_t ldr_elems, void* d, int64_t ldd_elems, void* z, int64_t ldz_elems, int M, int N, int K, int dtype,
+                           int64_t ldr_elems, void* d, int64_t ldd_elems, int16_t* slopes, int64_t lds_elems, int M, int N, int K, int dtype,
                            int out_dtype, int activation, int32_t* device_status, void* stream);
-NVFP4_API int nvfp4_linear_dz(const void* dd, int64_t ldd_elems, const void* z, int64_t ldz_elems, void* dz, int64_t lddz_elems, void* db, int M,
-                              int N, int dtype, int out_dtype, int activation, void* stream);
+NVFP4_API int nvfp4_linear_dz(const void* dd, int64_t ldd_elems, const int16_t* slopes, int64_t lds_elems, void* dz, int64_t lddz_elems, void* db,
+                              int M, int N, int dtype, int out_dtype, void* stream);
 NVFP4_API int nvfp4_linear_dx(const void* dz, int64_t lddz_elems, const void* w, int64_t ldw_elems, void* dx, int64_t lddx_elems, int M, int N,
                               int K, int dtype, int32_t* device_status, void* stream);
 NVFP4_API int nvfp4_linear_dw(const void* dz, int64_t lddz_elems, const void* x, int64_t ldx_elems, void* dw, int64_t lddw_elems, int M, int N,

@@ -104,7 +104,7 @@ def lib() -> ctypes.CDLL:
         L.nvfp4_unsort_tokens.argtypes = [vp, i64, i32, i64, vp, vp, i64, i32, i32, vp, vp]
         L.nvfp4_unsort_tokens_backward.argtypes = [vp, i64, vp, i64, i32, i64, vp, vp, vp, i64, i32, i32, vp, vp, vp]
         L.nvfp4_linear.argtypes = [vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, i32, i32, vp, vp]
-        L.nvfp4_linear_dz.argtypes = [vp, i64, vp, i64, vp, i64, vp, i32, i32, i32, i32, i32, vp]
+        L.nvfp4_linear_dz.argtypes = [vp, i64, vp, i64, vp, i64, vp, i32, i32, i32, i32, vp]
         L.nvfp4_linear_dx.argtypes = [vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp]
         L.nvfp4_linear_dw.argtypes = [vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp]
         _contiguous_call = _bind(L)
@@ -814,13 +814,13 @@ def _operand(t, name: str) -> int:
     return ld
 
 
-def _padded(rows: int, columns: int, like: torch.Tensor) -> torch.Tensor:
-    """(rows, columns) whose row stride is a multiple of 8."""
-    return torch.empty(rows, (columns + 7) // 8 * 8, dtype=like.dtype, device=like.device)[:, :columns]
+def _padded(rows: int, columns: int, dtype, device) -> torch.Tensor:
+    """Room for (rows, columns) with a row stride that is a multiple of 8."""
+    return torch.empty(rows, (columns + 7) // 8 * 8, dtype=dtype, device=device)
 
 
 def linear(x: torch.Tensor, w: torch.Tensor, bias, residual, activation: str, out_dtype, keep: bool = False, device_status=None):
-    """(d, z): d = activation(x w^T + bias) + residual, z what the activation is applied to, None without `keep`; see nvfp4_linear."""
+    """(d, slopes): d = activation(x w^T + bias) + residual, slopes for the backward pass, None without `keep`; see nvfp4_linear."""
     ldx, ldw = _operand(x, "x"), _operand(w, "w")
     (m, k), n, dev = x.shape, w.shape[0], _one_device(x, w, bias, residual, device_status)
     out_dtype = x.dtype if out_dtype is None else out_dtype
@@ -832,46 +832,47 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias, residual, activation: str, ou
     _require(residual is None or (residual.dtype == out_dtype and residual.shape == (m, n)), "residual is (M, N), of the output's type")
     ldr = _matrix(residual, "residual") if residual is not None else 0
     d = torch.empty(m, n, dtype=out_dtype, device=dev)
-    z = _padded(m, n, x) if keep else None
+    slopes = _padded(m, n, torch.int16, dev) if keep else None
     with _on(dev):
         _check(lib().nvfp4_linear(x.data_ptr(), ldx, w.data_ptr(), ldw, bias.data_ptr() if bias is not None else None,
                                   residual.data_ptr() if residual is not None else None, ldr, d.data_ptr(), n,
-                                  z.data_ptr() if keep else None, z.stride(0) if keep else 0, m, n, k, DTYPE_CODES[x.dtype],
+                                  slopes.data_ptr() if keep else None, slopes.shape[1] if keep else 0, m, n, k, DTYPE_CODES[x.dtype],
                                   DTYPE_CODES[out_dtype], ACTIVATION_CODES[activation],
                                   device_status.data_ptr() if device_status is not None else None, _stream()))
-    return d, z
+    return d, slopes
 
 
-def linear_backward(dd: torch.Tensor, x, w, z, dtype: torch.dtype, activation: str, want_x: bool, want_w: bool, want_bias: bool, device_status=None):
-    """(dx, dw, db) of `linear`, None where not wanted; dd contiguous along its rows."""
+def linear_backward(dd: torch.Tensor, x, w, slopes, dtype: torch.dtype, want_bias: bool, device_status=None):
+    """(dx, dw, db) of `linear`: dx if w is given, dw if x is, None otherwise; slopes None: no activation."""
     ldd, (m, n) = _matrix(dd, "dd"), dd.shape
-    dev = _one_device(dd, x, w, z, device_status)
-    like = torch.empty(0, dtype=dtype, device=dev)
+    dev = _one_device(dd, x, w, slopes, device_status)
     status = device_status.data_ptr() if device_status is not None else None
-    code = DTYPE_CODES[dtype]
-    k = x.shape[1] if x is not None else w.shape[1] if w is not None else 0
-    products = want_x or want_w
+    code, products = DTYPE_CODES[dtype], x is not None or w is not None
     # without an activation the incoming gradient is dz itself, where it can be an operand
-    as_it_is = activation == "none" and dd.dtype == dtype and ldd % 8 == 0 and dd.data_ptr() % 16 == 0
-    dz = dd if as_it_is else _padded(m, n, like) if products else None
+    as_it_is = slopes is None and dd.dtype == dtype and ldd % 8 == 0 and dd.data_ptr() % 16 == 0
     db = torch.empty(n, dtype=dtype, device=dev) if want_bias else None
-    dx = torch.empty(m, k, dtype=dtype, device=dev) if want_x else None
-    dw = torch.empty(n, k, dtype=dtype, device=dev) if want_w else None
+    dx = torch.empty(m, w.shape[1], dtype=dtype, device=dev) if w is not None else None
+    dw = torch.empty(n, x.shape[1], dtype=dtype, device=dev) if x is not None else None
     if m == 0 or n == 0:                                 # sums over nothing
         for t in (dx, dw, db):
             if t is not None:
                 t.zero_()
         return dx, dw, db
-    ldz = dz.stride(0) if products and m > 1 else (n + 7) // 8 * 8
+    dz, ldz = (dd, ldd) if as_it_is else (None, 0)
+    if products and not as_it_is:
+        dz = _padded(m, n, dtype, dev)
+        ldz = dz.shape[1]
     with _on(dev):
         if want_bias or (products and not as_it_is):
-            _check(lib().nvfp4_linear_dz(dd.data_ptr(), ldd, z.data_ptr() if z is not None else None, z.stride(0) if z is not None else 0,
+            _check(lib().nvfp4_linear_dz(dd.data_ptr(), ldd, slopes.data_ptr() if slopes is not None else None, slopes.shape[1] if slopes is not None else 0,
                                          None if as_it_is or not products else dz.data_ptr(), ldz, db.data_ptr() if want_bias else None, m, n,
-                                         code, DTYPE_CODES[dd.dtype], ACTIVATION_CODES[activation], _stream()))
-        if want_x:
-            _check(lib().nvfp4_linear_dx(dz.data_ptr(), ldz, w.data_ptr(), _operand(w, "w"), dx.data_ptr(), k, m, n, k, code, status, _stream()))
-        if want_w:
-            _check(lib().nvfp4_linear_dw(dz.data_ptr(), ldz, x.data_ptr(), _operand(x, "x"), dw.data_ptr(), k, m, n, k, code, status, _stream()))
+                                         code, DTYPE_CODES[dd.dtype], _stream()))
+        if w is not None:
+            _check(lib().nvfp4_linear_dx(dz.data_ptr(), ldz, w.data_ptr(), _operand(w, "w"), dx.data_ptr(), dx.shape[1], m, n, dx.shape[1], code, status,
+                                         _stream()))
+        if x is not None:
+            _check(lib().nvfp4_linear_dw(dz.data_ptr(), ldz, x.data_ptr(), _operand(x, "x"), dw.data_ptr(), dw.shape[1], m, n, dw.shape[1], code, status,
+                                         _stream()))
     return dx, dw, db
 
 

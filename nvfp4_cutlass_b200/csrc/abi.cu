@@ -876,8 +876,8 @@ static int tensor_core_device(host::DeviceInfo** dev)
 }
 
 int nvfp4_linear(const void* x, int64_t ldx_elems, const void* w, int64_t ldw_elems, const void* bias, const void* residual, int64_t ldr_elems, void* d,
-                 int64_t ldd_elems, void* z, int64_t ldz_elems, int M, int N, int K, int dtype, int out_dtype, int activation, int32_t* device_status,
-                 void* stream)
+                 int64_t ldd_elems, int16_t* slopes, int64_t lds_elems, int M, int N, int K, int dtype, int out_dtype, int activation,
+                 int32_t* device_status, void* stream)
 {
     host::clear_error();
     if (int rc = check_linear(M, N, K, dtype)) return rc;
@@ -886,35 +886,34 @@ int nvfp4_linear(const void* x, int64_t ldx_elems, const void* w, int64_t ldw_el
     if (M == 0 || N == 0) return NVFP4_OK;
     if (int rc = check_operand("x", x, ldx_elems, K)) return rc;
     if (int rc = check_operand("w", w, ldw_elems, K)) return rc;
-    NVFP4_REQUIRE(d != nullptr && ldd_elems >= N && (residual == nullptr || ldr_elems >= N) && (z == nullptr || ldz_elems >= N),
+    NVFP4_REQUIRE(d != nullptr && ldd_elems >= N && (residual == nullptr || ldr_elems >= N) && (slopes == nullptr || lds_elems >= N),
                   "null output, or row strides smaller than the row");
-    NVFP4_REQUIRE(on_elements(d, out_dtype) && on_elements(residual, out_dtype) && on_elements(bias, dtype) && on_elements(z, dtype),
+    NVFP4_REQUIRE(on_elements(d, out_dtype) && on_elements(residual, out_dtype) && on_elements(bias, dtype) && on_elements(slopes, dtype),
                   "output, bias or residual is not aligned to its type");
     host::DeviceInfo* dev;
     if (int rc = tensor_core_device(&dev)) return rc;
-    return launch_linear(x, ldx_elems, w, ldw_elems, bias, residual, ldr_elems, d, ldd_elems, z, ldz_elems, M, N, K, dtype == NVFP4_DTYPE_BF16,
+    return launch_linear(x, ldx_elems, w, ldw_elems, bias, residual, ldr_elems, d, ldd_elems, slopes, lds_elems, M, N, K, dtype == NVFP4_DTYPE_BF16,
                          out_dtype == NVFP4_DTYPE_F32, activation, device_status, dev->num_sms, static_cast<cudaStream_t>(stream));
 }
 
-int nvfp4_linear_dz(const void* dd, int64_t ldd_elems, const void* z, int64_t ldz_elems, void* dz, int64_t lddz_elems, void* db, int M, int N, int dtype,
-                    int out_dtype, int activation, void* stream)
+int nvfp4_linear_dz(const void* dd, int64_t ldd_elems, const int16_t* slopes, int64_t lds_elems, void* dz, int64_t lddz_elems, void* db, int M, int N,
+                    int dtype, int out_dtype, void* stream)
 {
     host::clear_error();
     if (int rc = check_linear(M, N, 8, dtype)) return rc;
     NVFP4_REQUIRE(out_dtype == dtype || out_dtype == NVFP4_DTYPE_F32, "the output has the operands' type or FP32 (type codes %d, %d)", out_dtype, dtype);
-    NVFP4_REQUIRE(activation >= NVFP4_ACTIVATION_NONE && activation <= NVFP4_ACTIVATION_SILU, "unknown activation %d", activation);
     if (M == 0 || N == 0 || (dz == nullptr && db == nullptr)) return NVFP4_OK;
     const int64_t padded = (static_cast<int64_t>(N) + 7) / 8 * 8;
     NVFP4_REQUIRE(dd != nullptr && ldd_elems >= N && on_elements(dd, out_dtype), "dd is null, not aligned to its type, or its rows overlap");
     NVFP4_REQUIRE(on_elements(db, dtype), "db is not aligned to its type");
-    if (activation != NVFP4_ACTIVATION_NONE)
-        if (int rc = check_operand("z", z, ldz_elems, padded)) return rc;
+    if (slopes != nullptr)
+        if (int rc = check_operand("slopes", slopes, lds_elems, padded)) return rc;
     if (dz != nullptr)
         if (int rc = check_operand("dz", dz, lddz_elems, padded)) return rc;
     host::DeviceInfo* dev;
     if (int rc = tensor_core_device(&dev)) return rc;
-    return launch_linear_dz(dd, ldd_elems, out_dtype == NVFP4_DTYPE_F32, z, ldz_elems, dz, lddz_elems, db, M, N, dtype == NVFP4_DTYPE_BF16, activation,
-                            dev->hw_sms, static_cast<cudaStream_t>(stream));
+    return launch_linear_dz(dd, ldd_elems, out_dtype == NVFP4_DTYPE_F32, slopes, lds_elems, dz, lddz_elems, db, M, N, dtype == NVFP4_DTYPE_BF16, dev->hw_sms,
+                            static_cast<cudaStream_t>(stream));
 }
 
 int nvfp4_linear_dx(const void* dz, int64_t lddz_elems, const void* w, int64_t ldw_elems, void* dx, int64_t lddx_elems, int M, int N, int K, int dtype,

@@ -42,8 +42,8 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(f
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
 // ---- activations -----------------------------------------------------------------------------------------------------
-// gelu(z) = z Phi(z); its tanh form 0.5 z (1 + tanh u), u = c (z + 0.044715 z^3), is z / (1 + exp(-2 u)): neither loses the digits of
-// small values to a sum near zero.
+// gelu(z) = z Phi(z); its tanh form 0.5 z (1 + tanh u), u = c (z + 0.044715 z^3), is z sigmoid(2 u) as silu is z sigmoid(z): none of
+// them loses the digits of small values to a sum near zero.
 constexpr float kGeluC = 0.7978845608028654f;        // sqrt(2 / pi)
 template <int kAct>
 __device__ __forceinline__ float activate(float z)
@@ -67,6 +67,12 @@ __device__ __forceinline__ float slope(float z)
     const float e = expf(-fabsf(u2)), near = 1.0f / (1.0f + e), far = e * near;           // of sigmoid(u2) and 1 - sigmoid(u2) the larger, the smaller
     return fmaf(z * du2, near * far, u2 >= 0.0f ? near : far);
 }
+// For the backward pass a slope, all of which lie in (-0.2, 1.2), is kept as a multiple of 2^-14 in 16 bits: off by 2^-15 at most, less
+// than the rounding of the gradient that it multiplies, where z kept in BF16 would cost as much as that rounding again.
+constexpr int kSlopeNan = -32768;
+__device__ __forceinline__ int16_t pack_slope(float s) { return static_cast<int16_t>(s != s ? kSlopeNan : __float2int_rn(s * 16384.0f)); }
+__device__ __forceinline__ float unpack_slope(int16_t c) { return c == kSlopeNan ? __uint_as_float(0x7fc00000u) : c * (1.0f / 16384.0f); }
+
 // Calls f(std::integral_constant<int, activation>) for a code: one switch around a loop of elements.
 template <typename F>
 __device__ __forceinline__ void with_activation(int code, F&& f)
@@ -84,57 +90,55 @@ __device__ __forceinline__ void with_activation(int code, F&& f)
 
 struct Epilogue {
     void* d; int64_t ldd;                            // (rows, cols), of the operands' type or FP32
-    void* z; int64_t ldz;                            // what the activation is applied to, for the backward pass, or NULL
+    int16_t* slopes; int64_t lds;                    // activation'(z) for the backward pass, or NULL
     const void* bias;                                // (cols) or NULL
     const void* residual; int64_t ldr;               // of d's type, or NULL
     uint32_t rows, cols;
     int activation;
-    bool out32;
 };
 
 // Up to kN accumulators of a lane: output column `col`, rows row0 + i, i < count.  The lanes of a warp hold neighbouring columns, so that
-// every access of the warp is one run of an output row, whatever its alignment.
-template <typename T, uint32_t kN>
+// every access of the warp is one run of an output row, whatever its alignment.  T: operands and bias, D: output and residual.
+// The residual's loads go out together, from rows and columns that exist (a load in a branch of its own waits for its value there: 8192 x
+// 4096 x 4096 took 465 us in place of the 184 without a residual).  All of them are plain loads: __ldg is an asm statement that the
+// compiler may move, and it was moved ahead of the test for a NULL bias, out of the loop over a tile's columns.
+template <typename T, typename D, uint32_t kN>
 __device__ __forceinline__ void finish(float (&v)[kN], uint32_t row0, uint32_t count, uint32_t col, const Epilogue& e)
 {
-    const uint32_t rows = row0 < e.rows && col < e.cols ? min(count, e.rows - row0) : 0u;
-    float r[kN];
+    if (row0 >= e.rows || count == 0) return;
+    const uint32_t rows = min(count, e.rows - row0), last = rows - 1, at = min(col, e.cols - 1);
+    const bool mine = col < e.cols;
+    D r[kN];
     if (e.residual != nullptr) {
+        const D* from = static_cast<const D*>(e.residual) + static_cast<int64_t>(row0) * e.ldr + at;
 #pragma unroll
-        for (uint32_t i = 0; i < kN; ++i) {
-            r[i] = 0.0f;
-            const int64_t at = static_cast<int64_t>(row0 + i) * e.ldr + col;
-            if (i < rows) r[i] = e.out32 ? static_cast<const float*>(e.residual)[at] : to_float(static_cast<const T*>(e.residual)[at]);
-        }
+        for (uint32_t i = 0; i < kN; ++i) r[i] = from[static_cast<int64_t>(min(i, last)) * e.ldr];
     }
     if (e.bias != nullptr) {
-        const float b = col < e.cols ? to_float(static_cast<const T*>(e.bias)[col]) : 0.0f;
+        const float b = to_float(static_cast<const T*>(e.bias)[at]);
 #pragma unroll
         for (uint32_t i = 0; i < kN; ++i) v[i] += b;
     }
-    if (e.z != nullptr) {
-#pragma unroll
-        for (uint32_t i = 0; i < kN; ++i)
-            if (i < rows) static_cast<T*>(e.z)[static_cast<int64_t>(row0 + i) * e.ldz + col] = from_float<T>(v[i]);
-    }
     if (e.activation != NVFP4_ACTIVATION_NONE)
         with_activation(e.activation, [&](auto act) {
+            constexpr int kAct = decltype(act)::value;
+            if (e.slopes != nullptr) {
+                int16_t* to = e.slopes + static_cast<int64_t>(row0) * e.lds + at;
 #pragma unroll
-            for (uint32_t i = 0; i < kN; ++i) v[i] = activate<decltype(act)::value>(v[i]);
+                for (uint32_t i = 0; i < kN; ++i)
+                    if (i < rows && mine) to[i * e.lds] = pack_slope(slope<kAct>(v[i]));
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < kN; ++i) v[i] = activate<kAct>(v[i]);
         });
     if (e.residual != nullptr) {
 #pragma unroll
-        for (uint32_t i = 0; i < kN; ++i) v[i] += r[i];
+        for (uint32_t i = 0; i < kN; ++i) v[i] += to_float(r[i]);
     }
-    if (e.out32) {
+    D* to = static_cast<D*>(e.d) + static_cast<int64_t>(row0) * e.ldd + at;
 #pragma unroll
-        for (uint32_t i = 0; i < kN; ++i)
-            if (i < rows) static_cast<float*>(e.d)[static_cast<int64_t>(row0 + i) * e.ldd + col] = v[i];
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < kN; ++i)
-            if (i < rows) static_cast<T*>(e.d)[static_cast<int64_t>(row0 + i) * e.ldd + col] = from_float<T>(v[i]);
-    }
+    for (uint32_t i = 0; i < kN; ++i)
+        if (i < rows && mine) to[i * e.ldd] = from_float<D>(v[i]);
 }
 
 // 32 x 32 values, lane l holding row l: afterwards lane l holds column l.  Five butterfly steps.
@@ -195,19 +199,24 @@ struct Product {
 // ---- one tile to a CTA or cluster --------------------------------------------------------------------------------------
 
 constexpr int kTileThreads = 192;                    // warp 0: TMA, warp 1: products, warps 2-5: epilogue
+constexpr uint32_t kTileEpiWarps = 4;
 constexpr uint32_t tile_stage(uint32_t bn) { return kSlotA + bn * kRowBytes; }
 constexpr uint32_t tile_smem(uint32_t bn, uint32_t depth, bool split)
 {
-    return 1024 + depth * tile_stage(bn) + (split ? bn * BM * 4 : 0) + (2 * kMaxDepth + 1) * 8 + 16;
+    return 1024 + depth * tile_stage(bn) + (split ? bn * BM * 4 : 0) + (2 * kMaxDepth + 4) * 8 + 16;
 }
+// For an FP32 output the epilogue warps take the accumulators over every four K blocks and add them up in registers, two accumulators in
+// turn: the tensor core cuts what it adds to a long sum (K = 4096 in one accumulator: off by 4.3e-6 of the result, FP32 sums by 6e-7).
+constexpr uint32_t kChunkBlocks = 4;
 
 // kSwap: A is the weight and the output's columns lie on the tensor memory's lanes; else A is x and a warp's 32 x 32 accumulators are
-// transposed first.
-template <typename T, uint32_t BN, bool kSwap>
-__global__ void __launch_bounds__(kTileThreads, 2)
+// transposed first.  D: type of the output.
+template <typename T, typename D, uint32_t BN, bool kSwap>
+__global__ void __launch_bounds__(kTileThreads, std::is_same<D, float>::value && BN > 64 ? 1 : 2)
 product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Product p, const Epilogue e)
 {
-    constexpr uint32_t kChunk = BN < 32 ? BN : 32, kStage = tile_stage(BN);
+    constexpr bool kWide = std::is_same<D, float>::value;
+    constexpr uint32_t kChunk = BN < 32 ? BN : 32, kStage = tile_stage(BN), kCols = (kWide ? 2 : 1) * BN < 32 ? 32 : (kWide ? 2 : 1) * BN;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (smem - ptx::smem_u32(smem_raw));
@@ -215,21 +224,22 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     float* partial = reinterpret_cast<float*>(gen + depth * kStage);          // [splits][BN / splits][BM], from each CTA of the cluster
     uint64_t* full = reinterpret_cast<uint64_t*>(gen + depth * kStage + (splits > 1 ? BN * BM * 4 : 0));
     uint64_t* drained = full + kMaxDepth;
-    uint64_t* tmem_full = drained + kMaxDepth;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_full + 1);
+    uint64_t* tmem_full = drained + kMaxDepth;       // per accumulator
+    uint64_t* tmem_empty = tmem_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
     volatile uint32_t* abort_flag = tmem_slot + 1;
 
     const uint32_t warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const uint32_t rank = blockIdx.x & (splits - 1), tile = blockIdx.x >> p.splits_log2;
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < depth; ++i) { ptx::mbar_init(full + i, 1); ptx::mbar_init(drained + i, 1); }
-        ptx::mbar_init(tmem_full, 1);
+        for (uint32_t i = 0; i < 2; ++i) { ptx::mbar_init(tmem_full + i, 1); ptx::mbar_init(tmem_empty + i, kTileEpiWarps); }
         *abort_flag = 0;
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&tm_a);
         ptx::prefetch_tensormap(&tm_b);
     }
-    if (warp == 1) ptx::tmem_alloc<BN < 32 ? 32 : BN>(tmem_slot);
+    if (warp == 1) ptx::tmem_alloc<kCols>(tmem_slot);
     ptx::tcgen05_fence_before_sync();
     if (splits > 1) ptx::cluster_sync();             // every CTA of the cluster runs before anybody writes into its shared memory
     else __syncthreads();
@@ -242,6 +252,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     const uint32_t a0 = a_blk * BM, b0 = b_blk * BN;
     const uint32_t kb0 = static_cast<uint32_t>(static_cast<uint64_t>(p.k_blocks) * rank >> p.splits_log2);
     const uint32_t kb1 = static_cast<uint32_t>(static_cast<uint64_t>(p.k_blocks) * (rank + 1) >> p.splits_log2);
+    const uint32_t chunks = kWide ? (kb1 - kb0 + kChunkBlocks - 1) / kChunkBlocks : 1;
     bool ok = true;
     auto give_up = [&] {
         *abort_flag = 1;
@@ -251,6 +262,9 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     auto next = [&](Ring& r) {
         if (++r.slot == depth) { r.slot = 0; r.phase ^= 1; }
     };
+    const uint32_t quad = warp & 3, row = quad * 32 + lane;                   // epilogue: the warp's quarter of the lanes
+    const uint32_t taddr = tmem + ((quad * 32) << 16);
+    [[maybe_unused]] float sum[kWide ? BN : 1];
     if (warp == 0) {
         const uint32_t issue = ptx::elect_one();
         Ring r;
@@ -274,46 +288,74 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         const uint32_t idesc = ptx::make_idesc_f16(BM, BN, std::is_same<T, __nv_bfloat16>::value, p.a_mn, p.b_mn);
         Ring r;
         for (uint32_t kb = kb0; kb < kb1; ++kb) {
+            const uint32_t n = kb - kb0, c = kWide ? n / kChunkBlocks : 0, acc = c & 1;
+            const bool first = kWide ? n % kChunkBlocks == 0 : n == 0;
+            if (kWide && first && !ptx::all_lanes(ptx::mbar_wait_impl(tmem_empty + acc, ((c >> 1) & 1) ^ 1, abort_flag))) { give_up(); break; }
             if (!ptx::all_lanes(ptx::mbar_wait_impl(full + r.slot, r.phase, abort_flag))) { give_up(); break; }
             ptx::tcgen05_fence_after_sync();
             const uint32_t at = smem + r.slot * kStage;
 #pragma unroll
             for (uint32_t s = 0; s < BK / 16; ++s)
-                ptx::tcgen05_mma_f16(tmem, operand_desc(at, p.a_mn, s), operand_desc(at + kSlotA, p.b_mn, s), idesc, (kb != kb0) | s, issue);
+                ptx::tcgen05_mma_f16(tmem + acc * BN, operand_desc(at, p.a_mn, s), operand_desc(at + kSlotA, p.b_mn, s), idesc, first && s == 0 ? 0u : 1u, issue);
             ptx::tcgen05_commit(drained + r.slot, issue);
+            if (kb + 1 == kb1 || (kWide && n % kChunkBlocks == kChunkBlocks - 1)) ptx::tcgen05_commit(tmem_full + acc, issue);
             next(r);
         }
-        if (ok) ptx::tcgen05_commit(tmem_full, issue);
     } else {
-        if (!ptx::all_lanes(ptx::mbar_wait_relaxed(tmem_full, 0, abort_flag, 20))) give_up();
-        ptx::tcgen05_fence_after_sync();
+        if constexpr (kWide) {
+#pragma unroll
+            for (uint32_t i = 0; i < BN; ++i) sum[i] = 0.0f;
+        }
+        for (uint32_t c = 0; c < chunks; ++c) {
+            const uint32_t acc = c & 1;
+            if (!ptx::all_lanes(ptx::mbar_wait_relaxed(tmem_full + acc, (c >> 1) & 1, abort_flag, 20))) { give_up(); break; }
+            ptx::tcgen05_fence_after_sync();
+            if constexpr (kWide) {
+#pragma unroll
+                for (uint32_t c0 = 0; c0 < BN; c0 += kChunk) {
+                    float v[kChunk];
+                    load_accumulators(taddr + acc * BN + c0, v);
+#pragma unroll
+                    for (uint32_t i = 0; i < kChunk; ++i) sum[c0 + i] += v[i];
+                }
+                ptx::tcgen05_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(tmem_empty + acc);
+            }
+        }
     }
 
-    // epilogue: warp's quadrant of the lanes, 128 rows of A in all
-    const uint32_t quad = warp & 3, row = quad * 32 + lane;
-    const uint32_t taddr = tmem + ((quad * 32) << 16);
-    const uint32_t live = kSwap ? min(BN, e.rows - b0) : BN;                  // columns of the tile that anybody wants
+    // epilogue: 128 rows of A in all
+    const uint32_t live = kSwap ? min(BN, e.rows - b0) : min(BN, e.cols - b0);          // columns of the tile that anybody wants
+    auto take = [&](float (&v)[kChunk], uint32_t c0) {
+        if constexpr (kWide) {
+#pragma unroll
+            for (uint32_t i = 0; i < kChunk; ++i) v[i] = sum[c0 + i];
+        } else {
+            load_accumulators(taddr + c0, v);
+        }
+    };
     auto give = [&](float (&v)[kChunk], uint32_t column, uint32_t count) {    // columns [column, column + count) of the tile
         if constexpr (kSwap) {
-            finish<T>(v, b0 + column, count, a0 + row, e);
+            finish<T, D>(v, b0 + column, count, a0 + row, e);
         } else {
             transpose(v, lane);
-            finish<T>(v, a0 + quad * 32, 32, b0 + column + lane, e);
+            finish<T, D>(v, a0 + quad * 32, 32, b0 + column + lane, e);
         }
     };
     if (splits > 1) {
         const uint32_t width_log2 = __popc(BN - 1) - p.splits_log2, width = 1u << width_log2;          // columns that a CTA finishes
         if (warp >= 2 && ok) {
-#pragma unroll 1
+            const uint32_t mine = ptx::smem_u32(partial + ((rank << width_log2) * BM + row));
+#pragma unroll
             for (uint32_t c0 = 0; c0 < BN; c0 += kChunk) {
-                if (c0 >= live) break;
+                if (c0 >= live) continue;
                 float v[kChunk];
-                load_accumulators(taddr + c0, v);
+                take(v, c0);
 #pragma unroll
                 for (uint32_t i = 0; i < kChunk; ++i) {
                     const uint32_t c = c0 + i;
-                    if (c < live)
-                        ptx::st_cluster_f32(ptx::map_to_cta(ptx::smem_u32(partial + ((rank << width_log2) + (c & (width - 1))) * BM + row), c >> width_log2), v[i]);
+                    if (c < live) ptx::st_cluster_f32(ptx::map_to_cta(mine + (c & (width - 1)) * BM * 4, c >> width_log2), v[i]);
                 }
             }
         }
@@ -326,28 +368,30 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                 const uint32_t count = min(min(width - c0, kChunk), live - first);
                 float v[kChunk];
 #pragma unroll
-                for (uint32_t i = 0; i < kChunk; ++i) {
-                    v[i] = 0.0f;
-                    if (i < count)
-                        for (uint32_t s = 0; s < splits; ++s) v[i] += partial[((s << width_log2) + c0 + i) * BM + row];
+                for (uint32_t i = 0; i < kChunk; ++i) v[i] = 0.0f;
+                for (uint32_t s = 0; s < splits; ++s) {
+                    const float* from = partial + ((s << width_log2) + c0) * BM + row;
+#pragma unroll
+                    for (uint32_t i = 0; i < kChunk; ++i)
+                        if (i < count) v[i] += from[i * BM];
                 }
-                give(v, first, count);
+                give(v, first, kSwap ? count : 32);
             }
         }
     } else if (warp >= 2 && ok) {
-#pragma unroll 1
+#pragma unroll
         for (uint32_t c0 = 0; c0 < BN; c0 += kChunk) {
-            if (c0 >= live || (!kSwap && b0 + c0 >= e.cols)) break;
+            if (c0 >= live) continue;
             float v[kChunk];
-            load_accumulators(taddr + c0, v);
-            give(v, c0, kChunk);
+            take(v, c0);
+            give(v, c0, kSwap ? min(kChunk, live - c0) : 32);
         }
     }
     ptx::tcgen05_fence_before_sync();
     __syncthreads();
     if (warp == 1) {
         ptx::tcgen05_fence_after_sync();
-        ptx::tmem_dealloc<BN < 32 ? 32 : BN>(tmem);
+        ptx::tmem_dealloc<kCols>(tmem);
     }
 }
 
@@ -464,7 +508,7 @@ product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                 }
                 if (row0 < e.rows && col0 + c < e.cols) {
                     transpose(v, lane);
-                    finish<T>(v, row0, 32, col0 + c + lane, e);
+                    finish<T, T>(v, row0, 32, col0 + c + lane, e);
                 }
             }
         }
@@ -498,7 +542,7 @@ struct Operands {
     int32_t* status;
 };
 
-template <typename T, uint32_t BN, bool kSwap>
+template <typename T, typename D, uint32_t BN, bool kSwap>
 int launch_tiles(const Operands& o, const Epilogue& e, uint32_t splits_log2, int num_sms, cudaStream_t stream)
 {
     CUtensorMap tm_a, tm_b;
@@ -521,11 +565,11 @@ int launch_tiles(const Operands& o, const Epilogue& e, uint32_t splits_log2, int
     NVFP4_CUDA_CHECK(cudaGetDevice(&dev));
     static bool attr_set[host::kMaxDevices] = {};
     if (!attr_set[dev]) {
-        NVFP4_CUDA_CHECK(cudaFuncSetAttribute(product_kernel<T, BN, kSwap>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+        NVFP4_CUDA_CHECK(cudaFuncSetAttribute(product_kernel<T, D, BN, kSwap>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
         attr_set[dev] = true;
     }
     NVFP4_REQUIRE(ctas <= INT32_MAX, "too many tiles (%llu)", static_cast<unsigned long long>(ctas));
-    return host::launch_kernel_cluster(product_kernel<T, BN, kSwap>, dim3(static_cast<unsigned>(ctas)), dim3(kTileThreads),
+    return host::launch_kernel_cluster(product_kernel<T, D, BN, kSwap>, dim3(static_cast<unsigned>(ctas)), dim3(kTileThreads),
                                        tile_smem(BN, p.depth, splits_log2 != 0), stream, true, 1u << splits_log2, tm_a, tm_b, p, e);
 }
 
@@ -555,8 +599,8 @@ int launch_pairs(const Operands& o, const Epilogue& e, int num_sms, cudaStream_t
                                        kPairSmem, stream, true, 2u, tm_a, tm_b, p, e);
 }
 
-// D of (rows_a, rows_b) = (e.rows, e.cols).
-template <typename T>
+// The output (rows_a, rows_b), of type D.
+template <typename T, typename D>
 int launch_product(const Operands& o, const Epilogue& e, int num_sms, cudaStream_t stream)
 {
     const uint32_t k_blocks = (o.k + BK - 1) / BK;
@@ -569,28 +613,30 @@ int launch_product(const Operands& o, const Epilogue& e, int num_sms, cudaStream
     if (o.rows_a <= 128 && !o.a_mn && !o.b_mn) {
         const Operands s{o.b, o.ldb, false, o.rows_b, o.a, o.lda, false, o.rows_a, o.k, o.status};
         const uint32_t splits = splits_for((o.rows_b + BM - 1) / BM, 3);
-        if (o.rows_a <= 16) return launch_tiles<T, 16, true>(s, e, splits, num_sms, stream);
-        if (o.rows_a <= 32) return launch_tiles<T, 32, true>(s, e, splits, num_sms, stream);
-        if (o.rows_a <= 64) return launch_tiles<T, 64, true>(s, e, splits, num_sms, stream);
-        return launch_tiles<T, 128, true>(s, e, splits, num_sms, stream);
+        if (o.rows_a <= 16) return launch_tiles<T, D, 16, true>(s, e, splits, num_sms, stream);
+        if (o.rows_a <= 32) return launch_tiles<T, D, 32, true>(s, e, splits, num_sms, stream);
+        if (o.rows_a <= 64) return launch_tiles<T, D, 64, true>(s, e, splits, num_sms, stream);
+        return launch_tiles<T, D, 128, true>(s, e, splits, num_sms, stream);
     }
-    const uint64_t pair_tiles = static_cast<uint64_t>((o.rows_a + 255) / 256) * ((o.rows_b + 255) / 256);
-    if (pair_tiles * 2 >= static_cast<uint64_t>(num_sms / 2) && o.rows_b > 128) return launch_pairs<T>(o, e, num_sms, stream);
+    if constexpr (std::is_same<D, T>::value) {
+        const uint64_t pair_tiles = static_cast<uint64_t>((o.rows_a + 255) / 256) * ((o.rows_b + 255) / 256);
+        if (pair_tiles * 2 >= static_cast<uint64_t>(num_sms / 2) && o.rows_b > 128) return launch_pairs<T>(o, e, num_sms, stream);
+    }
     const uint64_t tiles_128 = static_cast<uint64_t>((o.rows_a + 127) / 128) * ((o.rows_b + 127) / 128);
-    if (o.rows_b <= 64) return launch_tiles<T, 64, false>(o, e, splits_for((o.rows_a + 127) / 128, 1), num_sms, stream);
-    return launch_tiles<T, 128, false>(o, e, splits_for(tiles_128, 2), num_sms, stream);
+    if (o.rows_b <= 64) return launch_tiles<T, D, 64, false>(o, e, splits_for((o.rows_a + 127) / 128, 1), num_sms, stream);
+    return launch_tiles<T, D, 128, false>(o, e, splits_for(tiles_128, 2), num_sms, stream);
 }
 
 // ---- dz and the bias' gradient -----------------------------------------------------------------------------------------
 
 // dz = dd * activation'(z), rounded once for the tensor cores, and per block of rows the sums of its columns before that rounding.
-// A thread takes eight columns (16 bytes of z and dz, whose rows are padded to that) of every eighth row of its block's; a block 256
-// columns.  One pass over dd and z, bound by their bytes.
+// A thread takes eight columns (16 bytes of the slopes and of dz, whose rows are padded to that) of every eighth row of its block's; a
+// block 256 columns.  One pass over dd and the slopes, bound by their bytes.
 constexpr int kGradThreads = 256, kGradColumns = 256, kGradRowLanes = 8;
 template <typename T, typename D>
 __global__ void __launch_bounds__(kGradThreads)
-linear_dz_kernel(const D* __restrict__ dd, int64_t ldd, bool wide, const T* __restrict__ z, int64_t ldz, T* __restrict__ dz, int64_t lddz, uint32_t rows,
-                 uint32_t cols, uint32_t rows_each, int activation, float* __restrict__ sums)
+linear_dz_kernel(const D* __restrict__ dd, int64_t ldd, bool wide, const int16_t* __restrict__ slopes, int64_t lds, T* __restrict__ dz, int64_t lddz, uint32_t rows,
+                 uint32_t cols, uint32_t rows_each, float* __restrict__ sums)
 {
     __shared__ float part[kGradRowLanes][kGradColumns];
     const uint32_t group = threadIdx.x % 32, row_lane = threadIdx.x / 32;
@@ -598,33 +644,31 @@ linear_dz_kernel(const D* __restrict__ dd, int64_t ldd, bool wide, const T* __re
     const uint32_t first = blockIdx.y * rows_each, last = min(rows, first + rows_each);
     ptx::grid_dependency_wait();
     float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    with_activation(activation, [&](auto act) {
-        if (col0 >= cols) return;
+    if (col0 < cols) {
         const uint32_t here = min(8u, cols - col0);
         for (uint32_t r = first + row_lane; r < last; r += kGradRowLanes) {
             const D* from = dd + static_cast<int64_t>(r) * ldd + col0;
             alignas(16) D g[8];
             if (wide) {
 #pragma unroll
-                for (uint32_t i = 0; i < sizeof(g) / 16; ++i) reinterpret_cast<uint4*>(g)[i] = __ldg(reinterpret_cast<const uint4*>(from) + i);
+                for (uint32_t i = 0; i < sizeof(g) / 16; ++i) reinterpret_cast<uint4*>(g)[i] = reinterpret_cast<const uint4*>(from)[i];
             } else {
 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i) g[i] = i < here ? from[i] : from_float<D>(0.0f);
             }
-            alignas(16) T pre[8];
-            if constexpr (decltype(act)::value != NVFP4_ACTIVATION_NONE)
-                *reinterpret_cast<uint4*>(pre) = __ldg(reinterpret_cast<const uint4*>(z + static_cast<int64_t>(r) * ldz + col0));
+            alignas(16) int16_t code[8];
+            if (slopes != nullptr) *reinterpret_cast<uint4*>(code) = *reinterpret_cast<const uint4*>(slopes + static_cast<int64_t>(r) * lds + col0);
             alignas(16) T out[8];
 #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) {
                 float v = to_float(g[i]);
-                if constexpr (decltype(act)::value != NVFP4_ACTIVATION_NONE) v *= slope<decltype(act)::value>(to_float(pre[i]));
+                if (slopes != nullptr) v *= unpack_slope(code[i]);
                 sum[i] += v;
                 out[i] = from_float<T>(v);
             }
             if (dz != nullptr) *reinterpret_cast<uint4*>(dz + static_cast<int64_t>(r) * lddz + col0) = *reinterpret_cast<const uint4*>(out);
         }
-    });
+    }
     if (sums == nullptr) return;
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) part[row_lane][group * 8 + i] = sum[i];
@@ -649,8 +693,8 @@ linear_db_kernel(const float* __restrict__ sums, uint32_t blocks, uint32_t cols,
 }
 
 template <typename T, typename D>
-int launch_dz(const void* dd, int64_t ldd, const void* z, int64_t ldz, void* dz, int64_t lddz, void* db, uint32_t rows, uint32_t cols, int activation,
-              int num_sms, cudaStream_t stream)
+int launch_dz(const void* dd, int64_t ldd, const int16_t* slopes, int64_t lds, void* dz, int64_t lddz, void* db, uint32_t rows, uint32_t cols, int num_sms,
+              cudaStream_t stream)
 {
     const unsigned columns = (cols + kGradColumns - 1) / kGradColumns;
     // about four blocks to an SM, at least eight rows to a block
@@ -668,7 +712,7 @@ int launch_dz(const void* dd, int64_t ldd, const void* z, int64_t ldz, void* dz,
         NVFP4_CUDA_CHECK(cudaMallocFromPoolAsync(reinterpret_cast<void**>(&sums), static_cast<size_t>(blocks) * cols * sizeof(float), pool, stream));
     }
     int rc = host::launch_kernel(linear_dz_kernel<T, D>, dim3(columns, blocks), dim3(kGradThreads), 0, stream, true, static_cast<const D*>(dd), ldd, wide,
-                                 static_cast<const T*>(z), ldz, static_cast<T*>(dz), lddz, rows, cols, rows_each, activation, sums);
+                                 slopes, lds, static_cast<T*>(dz), lddz, rows, cols, rows_each, sums);
     if (db != nullptr) {
         if (rc == NVFP4_OK)
             rc = host::launch_kernel(linear_db_kernel<T>, dim3((cols + kGradThreads - 1) / kGradThreads), dim3(kGradThreads), 0, stream, true, sums,
@@ -680,39 +724,46 @@ int launch_dz(const void* dd, int64_t ldd, const void* z, int64_t ldz, void* dz,
 
 }  // namespace
 
-int launch_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual, int64_t ldr, void* d, int64_t ldd,
-                  void* z, int64_t ldz, int M, int N, int K, bool bf16, bool out32, int activation, int32_t* status, int num_sms, cudaStream_t stream)
+template <typename T>
+static int product(const Operands& o, const Epilogue& e, bool out32, int num_sms, cudaStream_t stream)
 {
-    const Operands o{x, ldx, false, static_cast<uint32_t>(M), w, ldw, false, static_cast<uint32_t>(N), static_cast<uint32_t>(K), status};
-    const Epilogue e{d, ldd, z, ldz, bias, residual, ldr, static_cast<uint32_t>(M), static_cast<uint32_t>(N), activation, out32};
-    return bf16 ? launch_product<__nv_bfloat16>(o, e, num_sms, stream) : launch_product<__half>(o, e, num_sms, stream);
+    return out32 ? launch_product<T, float>(o, e, num_sms, stream) : launch_product<T, T>(o, e, num_sms, stream);
 }
 
-int launch_linear_dz(const void* dd, int64_t ldd, bool dd32, const void* z, int64_t ldz, void* dz, int64_t lddz, void* db, int M, int N, bool bf16,
-                     int activation, int num_sms, cudaStream_t stream)
+int launch_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual, int64_t ldr, void* d, int64_t ldd,
+                  int16_t* slopes, int64_t lds, int M, int N, int K, bool bf16, bool out32, int activation, int32_t* status, int num_sms,
+                  cudaStream_t stream)
+{
+    const Operands o{x, ldx, false, static_cast<uint32_t>(M), w, ldw, false, static_cast<uint32_t>(N), static_cast<uint32_t>(K), status};
+    const Epilogue e{d, ldd, slopes, lds, bias, residual, ldr, static_cast<uint32_t>(M), static_cast<uint32_t>(N), activation};
+    return bf16 ? product<__nv_bfloat16>(o, e, out32, num_sms, stream) : product<__half>(o, e, out32, num_sms, stream);
+}
+
+int launch_linear_dz(const void* dd, int64_t ldd, bool dd32, const int16_t* slopes, int64_t lds, void* dz, int64_t lddz, void* db, int M, int N,
+                     bool bf16, int num_sms, cudaStream_t stream)
 {
     const uint32_t m = static_cast<uint32_t>(M), n = static_cast<uint32_t>(N);
     if (bf16)
-        return dd32 ? launch_dz<__nv_bfloat16, float>(dd, ldd, z, ldz, dz, lddz, db, m, n, activation, num_sms, stream)
-                    : launch_dz<__nv_bfloat16, __nv_bfloat16>(dd, ldd, z, ldz, dz, lddz, db, m, n, activation, num_sms, stream);
-    return dd32 ? launch_dz<__half, float>(dd, ldd, z, ldz, dz, lddz, db, m, n, activation, num_sms, stream)
-                : launch_dz<__half, __half>(dd, ldd, z, ldz, dz, lddz, db, m, n, activation, num_sms, stream);
+        return dd32 ? launch_dz<__nv_bfloat16, float>(dd, ldd, slopes, lds, dz, lddz, db, m, n, num_sms, stream)
+                    : launch_dz<__nv_bfloat16, __nv_bfloat16>(dd, ldd, slopes, lds, dz, lddz, db, m, n, num_sms, stream);
+    return dd32 ? launch_dz<__half, float>(dd, ldd, slopes, lds, dz, lddz, db, m, n, num_sms, stream)
+                : launch_dz<__half, __half>(dd, ldd, slopes, lds, dz, lddz, db, m, n, num_sms, stream);
 }
 
 int launch_linear_dx(const void* dz, int64_t lddz, const void* w, int64_t ldw, void* dx, int64_t lddx, int M, int N, int K, bool bf16, int32_t* status,
                      int num_sms, cudaStream_t stream)
 {
     const Operands o{dz, lddz, false, static_cast<uint32_t>(M), w, ldw, true, static_cast<uint32_t>(K), static_cast<uint32_t>(N), status};
-    const Epilogue e{dx, lddx, nullptr, 0, nullptr, nullptr, 0, static_cast<uint32_t>(M), static_cast<uint32_t>(K), NVFP4_ACTIVATION_NONE, false};
-    return bf16 ? launch_product<__nv_bfloat16>(o, e, num_sms, stream) : launch_product<__half>(o, e, num_sms, stream);
+    const Epilogue e{dx, lddx, nullptr, 0, nullptr, nullptr, 0, static_cast<uint32_t>(M), static_cast<uint32_t>(K), NVFP4_ACTIVATION_NONE};
+    return bf16 ? product<__nv_bfloat16>(o, e, false, num_sms, stream) : product<__half>(o, e, false, num_sms, stream);
 }
 
 int launch_linear_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, void* dw, int64_t lddw, int M, int N, int K, bool bf16, int32_t* status,
                      int num_sms, cudaStream_t stream)
 {
     const Operands o{dz, lddz, true, static_cast<uint32_t>(N), x, ldx, true, static_cast<uint32_t>(K), static_cast<uint32_t>(M), status};
-    const Epilogue e{dw, lddw, nullptr, 0, nullptr, nullptr, 0, static_cast<uint32_t>(N), static_cast<uint32_t>(K), NVFP4_ACTIVATION_NONE, false};
-    return bf16 ? launch_product<__nv_bfloat16>(o, e, num_sms, stream) : launch_product<__half>(o, e, num_sms, stream);
+    const Epilogue e{dw, lddw, nullptr, 0, nullptr, nullptr, 0, static_cast<uint32_t>(N), static_cast<uint32_t>(K), NVFP4_ACTIVATION_NONE};
+    return bf16 ? product<__nv_bfloat16>(o, e, false, num_sms, stream) : product<__half>(o, e, false, num_sms, stream);
 }
 
 }  // namespace nvfp4

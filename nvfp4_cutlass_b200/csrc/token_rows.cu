@@ -192,7 +192,7 @@ sort_one_kernel(const W* __restrict__ x, int64_t ldx, const int64_t* __restrict_
 #pragma unroll
         for (int i = 0; i < kPieceWords; ++i) {
             v[i] = W{};
-            if (live && c0 + i * 32 < row_words) v[i] = __ldg(from + c0 + i * 32);
+            if (live && c0 + i * 32 < row_words) v[i] = from[c0 + i * 32];
         }
 #pragma unroll
         for (int i = 0; i < kPieceWords; ++i)
@@ -282,7 +282,7 @@ sort_move_kernel(const W* __restrict__ x, int64_t ldx, uint32_t tokens, int k, i
             W v[kPieceWords];
 #pragma unroll
             for (int i = 0; i < kPieceWords; ++i)
-                if (c0 + i * 32 < row_words) v[i] = __ldg(from + c0 + i * 32);
+                if (c0 + i * 32 < row_words) v[i] = from[c0 + i * 32];
             for (int j0 = 0; j0 < k; j0 += 32) {
                 const int64_t mine = j0 + static_cast<int>(lane) < k ? place[static_cast<int64_t>(t) * k + j0 + lane] : -1;
                 const int here = min(32, k - j0);
@@ -315,7 +315,8 @@ sort_move_kernel(const W* __restrict__ x, int64_t ldx, uint32_t tokens, int k, i
 
 // ---- back: y[t] = sum_j w[t, j] * rows[place[t, j]] ------------------------------------------------------------------------------------
 
-// kN elements of T as one access
+// kN elements of T as one access.  Loads are plain here as elsewhere in this file: __ldg, an asm statement, may be moved ahead of the test
+// that guards it.
 template <typename T, int kN>
 struct alignas(sizeof(T) * kN) Pack {
     T v[kN];
@@ -324,7 +325,7 @@ template <typename P>
 __device__ __forceinline__ P load_pack(const P* at)
 {
     if constexpr (sizeof(P) == 16) {
-        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(at));
+        const uint4 raw = *reinterpret_cast<const uint4*>(at);
         return *reinterpret_cast<const P*>(&raw);
     } else {
         return *at;

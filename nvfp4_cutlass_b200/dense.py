@@ -19,21 +19,19 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, w, bias, residual, activation, out_dtype, device_status):
         want_x, want_w, want_bias, _ = ctx.needs_input_grad[:4]
         keep = activation != "none" and (want_x or want_w or want_bias)
-        d, z = _C.linear(x, w, bias, residual, activation, out_dtype, keep, device_status)
-        ctx.save_for_backward(x if want_w else None, w if want_x else None, z)
-        ctx.form = (x.dtype, activation)
-        ctx.device_status = device_status
+        d, slopes = _C.linear(x, w, bias, residual, activation, out_dtype, keep, device_status)
+        ctx.save_for_backward(x if want_w else None, w if want_x else None, slopes)
+        ctx.form = (x.dtype, want_bias, device_status)
         return d
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dd):
-        want_x, want_w, want_bias, want_residual = ctx.needs_input_grad[:4]
         dx = dw = db = None
-        if want_x or want_w or want_bias:
+        if any(ctx.needs_input_grad[:3]):
             rows = dd if dd.stride(-1) == 1 and dd.stride(0) >= dd.shape[1] else dd.contiguous()
-            dx, dw, db = _C.linear_backward(rows, *ctx.saved_tensors, *ctx.form, want_x, want_w, want_bias, ctx.device_status)
-        return dx, dw, db, dd if want_residual else None, None, None, None
+            dx, dw, db = _C.linear_backward(rows, *ctx.saved_tensors, *ctx.form)
+        return dx, dw, db, dd if ctx.needs_input_grad[3] else None, None, None, None
 
 
 def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, *,
@@ -45,8 +43,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     ``out_dtype``: the operands' type, or float32.  ``activation``: none, relu, gelu, gelu_tanh or silu.  Sums, bias, activation and residual
     are FP32, rounded once.  ``device_status``: int32 on the device that receives bit 0 should a bounded wait in the kernels expire.
 
-    Differentiable in x, w, bias and residual.  The backward pass keeps x w^T + bias rounded to the operands' type, and rounds the
-    gradient in front of the activation to it: the tensor cores take no wider operands."""
+    Differentiable in x, w, bias and residual.  The backward pass keeps the activation's slope, off by 2^-15 at most, and rounds the
+    gradient in front of the activation to the operands' type: the tensor cores take no wider operands."""
     if not _differentiable(x, w, bias, residual):
         return _C.linear(x, w, bias, residual, activation, out_dtype, device_status=device_status)[0]
     return _Linear.apply(x, w, bias, residual, activation, out_dtype, device_status)

@@ -64,8 +64,8 @@ def error_of(rc):
     return _C.lib().nvfp4_last_error().decode()
 
 
-def call(x=1024, ldx=64, w=1024, ldw=64, bias=None, residual=None, ldr=0, d=1024, ldd=32, z=None, ldz=0, m=4, n=32, k=64, dtype=0, out=0, act=0):
-    return _C.lib().nvfp4_linear(x, ldx, w, ldw, bias, residual, ldr, d, ldd, z, ldz, m, n, k, dtype, out, act, None, None)
+def call(x=1024, ldx=64, w=1024, ldw=64, bias=None, residual=None, ldr=0, d=1024, ldd=32, slopes=None, lds=0, m=4, n=32, k=64, dtype=0, out=0, act=0):
+    return _C.lib().nvfp4_linear(x, ldx, w, ldw, bias, residual, ldr, d, ldd, slopes, lds, m, n, k, dtype, out, act, None, None)
 
 
 @pytest.mark.parametrize("change, text", [
@@ -73,7 +73,7 @@ def call(x=1024, ldx=64, w=1024, ldw=64, bias=None, residual=None, ldr=0, d=1024
     (dict(ldx=68), "multiple of 8"), (dict(ldx=56), "cover the row"), (dict(ldw=60), "multiple of 8"), (dict(k=60), "K must be"), (dict(k=0), "K must be"),
     (dict(m=-1), "negative"), (dict(dtype=1), "BF16 or FP16"), (dict(dtype=3), "BF16 or FP16"), (dict(out=2), "operands' type"), (dict(act=5), "activation"),
     (dict(act=-1), "activation"), (dict(ldd=31), "smaller than the row"), (dict(residual=1024, ldr=8), "smaller than the row"), (dict(d=1025), "aligned"),
-    (dict(bias=1025), "aligned"), (dict(out=1, d=1026), "aligned"), (dict(z=1024, ldz=31), "smaller than the row")])
+    (dict(bias=1025), "aligned"), (dict(out=1, d=1026), "aligned"), (dict(slopes=1024, lds=31), "smaller than the row")])
 def test_products_refuse(change, text):
     assert text in error_of(call(**change))
 
@@ -85,10 +85,10 @@ def test_gradients_refuse():
     assert "empty contraction" in error_of(lib.nvfp4_linear_dx(1024, 32, 1024, 64, 1024, 64, 4, 0, 64, 0, None, None))
     assert "empty contraction" in error_of(lib.nvfp4_linear_dw(1024, 32, 1024, 64, 1024, 64, 0, 32, 64, 0, None, None))
     assert "rows overlap" in error_of(lib.nvfp4_linear_dw(1024, 32, 1024, 64, 1024, 56, 4, 32, 64, 0, None, None))
-    assert "z" in error_of(lib.nvfp4_linear_dz(1024, 32, None, 32, 1024, 32, None, 4, 32, 0, 0, 4, None))
-    assert "stride of dz" in error_of(lib.nvfp4_linear_dz(1024, 33, 1024, 40, 1024, 32, None, 4, 33, 0, 0, 4, None))
-    assert "operands' type" in error_of(lib.nvfp4_linear_dz(1024, 32, 1024, 32, 1024, 32, None, 4, 32, 0, 2, 4, None))
-    assert lib.nvfp4_linear_dz(1024, 32, 1024, 32, None, 32, None, 4, 32, 0, 0, 4, None) == 0
+    assert "stride of slopes" in error_of(lib.nvfp4_linear_dz(1024, 33, 1024, 32, 1024, 40, None, 4, 33, 0, 0, None))
+    assert "stride of dz" in error_of(lib.nvfp4_linear_dz(1024, 33, 1024, 40, 1024, 32, None, 4, 33, 0, 0, None))
+    assert "operands' type" in error_of(lib.nvfp4_linear_dz(1024, 32, 1024, 32, 1024, 32, None, 4, 32, 0, 2, None))
+    assert lib.nvfp4_linear_dz(1024, 32, 1024, 32, None, 32, None, 4, 32, 0, 0, None) == 0
 
 
 def test_empty_products_are_nothing():
@@ -194,14 +194,15 @@ def test_gradients_against_the_formulas(m, n, k, activation):
         z = (x.double() @ w.double().t() + bias.double()).requires_grad_()
         (dz,) = torch.autograd.grad(act64(z, activation), z, dd.double())
         z = z.detach()
-        # z is kept rounded: half a step of it times the curvature; a sign that the forward sum's error can flip costs relu the whole slope
-        z_error = sum_error(x, w.t()) + z.abs() * (HALF_STEP[dtype] * 1.01 + 2.0 ** -23) + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+        # the slope is kept in steps of 2^-14; it is taken at the z that the forward sum gave, curvature times that sum's error away, and
+        # costs some 16 roundings itself; a sign that the sum's error can flip costs relu the whole slope
+        z_error = sum_error(x, w.t()) + z.abs() * 2.0 ** -23
         if activation == "none":
             dz_error = torch.zeros_like(z)
         elif activation == "relu":
-            dz_error = torch.where(z.abs() <= sum_error(x, w.t()) + z.abs() * 2.0 ** -23 + (2.0 ** -24 if dtype == torch.float16 else 0.0), dd.double().abs(), 0.0)
+            dz_error = torch.where(z.abs() <= z_error, dd.double().abs(), 0.0)
         else:
-            dz_error = dd.double().abs() * (CURVATURE * z_error + 16 * 2.0 ** -23)
+            dz_error = dd.double().abs() * (2.0 ** -15 + CURVATURE * z_error + 16 * 2.0 ** -23)
         tiny = 2.0 ** -25 if dtype == torch.float16 else 1e-40
         db_error = dz_error.sum(dim=0) + dz.abs().sum(dim=0) * (m + 4) * 2.0 ** -24
         assert (db.cpu().double() - dz.sum(dim=0)).abs().le(db_error + (dz.sum(dim=0).abs() + db_error) * 1.01 * HALF_STEP[dtype] + tiny).all()
@@ -234,7 +235,7 @@ def test_gradients_against_differences():
                     args[which].view(-1)[at] += sign
                     moved.append(f(*args))
                 slope = (moved[0] - moved[1]) / (2 * h)
-                # z and dz rounded to FP16 (2^-11 each, values of a few) in sums of up to 16 terms, the result rounded once
+                # dz rounded to FP16 (2^-11, values of a few) in sums of up to 16 terms, the result rounded once
                 assert abs(slope - float(grad.reshape(-1)[at])) < 16 * 4 * 2 * 2.0 ** -11
 
 
