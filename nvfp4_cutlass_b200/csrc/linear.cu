@@ -44,28 +44,59 @@ template <> __device__ __forceinline__ __half from_float<__half>(float v) { retu
 // ---- activations -----------------------------------------------------------------------------------------------------
 // gelu(z) = z Phi(z); its tanh form 0.5 z (1 + tanh u), u = c (z + 0.044715 z^3), is z sigmoid(2 u) as silu is z sigmoid(z): none of
 // them loses the digits of small values to a sum near zero.
+// kExact, for FP32 outputs: CUDA's full-precision functions.  For 16-bit outputs the epilogue would be bound by them (an IEEE division alone
+// takes more instructions than the rest; 16384 x 1024 x 1024 with silu took 86 us, 37 without): hardware exponential and
+// reciprocal, off by 2^-21 or so of the value, and erfc by the rational Chebyshev fit of Press et al., Numerical Recipes,
+// 6.2, off by 1.2e-7 of its value everywhere.
 constexpr float kGeluC = 0.7978845608028654f;        // sqrt(2 / pi)
-template <int kAct>
-__device__ __forceinline__ float activate(float z)
+template <bool kExact> __device__ __forceinline__ float exponential(float x) { return kExact ? expf(x) : __expf(x); }
+template <bool kExact> __device__ __forceinline__ float reciprocal(float x) { return kExact ? 1.0f / x : __fdividef(1.0f, x); }
+template <bool kExact>
+__device__ __forceinline__ float normal_cdf(float z)
 {
-    if constexpr (kAct == NVFP4_ACTIVATION_RELU) return z > 0.0f || z != z ? z : 0.0f;
-    else if constexpr (kAct == NVFP4_ACTIVATION_GELU) return z * normcdff(z);
-    else if constexpr (kAct == NVFP4_ACTIVATION_GELU_TANH) return z / (1.0f + expf(-2.0f * kGeluC * z * fmaf(0.044715f * z, z, 1.0f)));
-    else if constexpr (kAct == NVFP4_ACTIVATION_SILU) return z / (1.0f + expf(-z));
-    else return z;
+    if constexpr (kExact) return normcdff(z);
+    const float x = fabsf(z) * 0.7071067811865476f, t = reciprocal<false>(fmaf(0.5f, x, 1.0f));
+    float p = 0.17087277f;
+    p = fmaf(p, t, -0.82215223f);
+    p = fmaf(p, t, 1.48851587f);
+    p = fmaf(p, t, -1.13520398f);
+    p = fmaf(p, t, 0.27886807f);
+    p = fmaf(p, t, -0.18628806f);
+    p = fmaf(p, t, 0.09678418f);
+    p = fmaf(p, t, 0.37409196f);
+    p = fmaf(p, t, 1.00002368f);
+    p = fmaf(p, t, -1.26551223f);
+    const float half_erfc = 0.5f * t * exponential<false>(fmaf(-x, x, p));
+    return z < 0.0f ? half_erfc : 1.0f - half_erfc;
 }
-template <int kAct>
-__device__ __forceinline__ float slope(float z)
+// y = activation(z) and, with kSlope, its derivative there.
+template <int kAct, bool kExact, bool kSlope>
+__device__ __forceinline__ void activate(float z, float& y, float& slope)
 {
-    if constexpr (kAct == NVFP4_ACTIVATION_NONE) return 1.0f;
-    if (z != z) return z;
-    if constexpr (kAct == NVFP4_ACTIVATION_RELU) return z > 0.0f ? 1.0f : 0.0f;
-    z = fminf(fmaxf(z, -40.0f), 40.0f);              // constant to FP32 beyond: no infinity times zero
-    if constexpr (kAct == NVFP4_ACTIVATION_GELU) return fmaf(z, 0.3989422804014327f * expf(-0.5f * z * z), normcdff(z));
-    const float u2 = kAct == NVFP4_ACTIVATION_SILU ? z : 2.0f * kGeluC * z * fmaf(0.044715f * z, z, 1.0f);
-    const float du2 = kAct == NVFP4_ACTIVATION_SILU ? 1.0f : 2.0f * kGeluC * fmaf(3.0f * 0.044715f * z, z, 1.0f);
-    const float e = expf(-fabsf(u2)), near = 1.0f / (1.0f + e), far = e * near;           // of sigmoid(u2) and 1 - sigmoid(u2) the larger, the smaller
-    return fmaf(z * du2, near * far, u2 >= 0.0f ? near : far);
+    if constexpr (kAct == NVFP4_ACTIVATION_RELU) {
+        y = z > 0.0f || z != z ? z : 0.0f;
+        slope = z > 0.0f ? 1.0f : z != z ? z : 0.0f;
+    } else if constexpr (kAct == NVFP4_ACTIVATION_NONE) {
+        y = z;
+        slope = 1.0f;
+    } else {
+        const float bounded = fminf(fmaxf(z, -40.0f), 40.0f);                 // beyond, the slope is constant: no infinity times zero
+        if constexpr (kAct == NVFP4_ACTIVATION_GELU) {
+            const float cdf = normal_cdf<kExact>(z);
+            y = z * cdf;
+            if constexpr (kSlope) slope = fmaf(bounded, 0.3989422804014327f * exponential<kExact>(-0.5f * bounded * bounded), cdf);
+        } else {
+            constexpr bool kSilu = kAct == NVFP4_ACTIVATION_SILU;
+            const float u2 = kSilu ? z : 2.0f * kGeluC * z * fmaf(0.044715f * z, z, 1.0f);
+            const float e = exponential<kExact>(-fabsf(u2)), near = reciprocal<kExact>(1.0f + e), far = e * near;
+            const float sigmoid = u2 >= 0.0f ? near : far;                    // the larger of sigmoid(u2) and 1 - sigmoid(u2), or the smaller
+            y = z * sigmoid;
+            if constexpr (kSlope) {
+                const float du2 = kSilu ? 1.0f : 2.0f * kGeluC * fmaf(3.0f * 0.044715f * bounded, bounded, 1.0f);
+                slope = fmaf(bounded * du2, near * far, sigmoid);
+            }
+        }
+    }
 }
 // For the backward pass a slope, all of which lie in (-0.2, 1.2), is kept as a multiple of 2^-14 in 16 bits: off by 2^-15 at most, less
 // than the rounding of the gradient that it multiplies, where z kept in BF16 would cost as much as that rounding again.
@@ -95,6 +126,7 @@ struct Epilogue {
     const void* residual; int64_t ldr;               // of d's type, or NULL
     uint32_t rows, cols;
     int activation;
+    bool staged;                                     // rows of d, residual and slopes are multiples of 16 bytes: see Stage
 };
 
 // Up to kN accumulators of a lane: output column `col`, rows row0 + i, i < count.  The lanes of a warp hold neighbouring columns, so that
@@ -122,14 +154,19 @@ __device__ __forceinline__ void finish(float (&v)[kN], uint32_t row0, uint32_t c
     if (e.activation != NVFP4_ACTIVATION_NONE)
         with_activation(e.activation, [&](auto act) {
             constexpr int kAct = decltype(act)::value;
+            constexpr bool kExact = std::is_same<D, float>::value;
+            float slope;
             if (e.slopes != nullptr) {
                 int16_t* to = e.slopes + static_cast<int64_t>(row0) * e.lds + at;
 #pragma unroll
-                for (uint32_t i = 0; i < kN; ++i)
-                    if (i < rows && mine) to[i * e.lds] = pack_slope(slope<kAct>(v[i]));
-            }
+                for (uint32_t i = 0; i < kN; ++i) {
+                    activate<kAct, kExact, true>(v[i], v[i], slope);
+                    if (i < rows && mine) to[i * e.lds] = pack_slope(slope);
+                }
+            } else {
 #pragma unroll
-            for (uint32_t i = 0; i < kN; ++i) v[i] = activate<kAct>(v[i]);
+                for (uint32_t i = 0; i < kN; ++i) activate<kAct, kExact, false>(v[i], v[i], slope);
+            }
         });
     if (e.residual != nullptr) {
 #pragma unroll
@@ -157,6 +194,25 @@ __device__ __forceinline__ void transpose(float (&v)[32], uint32_t lane)
     }
 }
 
+template <typename T> struct Pair2;
+template <> struct Pair2<__nv_bfloat16> { using type = __nv_bfloat162; };
+template <> struct Pair2<__half> { using type = __half2; };
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w)
+{
+    const typename Pair2<T>::type h = *reinterpret_cast<const typename Pair2<T>::type*>(&w);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) return __bfloat1622float2(h);
+    else return __half22float2(h);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b)
+{
+    typename Pair2<T>::type h;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) h = __floats2bfloat162_rn(a, b);
+    else h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 template <uint32_t kN>
 __device__ __forceinline__ void load_accumulators(uint32_t taddr, float (&v)[kN])
 {
@@ -167,6 +223,128 @@ __device__ __forceinline__ void load_accumulators(uint32_t taddr, float (&v)[kN]
 #pragma unroll
     for (uint32_t i = 0; i < kN; ++i) v[i] = __uint_as_float(raw[i]);
 }
+
+// An epilogue warp's way out through shared memory, where TMA can address the output: 32 rows x 64 columns at a time, a row (128 bytes,
+// 128-byte swizzle) to a lane as tensor memory gives them, so that nothing has to be transposed and every line of the output is
+// written whole.  The residual comes into the same buffer by TMA beforehand and is replaced by the result in place.
+constexpr uint32_t kBox = 64, kBoxBytes = 32 * kBox * 2;
+struct Maps {
+    CUtensorMap d, residual, slopes;                 // boxes of 32 rows x 64 columns
+};
+template <typename T>
+struct Stage {
+    uint32_t out, out_step, slopes, slopes_step;     // shared memory: buffers of the output (and residual) and of the slopes, of box 0 and from there to box 1's
+    uint64_t* landed;                                // [2] residual of a box is there
+    uint32_t phase = 0;
+    const Maps* maps;
+
+    // Everything that the warp has given to TMA has been read: the buffers may be written.
+    __device__ __forceinline__ void reclaim(uint32_t lane) const
+    {
+        if (lane == 0) ptx::bulk_wait_read();
+        __syncwarp();
+    }
+    __device__ __forceinline__ void request(uint32_t box, uint32_t col, uint32_t row0, uint32_t lane) const
+    {
+        if (lane == 0) {
+            ptx::mbar_arrive_expect_tx(landed + box, kBoxBytes);
+            tma_load(out + box * out_step, &maps->residual, landed + box, col, row0);
+        }
+    }
+    static __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int32_t c0, int32_t c1)
+    {
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(ptx::smem_u32(bar)), "r"(c0), "r"(c1)
+                     : "memory");
+    }
+    // Bias of the columns [col, col + 32), two to a word: the same for every lane
+    static __device__ __forceinline__ void load_bias(const Epilogue& e, uint32_t col, uint32_t (&b)[16])
+    {
+        const T* from = static_cast<const T*>(e.bias) + col;
+        if (col + 32 <= e.cols && (reinterpret_cast<uintptr_t>(from) & 15u) == 0) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint4 q = reinterpret_cast<const uint4*>(from)[i];
+                b[4 * i] = q.x; b[4 * i + 1] = q.y; b[4 * i + 2] = q.z; b[4 * i + 3] = q.w;
+            }
+        } else {
+            const uint16_t* bits = reinterpret_cast<const uint16_t*>(e.bias);
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i)
+                b[i] = bits[min(col + 2 * i, e.cols - 1)] | static_cast<uint32_t>(bits[min(col + 2 * i + 1, e.cols - 1)]) << 16;
+        }
+    }
+    // One box: accumulators at taddr, columns [col, col + 64).  False: the residual never came.
+    __device__ __forceinline__ bool finish(uint32_t taddr, uint32_t box, uint32_t col, uint32_t row0, uint32_t lane, const Epilogue& e,
+                                           volatile uint32_t* abort_flag)
+    {
+        if (e.residual != nullptr) {
+            if (!ptx::all_lanes(ptx::mbar_wait_impl(landed + box, phase >> box & 1u, abort_flag))) return false;
+            phase ^= 1u << box;
+        }
+#pragma unroll
+        for (uint32_t half = 0; half < 2; ++half) {
+            float v[32];
+            uint32_t b[16];
+            if (e.bias != nullptr) load_bias(e, col + half * 32, b);
+            load_accumulators(taddr + half * 32, v);
+            if (e.bias != nullptr) {
+#pragma unroll
+                for (uint32_t i = 0; i < 16; ++i) {
+                    const float2 f = unpack2<T>(b[i]);
+                    v[2 * i] += f.x;
+                    v[2 * i + 1] += f.y;
+                }
+            }
+            auto piece = [&](uint32_t buffer, uint32_t q) { return buffer + lane * 128 + (((half * 4 + q) ^ (lane & 7u)) << 4); };
+            if (e.activation != NVFP4_ACTIVATION_NONE)
+                with_activation(e.activation, [&](auto act) {
+                    constexpr int kAct = decltype(act)::value;
+                    float slope[2];
+                    if (e.slopes != nullptr) {
+#pragma unroll
+                        for (uint32_t q = 0; q < 4; ++q) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (uint32_t i = 0; i < 4; ++i) {
+#pragma unroll
+                                for (uint32_t j = 0; j < 2; ++j) activate<kAct, false, true>(v[8 * q + 2 * i + j], v[8 * q + 2 * i + j], slope[j]);
+                                w[i] = static_cast<uint16_t>(pack_slope(slope[0])) | static_cast<uint32_t>(static_cast<uint16_t>(pack_slope(slope[1]))) << 16;
+                            }
+                            ptx::sts128(piece(slopes + box * slopes_step, q), w[0], w[1], w[2], w[3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; ++i) activate<kAct, false, false>(v[i], v[i], slope[0]);
+                    }
+                });
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q) {
+                const uint32_t to = piece(out + box * out_step, q);
+                if (e.residual != nullptr) {
+                    const uint4 r = ptx::lds128(to);
+                    const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        const float2 f = unpack2<T>(rw[i]);
+                        v[8 * q + 2 * i] += f.x;
+                        v[8 * q + 2 * i + 1] += f.y;
+                    }
+                }
+                ptx::sts128(to, pack2<T>(v[8 * q], v[8 * q + 1]), pack2<T>(v[8 * q + 2], v[8 * q + 3]), pack2<T>(v[8 * q + 4], v[8 * q + 5]),
+                            pack2<T>(v[8 * q + 6], v[8 * q + 7]));
+            }
+        }
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            ptx::tma_store_2d(&maps->d, out + box * out_step, col, row0);
+            if (e.slopes != nullptr) ptx::tma_store_2d(&maps->slopes, slopes + box * slopes_step, col, row0);
+            ptx::bulk_commit();
+        }
+        return true;
+    }
+};
 
 // ---- operands --------------------------------------------------------------------------------------------------------
 
@@ -203,7 +381,7 @@ constexpr uint32_t kTileEpiWarps = 4;
 constexpr uint32_t tile_stage(uint32_t bn) { return kSlotA + bn * kRowBytes; }
 constexpr uint32_t tile_smem(uint32_t bn, uint32_t depth, bool split)
 {
-    return 1024 + depth * tile_stage(bn) + (split ? bn * BM * 4 : 0) + (2 * kMaxDepth + 4) * 8 + 16;
+    return 1024 + depth * tile_stage(bn) + (split ? bn * BM * 4 : 0) + (2 * kMaxDepth + 4) * 8 + 16 + kTileEpiWarps * 16;
 }
 // For an FP32 output the epilogue warps take the accumulators over every four K blocks and add them up in registers, two accumulators in
 // turn: the tensor core cuts what it adds to a long sum (K = 4096 in one accumulator: off by 4.3e-6 of the result, FP32 sums by 6e-7).
@@ -213,7 +391,8 @@ constexpr uint32_t kChunkBlocks = 4;
 // transposed first.  D: type of the output.
 template <typename T, typename D, uint32_t BN, bool kSwap>
 __global__ void __launch_bounds__(kTileThreads, std::is_same<D, float>::value && BN > 64 ? 1 : 2)
-product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Product p, const Epilogue e)
+product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ Maps maps, const Product p,
+               const Epilogue e)
 {
     constexpr bool kWide = std::is_same<D, float>::value;
     constexpr uint32_t kChunk = BN < 32 ? BN : 32, kStage = tile_stage(BN), kCols = (kWide ? 2 : 1) * BN < 32 ? 32 : (kWide ? 2 : 1) * BN;
@@ -226,7 +405,8 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     uint64_t* drained = full + kMaxDepth;
     uint64_t* tmem_full = drained + kMaxDepth;       // per accumulator
     uint64_t* tmem_empty = tmem_full + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
+    uint64_t* landed = tmem_empty + 2;               // [epilogue warp][2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(landed + 2 * kTileEpiWarps);
     volatile uint32_t* abort_flag = tmem_slot + 1;
 
     const uint32_t warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -234,6 +414,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < depth; ++i) { ptx::mbar_init(full + i, 1); ptx::mbar_init(drained + i, 1); }
         for (uint32_t i = 0; i < 2; ++i) { ptx::mbar_init(tmem_full + i, 1); ptx::mbar_init(tmem_empty + i, kTileEpiWarps); }
+        for (uint32_t i = 0; i < 2 * kTileEpiWarps; ++i) ptx::mbar_init(landed + i, 1);
         *abort_flag = 0;
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&tm_a);
@@ -378,6 +559,20 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                 give(v, first, kSwap ? count : 32);
             }
         }
+    } else if (warp >= 2 && ok && e.staged) {
+        // the ring is at rest (the accumulators are complete): its memory takes the boxes, out and slopes of two for every warp
+        if constexpr (!kSwap && !kWide) {
+            const uint32_t at = smem + (warp - 2) * 4 * kBoxBytes, row0 = a0 + quad * 32;
+            Stage<T> stage{at, kBoxBytes, at + 2 * kBoxBytes, kBoxBytes, landed + 2 * (warp - 2), 0, &maps};
+            if (row0 < e.rows) {
+                if (e.residual != nullptr)
+                    for (uint32_t c = 0; c < live; c += kBox) stage.request(c / kBox, b0 + c, row0, lane);
+#pragma unroll 1
+                for (uint32_t c = 0; c < live; c += kBox)
+                    if (!stage.finish(taddr + c, c / kBox, b0 + c, row0, lane, e, abort_flag)) { give_up(); break; }
+                if (lane == 0) ptx::bulk_wait();
+            }
+        }
     } else if (warp >= 2 && ok) {
 #pragma unroll
         for (uint32_t c0 = 0; c0 < BN; c0 += kChunk) {
@@ -397,22 +592,28 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
 
 // ---- persistent CTA pairs ----------------------------------------------------------------------------------------------
 
-constexpr int kPairThreads = 384;                    // warp 0: TMA, warp 1: products (even CTA), warps 4-11: epilogue
-constexpr uint32_t kPairDepth = 6, kPairStage = 2 * kSlotA, kPairBN = 256, kPairEpiWarps = 8;
-constexpr uint32_t kPairSmem = 1024 + kPairDepth * kPairStage + (2 * kPairDepth + 4) * 8 + 16;
+constexpr int kPairThreads = 320;                    // warp 0: TMA, warp 1: products (even CTA), warps 2-9: epilogue
+constexpr uint32_t kPairFirstEpi = 2;
+constexpr uint32_t kPairDepth = 5, kPairStage = 2 * kSlotA, kPairBN = 256, kPairEpiWarps = 8;
+// behind the ring: two boxes for every epilogue warp (of the output, or of the output and the slopes), barriers
+constexpr uint32_t kPairSmem = 1024 + kPairDepth * kPairStage + kPairEpiWarps * 2 * kBoxBytes + (2 * kPairDepth + 4 + 2 * kPairEpiWarps) * 8 + 16;
+static_assert(kPairSmem <= 232448, "shared memory of an SM");
 
 template <typename T>
 __global__ void __launch_bounds__(kPairThreads, 1)
-product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Product p, const Epilogue e)
+product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ Maps maps,
+                    const Product p, const Epilogue e)
 {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (smem - ptx::smem_u32(smem_raw));
-    uint64_t* full = reinterpret_cast<uint64_t*>(gen + kPairDepth * kPairStage);       // even CTA: both CTAs' operands have landed
+    constexpr uint32_t kOffBoxes = kPairDepth * kPairStage;
+    uint64_t* full = reinterpret_cast<uint64_t*>(gen + kOffBoxes + kPairEpiWarps * 2 * kBoxBytes);       // even CTA: both CTAs' operands have landed
     uint64_t* drained = full + kPairDepth;           // each CTA: the products that read a ring position are done
     uint64_t* tmem_full = drained + kPairDepth;      // each CTA, per accumulator: complete
     uint64_t* tmem_empty = tmem_full + 2;            // even CTA, per accumulator: read by the epilogue warps of both
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
+    uint64_t* landed = tmem_empty + 2;               // [epilogue warp][2] residual of a box
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(landed + 2 * kPairEpiWarps);
     volatile uint32_t* abort_flag = tmem_slot + 1;
 
     const uint32_t warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -420,6 +621,7 @@ product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kPairDepth; ++i) { ptx::mbar_init(full + i, 1); ptx::mbar_init(drained + i, 1); }
         for (uint32_t i = 0; i < 2; ++i) { ptx::mbar_init(tmem_full + i, 1); ptx::mbar_init(tmem_empty + i, 2 * kPairEpiWarps); }
+        for (uint32_t i = 0; i < 2 * kPairEpiWarps; ++i) ptx::mbar_init(landed + i, 1);
         *abort_flag = 0;
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&tm_a);
@@ -485,33 +687,53 @@ product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                 if (ok) ptx::tcgen05_commit_pair(tmem_full + acc, kBoth, issue);
             }
         }
-    } else if (warp >= 4) {
-        const uint32_t quad = warp & 3, half = (warp - 4) >> 2;               // its lanes; columns [128 half, 128 half + 128) of the tile
+    } else {
+        const uint32_t quad = warp & 3, half = (warp - kPairFirstEpi) >> 2;   // its lanes; columns [128 half, 128 half + 128) of the tile
         const uint32_t tmem_empty_even = ptx::map_to_cta(ptx::smem_u32(tmem_empty), 0);
+        const uint32_t boxes = smem + kOffBoxes + (warp - kPairFirstEpi) * 2 * kBoxBytes;
+        const bool both = e.slopes != nullptr;       // the second buffer takes the slopes
+        Stage<T> stage{boxes, both ? 0u : kBoxBytes, boxes + kBoxBytes, 0u, landed + 2 * (warp - kPairFirstEpi), 0, &maps};
         uint32_t n = 0;
         for (uint32_t tile = pair_id; ok && tile < tiles; tile += num_pairs, ++n) {
             const uint32_t acc = n & 1;
             uint32_t a_blk, b_blk;
             gemm::tile_coords(tile, p.tiles_a, p.tiles_b, 8, a_blk, b_blk);
             const uint32_t row0 = (a_blk * 2 + rank) * BM + quad * 32, col0 = b_blk * kPairBN + half * 128;
+            const bool wanted = row0 < e.rows && col0 < e.cols, second = col0 + kBox < e.cols;
+            if (e.staged && wanted) {
+                stage.reclaim(lane);
+                if (e.residual != nullptr) {
+                    stage.request(0, col0, row0, lane);
+                    if (second && !both) stage.request(1, col0 + kBox, row0, lane);
+                }
+            }
             if (!ptx::all_lanes(ptx::mbar_wait_relaxed(tmem_full + acc, (n >> 1) & 1, abort_flag, 50))) { give_up(); break; }
             ptx::tcgen05_fence_after_sync();
             const uint32_t taddr = tmem + ((quad * 32) << 16) + acc * kPairBN + half * 128;
+            if (e.staged) {
 #pragma unroll 1
-            for (uint32_t c = 0; c < 128; c += 32) {
-                float v[32];
-                load_accumulators(taddr + c, v);
-                if (c == 96) {                                               // everything of this warp's is in registers
-                    ptx::tcgen05_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive_remote(tmem_empty_even + acc * 8);
+                for (uint32_t box = 0; wanted && ok && box < (second ? 2u : 1u); ++box) {
+                    if (box == 1 && both) {
+                        stage.reclaim(lane);
+                        if (e.residual != nullptr) stage.request(1, col0 + kBox, row0, lane);
+                    }
+                    if (!stage.finish(taddr + box * kBox, box, col0 + box * kBox, row0, lane, e, abort_flag)) give_up();
                 }
-                if (row0 < e.rows && col0 + c < e.cols) {
+            } else if (wanted) {
+#pragma unroll 1
+                for (uint32_t c = 0; c < 128; c += 32) {
+                    if (col0 + c >= e.cols) break;
+                    float v[32];
+                    load_accumulators(taddr + c, v);
                     transpose(v, lane);
                     finish<T, T>(v, row0, 32, col0 + c + lane, e);
                 }
             }
+            ptx::tcgen05_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_remote(tmem_empty_even + acc * 8);
         }
+        if (lane == 0) ptx::bulk_wait();
     }
     // neither CTA leaves, or gives up its tensor memory, while the other can still signal it or read its operands
     ptx::tcgen05_fence_before_sync();
@@ -535,6 +757,25 @@ int operand_map(CUtensorMap* map, const void* base, int64_t ld, bool mn_major, u
                                       mn_major ? 64 : tile, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Maps of what the epilogue moves by TMA, if it can; T has 16 bits, as the slopes have.
+template <typename T>
+int output_maps(Maps* maps, Epilogue* e)
+{
+    auto aligned = [](const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0; };
+    *maps = Maps{};
+    e->staged = aligned(e->d, e->ldd) && (e->residual == nullptr || aligned(e->residual, e->ldr)) && (e->slopes == nullptr || aligned(e->slopes, e->lds));
+    if (!e->staged) return NVFP4_OK;
+    auto map = [&](CUtensorMap* m, CUtensorMapDataType type, const void* base, int64_t ld) {
+        return host::encode_tensor_map_2d(m, type, 2, base, e->cols, e->rows, static_cast<uint64_t>(ld) * 2, kBox, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    if (int rc = map(&maps->d, kMapType<T>, e->d, e->ldd)) return rc;
+    if (e->residual != nullptr)
+        if (int rc = map(&maps->residual, kMapType<T>, e->residual, e->ldr)) return rc;
+    if (e->slopes != nullptr)
+        if (int rc = map(&maps->slopes, CU_TENSOR_MAP_DATA_TYPE_UINT16, e->slopes, e->lds)) return rc;
+    return NVFP4_OK;
+}
+
 struct Operands {
     const void* a; int64_t lda; bool a_mn; uint32_t rows_a;
     const void* b; int64_t ldb; bool b_mn; uint32_t rows_b;
@@ -543,9 +784,13 @@ struct Operands {
 };
 
 template <typename T, typename D, uint32_t BN, bool kSwap>
-int launch_tiles(const Operands& o, const Epilogue& e, uint32_t splits_log2, int num_sms, cudaStream_t stream)
+int launch_tiles(const Operands& o, Epilogue e, uint32_t splits_log2, int num_sms, cudaStream_t stream)
 {
     CUtensorMap tm_a, tm_b;
+    Maps maps{};
+    if constexpr (!kSwap && std::is_same<D, T>::value)
+        if (splits_log2 == 0)
+            if (int rc = output_maps<T>(&maps, &e)) return rc;
     if (int rc = operand_map<T>(&tm_a, o.a, o.lda, o.a_mn, o.rows_a, o.k, BM)) return rc;
     if (int rc = operand_map<T>(&tm_b, o.b, o.ldb, o.b_mn, o.rows_b, o.k, BN)) return rc;
     Product p{};
@@ -570,13 +815,15 @@ int launch_tiles(const Operands& o, const Epilogue& e, uint32_t splits_log2, int
     }
     NVFP4_REQUIRE(ctas <= INT32_MAX, "too many tiles (%llu)", static_cast<unsigned long long>(ctas));
     return host::launch_kernel_cluster(product_kernel<T, D, BN, kSwap>, dim3(static_cast<unsigned>(ctas)), dim3(kTileThreads),
-                                       tile_smem(BN, p.depth, splits_log2 != 0), stream, true, 1u << splits_log2, tm_a, tm_b, p, e);
+                                       tile_smem(BN, p.depth, splits_log2 != 0), stream, true, 1u << splits_log2, tm_a, tm_b, maps, p, e);
 }
 
 template <typename T>
-int launch_pairs(const Operands& o, const Epilogue& e, int num_sms, cudaStream_t stream)
+int launch_pairs(const Operands& o, Epilogue e, int num_sms, cudaStream_t stream)
 {
     CUtensorMap tm_a, tm_b;
+    Maps maps;
+    if (int rc = output_maps<T>(&maps, &e)) return rc;
     if (int rc = operand_map<T>(&tm_a, o.a, o.lda, o.a_mn, o.rows_a, o.k, BM)) return rc;
     if (int rc = operand_map<T>(&tm_b, o.b, o.ldb, o.b_mn, o.rows_b, o.k, BM)) return rc;
     Product p{};
@@ -596,7 +843,7 @@ int launch_pairs(const Operands& o, const Epilogue& e, int num_sms, cudaStream_t
     const uint64_t tiles = static_cast<uint64_t>(p.tiles_a) * p.tiles_b, pairs = static_cast<uint64_t>(num_sms / 2);
     NVFP4_REQUIRE(tiles <= INT32_MAX, "too many tiles (%llu)", static_cast<unsigned long long>(tiles));
     return host::launch_kernel_cluster(product_pair_kernel<T>, dim3(static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs))), dim3(kPairThreads),
-                                       kPairSmem, stream, true, 2u, tm_a, tm_b, p, e);
+                                       kPairSmem, stream, true, 2u, tm_a, tm_b, maps, p, e);
 }
 
 // The output (rows_a, rows_b), of type D.
@@ -735,7 +982,7 @@ int launch_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const 
                   cudaStream_t stream)
 {
     const Operands o{x, ldx, false, static_cast<uint32_t>(M), w, ldw, false, static_cast<uint32_t>(N), static_cast<uint32_t>(K), status};
-    const Epilogue e{d, ldd, slopes, lds, bias, residual, ldr, static_cast<uint32_t>(M), static_cast<uint32_t>(N), activation};
+    const Epilogue e{d, ldd, slopes, lds, bias, residual, ldr, static_cast<uint32_t>(M), static_cast<uint32_t>(N), activation, false};
     return bf16 ? product<__nv_bfloat16>(o, e, out32, num_sms, stream) : product<__half>(o, e, out32, num_sms, stream);
 }
 
@@ -754,7 +1001,7 @@ int launch_linear_dx(const void* dz, int64_t lddz, const void* w, int64_t ldw, v
                      int num_sms, cudaStream_t stream)
 {
     const Operands o{dz, lddz, false, static_cast<uint32_t>(M), w, ldw, true, static_cast<uint32_t>(K), static_cast<uint32_t>(N), status};
-    const Epilogue e{dx, lddx, nullptr, 0, nullptr, nullptr, 0, static_cast<uint32_t>(M), static_cast<uint32_t>(K), NVFP4_ACTIVATION_NONE};
+    const Epilogue e{dx, lddx, nullptr, 0, nullptr, nullptr, 0, static_cast<uint32_t>(M), static_cast<uint32_t>(K), NVFP4_ACTIVATION_NONE, false};
     return bf16 ? product<__nv_bfloat16>(o, e, false, num_sms, stream) : product<__half>(o, e, false, num_sms, stream);
 }
 
@@ -762,7 +1009,7 @@ int launch_linear_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, v
                      int num_sms, cudaStream_t stream)
 {
     const Operands o{dz, lddz, true, static_cast<uint32_t>(N), x, ldx, true, static_cast<uint32_t>(K), static_cast<uint32_t>(M), status};
-    const Epilogue e{dw, lddw, nullptr, 0, nullptr, nullptr, 0, static_cast<uint32_t>(N), static_cast<uint32_t>(K), NVFP4_ACTIVATION_NONE};
+    const Epilogue e{dw, lddw, nullptr, 0, nullptr, nullptr, 0, static_cast<uint32_t>(N), static_cast<uint32_t>(K), NVFP4_ACTIVATION_NONE, false};
     return bf16 ? product<__nv_bfloat16>(o, e, false, num_sms, stream) : product<__half>(o, e, false, num_sms, stream);
 }
 

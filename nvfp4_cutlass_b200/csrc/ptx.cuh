@@ -172,6 +172,19 @@ NVFP4_DEVICE void tma_load_2d_hint(void* smem_dst, const CUtensorMap* map, uint6
         : "memory");
 }
 
+// Tiled store of a box from this CTA's shared memory (what lies outside of the tensor is not written); the writes of the generic proxy
+// come before it by fence_proxy_async_smem.  Part of the thread's bulk group.
+NVFP4_DEVICE void tma_store_2d(const CUtensorMap* map, uint32_t smem_src, int32_t c0, int32_t c1)
+{
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_src), "r"(c0), "r"(c1)
+                 : "memory");
+}
+NVFP4_DEVICE void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// The thread's committed bulk groups have read their shared memory / are complete.
+NVFP4_DEVICE void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+NVFP4_DEVICE void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 NVFP4_DEVICE uint64_t l2_policy_evict_first()
 {
     uint64_t p;

@@ -45,8 +45,10 @@ def check_forward(got, x, w, bias, residual, activation, out):
     if bias is not None:
         z = z + bias.double()
     want = act64(z, activation)
-    # activation: its argument's error times the slope, and a few steps of its own (exp, a division, products: 8 roundings)
-    error = SLOPE * (sum_error(x, w.t()) + z.abs() * 2.0 ** -23) + want.abs() * 8 * 2.0 ** -23
+    # activation: its argument's error times the slope; 16 roundings of its own, and those of the exponential's argument (three, and one more
+    # in the hardware's base 2), which count as that argument's size
+    argument = {"gelu": z * z / 2 + 2, "gelu_tanh": 1.6 * (z.abs() + 0.044715 * z.abs() ** 3)}.get(activation, z.abs()).clamp(max=200)
+    error = SLOPE * (sum_error(x, w.t()) + z.abs() * 2.0 ** -23) + want.abs() * (16 + 4 * argument) * 2.0 ** -23
     if residual is not None:
         want = want + residual.double()
         error = error + want.abs() * 2.0 ** -23
@@ -195,14 +197,14 @@ def test_gradients_against_the_formulas(m, n, k, activation):
         (dz,) = torch.autograd.grad(act64(z, activation), z, dd.double())
         z = z.detach()
         # the slope is kept in steps of 2^-14; it is taken at the z that the forward sum gave, curvature times that sum's error away, and
-        # costs some 16 roundings itself; a sign that the sum's error can flip costs relu the whole slope
+        # costs some 64 roundings itself; a sign that the sum's error can flip costs relu the whole slope
         z_error = sum_error(x, w.t()) + z.abs() * 2.0 ** -23
         if activation == "none":
             dz_error = torch.zeros_like(z)
         elif activation == "relu":
             dz_error = torch.where(z.abs() <= z_error, dd.double().abs(), 0.0)
         else:
-            dz_error = dd.double().abs() * (2.0 ** -15 + CURVATURE * z_error + 16 * 2.0 ** -23)
+            dz_error = dd.double().abs() * (2.0 ** -15 + CURVATURE * z_error + 64 * 2.0 ** -23)
         tiny = 2.0 ** -25 if dtype == torch.float16 else 1e-40
         db_error = dz_error.sum(dim=0) + dz.abs().sum(dim=0) * (m + 4) * 2.0 ** -24
         assert (db.cpu().double() - dz.sum(dim=0)).abs().le(db_error + (dz.sum(dim=0).abs() + db_error) * 1.01 * HALF_STEP[dtype] + tiny).all()
