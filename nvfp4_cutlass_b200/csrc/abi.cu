@@ -843,13 +843,14 @@ int nvfp4_unsort_tokens_backward(const void* dy, int64_t ldy_elems, const void* 
     host::clear_error();
     if (int rc = check_token_rows(dtype, M, tokens, k, hidden, ld_elems)) return rc;
     NVFP4_REQUIRE(ldy_elems >= hidden, "row stride (%lld) smaller than the row (%d)", static_cast<long long>(ldy_elems), hidden);
-    NVFP4_REQUIRE(tokens + (M + 7) / 8 <= INT_MAX, "too many tokens and rows");
     if ((drows == nullptr && dw == nullptr) || (tokens == 0 && M == 0)) return NVFP4_OK;
     NVFP4_REQUIRE(tokens == 0 || (dy && place), "null pointer argument");
     NVFP4_REQUIRE(dw == nullptr || rows != nullptr || M == 0, "the weights' gradient needs the rows");
     NVFP4_REQUIRE(drows == nullptr || source != nullptr || M == 0, "the rows' gradient needs their sources");
     NVFP4_REQUIRE(on_elements(dy, dtype) && on_elements(rows, dtype) && on_elements(drows, dtype), "rows are not aligned to their type");
-    return launch_unsort_tokens_backward(dy, ldy_elems, rows, ld_elems, dtype, M, place, source, w, tokens, k, hidden, drows, dw,
+    host::DeviceInfo* dev;
+    if (int rc = host::device_info(-1, &dev)) return rc;
+    return launch_unsort_tokens_backward(dy, ldy_elems, rows, ld_elems, dtype, M, place, source, w, tokens, k, hidden, drows, dw, dev->hw_sms,
                                          static_cast<cudaStream_t>(stream));
 }
 

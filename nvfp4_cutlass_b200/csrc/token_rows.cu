@@ -14,6 +14,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "host_common.hpp"
 #include "launchers.hpp"
@@ -315,37 +316,72 @@ sort_move_kernel(const W* __restrict__ x, int64_t ldx, uint32_t tokens, int k, i
 
 // ---- back: y[t] = sum_j w[t, j] * rows[place[t, j]] ------------------------------------------------------------------------------------
 
-// kN elements of T as one access.  Loads are plain here as elsewhere in this file: __ldg, an asm statement, may be moved ahead of the test
-// that guards it.
-template <typename T, int kN>
-struct alignas(sizeof(T) * kN) Pack {
-    T v[kN];
-};
-template <typename P>
-__device__ __forceinline__ P load_pack(const P* at)
-{
-    if constexpr (sizeof(P) == 16) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(at);
-        return *reinterpret_cast<const P*>(&raw);
-    } else {
-        return *at;
+// What a lane moves at a time: 16 bytes of elements of T, or one of them, as bits.  (Arrays of the 16-bit types' classes end up in local
+// memory.)  Loads are plain here as elsewhere in this file: __ldg, an asm statement, may be moved ahead of the test that guards it.
+template <typename T, bool kWide>
+struct Pack {
+    using Bits = std::conditional_t<kWide, uint4, std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>>;
+    static constexpr int kN = kWide ? 16 / static_cast<int>(sizeof(T)) : 1;
+    static __device__ __forceinline__ float2 two(uint32_t w)
+    {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+        else return __half22float2(*reinterpret_cast<const __half2*>(&w));
     }
-}
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ void from_float(float v, float& out) { out = v; }
-__device__ __forceinline__ void from_float(float v, __nv_bfloat16& out) { out = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void from_float(float v, __half& out) { out = __float2half_rn(v); }
+    static __device__ __forceinline__ uint32_t one_word(float a, float b)
+    {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+            return *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+            const __half2 h = __floats2half2_rn(a, b);
+            return *reinterpret_cast<const uint32_t*>(&h);
+        }
+    }
+    static __device__ __forceinline__ void unpack(const Bits& bits, float (&f)[kN])
+    {
+        if constexpr (!kWide) {
+            if constexpr (sizeof(T) == 4) f[0] = __uint_as_float(bits);
+            else f[0] = two(bits).x;
+        } else {
+            const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (sizeof(T) == 4) {
+                    f[i] = __uint_as_float(w[i]);
+                } else {
+                    const float2 v = two(w[i]);
+                    f[2 * i] = v.x;
+                    f[2 * i + 1] = v.y;
+                }
+            }
+        }
+    }
+    static __device__ __forceinline__ Bits pack(const float (&f)[kN])
+    {
+        if constexpr (!kWide) {
+            if constexpr (sizeof(T) == 4) return __float_as_uint(f[0]);
+            else return static_cast<uint16_t>(one_word(f[0], 0.0f));
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(f[i]);
+                else w[i] = one_word(f[2 * i], f[2 * i + 1]);
+            }
+            return make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+};
 
 // A warp takes a piece of a token, kPer packs a lane; the rows of up to four choices are under way together.  FP32, ascending j.
 // The gradient of the sort is the same sum without weights.
 constexpr int kPer = 2, kFlight = 4;
-template <typename T, int kN>
-__global__ void __launch_bounds__(256)
-unsort_kernel(const Pack<T, kN>* __restrict__ rows, int64_t ld, const int64_t* __restrict__ place, const float* __restrict__ w, uint32_t tokens,
-              int k, int64_t m, uint32_t row_packs, Pack<T, kN>* __restrict__ y)
+template <typename P>
+__global__ void __launch_bounds__(256, 3)
+unsort_kernel(const typename P::Bits* __restrict__ rows, int64_t ld, const int64_t* __restrict__ place, const float* __restrict__ w, uint32_t tokens,
+              int k, int64_t m, uint32_t row_packs, typename P::Bits* __restrict__ y)
 {
+    constexpr int kN = P::kN;
     const uint32_t lane = threadIdx.x & 31, pieces = (row_packs + 32 * kPer - 1) / (32 * kPer);
     const uint64_t units = static_cast<uint64_t>(tokens) * pieces;
     ptx::grid_dependency_wait();
@@ -366,7 +402,7 @@ unsort_kernel(const Pack<T, kN>* __restrict__ rows, int64_t ld, const int64_t* _
             }
             const int here = min(32, k - j0);
             for (int j1 = 0; j1 < here; j1 += kFlight) {
-                Pack<T, kN> v[kFlight][kPer];
+                typename P::Bits v[kFlight][kPer];
                 bool live[kFlight];
                 float wj[kFlight];
 #pragma unroll
@@ -377,114 +413,229 @@ unsort_kernel(const Pack<T, kN>* __restrict__ rows, int64_t ld, const int64_t* _
                     if (live[u]) {
 #pragma unroll
                         for (int i = 0; i < kPer; ++i)
-                            if (c0 + i * 32 < row_packs) v[u][i] = load_pack(rows + r * ld + c0 + i * 32);
+                            if (c0 + i * 32 < row_packs) v[u][i] = rows[r * ld + c0 + i * 32];
                     }
                 }
 #pragma unroll
                 for (int u = 0; u < kFlight; ++u) {
                     if (!live[u]) continue;
 #pragma unroll
-                    for (int i = 0; i < kPer; ++i)
+                    for (int i = 0; i < kPer; ++i) {
+                        float f[kN];
+                        P::unpack(v[u][i], f);
 #pragma unroll
-                        for (int q = 0; q < kN; ++q) acc[i][q] = fmaf(wj[u], to_float(v[u][i].v[q]), acc[i][q]);
+                        for (int q = 0; q < kN; ++q) acc[i][q] = fmaf(wj[u], f[q], acc[i][q]);
+                    }
                 }
             }
         }
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             if (c0 + i * 32 >= row_packs) continue;
-            Pack<T, kN> o;
-#pragma unroll
-            for (int q = 0; q < kN; ++q) from_float(acc[i][q], o.v[q]);
-            y[static_cast<int64_t>(t) * row_packs + c0 + i * 32] = o;
+            y[static_cast<int64_t>(t) * row_packs + c0 + i * 32] = P::pack(acc[i]);
         }
     }
 }
 
-// Gradients of that sum: drows[place[t, j]] = w[t, j] * dy[t], zero for rows without a pair, dw[t, j] = <dy[t], rows[place[t, j]]>.
-// A block takes a token: dy is read once for every group of eight choices (from L1 after the first), every row of `rows` once, every
-// row of `drows` is written once.  A token's dot products stay inside its block and are added in a fixed order.  Behind the
-// tokens: blocks that zero the rows whose source is -1.  drows or dw may be NULL; rows is read for dw alone.
-constexpr int kBackThreads = 256, kBackWarps = kBackThreads / 32, kGroup = 8;
-template <typename T, int kN>
-__global__ void __launch_bounds__(kBackThreads)
-unsort_backward_kernel(const Pack<T, kN>* __restrict__ dy, int64_t ldy, const Pack<T, kN>* __restrict__ rows, int64_t ld,
-                       const int64_t* __restrict__ place, const int32_t* __restrict__ source, const float* __restrict__ w, uint32_t tokens, int k,
-                       int64_t m, uint32_t row_packs, Pack<T, kN>* __restrict__ drows, float* __restrict__ dw)
+// The same sum for many tokens with rows of whole 16-byte words: the rows come by bulk copies into a ring in shared memory, whole pieces
+// of up to 8 KB a request, and a block has its entire shared memory under way, where the loads of the kernel above come in pieces of 1 KB
+// and no faster than registers for them are to be had (8192 tokens x 8 rows of 8 KB: 171 us, 3.5 TB/s).
+// A unit is a piece of one token's rows, or `group` whole tokens whose rows are short; a slot of the ring takes a unit's pairs (at most
+// 32), `stride` bytes each.  Warp 0 looks up a pair per lane, one unit ahead, leaves the weights and the mask of pairs with a row beside
+// the slot and requests the rows; the other warps add them up in FP32 in ascending j, the order of the kernel above: the same bits.
+// Every wait is bounded; a block whose wait ran out leaves NaN in what it did not finish.
+constexpr int kRingWorkers = 16, kRingThreads = 32 * (1 + kRingWorkers), kRingPairs = 32, kRingMaxDepth = 12;
+struct RingSlot {
+    float w[kRingPairs];
+    uint32_t live;                                   // bit p: pair p has a row, whose bytes were requested
+};
+// units to an SM from which on the ring is taken
+constexpr uint32_t kRingLeast = 2;
+struct RingShape {
+    uint32_t tokens, k, group, units, pieces, row_bytes, stride, depth;
+};
+template <typename P>
+__global__ void __launch_bounds__(kRingThreads, 1)
+unsort_ring_kernel(const uint8_t* __restrict__ rows, int64_t ld_bytes, const int64_t* __restrict__ place, const float* __restrict__ w, int64_t m,
+                   const RingShape shape, uint4* __restrict__ y)
 {
-    __shared__ float part[kBackWarps][kGroup];
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem = (ptx::smem_u32(smem_raw) + 127u) & ~127u;
+    uint8_t* gen = smem_raw + (smem - ptx::smem_u32(smem_raw));
+    const uint32_t pairs = shape.group * shape.k, slot_bytes = pairs * shape.stride;
+    uint64_t* full = reinterpret_cast<uint64_t*>(gen + static_cast<size_t>(shape.depth) * slot_bytes);
+    uint64_t* freed = full + kRingMaxDepth;
+    RingSlot* info = reinterpret_cast<RingSlot*>(freed + kRingMaxDepth);
+    volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(info + kRingMaxDepth);
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < shape.depth; ++i) { ptx::mbar_init(full + i, 1); ptx::mbar_init(freed + i, kRingWorkers); }
+        *abort_flag = 0;
+        ptx::fence_mbar_init();
+    }
+    __syncthreads();
     ptx::grid_dependency_wait();
-    if (blockIdx.x >= tokens) {                                              // a warp per row
-        const int64_t r = static_cast<int64_t>(blockIdx.x - tokens) * kBackWarps + warp;
-        if (r >= m || source[r] >= 0) return;
-        for (uint32_t c = lane; c < row_packs; c += 32) drows[r * row_packs + c] = Pack<T, kN>{};
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t slot = 0, phase = 0;
+    auto next = [&] { if (++slot == shape.depth) { slot = 0; phase ^= 1; } };
+    if (warp == 0) {
+        int64_t row = -1;
+        float weight = 0.0f;
+        auto look_up = [&](uint32_t unit) {
+            row = -1;
+            if (unit >= shape.units || lane >= pairs) return;
+            const uint32_t t0 = unit / shape.pieces * shape.group;
+            if (lane >= min(shape.group, shape.tokens - t0) * shape.k) return;
+            const int64_t at = static_cast<int64_t>(t0) * shape.k + lane;
+            row = place[at];
+            if (row >= m) row = -1;
+            weight = w != nullptr ? w[at] : 1.0f;
+        };
+        look_up(blockIdx.x);
+        for (uint32_t unit = blockIdx.x; unit < shape.units; unit += gridDim.x) {
+            if (!ptx::all_lanes(ptx::mbar_wait_impl(freed + slot, phase ^ 1, abort_flag))) { *abort_flag = 1; break; }
+            const uint32_t from = unit % shape.pieces * shape.stride, bytes = min(shape.stride, shape.row_bytes - from);
+            const unsigned live = __ballot_sync(kAll, row >= 0);
+            if (lane < pairs) info[slot].w[lane] = weight;
+            if (lane == 0) info[slot].live = live;
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_expect_tx(full + slot, __popc(live) * bytes);
+            __syncwarp();
+            if (row >= 0) ptx::bulk_load(gen + static_cast<size_t>(slot) * slot_bytes + lane * shape.stride, rows + row * ld_bytes + from, bytes, full + slot);
+            look_up(unit + gridDim.x);
+            next();
+        }
         return;
     }
-    const int64_t t = blockIdx.x;
-    for (int j0 = 0; j0 < k; j0 += kGroup) {
-        int64_t r[kGroup];
-        float wj[kGroup], dot[kGroup];
+    bool ok = true;
+    for (uint32_t unit = blockIdx.x; unit < shape.units; unit += gridDim.x) {
+        if (ok && !ptx::all_lanes(ptx::mbar_wait_impl(full + slot, phase, abort_flag))) { *abort_flag = 1; ok = false; }
+        const uint32_t base = smem + slot * slot_bytes, live = ok ? info[slot].live : 0u;
+        const uint32_t t0 = unit / shape.pieces * shape.group, here = min(shape.group, shape.tokens - t0);
+        const uint32_t from = unit % shape.pieces * shape.stride, words = min(shape.stride, shape.row_bytes - from) / 16;
+        for (uint32_t c = threadIdx.x - 32; c < here * words; c += 32 * kRingWorkers) {
+            const uint32_t g = c / words, word = c % words, first = g * shape.k;
+            float acc[P::kN];
 #pragma unroll
-        for (int u = 0; u < kGroup; ++u) {
-            r[u] = j0 + u < k ? place[t * k + j0 + u] : -1;
-            if (r[u] >= m) r[u] = -1;
-            wj[u] = w != nullptr && j0 + u < k ? w[t * k + j0 + u] : 1.0f;
-            dot[u] = 0.0f;
-        }
-        for (uint32_t c = threadIdx.x; c < row_packs; c += kBackThreads) {
-            const Pack<T, kN> g = load_pack(dy + t * ldy + c);
-            float gf[kN];
+            for (int q = 0; q < P::kN; ++q) acc[q] = ok ? 0.0f : __uint_as_float(0x7fc00000u);
+            for (uint32_t j0 = 0; j0 < shape.k; j0 += 8) {
+                uint4 v[8];
+                const uint32_t mask = (live >> (first + j0)) & ((2u << min(7u, shape.k - 1 - j0)) - 1);
 #pragma unroll
-            for (int q = 0; q < kN; ++q) gf[q] = to_float(g.v[q]);
-            if (dw != nullptr) {
-                Pack<T, kN> v[kGroup];
+                for (uint32_t u = 0; u < 8; ++u)
+                    if (mask >> u & 1u) v[u] = ptx::lds128(base + (first + j0 + u) * shape.stride + word * 16);
 #pragma unroll
-                for (int u = 0; u < kGroup; ++u)
-                    if (r[u] >= 0) v[u] = load_pack(rows + r[u] * ld + c);
+                for (uint32_t u = 0; u < 8; ++u) {
+                    if (!(mask >> u & 1u)) continue;
+                    const float wj = info[slot].w[first + j0 + u];
+                    float f[P::kN];
+                    P::unpack(v[u], f);
 #pragma unroll
-                for (int u = 0; u < kGroup; ++u) {
-                    if (r[u] < 0) continue;
-#pragma unroll
-                    for (int q = 0; q < kN; ++q) dot[u] = fmaf(gf[q], to_float(v[u].v[q]), dot[u]);
+                    for (int q = 0; q < P::kN; ++q) acc[q] = fmaf(wj, f[q], acc[q]);
                 }
             }
-            if (drows != nullptr) {
+            y[(static_cast<int64_t>(t0 + g) * shape.row_bytes + from) / 16 + word] = P::pack(acc);
+        }
+        // the slot's loads are over: what they brought went into the words that were stored
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(freed + slot);
+        next();
+    }
+}
+constexpr size_t kRingExtra = 128 + kRingMaxDepth * (2 * sizeof(uint64_t) + sizeof(RingSlot)) + 16, kRingSmem = 232448 - 1024;
+// The ring for these rows; depth 0: there is none.
+RingShape ring_shape(int64_t tokens, int k, int64_t row_bytes)
+{
+    RingShape r{static_cast<uint32_t>(tokens), static_cast<uint32_t>(k), 1, 0, 1, static_cast<uint32_t>(row_bytes), static_cast<uint32_t>(row_bytes), 0};
+    if (k > kRingPairs || row_bytes % 16 != 0) return r;
+    for (r.stride = 8192; r.stride > 1024 && 3 * static_cast<int64_t>(r.stride) * k > static_cast<int64_t>(kRingSmem - kRingExtra); r.stride /= 2) {}
+    if (row_bytes <= r.stride) {
+        r.stride = static_cast<uint32_t>(row_bytes);
+        while ((r.group + 1) * r.k <= kRingPairs && (r.group + 1) * row_bytes <= 8192) ++r.group;
+    }
+    r.pieces = static_cast<uint32_t>((row_bytes + r.stride - 1) / r.stride);
+    const int64_t units = (tokens + r.group - 1) / r.group * r.pieces, depth = static_cast<int64_t>(kRingSmem - kRingExtra) / (static_cast<int64_t>(r.group) * k * r.stride);
+    if (units > INT32_MAX) return r;
+    r.units = static_cast<uint32_t>(units);
+    r.depth = static_cast<uint32_t>(depth > kRingMaxDepth ? kRingMaxDepth : depth);
+    return r;
+}
+
+// Gradients of that sum: drows[place[t, j]] = w[t, j] * dy[t], zero for rows without a pair, dw[t, j] = <dy[t], rows[place[t, j]]>.
+// A warp takes a pair: its dot product stays inside the warp, in a fixed order, and four packs a lane of the row and of dy are under way
+// at a time in few registers.  The pairs of a token are neighbouring warps', which read dy from L1 behind the first.  (A block to a token,
+// eight rows at a time to a thread, took 138 registers and ran at an eighth of the warps: 455 us for 8192 x 8 rows of 8 KB.)
+// Behind the pairs: warps that zero the rows whose source is -1.  drows or dw may be NULL; rows is read for dw alone.
+constexpr int kBackThreads = 256, kBackWarps = kBackThreads / 32, kBackPer = 4;
+template <typename P>
+__global__ void __launch_bounds__(kBackThreads, 4)
+unsort_backward_kernel(const typename P::Bits* __restrict__ dy, int64_t ldy, const typename P::Bits* __restrict__ rows, int64_t ld,
+                       const int64_t* __restrict__ place, const int32_t* __restrict__ source, const float* __restrict__ w, uint32_t pairs, uint32_t k,
+                       uint32_t m, uint32_t row_packs, typename P::Bits* __restrict__ drows, float* __restrict__ dw)
+{
+    using Bits = typename P::Bits;
+    constexpr int kN = P::kN;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint64_t units = static_cast<uint64_t>(pairs) + (drows != nullptr ? m : 0);
+    ptx::grid_dependency_wait();
+    for (uint64_t unit = static_cast<uint64_t>(blockIdx.x) * kBackWarps + (threadIdx.x >> 5); unit < units; unit += static_cast<uint64_t>(gridDim.x) * kBackWarps) {
+        if (unit >= pairs) {
+            const uint32_t r = static_cast<uint32_t>(unit - pairs);
+            if (source[r] >= 0) continue;
+            for (uint32_t c = lane; c < row_packs; c += 32) drows[static_cast<int64_t>(r) * row_packs + c] = Bits{};
+            continue;
+        }
+        const uint32_t p = static_cast<uint32_t>(unit);
+        const int64_t r = place[p];
+        if (r < 0 || r >= m) {
+            if (dw != nullptr && lane == 0) dw[p] = 0.0f;
+            continue;
+        }
+        const float weight = w != nullptr ? w[p] : 1.0f;
+        const Bits* from = dy + static_cast<int64_t>(p / k) * ldy;
+        const Bits* row = rows + r * ld;
+        Bits* to = drows + r * row_packs;
+        float dot = 0.0f;
+        for (uint32_t c0 = lane; c0 < row_packs; c0 += 32 * kBackPer) {
+            Bits g[kBackPer], v[kBackPer];
 #pragma unroll
-                for (int u = 0; u < kGroup; ++u) {
-                    if (r[u] < 0) continue;
-                    Pack<T, kN> o;
+            for (int i = 0; i < kBackPer; ++i)
+                if (c0 + i * 32 < row_packs) g[i] = from[c0 + i * 32];
+            if (dw != nullptr) {
 #pragma unroll
-                    for (int q = 0; q < kN; ++q) from_float(wj[u] * gf[q], o.v[q]);
-                    drows[r[u] * row_packs + c] = o;
+                for (int i = 0; i < kBackPer; ++i)
+                    if (c0 + i * 32 < row_packs) v[i] = row[c0 + i * 32];
+            }
+#pragma unroll
+            for (int i = 0; i < kBackPer; ++i) {
+                if (c0 + i * 32 >= row_packs) continue;
+                float gf[kN], f[kN];
+                P::unpack(g[i], gf);
+                if (dw != nullptr) {
+                    P::unpack(v[i], f);
+#pragma unroll
+                    for (int q = 0; q < kN; ++q) dot = fmaf(gf[q], f[q], dot);
+                }
+                if (drows != nullptr) {
+#pragma unroll
+                    for (int q = 0; q < kN; ++q) f[q] = weight * gf[q];
+                    to[c0 + i * 32] = P::pack(f);
                 }
             }
         }
         if (dw == nullptr) continue;
 #pragma unroll
-        for (int u = 0; u < kGroup; ++u) {
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) dot[u] += __shfl_xor_sync(kAll, dot[u], d);
-            if (lane == 0) part[warp][u] = dot[u];
-        }
-        __syncthreads();
-        if (threadIdx.x < kGroup && j0 + static_cast<int>(threadIdx.x) < k) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kBackWarps; ++i) sum += part[i][threadIdx.x];
-            dw[t * k + j0 + threadIdx.x] = sum;
-        }
-        __syncthreads();
+        for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(kAll, dot, d);
+        if (lane == 0) dw[p] = dot;
     }
 }
 
-// Calls f(T*, elements of a 16-byte pack or 1) for a type code.
+// Calls f(Pack<type, wide>*) for a type code.
 template <typename F>
 int with_pack(int dtype, bool wide, F&& f)
 {
     auto packs = [&](auto* type) {
-        constexpr int kN = 16 / static_cast<int>(sizeof(*type));
-        return wide ? f(type, std::integral_constant<int, kN>{}) : f(type, std::integral_constant<int, 1>{});
+        using T = std::remove_pointer_t<decltype(type)>;
+        return wide ? f(static_cast<Pack<T, true>*>(nullptr)) : f(static_cast<Pack<T, false>*>(nullptr));
     };
     switch (dtype) {
         case NVFP4_DTYPE_BF16: return packs(static_cast<__nv_bfloat16*>(nullptr));
@@ -564,31 +715,49 @@ int launch_unsort_tokens(const void* rows, int64_t ld, int dtype, int64_t m, con
 {
     const size_t size = elem_bytes(dtype);
     const bool wide = ((reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(y) | static_cast<uintptr_t>(ld * size) | hidden * size) & 15u) == 0;
-    return with_pack(dtype, wide, [&](auto* type, auto n) {
-        using T = std::remove_pointer_t<decltype(type)>;
-        constexpr int kN = decltype(n)::value;
+    return with_pack(dtype, wide, [&](auto* type) {
+        using P = std::remove_pointer_t<decltype(type)>;
+        using Bits = typename P::Bits;
+        constexpr int kN = P::kN;
+        if constexpr (kN > 1) {
+            const RingShape shape = ring_shape(tokens, k, static_cast<int64_t>(hidden * size));
+            if (shape.depth >= 2 && shape.units >= kRingLeast * static_cast<uint32_t>(num_sms)) {
+                static bool attr_set[host::kMaxDevices] = {};
+                int dev = 0;
+                NVFP4_CUDA_CHECK(cudaGetDevice(&dev));
+                if (!attr_set[dev]) {
+                    NVFP4_CUDA_CHECK(cudaFuncSetAttribute(unsort_ring_kernel<P>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kRingSmem)));
+                    attr_set[dev] = true;
+                }
+                return host::launch_kernel(unsort_ring_kernel<P>, dim3(static_cast<unsigned>(num_sms)), dim3(kRingThreads),
+                                           static_cast<size_t>(shape.depth) * shape.group * shape.k * shape.stride + kRingExtra, stream, true,
+                                           static_cast<const uint8_t*>(rows), static_cast<int64_t>(ld * size), place, w, m, shape, static_cast<uint4*>(y));
+            }
+        }
         const uint32_t packs = static_cast<uint32_t>(hidden / kN);
         const uint64_t units = static_cast<uint64_t>(tokens) * ((packs + 32 * kPer - 1) / (32 * kPer));
-        return host::launch_kernel(unsort_kernel<T, kN>, dim3(blocks_for(units, 8, num_sms, 8)), dim3(256), 0, stream, true,
-                                   static_cast<const Pack<T, kN>*>(rows), ld / kN, place, w, static_cast<uint32_t>(tokens), k, m, packs,
-                                   static_cast<Pack<T, kN>*>(y));
+        return host::launch_kernel(unsort_kernel<P>, dim3(blocks_for(units, 8, num_sms, 8)), dim3(256), 0, stream, true,
+                                   static_cast<const Bits*>(rows), ld / kN, place, w, static_cast<uint32_t>(tokens), k, m, packs,
+                                   static_cast<Bits*>(y));
     });
 }
 
 int launch_unsort_tokens_backward(const void* dy, int64_t ldy, const void* rows, int64_t ld, int dtype, int64_t m, const int64_t* place,
-                                  const int32_t* source, const float* w, int64_t tokens, int k, int hidden, void* drows, float* dw,
+                                  const int32_t* source, const float* w, int64_t tokens, int k, int hidden, void* drows, float* dw, int num_sms,
                                   cudaStream_t stream)
 {
     const size_t size = elem_bytes(dtype);
     const bool wide = ((reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(drows) |
                         static_cast<uintptr_t>(ldy * size) | static_cast<uintptr_t>(ld * size) | hidden * size) & 15u) == 0;
-    return with_pack(dtype, wide, [&](auto* type, auto n) {
-        using T = std::remove_pointer_t<decltype(type)>;
-        constexpr int kN = decltype(n)::value;
-        const int64_t zeroing = drows != nullptr ? (m + kBackWarps - 1) / kBackWarps : 0;
-        return host::launch_kernel(unsort_backward_kernel<T, kN>, dim3(static_cast<unsigned>(tokens + zeroing)), dim3(kBackThreads), 0, stream, true,
-                                   static_cast<const Pack<T, kN>*>(dy), ldy / kN, static_cast<const Pack<T, kN>*>(rows), ld / kN, place, source, w,
-                                   static_cast<uint32_t>(tokens), k, m, static_cast<uint32_t>(hidden / kN), static_cast<Pack<T, kN>*>(drows), dw);
+    return with_pack(dtype, wide, [&](auto* type) {
+        using P = std::remove_pointer_t<decltype(type)>;
+        using Bits = typename P::Bits;
+        constexpr int kN = P::kN;
+        const uint64_t pairs = static_cast<uint64_t>(tokens) * k, units = pairs + (drows != nullptr ? m : 0);
+        return host::launch_kernel(unsort_backward_kernel<P>, dim3(blocks_for(units, kBackWarps, num_sms, 8)), dim3(kBackThreads), 0, stream, true,
+                                   static_cast<const Bits*>(dy), ldy / kN, static_cast<const Bits*>(rows), ld / kN, place, source, w,
+                                   static_cast<uint32_t>(pairs), static_cast<uint32_t>(k), static_cast<uint32_t>(m), static_cast<uint32_t>(hidden / kN),
+                                   static_cast<Bits*>(drows), dw);
     });
 }
 
