@@ -29,6 +29,7 @@ def _no_binding(*args):
 
 
 _contiguous_call = _no_binding
+_binding = None                  # binding.cpp's module, once it is bound: the operators' calls in tokens.py and dense.py go through it
 
 POLICY_CODES = {"derived_div8": 0, "residual_amax": 1, "derived_div4": 2, "div4_radix8": 3}
 
@@ -115,6 +116,7 @@ def lib() -> ctypes.CDLL:
 def _bind(library):
     """binding.cpp's form of the contiguous GEMM call, bound to the library's entry.  It is a faster way to the same entry and nothing
     else needs it: without it (a build without torch's headers, a torch without CUDA) every call goes the general way."""
+    global _binding
     try:
         loader = importlib.machinery.ExtensionFileLoader("_binding", _BINDING_PATH)
         binding = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_binding", _BINDING_PATH, loader=loader))
@@ -122,8 +124,12 @@ def _bind(library):
     except (ImportError, OSError) as e:
         if torch.version.cuda is not None:
             warnings.warn(f"{_BINDING_PATH} does not load ({e}): GEMM calls take some 6 us more on the host", RuntimeWarning, stacklevel=3)
+        _binding = None
         return _no_binding
-    binding.bind(ctypes.cast(library.nvfp4_grouped_gemm_contiguous, ctypes.c_void_p).value)
+    address = lambda entry: ctypes.cast(entry, ctypes.c_void_p).value
+    binding.bind(address(library.nvfp4_grouped_gemm_contiguous))
+    binding.bind_operators(*map(address, (library.nvfp4_route_tokens, library.nvfp4_sort_tokens, library.nvfp4_unsort_tokens, library.nvfp4_linear)))
+    _binding = binding
     return binding.contiguous
 
 
@@ -700,6 +706,13 @@ def combine_rows_peer(peers: torch.Tensor, rows_ld_elems: int, src_rank: torch.T
 
 
 # ---- operators around the grouped GEMM: routing, rows sorted by expert and back (tokens.py puts the gradients on top) ----
+
+def answered(result):
+    """Whether binding.cpp took the call (its result is the caller's then); raises for an error code of the library."""
+    if type(result) is int:
+        _check(result)
+    return result is not None
+
 
 DTYPE_CODES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 SCORE_CODES = {"softmax": 0, "sigmoid": 1}

@@ -47,6 +47,10 @@ def route_tokens(logits: torch.Tensor, k: int, *, scores: str = "softmax", renor
     softmax (over all experts) or sigmoid scores, with ``renormalize`` divided by the sum of the chosen ones.  A logit of -inf is an
     expert that is not to be had: it is never chosen, and where fewer than k others are left the remaining ids are -1 and their weights 0
     (``sort_tokens`` gives such a pair no row).  experts <= 1024, k <= 32.  Differentiable in ``logits``."""
+    if _C._binding is not None and scores in _C.SCORE_CODES:
+        result = _C._binding.route(logits, k, _C.SCORE_CODES[scores], 1 if renormalize else 0)
+        if _C.answered(result):
+            return result
     if not _differentiable(logits):
         return _C.route_tokens(logits, int(k), scores, bool(renormalize))
     return _Route.apply(logits, int(k), scores, bool(renormalize))
@@ -81,6 +85,10 @@ def sort_tokens(x: torch.Tensor, ids: torch.Tensor, num_experts: int, *, alignme
     their pairs; rows without a pair are zero.  M depends on the sizes alone:
     (pairs + min(num_experts, pairs) * (alignment - 1)) rounded down to a multiple of alignment.  BF16 rows go into the GEMM as they
     are; FP16 and FP32 rows are moved too.  num_experts <= 1024.  Differentiable in ``x``."""
+    if _C._binding is not None:
+        result = _C._binding.sort(x, ids, num_experts, alignment)
+        if _C.answered(result):
+            return result[0], TokenOrder(*result[1:])
     call = _Sort.apply if _differentiable(x) else _C.sort_tokens
     rows, place, source, m_indices = call(x, ids, int(num_experts), int(alignment))
     return rows, TokenOrder(place, source, m_indices)
@@ -109,6 +117,10 @@ def unsort_tokens(rows: torch.Tensor, order: TokenOrder, weights: Optional[torch
     ascending j, rounded once.  A pair without a row contributes nothing, and its weight's gradient is 0.  Differentiable in ``rows`` and
     ``weights``; the gradient of rows without a pair is zero."""
     place, source = order.place, order.source
+    if _C._binding is not None and rows.shape[0] == source.shape[0]:
+        result = _C._binding.unsort(rows, place, weights)
+        if _C.answered(result):
+            return result
     _C._require(isinstance(rows, torch.Tensor) and source.dtype == torch.int32 and source.dim() == 1 and source.is_contiguous() and
                 rows.dim() == 2 and rows.shape[0] == source.shape[0], "rows has the rows of the order")
     _C._one_device(rows, weights, place, source)

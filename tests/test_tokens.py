@@ -482,3 +482,49 @@ def test_an_expert_layer_out_of_the_public_calls():
     y = unsort_tokens(out, order, w)
     layer = ExpertParallelMoE(experts, hidden, inter, up, down)
     assert torch.equal(y, layer(x, ids, w))
+
+
+# ---- the calls in binding.cpp ----------------------------------------------------------------------------------------
+
+
+def test_the_binding_takes_no_host_tensors_and_no_odd_arguments():
+    _C.lib()
+    b = _C._binding
+    assert b is not None
+    x, ids = torch.zeros(4, 8), torch.zeros(4, 2, dtype=torch.int64)
+    assert b.route(x, 2, 0, 1) is None and b.route(None, 2, 0, 1) is None and b.route(x, "2", 0, 1) is None and b.route(x) is None
+    assert b.sort(x, ids, 4, 16) is None and b.sort(x, None, 4, 16) is None and b.sort(x, ids, -4, 16) is None
+    assert b.unsort(x, ids, None) is None and b.unsort(x, ids, 3) is None and b.unsort(x) is None
+    assert b.linear(x, x, None, None, 0, 0) is None and b.linear(x, x, None, None, 1 << 40, 0) is None and b.linear(x) is None
+    with pytest.raises(TypeError):
+        b.bind_operators(1)
+
+
+@gpu
+def test_the_binding_gives_the_general_way_s_results(monkeypatch):
+    g = gen(6)
+    logits, x = torch.randn(50, 24, generator=g).cuda(), torch.randn(50, 72, generator=g).to(torch.bfloat16).cuda()
+    w, bias = torch.randn(40, 72, generator=g).to(torch.bfloat16).cuda(), torch.randn(40, generator=g).to(torch.bfloat16).cuda()
+    residual = torch.randn(50, 40, generator=g).cuda()
+
+    def calls():
+        ids, weights = route_tokens(logits, 3, scores="sigmoid", renormalize=False)
+        rows, order = sort_tokens(x, ids, 24, alignment=16)
+        return [ids, weights, rows, *order, unsort_tokens(rows, order, weights), unsort_tokens(rows, order),
+                nvfp4_gemm.linear(x, w, bias, residual, activation="silu", out_dtype=torch.float32), nvfp4_gemm.linear(x, w)]
+
+    _C.lib()
+    assert _C._binding is not None
+    fast = calls()
+    # what it leaves to the general way: strided index tensors, tensors that need a gradient, empty ones
+    b = _C._binding
+    ids = fast[0]
+    assert b.sort(x, ids.t().contiguous().t(), 24, 16) is None and b.route(logits.clone().requires_grad_(), 3, 0, 1) is None
+    assert b.linear(x, w.clone().requires_grad_(), None, None, 0, 0) is None and b.linear(x[:0], w, None, None, 0, 0) is None
+    with torch.no_grad():
+        assert b.linear(x, w.clone().requires_grad_(), None, None, 0, 0) is not None
+    assert torch.equal(sort_tokens(x, ids.t().contiguous().t(), 24, alignment=16)[0], fast[2])
+    with pytest.raises(RuntimeError, match="K must be"):
+        nvfp4_gemm.linear(x[:, :60], w[:, :60])
+    monkeypatch.setattr(_C, "_binding", None)
+    assert all(torch.equal(a, b) for a, b in zip(fast, calls()))
