@@ -445,7 +445,6 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     };
     const uint32_t quad = warp & 3, row = quad * 32 + lane;                   // epilogue: the warp's quarter of the lanes
     const uint32_t taddr = tmem + ((quad * 32) << 16);
-    [[maybe_unused]] float sum[kWide ? BN : 1];
     if (warp == 0) {
         const uint32_t issue = ptx::elect_one();
         Ring r;
@@ -483,6 +482,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
             next(r);
         }
     } else {
+        [[maybe_unused]] float sum[kWide ? BN : 1];
         if constexpr (kWide) {
 #pragma unroll
             for (uint32_t i = 0; i < BN; ++i) sum[i] = 0.0f;
@@ -504,18 +504,20 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                 if (lane == 0) ptx::mbar_arrive(tmem_empty + acc);
             }
         }
+        if constexpr (kWide) {                       // back to tensor memory, which can be indexed: what follows is there once, not once per chunk
+#pragma unroll
+            for (uint32_t c0 = 0; c0 < BN; c0 += kChunk) {
+                uint32_t raw[kChunk];
+#pragma unroll
+                for (uint32_t i = 0; i < kChunk; ++i) raw[i] = __float_as_uint(sum[c0 + i]);
+                ptx::tmem_st_32x32b(taddr + c0, raw);
+            }
+            ptx::tmem_st_wait();
+        }
     }
 
     // epilogue: 128 rows of A in all
     const uint32_t live = kSwap ? min(BN, e.rows - b0) : min(BN, e.cols - b0);          // columns of the tile that anybody wants
-    auto take = [&](float (&v)[kChunk], uint32_t c0) {
-        if constexpr (kWide) {
-#pragma unroll
-            for (uint32_t i = 0; i < kChunk; ++i) v[i] = sum[c0 + i];
-        } else {
-            load_accumulators(taddr + c0, v);
-        }
-    };
     auto give = [&](float (&v)[kChunk], uint32_t column, uint32_t count) {    // columns [column, column + count) of the tile
         if constexpr (kSwap) {
             finish<T, D>(v, b0 + column, count, a0 + row, e);
@@ -528,11 +530,10 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         const uint32_t width_log2 = __popc(BN - 1) - p.splits_log2, width = 1u << width_log2;          // columns that a CTA finishes
         if (warp >= 2 && ok) {
             const uint32_t mine = ptx::smem_u32(partial + ((rank << width_log2) * BM + row));
-#pragma unroll
-            for (uint32_t c0 = 0; c0 < BN; c0 += kChunk) {
-                if (c0 >= live) continue;
+#pragma unroll 1
+            for (uint32_t c0 = 0; c0 < live; c0 += kChunk) {
                 float v[kChunk];
-                take(v, c0);
+                load_accumulators(taddr + c0, v);
 #pragma unroll
                 for (uint32_t i = 0; i < kChunk; ++i) {
                     const uint32_t c = c0 + i;
@@ -574,11 +575,11 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
             }
         }
     } else if (warp >= 2 && ok) {
-#pragma unroll
-        for (uint32_t c0 = 0; c0 < BN; c0 += kChunk) {
-            if (c0 >= live) continue;
+        // (unrolled, a cold call spent 3 us a chunk fetching instructions: 13 us of a router's 41)
+#pragma unroll 1
+        for (uint32_t c0 = 0; c0 < live; c0 += kChunk) {
             float v[kChunk];
-            take(v, c0);
+            load_accumulators(taddr + c0, v);
             give(v, c0, kSwap ? min(kChunk, live - c0) : 32);
         }
     }
