@@ -128,7 +128,9 @@ def _bind(library):
         return _no_binding
     address = lambda entry: ctypes.cast(entry, ctypes.c_void_p).value
     binding.bind(address(library.nvfp4_grouped_gemm_contiguous))
-    binding.bind_operators(*map(address, (library.nvfp4_route_tokens, library.nvfp4_sort_tokens, library.nvfp4_unsort_tokens, library.nvfp4_linear)))
+    binding.bind_operators(*(address(getattr(library, "nvfp4_" + name)) for name in (
+        "last_error", "route_tokens", "route_tokens_backward", "sort_tokens", "unsort_tokens", "unsort_tokens_backward", "linear", "linear_dz",
+        "linear_dx", "linear_dw")))
     _binding = binding
     return binding.contiguous
 
@@ -706,13 +708,6 @@ def combine_rows_peer(peers: torch.Tensor, rows_ld_elems: int, src_rank: torch.T
 
 
 # ---- operators around the grouped GEMM: routing, rows sorted by expert and back (tokens.py puts the gradients on top) ----
-
-def answered(result):
-    """Whether binding.cpp took the call (its result is the caller's then); raises for an error code of the library."""
-    if type(result) is int:
-        _check(result)
-    return result is not None
-
 
 DTYPE_CODES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 SCORE_CODES = {"softmax": 0, "sigmoid": 1}

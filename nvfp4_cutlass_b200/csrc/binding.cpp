@@ -8,13 +8,16 @@
 // that does not hold.  The C ABI's entry point comes from the caller (bind), so that nothing here is linked to it.
 //
 // The same for the operators around it, which take a few microseconds on the GPU and took three to five times that in the interpreter
-// (route_tokens of 64 tokens 12 us, linear of one token 18): route, sort, unsort and linear allocate their outputs and call the ABI; they
-// leave calls that autograd has to record to Python, too.
+// (route_tokens of 64 tokens 12 us, linear of one token 18): route, sort, unsort and linear allocate their outputs and call the ABI, and record
+// what autograd needs.
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <algorithm>
@@ -95,52 +98,69 @@ PyObject* contiguous(PyObject*, PyObject* const* args, Py_ssize_t count)
 }
 
 // ---- operators around the GEMM -----------------------------------------------------------------------------------
+//
+// route, sort, unsort and linear answer None to a call for the general way.  What autograd has to record goes through nodes of its own
+// below: a backward pass that enters the interpreter from the engine's thread costs some 50 us a node.
 
-decltype(&nvfp4_route_tokens) g_route = nullptr;
-decltype(&nvfp4_sort_tokens) g_sort = nullptr;
-decltype(&nvfp4_unsort_tokens) g_unsort = nullptr;
-decltype(&nvfp4_linear) g_linear = nullptr;
+struct Entries {
+    decltype(&nvfp4_last_error) last_error;
+    decltype(&nvfp4_route_tokens) route;
+    decltype(&nvfp4_route_tokens_backward) route_backward;
+    decltype(&nvfp4_sort_tokens) sort;
+    decltype(&nvfp4_unsort_tokens) unsort;
+    decltype(&nvfp4_unsort_tokens_backward) unsort_backward;
+    decltype(&nvfp4_linear) linear;
+    decltype(&nvfp4_linear_dz) linear_dz;
+    decltype(&nvfp4_linear_dx) linear_dx;
+    decltype(&nvfp4_linear_dw) linear_dw;
+} g_entry = {};
 
-// bind_operators(addresses of nvfp4_route_tokens, nvfp4_sort_tokens, nvfp4_unsort_tokens, nvfp4_linear)
+// bind_operators(addresses of the entries in the order of Entries)
 PyObject* bind_operators(PyObject*, PyObject* const* args, Py_ssize_t count)
 {
-    if (count != 4) { PyErr_SetString(PyExc_TypeError, "bind_operators() takes four addresses"); return nullptr; }
-    void* p[4];
-    for (int i = 0; i < 4; ++i) {
+    constexpr int kEntries = sizeof(Entries) / sizeof(void*);
+    if (count != kEntries) { PyErr_SetString(PyExc_TypeError, "bind_operators() takes the addresses of the operators' entries"); return nullptr; }
+    void* p[kEntries];
+    for (int i = 0; i < kEntries; ++i) {
         p[i] = PyLong_AsVoidPtr(args[i]);
-        if (p[i] == nullptr && PyErr_Occurred()) return nullptr;
+        if (p[i] == nullptr) { if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "a null address"); return nullptr; }
     }
-    g_route = reinterpret_cast<decltype(g_route)>(p[0]);
-    g_sort = reinterpret_cast<decltype(g_sort)>(p[1]);
-    g_unsort = reinterpret_cast<decltype(g_unsort)>(p[2]);
-    g_linear = reinterpret_cast<decltype(g_linear)>(p[3]);
+    g_entry = Entries{reinterpret_cast<decltype(Entries::last_error)>(p[0]), reinterpret_cast<decltype(Entries::route)>(p[1]),
+                      reinterpret_cast<decltype(Entries::route_backward)>(p[2]), reinterpret_cast<decltype(Entries::sort)>(p[3]),
+                      reinterpret_cast<decltype(Entries::unsort)>(p[4]), reinterpret_cast<decltype(Entries::unsort_backward)>(p[5]),
+                      reinterpret_cast<decltype(Entries::linear)>(p[6]), reinterpret_cast<decltype(Entries::linear_dz)>(p[7]),
+                      reinterpret_cast<decltype(Entries::linear_dx)>(p[8]), reinterpret_cast<decltype(Entries::linear_dw)>(p[9])};
     Py_RETURN_NONE;
 }
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
 // NVFP4_DTYPE_* of a tensor's type, -1 for others
 int dtype_code(at::ScalarType type)
 {
     return type == at::kBFloat16 ? NVFP4_DTYPE_BF16 : type == at::kHalf ? NVFP4_DTYPE_F16 : type == at::kFloat ? NVFP4_DTYPE_F32 : -1;
 }
-// A 2-D tensor of one of the three types on the current device with contiguous rows that do not overlap, at least a row and a column, that
-// needs no gradient; ld: its row stride (of a single row: its length).
-const at::Tensor* matrix(PyObject* o, int64_t& ld)
+// A 2-D tensor of one of the three types on the current device with contiguous rows that do not overlap, at least a row and a column.
+const at::Tensor* matrix(PyObject* o)
 {
     if (!THPVariable_CheckExact(o)) return nullptr;
     const at::Tensor& t = THPVariable_Unpack(o);
-    if (!t.is_cuda() || t.layout() != at::kStrided || !t.has_storage() || t.dim() != 2 || dtype_code(t.scalar_type()) < 0 || t.size(0) < 1 || t.size(1) < 1 ||
-        t.size(0) > INT32_MAX || t.size(1) > INT32_MAX || (t.size(1) > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < t.size(1)) ||
-        t.get_device() != c10::cuda::current_device() || t.is_conj() || t.is_neg() || (t.requires_grad() && at::GradMode::is_enabled()))
-        return nullptr;
-    ld = t.size(0) > 1 ? t.stride(0) : t.size(1);
-    return &t;
+    return t.is_cuda() && t.layout() == at::kStrided && t.has_storage() && t.dim() == 2 && dtype_code(t.scalar_type()) >= 0 && t.size(0) >= 1 &&
+                   t.size(1) >= 1 && t.size(0) <= INT32_MAX && t.size(1) <= INT32_MAX && (t.size(1) == 1 || t.stride(1) == 1) &&
+                   (t.size(0) == 1 || t.stride(0) >= t.size(1)) && t.get_device() == c10::cuda::current_device() && !t.is_conj() && !t.is_neg()
+               ? &t
+               : nullptr;
 }
-// A contiguous tensor of the given type beside `like` that needs no gradient.
+// Row stride of such a tensor; of a single row its length
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+// A contiguous tensor of the given type beside `like`.
 const at::Tensor* beside(PyObject* o, at::ScalarType type, int64_t dim, const at::Tensor& like)
 {
     const at::Tensor* t = plain(o, type, dim);
-    return t != nullptr && t->get_device() == like.get_device() && t->is_contiguous() && !(t->requires_grad() && at::GradMode::is_enabled()) ? t : nullptr;
+    return t != nullptr && t->get_device() == like.get_device() && t->is_contiguous() ? t : nullptr;
 }
+bool wants_gradient(const at::Tensor* t) { return t != nullptr && t->requires_grad(); }
 // A small int argument; false where it is none.
 bool number(PyObject* o, int& value)
 {
@@ -150,9 +170,9 @@ bool number(PyObject* o, int& value)
     return v >= 0 && v <= INT32_MAX;
 }
 // Results as the interpreter has them: a tensor, or a tuple of them
-PyObject* wrapped(std::initializer_list<at::Tensor> tensors)
+PyObject* wrapped(const variable_list& tensors)
 {
-    if (tensors.size() == 1) return THPVariable_Wrap(*tensors.begin());
+    if (tensors.size() == 1) return THPVariable_Wrap(tensors[0]);
     PyObject* tuple = PyTuple_New(static_cast<Py_ssize_t>(tensors.size()));
     if (tuple == nullptr) return nullptr;
     Py_ssize_t i = 0;
@@ -163,113 +183,290 @@ PyObject* wrapped(std::initializer_list<at::Tensor> tensors)
     }
     return tuple;
 }
-template <typename F>
-int unlocked(F&& launch)
-{
-    Unlocked state;
-    return launch();
-}
 at::Tensor fresh(const at::Tensor& like, at::ScalarType type, at::IntArrayRef size) { return at::empty(size, like.options().dtype(type).requires_grad(false)); }
+cudaStream_t stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
+// An error of the library as an exception: in a forward call it sends the call the general way, which meets and names it again.
+void check(int rc)
+{
+    TORCH_CHECK(rc == 0, "nvfp4_b200 error ", rc, ": ", g_entry.last_error());
+}
+template <typename F>
+void forward(F&& launch)                 // holding the interpreter's lock
+{
+    int rc;
+    {
+        Unlocked unlocked;
+        rc = launch();
+    }
+    check(rc);
+}
+template <typename T>
+T* pointer(const at::Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
+// The gradient of an output in rows that the kernels can read
+at::Tensor in_rows(const at::Tensor& t) { return t.size(0) > 0 && t.size(1) > 0 && t.stride(1) == 1 && t.stride(0) >= t.size(1) ? t : t.contiguous(); }
+// Gradients that were computed without being recorded: whoever differentiates them again gets an error instead of nothing.
+variable_list once(variable_list grads)
+{
+    if (!at::GradMode::is_enabled()) return grads;
+    for (at::Tensor& t : grads)
+        if (t.defined()) t = t.detach().set_requires_grad(true);
+    auto guard = std::make_shared<torch::autograd::DelayedError>("the gradients of this operator are computed once and cannot be differentiated again",
+                                                                 static_cast<int64_t>(grads.size()));
+    return (*guard)(std::move(grads));
+}
 
-// The four below answer an error code of the library, or None to a call for the general way.
+variable_list route_forward(const at::Tensor& logits, int k, int scores, int renormalize)
+{
+    const int64_t tokens = logits.size(0);
+    at::Tensor ids = fresh(logits, at::kLong, {tokens, k}), weights = fresh(logits, at::kFloat, {tokens, k});
+    forward([&] {
+        return g_entry.route(logits.data_ptr(), row_stride(logits), dtype_code(logits.scalar_type()), tokens, static_cast<int>(logits.size(1)), k, scores,
+                             renormalize, pointer<int64_t>(ids), pointer<float>(weights), stream());
+    });
+    return {ids, weights};
+}
+struct RouteNode : torch::autograd::Function<RouteNode> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, int64_t k, int64_t scores, int64_t renormalize)
+    {
+        variable_list out = route_forward(logits, static_cast<int>(k), static_cast<int>(scores), static_cast<int>(renormalize));
+        ctx->set_materialize_grads(false);
+        ctx->mark_non_differentiable({out[0]});
+        ctx->save_for_backward({logits, out[0]});
+        ctx->saved_data["scores"] = scores;
+        ctx->saved_data["renormalize"] = renormalize;
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        if (!grads[1].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &logits = saved[0], &ids = saved[1], g = grads[1].contiguous();
+        const c10::cuda::CUDAGuard guard(logits.device());
+        at::Tensor dlogits = fresh(logits, logits.scalar_type(), logits.sizes());
+        check(g_entry.route_backward(logits.data_ptr(), row_stride(logits), dtype_code(logits.scalar_type()), logits.size(0), static_cast<int>(logits.size(1)),
+                                     static_cast<int>(ids.size(1)), static_cast<int>(ctx->saved_data["scores"].toInt()),
+                                     static_cast<int>(ctx->saved_data["renormalize"].toInt()), pointer<int64_t>(ids), pointer<float>(g), dlogits.data_ptr(),
+                                     stream()));
+        return once({dlogits, at::Tensor(), at::Tensor(), at::Tensor()});
+    }
+};
 
 // route(logits, k, scores code, renormalize) -> (ids, weights)
 PyObject* route(PyObject*, PyObject* const* args, Py_ssize_t count)
 {
-    int64_t ld;
     int k, scores, renormalize;
-    if (count != 4 || g_route == nullptr || !number(args[1], k) || !number(args[2], scores) || !number(args[3], renormalize)) Py_RETURN_NONE;
+    if (count != 4 || g_entry.route == nullptr || !number(args[1], k) || !number(args[2], scores) || !number(args[3], renormalize)) Py_RETURN_NONE;
     try {
-        const at::Tensor* logits = matrix(args[0], ld);
+        const at::Tensor* logits = matrix(args[0]);
         if (logits == nullptr || k < 1 || k > 32 || k > logits->size(1) || logits->size(1) > 1024) Py_RETURN_NONE;
-        const int64_t tokens = logits->size(0);
-        at::Tensor ids = fresh(*logits, at::kLong, {tokens, k}), weights = fresh(*logits, at::kFloat, {tokens, k});
-        const int rc = unlocked([&] { return g_route(logits->data_ptr(), ld, dtype_code(logits->scalar_type()), tokens, static_cast<int>(logits->size(1)), k, scores, renormalize,
-                               ids.data_ptr<int64_t>(), weights.data_ptr<float>(), c10::cuda::getCurrentCUDAStream().stream()); });
-        return rc == 0 ? wrapped({ids, weights}) : PyLong_FromLong(rc);
+        return wrapped(at::GradMode::is_enabled() && wants_gradient(logits) ? RouteNode::apply(*logits, k, scores, renormalize)
+                                                                            : route_forward(*logits, k, scores, renormalize));
     } catch (const std::exception&) {
         Py_RETURN_NONE;
     }
 }
+
+variable_list sort_forward(const at::Tensor& x, const at::Tensor& ids, int experts, int alignment)
+{
+    const int64_t tokens = x.size(0), k = ids.size(1), hidden = x.size(1), n = tokens * k;
+    const int64_t m = (n + std::min<int64_t>(experts, n) * (alignment - 1)) / alignment * alignment;
+    at::Tensor rows = fresh(x, x.scalar_type(), {m, hidden}), place = fresh(x, at::kLong, {tokens, k}), source = fresh(x, at::kInt, {m}),
+               m_indices = fresh(x, at::kInt, {m});
+    forward([&] {
+        return g_entry.sort(x.data_ptr(), row_stride(x), dtype_code(x.scalar_type()), tokens, static_cast<int>(k), static_cast<int>(hidden),
+                            pointer<int64_t>(ids), experts, alignment, m, rows.data_ptr(), pointer<int64_t>(place), pointer<int32_t>(source),
+                            pointer<int32_t>(m_indices), stream());
+    });
+    return {rows, place, source, m_indices};
+}
+at::Tensor sum_rows(const at::Tensor& rows, const at::Tensor& place, const at::Tensor& weights, bool locked)
+{
+    at::Tensor y = fresh(rows, rows.scalar_type(), {place.size(0), rows.size(1)});
+    auto launch = [&] {
+        return g_entry.unsort(rows.data_ptr(), row_stride(rows), dtype_code(rows.scalar_type()), rows.size(0), pointer<int64_t>(place),
+                              pointer<float>(weights), place.size(0), static_cast<int>(place.size(1)), static_cast<int>(rows.size(1)), y.data_ptr(),
+                              stream());
+    };
+    if (locked) forward(launch);
+    else check(launch());
+    return y;
+}
+struct SortNode : torch::autograd::Function<SortNode> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& ids, int64_t experts, int64_t alignment)
+    {
+        variable_list out = sort_forward(x, ids, static_cast<int>(experts), static_cast<int>(alignment));
+        ctx->set_materialize_grads(false);
+        ctx->mark_non_differentiable({out[1], out[2], out[3]});
+        ctx->save_for_backward({out[1]});
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        const c10::cuda::CUDAGuard guard(grads[0].device());
+        return once({sum_rows(in_rows(grads[0]), ctx->get_saved_variables()[0], at::Tensor(), false), at::Tensor(), at::Tensor(), at::Tensor()});
+    }
+};
 
 // sort(x, ids, num_experts, alignment) -> (rows, place, source, m_indices)
 PyObject* sort(PyObject*, PyObject* const* args, Py_ssize_t count)
 {
-    int64_t ld;
     int experts, alignment;
-    if (count != 4 || g_sort == nullptr || !number(args[2], experts) || !number(args[3], alignment)) Py_RETURN_NONE;
+    if (count != 4 || g_entry.sort == nullptr || !number(args[2], experts) || !number(args[3], alignment)) Py_RETURN_NONE;
     try {
-        const at::Tensor* x = matrix(args[0], ld);
+        const at::Tensor* x = matrix(args[0]);
         const at::Tensor* ids = x == nullptr ? nullptr : beside(args[1], at::kLong, 2, *x);
         if (ids == nullptr || ids->size(0) != x->size(0) || ids->size(1) < 1 || experts < 1 || experts > 1024 || alignment < 1 || alignment > (1 << 20))
             Py_RETURN_NONE;
-        const int64_t tokens = x->size(0), k = ids->size(1), hidden = x->size(1);
-        if (k > INT32_MAX / tokens) Py_RETURN_NONE;
-        const int64_t n = tokens * k, m = (n + std::min<int64_t>(experts, n) * (alignment - 1)) / alignment * alignment;
-        if (m > INT32_MAX) Py_RETURN_NONE;
-        at::Tensor rows = fresh(*x, x->scalar_type(), {m, hidden}), place = fresh(*x, at::kLong, {tokens, k}), source = fresh(*x, at::kInt, {m}),
-                   m_indices = fresh(*x, at::kInt, {m});
-        const int rc = unlocked([&] { return g_sort(x->data_ptr(), ld, dtype_code(x->scalar_type()), tokens, static_cast<int>(k), static_cast<int>(hidden), ids->data_ptr<int64_t>(),
-                              experts, alignment, m, rows.data_ptr(), place.data_ptr<int64_t>(), source.data_ptr<int32_t>(), m_indices.data_ptr<int32_t>(),
-                              c10::cuda::getCurrentCUDAStream().stream()); });
-        return rc == 0 ? wrapped({rows, place, source, m_indices}) : PyLong_FromLong(rc);
+        const int64_t n = x->size(0) * std::min<int64_t>(ids->size(1), INT32_MAX);
+        if (n > INT32_MAX || n + std::min<int64_t>(experts, n) * (alignment - 1) > INT32_MAX) Py_RETURN_NONE;
+        return wrapped(at::GradMode::is_enabled() && wants_gradient(x) ? SortNode::apply(*x, *ids, experts, alignment)
+                                                                       : sort_forward(*x, *ids, experts, alignment));
     } catch (const std::exception&) {
         Py_RETURN_NONE;
     }
 }
 
-// unsort(rows, place, weights or None) -> y
+struct UnsortNode : torch::autograd::Function<UnsortNode> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& rows, const at::Tensor& weights, const at::Tensor& place, const at::Tensor& source)
+    {
+        const bool want_rows = rows.requires_grad(), want_weights = weights.defined() && weights.requires_grad();
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({want_weights ? rows : at::Tensor(), weights, place, source});
+        ctx->saved_data["rows"] = want_rows;
+        ctx->saved_data["weights"] = want_weights;
+        return sum_rows(rows, place, weights, true);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        variable_list out(4);
+        if (!grads[0].defined()) return out;
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &rows = saved[0], &weights = saved[1], &place = saved[2], &source = saved[3], dy = in_rows(grads[0]);
+        const c10::cuda::CUDAGuard guard(dy.device());
+        const bool want_weights = ctx->saved_data["weights"].toBool();
+        if (ctx->saved_data["rows"].toBool()) out[0] = fresh(dy, dy.scalar_type(), {source.size(0), dy.size(1)});
+        if (want_weights) out[1] = fresh(dy, at::kFloat, place.sizes());
+        check(g_entry.unsort_backward(dy.data_ptr(), row_stride(dy), want_weights ? rows.data_ptr() : nullptr, want_weights ? row_stride(rows) : dy.size(1),
+                                      dtype_code(dy.scalar_type()), source.size(0), pointer<int64_t>(place), pointer<int32_t>(source),
+                                      pointer<float>(weights), place.size(0), static_cast<int>(place.size(1)), static_cast<int>(dy.size(1)),
+                                      pointer<void>(out[0]), pointer<float>(out[1]), stream()));
+        return once(std::move(out));
+    }
+};
+
+// unsort(rows, place, source, weights or None) -> y
 PyObject* unsort(PyObject*, PyObject* const* args, Py_ssize_t count)
 {
-    int64_t ld;
-    if (count != 3 || g_unsort == nullptr) Py_RETURN_NONE;
+    if (count != 4 || g_entry.unsort == nullptr) Py_RETURN_NONE;
     try {
-        const at::Tensor* rows = matrix(args[0], ld);
+        const at::Tensor* rows = matrix(args[0]);
         const at::Tensor* place = rows == nullptr ? nullptr : beside(args[1], at::kLong, 2, *rows);
-        if (place == nullptr || place->size(0) < 1 || place->size(1) < 1 || place->size(1) > INT32_MAX) Py_RETURN_NONE;
+        const at::Tensor* source = place == nullptr ? nullptr : beside(args[2], at::kInt, 1, *rows);
+        if (source == nullptr || source->size(0) != rows->size(0) || place->size(0) < 1 || place->size(1) < 1 || place->size(1) > INT32_MAX) Py_RETURN_NONE;
         const at::Tensor* weights = nullptr;
-        if (args[2] != Py_None) {
-            weights = beside(args[2], at::kFloat, 2, *rows);
+        if (args[3] != Py_None) {
+            weights = beside(args[3], at::kFloat, 2, *rows);
             if (weights == nullptr || weights->sizes() != place->sizes()) Py_RETURN_NONE;
         }
-        const int64_t tokens = place->size(0), hidden = rows->size(1);
-        at::Tensor y = fresh(*rows, rows->scalar_type(), {tokens, hidden});
-        const int rc = unlocked([&] { return g_unsort(rows->data_ptr(), ld, dtype_code(rows->scalar_type()), rows->size(0), place->data_ptr<int64_t>(),
-                                weights != nullptr ? weights->data_ptr<float>() : nullptr, tokens, static_cast<int>(place->size(1)),
-                                static_cast<int>(hidden), y.data_ptr(), c10::cuda::getCurrentCUDAStream().stream()); });
-        return rc == 0 ? wrapped({y}) : PyLong_FromLong(rc);
+        const at::Tensor w = weights != nullptr ? *weights : at::Tensor();
+        return THPVariable_Wrap(at::GradMode::is_enabled() && (wants_gradient(rows) || wants_gradient(weights)) ? UnsortNode::apply(*rows, w, *place, *source)
+                                                                                                                : sum_rows(*rows, *place, w, true));
     } catch (const std::exception&) {
         Py_RETURN_NONE;
     }
 }
+
+// bias, residual and slopes may be undefined
+at::Tensor linear_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias, const at::Tensor& residual, int activation, bool out32,
+                          const at::Tensor& slopes)
+{
+    const at::ScalarType out = out32 ? at::kFloat : x.scalar_type();
+    const int64_t m = x.size(0), n = w.size(0);
+    at::Tensor d = fresh(x, out, {m, n});
+    forward([&] {
+        return g_entry.linear(x.data_ptr(), row_stride(x), w.data_ptr(), row_stride(w), pointer<void>(bias), pointer<void>(residual),
+                              residual.defined() ? row_stride(residual) : 0, d.data_ptr(), n, pointer<int16_t>(slopes), slopes.defined() ? slopes.size(1) : 0,
+                              static_cast<int>(m), static_cast<int>(n), static_cast<int>(x.size(1)), dtype_code(x.scalar_type()), dtype_code(out),
+                              activation, nullptr, stream());
+    });
+    return d;
+}
+struct LinearNode : torch::autograd::Function<LinearNode> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias, const at::Tensor& residual,
+                              int64_t activation, bool out32)
+    {
+        const bool want_x = x.requires_grad(), want_w = w.requires_grad(), want_bias = bias.defined() && bias.requires_grad();
+        at::Tensor slopes;
+        if (activation != NVFP4_ACTIVATION_NONE && (want_x || want_w || want_bias)) slopes = fresh(x, at::kShort, {x.size(0), (w.size(0) + 7) / 8 * 8});
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({want_w ? x : at::Tensor(), want_x ? w : at::Tensor(), slopes});
+        ctx->saved_data["bias"] = want_bias;
+        ctx->saved_data["residual"] = residual.defined() && residual.requires_grad();
+        ctx->saved_data["type"] = static_cast<int64_t>(x.scalar_type());
+        return linear_forward(x, w, bias, residual, static_cast<int>(activation), out32, slopes);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        variable_list out(6);
+        if (!grads[0].defined()) return out;
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &x = saved[0], &w = saved[1], &slopes = saved[2];
+        const bool want_bias = ctx->saved_data["bias"].toBool(), products = x.defined() || w.defined();
+        if (ctx->saved_data["residual"].toBool()) out[3] = grads[0];
+        if (products || want_bias) {
+            const at::Tensor dd = in_rows(grads[0]);
+            const c10::cuda::CUDAGuard guard(dd.device());
+            const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
+            const int m = static_cast<int>(dd.size(0)), n = static_cast<int>(dd.size(1)), code = dtype_code(type);
+            // without an activation the incoming gradient is dz itself, where it can be an operand
+            const bool as_it_is = !slopes.defined() && dd.scalar_type() == type && row_stride(dd) % 8 == 0 && reinterpret_cast<uintptr_t>(dd.data_ptr()) % 16 == 0;
+            at::Tensor dz = as_it_is ? dd : products ? fresh(dd, type, {m, (n + 7) / 8 * 8}) : at::Tensor();
+            const int64_t ldz = dz.defined() ? row_stride(dz) : 0;
+            if (want_bias) out[2] = fresh(dd, type, {n});
+            if (want_bias || (products && !as_it_is))
+                check(g_entry.linear_dz(dd.data_ptr(), row_stride(dd), pointer<int16_t>(slopes), slopes.defined() ? slopes.size(1) : 0,
+                                        as_it_is ? nullptr : pointer<void>(dz), ldz, pointer<void>(out[2]), m, n, code, dtype_code(dd.scalar_type()), stream()));
+            if (w.defined()) {
+                out[0] = fresh(dd, type, {m, w.size(1)});
+                check(g_entry.linear_dx(dz.data_ptr(), ldz, w.data_ptr(), row_stride(w), out[0].data_ptr(), w.size(1), m, n, static_cast<int>(w.size(1)), code,
+                                        nullptr, stream()));
+            }
+            if (x.defined()) {
+                out[1] = fresh(dd, type, {n, x.size(1)});
+                check(g_entry.linear_dw(dz.data_ptr(), ldz, x.data_ptr(), row_stride(x), out[1].data_ptr(), x.size(1), m, n, static_cast<int>(x.size(1)), code,
+                                        nullptr, stream()));
+            }
+        }
+        return once(std::move(out));
+    }
+};
 
 // linear(x, w, bias or None, residual or None, activation code, FP32 output) -> d
 PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count)
 {
-    int64_t ldx, ldw, ldr = 0;
     int activation, out32;
-    if (count != 6 || g_linear == nullptr || !number(args[4], activation) || !number(args[5], out32)) Py_RETURN_NONE;
+    if (count != 6 || g_entry.linear == nullptr || !number(args[4], activation) || !number(args[5], out32)) Py_RETURN_NONE;
     try {
-        const at::Tensor* x = matrix(args[0], ldx);
-        const at::Tensor* w = matrix(args[1], ldw);
+        const at::Tensor* x = matrix(args[0]);
+        const at::Tensor* w = matrix(args[1]);
         if (x == nullptr || w == nullptr || x->scalar_type() == at::kFloat || w->scalar_type() != x->scalar_type() || w->size(1) != x->size(1)) Py_RETURN_NONE;
-        const int64_t m = x->size(0), n = w->size(0), k = x->size(1);
-        const at::ScalarType out = out32 ? at::kFloat : x->scalar_type();
-        const at::Tensor *bias = nullptr, *residual = nullptr;
+        at::Tensor bias, residual;
         if (args[2] != Py_None) {
-            bias = beside(args[2], x->scalar_type(), 1, *x);
-            if (bias == nullptr || bias->size(0) != n) Py_RETURN_NONE;
+            const at::Tensor* t = beside(args[2], x->scalar_type(), 1, *x);
+            if (t == nullptr || t->size(0) != w->size(0)) Py_RETURN_NONE;
+            bias = *t;
         }
         if (args[3] != Py_None) {
-            residual = matrix(args[3], ldr);
-            if (residual == nullptr || residual->scalar_type() != out || residual->size(0) != m || residual->size(1) != n) Py_RETURN_NONE;
+            const at::Tensor* t = matrix(args[3]);
+            if (t == nullptr || t->scalar_type() != (out32 ? at::kFloat : x->scalar_type()) || t->size(0) != x->size(0) || t->size(1) != w->size(0))
+                Py_RETURN_NONE;
+            residual = *t;
         }
-        at::Tensor d = fresh(*x, out, {m, n});
-        const int rc = unlocked([&] { return g_linear(x->data_ptr(), ldx, w->data_ptr(), ldw, bias != nullptr ? bias->data_ptr() : nullptr,
-                                residual != nullptr ? residual->data_ptr() : nullptr, ldr, d.data_ptr(), n, nullptr, 0, static_cast<int>(m),
-                                static_cast<int>(n), static_cast<int>(k), dtype_code(x->scalar_type()), dtype_code(out), activation, nullptr,
-                                c10::cuda::getCurrentCUDAStream().stream()); });
-        return rc == 0 ? wrapped({d}) : PyLong_FromLong(rc);
+        const bool record = at::GradMode::is_enabled() && (wants_gradient(x) || wants_gradient(w) || (bias.defined() && bias.requires_grad()) ||
+                                                           (residual.defined() && residual.requires_grad()));
+        return THPVariable_Wrap(record ? LinearNode::apply(*x, *w, bias, residual, activation, out32 != 0)
+                                       : linear_forward(*x, *w, bias, residual, activation, out32 != 0, at::Tensor()));
     } catch (const std::exception&) {
         Py_RETURN_NONE;
     }

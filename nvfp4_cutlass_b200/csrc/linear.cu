@@ -14,6 +14,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cmath>
 #include <cstdint>
 #include <type_traits>
 
@@ -172,10 +173,21 @@ __device__ __forceinline__ void finish(float (&v)[kN], uint32_t row0, uint32_t c
 #pragma unroll
         for (uint32_t i = 0; i < kN; ++i) v[i] += to_float(r[i]);
     }
+    if (!mine) return;
+    // eight stores in a row where there are eight rows: each in a branch of its own they took a microsecond for 32
     D* to = static_cast<D*>(e.d) + static_cast<int64_t>(row0) * e.ldd + at;
 #pragma unroll
-    for (uint32_t i = 0; i < kN; ++i)
-        if (i < rows && mine) to[i * e.ldd] = from_float<D>(v[i]);
+    for (uint32_t g = 0; g < kN; g += 8) {
+        if (g + 8 <= rows) {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) to[i * e.ldd] = from_float<D>(v[g + i]);
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+                if (g + i < rows) to[i * e.ldd] = from_float<D>(v[g + i]);
+        }
+        to += 8 * e.ldd;
+    }
 }
 
 // 32 x 32 values, lane l holding row l: afterwards lane l holds column l.  Five butterfly steps.
@@ -367,6 +379,7 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t tile, bool mn_major, u
                     : ptx::make_smem_desc(tile + step * 32, 8 * kRowBytes, ptx::kSwizzle128B);
 }
 
+constexpr int kTileSmem = 216 * 1024;                // most that a block of product_kernel takes
 struct Product {
     uint32_t tiles_a, tiles_b, k_blocks;
     uint32_t splits_log2, depth;                     // product_kernel: CTAs to a tile, ring positions
@@ -379,9 +392,14 @@ struct Product {
 constexpr int kTileThreads = 192;                    // warp 0: TMA, warp 1: products, warps 2-5: epilogue
 constexpr uint32_t kTileEpiWarps = 4;
 constexpr uint32_t tile_stage(uint32_t bn) { return kSlotA + bn * kRowBytes; }
-constexpr uint32_t tile_smem(uint32_t bn, uint32_t depth, bool split)
+// Partial sums of a cluster: [source CTA][row][columns that a CTA finishes, and padding that keeps the rows on different banks].
+// A row moves `partial_words` at a time; sixteen columns among eight CTAs leave two to each, which need no padding.
+constexpr uint32_t partial_words(uint32_t bn) { return bn < 32 ? 2 : 4; }
+__host__ __device__ constexpr uint32_t partial_pad(uint32_t bn, uint32_t splits) { return bn >= 32 ? 4 : splits == 8 ? 0 : 2; }
+__host__ __device__ constexpr uint32_t partial_bytes(uint32_t bn, uint32_t splits) { return splits > 1 ? (bn + splits * partial_pad(bn, splits)) * BM * 4 : 0; }
+constexpr uint32_t tile_smem(uint32_t bn, uint32_t depth, uint32_t splits)
 {
-    return 1024 + depth * tile_stage(bn) + (split ? bn * BM * 4 : 0) + (2 * kMaxDepth + 4) * 8 + 16 + kTileEpiWarps * 16;
+    return 1024 + depth * tile_stage(bn) + partial_bytes(bn, splits) + (2 * kMaxDepth + 4) * 8 + 16 + kTileEpiWarps * 16;
 }
 // For an FP32 output the epilogue warps take the accumulators over every four K blocks and add them up in registers, two accumulators in
 // turn: the tensor core cuts what it adds to a long sum (K = 4096 in one accumulator: off by 4.3e-6 of the result, FP32 sums by 6e-7).
@@ -400,8 +418,8 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     const uint32_t smem = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (smem - ptx::smem_u32(smem_raw));
     const uint32_t splits = 1u << p.splits_log2, depth = p.depth;
-    float* partial = reinterpret_cast<float*>(gen + depth * kStage);          // [splits][BN / splits][BM], from each CTA of the cluster
-    uint64_t* full = reinterpret_cast<uint64_t*>(gen + depth * kStage + (splits > 1 ? BN * BM * 4 : 0));
+    const uint32_t partial = smem + depth * kStage;
+    uint64_t* full = reinterpret_cast<uint64_t*>(gen + depth * kStage + partial_bytes(BN, splits));
     uint64_t* drained = full + kMaxDepth;
     uint64_t* tmem_full = drained + kMaxDepth;       // per accumulator
     uint64_t* tmem_empty = tmem_full + 2;
@@ -528,21 +546,26 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     };
     if (splits > 1) {
         const uint32_t width_log2 = __popc(BN - 1) - p.splits_log2, width = 1u << width_log2;          // columns that a CTA finishes
+        constexpr uint32_t kWords = partial_words(BN);
+        const uint32_t pitch = (width + partial_pad(BN, splits)) * 4, block = BM * pitch;                       // of a row, of a source's rows
         if (warp >= 2 && ok) {
-            const uint32_t mine = ptx::smem_u32(partial + ((rank << width_log2) * BM + row));
+            const uint32_t mine = partial + rank * block + row * pitch;
 #pragma unroll 1
             for (uint32_t c0 = 0; c0 < live; c0 += kChunk) {
                 float v[kChunk];
                 load_accumulators(taddr + c0, v);
 #pragma unroll
-                for (uint32_t i = 0; i < kChunk; ++i) {
-                    const uint32_t c = c0 + i;
-                    if (c < live) ptx::st_cluster_f32(ptx::map_to_cta(mine + (c & (width - 1)) * BM * 4, c >> width_log2), v[i]);
+                for (uint32_t i = 0; i < kChunk; i += kWords) {
+                    const uint32_t c = c0 + i;               // columns that nobody wants included: they have their place, too
+                    const uint32_t to = ptx::map_to_cta(mine + (c & (width - 1)) * 4, c >> width_log2);
+                    if constexpr (kWords == 4) ptx::st_cluster_f32x4(to, v[i], v[i + 1], v[i + 2], v[i + 3]);
+                    else ptx::st_cluster_f32x2(to, v[i], v[i + 1]);
                 }
             }
         }
         ptx::cluster_sync();                         // partial sums have arrived; nobody touches another CTA's memory from here on
         if (warp >= 2 && ok) {
+            const float* mine = reinterpret_cast<const float*>(gen + (partial - smem) + row * pitch);
 #pragma unroll 1
             for (uint32_t c0 = 0; c0 < width; c0 += kChunk) {
                 const uint32_t first = rank * width + c0;
@@ -550,12 +573,30 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                 const uint32_t count = min(min(width - c0, kChunk), live - first);
                 float v[kChunk];
 #pragma unroll
-                for (uint32_t i = 0; i < kChunk; ++i) v[i] = 0.0f;
-                for (uint32_t s = 0; s < splits; ++s) {
-                    const float* from = partial + ((s << width_log2) + c0) * BM + row;
+                for (uint32_t i = 0; i < kChunk; i += kWords) {
 #pragma unroll
-                    for (uint32_t i = 0; i < kChunk; ++i)
-                        if (i < count) v[i] += from[i * BM];
+                    for (uint32_t j = 0; j < kWords; ++j) v[i + j] = 0.0f;
+                    if (i >= count) continue;                // (width is a multiple of kWords)
+                    // in the order of the sources, eight loads under way
+                    float4 part[8];
+#pragma unroll
+                    for (uint32_t s = 0; s < 8; ++s) {
+                        const float* from = mine + s * (block / 4) + c0 + i;
+                        if (s >= splits) continue;
+                        if constexpr (kWords == 4) {
+                            part[s] = *reinterpret_cast<const float4*>(from);
+                        } else {
+                            const float2 two = *reinterpret_cast<const float2*>(from);
+                            part[s] = make_float4(two.x, two.y, 0.0f, 0.0f);
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t s = 0; s < 8; ++s) {
+                        if (s >= splits) continue;
+                        v[i] += part[s].x;
+                        v[i + 1] += part[s].y;
+                        if constexpr (kWords == 4) { v[i + 2] += part[s].z; v[i + 3] += part[s].w; }
+                    }
                 }
                 give(v, first, kSwap ? count : 32);
             }
@@ -784,6 +825,9 @@ struct Operands {
     int32_t* status;
 };
 
+// CTAs that find an SM of their own: clusters of four and eight do not divide the SMs of every GPC.
+int ctas_at_once(uint32_t splits_log2, int num_sms) { return splits_log2 < 2 ? num_sms : num_sms * 13 / 15; }
+
 template <typename T, typename D, uint32_t BN, bool kSwap>
 int launch_tiles(const Operands& o, Epilogue e, uint32_t splits_log2, int num_sms, cudaStream_t stream)
 {
@@ -803,20 +847,21 @@ int launch_tiles(const Operands& o, Epilogue e, uint32_t splits_log2, int num_sm
     p.b_mn = o.b_mn;
     p.status = o.status;
     const uint64_t ctas = static_cast<uint64_t>(p.tiles_a) * p.tiles_b << splits_log2;
-    // one CTA to an SM: its ring may fill the shared memory; more: two share it
-    const uint32_t budget = ctas <= static_cast<uint64_t>(num_sms) ? 200 * 1024 : 112 * 1024;
+    // One CTA to an SM: its ring may fill the shared memory; more: two share it.  Clusters of eight, too, leave room for a second CTA: of
+    // those that fill their SMs not even sixteen run at once (256 x 128 x 4096, 16 of them: 8.9 us, a second wave; 5.7 so).
+    const uint32_t budget = ctas <= static_cast<uint64_t>(ctas_at_once(splits_log2, num_sms)) && splits_log2 < 3 ? kTileSmem : 112 * 1024;
     p.depth = kMaxDepth;
-    while (p.depth > 2 && tile_smem(BN, p.depth, splits_log2 != 0) > budget) --p.depth;
+    while (p.depth > 2 && tile_smem(BN, p.depth, 1u << splits_log2) > budget) --p.depth;
     int dev = 0;
     NVFP4_CUDA_CHECK(cudaGetDevice(&dev));
     static bool attr_set[host::kMaxDevices] = {};
     if (!attr_set[dev]) {
-        NVFP4_CUDA_CHECK(cudaFuncSetAttribute(product_kernel<T, D, BN, kSwap>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+        NVFP4_CUDA_CHECK(cudaFuncSetAttribute(product_kernel<T, D, BN, kSwap>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmem));
         attr_set[dev] = true;
     }
     NVFP4_REQUIRE(ctas <= INT32_MAX, "too many tiles (%llu)", static_cast<unsigned long long>(ctas));
     return host::launch_kernel_cluster(product_kernel<T, D, BN, kSwap>, dim3(static_cast<unsigned>(ctas)), dim3(kTileThreads),
-                                       tile_smem(BN, p.depth, splits_log2 != 0), stream, true, 1u << splits_log2, tm_a, tm_b, maps, p, e);
+                                       tile_smem(BN, p.depth, 1u << splits_log2), stream, true, 1u << splits_log2, tm_a, tm_b, maps, p, e);
 }
 
 template <typename T>
@@ -847,32 +892,68 @@ int launch_pairs(const Operands& o, Epilogue e, int num_sms, cudaStream_t stream
                                        kPairSmem, stream, true, 2u, tm_a, tm_b, maps, p, e);
 }
 
+// Which kernel, which tile and how many CTAs to a tile: the form with the smallest estimate, in microseconds,
+//     start + splitting + |(K blocks of a CTA * time of one * CTAs to an SM, operands / HBM)|
+// Measured on a B200 (BF16, alone on the GPU): a block of 64 of K takes a CTA 0.16 us at BN = 16 to 0.235 at 128, the time its bytes take into
+// one SM, and a CTA pair 0.29, the time of its products.  What is left at K -> 0 is the start.  Adding partial sums over a
+// cluster costs by the tile's columns.  Estimates are within a tenth or so of what was measured: 64 x 4096 x 4096 (swap 64 / 4) 10.4 for
+// 11.1, 256 x 1024 x 4096 (swap 64 / 4) 7.9 for 9.9, 512 x 4096 x 4096 (normal 128) 18 for 19, 1024 x 4096 x 4096 (pairs) 24 for 26.  Against the
+// best of all forms by measurement the choice loses up to 8 % over 1 to 2048 rows, 128 to 4096 columns, K 1024 and 4096.
+struct Form {
+    enum Kind { kSwap, kNormal, kPairs } kind;
+    uint32_t bn, splits_log2;
+};
+struct TileCost {
+    uint32_t bn;
+    double block, start_swap, start_normal, split;
+};
+constexpr TileCost kTileCosts[] = {{16, 0.16, 2.5, 0, 0.45}, {32, 0.17, 2.5, 0, 1.5}, {64, 0.20, 2.4, 2.6, 2.3}, {128, 0.235, 3.3, 3.0, 5.0}};
+Form choose_form(const Operands& o, bool wide, int num_sms)
+{
+    const double hbm = (static_cast<double>(o.rows_a) + o.rows_b) * o.k * 2 / 6.0e6;
+    const uint32_t k_blocks = (o.k + BK - 1) / BK;
+    auto blocks = [](uint32_t rows, uint32_t tile) { return (rows + tile - 1) / tile; };
+    Form best{Form::kNormal, 128, 0};
+    double least = 1e30;
+    auto consider = [&](Form::Kind kind, uint64_t tiles, const TileCost& c, double start, uint32_t most_log2) {
+        for (uint32_t s = 0; s <= most_log2 && (k_blocks >> s) >= 2; ++s) {
+            const uint64_t at_once = ctas_at_once(s, num_sms);
+            const double resident = static_cast<double>(((tiles << s) + at_once - 1) / at_once);
+            const double loop = ((k_blocks + (1u << s) - 1) >> s) * c.block * resident;
+            const double t = start * (resident > 2 ? resident / 2 : 1) + (s ? c.split : 0) + std::sqrt(loop * loop + hbm * hbm);
+            if (t < least) { least = t; best = Form{kind, c.bn, s}; }
+            if (tiles << (s + 1) > 2 * static_cast<uint64_t>(num_sms)) break;
+        }
+    };
+    for (const TileCost& c : kTileCosts) {
+        if (!o.a_mn && !o.b_mn) consider(Form::kSwap, static_cast<uint64_t>(blocks(o.rows_b, BM)) * blocks(o.rows_a, c.bn), c, c.start_swap, c.bn <= 32 ? 3 : 2);
+        if (c.start_normal > 0) consider(Form::kNormal, static_cast<uint64_t>(blocks(o.rows_a, BM)) * blocks(o.rows_b, c.bn), c, c.start_normal, c.bn / 64);
+    }
+    if (!wide && num_sms >= 2) {
+        const uint64_t tiles = static_cast<uint64_t>(blocks(o.rows_a, 2 * BM)) * blocks(o.rows_b, kPairBN), pairs = num_sms / 2;
+        const double loop = static_cast<double>((tiles + pairs - 1) / pairs) * k_blocks * 0.29, t = 5.0 + std::sqrt(loop * loop + hbm * hbm);
+        if (t < least) best = Form{Form::kPairs, kPairBN, 0};
+    }
+    return best;
+}
+
 // The output (rows_a, rows_b), of type D.
 template <typename T, typename D>
 int launch_product(const Operands& o, const Epilogue& e, int num_sms, cudaStream_t stream)
 {
-    const uint32_t k_blocks = (o.k + BK - 1) / BK;
-    auto splits_for = [&](uint64_t tiles, uint32_t most_log2) {
-        uint32_t s = 0;
-        while (s < most_log2 && (tiles << (s + 1)) <= static_cast<uint64_t>(num_sms) && k_blocks >> (s + 1) >= 4) ++s;
-        return s;
-    };
-    // a few rows: the weight's rows on the tensor memory's lanes, as many tokens to a tile as there are
-    if (o.rows_a <= 128 && !o.a_mn && !o.b_mn) {
+    const Form f = choose_form(o, !std::is_same<D, T>::value, num_sms);
+    if (f.kind == Form::kSwap) {                     // the weight's rows on the tensor memory's lanes
         const Operands s{o.b, o.ldb, false, o.rows_b, o.a, o.lda, false, o.rows_a, o.k, o.status};
-        const uint32_t splits = splits_for((o.rows_b + BM - 1) / BM, 3);
-        if (o.rows_a <= 16) return launch_tiles<T, D, 16, true>(s, e, splits, num_sms, stream);
-        if (o.rows_a <= 32) return launch_tiles<T, D, 32, true>(s, e, splits, num_sms, stream);
-        if (o.rows_a <= 64) return launch_tiles<T, D, 64, true>(s, e, splits, num_sms, stream);
-        return launch_tiles<T, D, 128, true>(s, e, splits, num_sms, stream);
+        switch (f.bn) {
+            case 16: return launch_tiles<T, D, 16, true>(s, e, f.splits_log2, num_sms, stream);
+            case 32: return launch_tiles<T, D, 32, true>(s, e, f.splits_log2, num_sms, stream);
+            case 64: return launch_tiles<T, D, 64, true>(s, e, f.splits_log2, num_sms, stream);
+            default: return launch_tiles<T, D, 128, true>(s, e, f.splits_log2, num_sms, stream);
+        }
     }
-    if constexpr (std::is_same<D, T>::value) {
-        const uint64_t pair_tiles = static_cast<uint64_t>((o.rows_a + 255) / 256) * ((o.rows_b + 255) / 256);
-        if (pair_tiles * 2 >= static_cast<uint64_t>(num_sms / 2) && o.rows_b > 128) return launch_pairs<T>(o, e, num_sms, stream);
-    }
-    const uint64_t tiles_128 = static_cast<uint64_t>((o.rows_a + 127) / 128) * ((o.rows_b + 127) / 128);
-    if (o.rows_b <= 64) return launch_tiles<T, D, 64, false>(o, e, splits_for((o.rows_a + 127) / 128, 1), num_sms, stream);
-    return launch_tiles<T, D, 128, false>(o, e, splits_for(tiles_128, 2), num_sms, stream);
+    if constexpr (std::is_same<D, T>::value)
+        if (f.kind == Form::kPairs) return launch_pairs<T>(o, e, num_sms, stream);
+    return f.bn == 64 ? launch_tiles<T, D, 64, false>(o, e, f.splits_log2, num_sms, stream) : launch_tiles<T, D, 128, false>(o, e, f.splits_log2, num_sms, stream);
 }
 
 // ---- dz and the bias' gradient -----------------------------------------------------------------------------------------

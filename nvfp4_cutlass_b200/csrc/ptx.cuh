@@ -478,10 +478,14 @@ NVFP4_DEVICE uint32_t map_to_cta(uint32_t smem_addr, uint32_t rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
     return r;
 }
-// One word into shared memory of a CTA of the cluster (address from map_to_cta).
-NVFP4_DEVICE void st_cluster_f32(uint32_t cluster_addr, float v)
+// Two or four words into shared memory of a CTA of the cluster (address from map_to_cta).
+NVFP4_DEVICE void st_cluster_f32x2(uint32_t cluster_addr, float a, float b)
 {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_addr), "f"(a), "f"(b) : "memory");
+}
+NVFP4_DEVICE void st_cluster_f32x4(uint32_t cluster_addr, float a, float b, float c, float d)
+{
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
 NVFP4_DEVICE void cluster_sync()
 {

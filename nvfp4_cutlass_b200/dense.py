@@ -47,7 +47,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     gradient in front of the activation to the operands' type: the tensor cores take no wider operands."""
     if _C._binding is not None and device_status is None and activation in _C.ACTIVATION_CODES and (out_dtype is None or out_dtype is torch.float32 or out_dtype is x.dtype):
         result = _C._binding.linear(x, w, bias, residual, _C.ACTIVATION_CODES[activation], 1 if out_dtype is torch.float32 else 0)
-        if _C.answered(result):
+        if result is not None:
             return result
     if not _differentiable(x, w, bias, residual):
         return _C.linear(x, w, bias, residual, activation, out_dtype, device_status=device_status)[0]

@@ -28,6 +28,7 @@ class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, k, scores, renormalize):
         ids, weights = _C.route_tokens(logits, k, scores, renormalize)
+        ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, ids)
         ctx.form = (scores, renormalize)
         ctx.mark_non_differentiable(ids)
@@ -36,6 +37,8 @@ class _Route(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, _, dweights):
+        if dweights is None:
+            return None, None, None, None
         logits, ids = ctx.saved_tensors
         return _C.route_tokens_backward(logits, ids, dweights, *ctx.form), None, None, None
 
@@ -49,7 +52,7 @@ def route_tokens(logits: torch.Tensor, k: int, *, scores: str = "softmax", renor
     (``sort_tokens`` gives such a pair no row).  experts <= 1024, k <= 32.  Differentiable in ``logits``."""
     if _C._binding is not None and scores in _C.SCORE_CODES:
         result = _C._binding.route(logits, k, _C.SCORE_CODES[scores], 1 if renormalize else 0)
-        if _C.answered(result):
+        if result is not None:
             return result
     if not _differentiable(logits):
         return _C.route_tokens(logits, int(k), scores, bool(renormalize))
@@ -67,6 +70,7 @@ class _Sort(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, ids, num_experts, alignment):
         rows, place, source, m_indices = _C.sort_tokens(x, ids, num_experts, alignment)
+        ctx.set_materialize_grads(False)
         ctx.save_for_backward(place)
         ctx.mark_non_differentiable(place, source, m_indices)
         return rows, place, source, m_indices
@@ -74,6 +78,8 @@ class _Sort(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, drows, *_):
+        if drows is None:
+            return None, None, None, None
         return _C.unsort_tokens(drows.contiguous(), ctx.saved_tensors[0], None), None, None, None
 
 
@@ -87,7 +93,7 @@ def sort_tokens(x: torch.Tensor, ids: torch.Tensor, num_experts: int, *, alignme
     are; FP16 and FP32 rows are moved too.  num_experts <= 1024.  Differentiable in ``x``."""
     if _C._binding is not None:
         result = _C._binding.sort(x, ids, num_experts, alignment)
-        if _C.answered(result):
+        if result is not None:
             return result[0], TokenOrder(*result[1:])
     call = _Sort.apply if _differentiable(x) else _C.sort_tokens
     rows, place, source, m_indices = call(x, ids, int(num_experts), int(alignment))
@@ -117,9 +123,9 @@ def unsort_tokens(rows: torch.Tensor, order: TokenOrder, weights: Optional[torch
     ascending j, rounded once.  A pair without a row contributes nothing, and its weight's gradient is 0.  Differentiable in ``rows`` and
     ``weights``; the gradient of rows without a pair is zero."""
     place, source = order.place, order.source
-    if _C._binding is not None and rows.shape[0] == source.shape[0]:
-        result = _C._binding.unsort(rows, place, weights)
-        if _C.answered(result):
+    if _C._binding is not None:
+        result = _C._binding.unsort(rows, place, source, weights)
+        if result is not None:
             return result
     _C._require(isinstance(rows, torch.Tensor) and source.dtype == torch.int32 and source.dim() == 1 and source.is_contiguous() and
                 rows.dim() == 2 and rows.shape[0] == source.shape[0], "rows has the rows of the order")

@@ -494,10 +494,12 @@ def test_the_binding_takes_no_host_tensors_and_no_odd_arguments():
     x, ids = torch.zeros(4, 8), torch.zeros(4, 2, dtype=torch.int64)
     assert b.route(x, 2, 0, 1) is None and b.route(None, 2, 0, 1) is None and b.route(x, "2", 0, 1) is None and b.route(x) is None
     assert b.sort(x, ids, 4, 16) is None and b.sort(x, None, 4, 16) is None and b.sort(x, ids, -4, 16) is None
-    assert b.unsort(x, ids, None) is None and b.unsort(x, ids, 3) is None and b.unsort(x) is None
+    assert b.unsort(x, ids, ids, None) is None and b.unsort(x, ids, 3, None) is None and b.unsort(x) is None
     assert b.linear(x, x, None, None, 0, 0) is None and b.linear(x, x, None, None, 1 << 40, 0) is None and b.linear(x) is None
     with pytest.raises(TypeError):
         b.bind_operators(1)
+    with pytest.raises(TypeError):
+        b.bind_operators(*[0] * 10)
 
 
 @gpu
@@ -516,15 +518,56 @@ def test_the_binding_gives_the_general_way_s_results(monkeypatch):
     _C.lib()
     assert _C._binding is not None
     fast = calls()
-    # what it leaves to the general way: strided index tensors, tensors that need a gradient, empty ones
-    b = _C._binding
-    ids = fast[0]
-    assert b.sort(x, ids.t().contiguous().t(), 24, 16) is None and b.route(logits.clone().requires_grad_(), 3, 0, 1) is None
-    assert b.linear(x, w.clone().requires_grad_(), None, None, 0, 0) is None and b.linear(x[:0], w, None, None, 0, 0) is None
-    with torch.no_grad():
-        assert b.linear(x, w.clone().requires_grad_(), None, None, 0, 0) is not None
+    # what it leaves to the general way: strided index tensors, empty ones
+    b, ids = _C._binding, fast[0]
+    assert b.sort(x, ids.t().contiguous().t(), 24, 16) is None and b.linear(x[:0], w, None, None, 0, 0) is None
     assert torch.equal(sort_tokens(x, ids.t().contiguous().t(), 24, alignment=16)[0], fast[2])
-    with pytest.raises(RuntimeError, match="K must be"):
+    with pytest.raises(RuntimeError, match="multiple of 8"):
         nvfp4_gemm.linear(x[:, :60], w[:, :60])
     monkeypatch.setattr(_C, "_binding", None)
     assert all(torch.equal(a, b) for a, b in zip(fast, calls()))
+
+
+@gpu
+def test_the_binding_s_gradients_are_the_general_way_s(monkeypatch):
+    g = gen(7)
+    leaf = lambda *shape, dtype=torch.bfloat16: torch.randn(*shape, generator=g).to(dtype).cuda().requires_grad_()
+    logits, x, w, bias, residual = leaf(50, 24, dtype=torch.float32), leaf(50, 72), leaf(41, 72), leaf(41), leaf(50, 41, dtype=torch.float32)
+    gw, gr, gy, gd = (torch.randn(*s, generator=g).cuda() for s in ((50, 3), (50, 72), (50, 72), (50, 41)))
+
+    def grads():
+        out = []
+        ids, weights = route_tokens(logits, 3, scores="sigmoid")
+        out += torch.autograd.grad(weights, logits, gw, retain_graph=True)
+        rows, order = sort_tokens(x, ids, 24, alignment=16)
+        y = unsort_tokens(rows, order, weights)
+        out += torch.autograd.grad(y, [x, logits, rows], gy.bfloat16(), retain_graph=True)
+        out += torch.autograd.grad(unsort_tokens(rows, order), rows, gy.bfloat16(), retain_graph=True)
+        for act in ("none", "silu"):
+            d = nvfp4_gemm.linear(x, w, bias, residual, activation=act, out_dtype=torch.float32)
+            out += torch.autograd.grad(d, [x, w, bias, residual], gd, retain_graph=True)
+            out += torch.autograd.grad(d, [residual], gd, retain_graph=True)
+            out += torch.autograd.grad(nvfp4_gemm.linear(x.detach(), w, bias, activation=act), [w], gd.bfloat16())
+        # a second derivative is an error, not nothing
+        (first,) = torch.autograd.grad(weights.sum(), logits, create_graph=True)
+        with pytest.raises(RuntimeError, match="once|does not require grad"):
+            first.sum().backward()
+        return out
+
+    _C.lib()
+    assert _C._binding is not None
+    fast = grads()
+    monkeypatch.setattr(_C, "_binding", None)
+    slow = grads()
+    assert len(fast) == len(slow) and all(torch.equal(a, b) for a, b in zip(fast, slow))
+
+
+@gpu
+def test_what_is_not_differentiated_costs_nothing():
+    x = torch.randn(6, 8, generator=gen(1)).cuda().requires_grad_()
+    rows, order = sort_tokens(x, some_ids(6, 2, 4, 1, "uniform").cuda(), 4, alignment=16)
+    assert rows.requires_grad and not any(t.requires_grad for t in order)
+    ids, weights = route_tokens(x, 2)
+    assert weights.requires_grad and not ids.requires_grad
+    with torch.no_grad():
+        assert not sort_tokens(x, ids, 8)[0].requires_grad and not route_tokens(x, 2)[1].requires_grad
