@@ -11,6 +11,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "host_common.hpp"
 #include "launchers.hpp"
@@ -42,6 +43,17 @@ __device__ __forceinline__ float value_of(uint32_t key)
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 constexpr uint32_t kMaskedKey = 0x007fffffu;                                  // of -inf
+
+// A 16-bit logit's rank in 21 bits (its place among the type's 2^16 values, masked ones and NaN as above) over the index, the lowest on top.
+// FP32 keys of BF16 values differ in their upper 16 bits alone; FP16 values take 10 digits and, subnormal ones included, 6 bits of
+// exponent in FP32 (2^-24 to 2^15), so that bits 13 to 31 tell them apart.
+constexpr uint32_t kIndexMask = 1023u;
+template <typename T>
+__device__ __forceinline__ uint32_t packed_key(uint32_t key, uint32_t index)
+{
+    constexpr uint32_t kShift = std::is_same<T, __nv_bfloat16>::value ? 16 : 13;
+    return (key >> kShift << 10) + (kIndexMask - index);
+}
 
 __device__ __forceinline__ float warp_sum(float v)
 {
@@ -93,21 +105,46 @@ route_kernel(const T* __restrict__ logits, int64_t ld, int64_t tokens, int exper
     }
     int id = -1;
     uint32_t chosen = kMaskedKey;
-    for (int j = 0; j < k; ++j) {
-        const uint32_t m = __reduce_max_sync(kAll, best);
-        if (m <= kMaskedKey) break;                                           // nothing left but masked experts
-        uint32_t at = 0xffffffffu;                                            // the lowest index of the lane with this key
+    if constexpr (sizeof(T) == 2) {
+        // A 16-bit logit's key has its digits in the upper half (both types' infinities and NaN included: the order of FP32 values that are
+        // exact in them is that of their upper bits), which leaves room for the index: one reduction a round.
+        best = 0;
 #pragma unroll
-        for (int r = V - 1; r >= 0; --r)
-            if (key[r] == m) at = r * 32 + lane;
-        const uint32_t winner = __reduce_min_sync(kAll, at);
-        if (lane == j) { id = static_cast<int>(winner); chosen = m; }
-        if ((winner & 31u) == static_cast<uint32_t>(lane)) {
-            best = 0;
+        for (int r = 0; r < V; ++r) {
+            if (r * 32 + lane < experts) key[r] = packed_key<T>(key[r], r * 32 + lane);
+            best = max(best, key[r]);
+        }
+        for (int j = 0; j < k; ++j) {
+            const uint32_t m = __reduce_max_sync(kAll, best);
+            if (m <= packed_key<T>(kMaskedKey, 0)) break;                     // nothing left but masked experts
+            if (lane == j) { id = static_cast<int>(kIndexMask - (m & kIndexMask)); }
+            if (best == m) {
+                best = 0;
 #pragma unroll
-            for (int r = 0; r < V; ++r) {
-                if (winner == static_cast<uint32_t>(r * 32 + lane)) key[r] = 0;
-                best = max(best, key[r]);
+                for (int r = 0; r < V; ++r) {
+                    if (key[r] == m) key[r] = 0;
+                    best = max(best, key[r]);
+                }
+            }
+        }
+        if (id >= 0) chosen = key_of(to_float(row[id]));
+    } else {
+        for (int j = 0; j < k; ++j) {
+            const uint32_t m = __reduce_max_sync(kAll, best);
+            if (m <= kMaskedKey) break;
+            uint32_t at = 0xffffffffu;                                        // the lowest index of the lane with this key
+#pragma unroll
+            for (int r = V - 1; r >= 0; --r)
+                if (key[r] == m) at = r * 32 + lane;
+            const uint32_t winner = __reduce_min_sync(kAll, at);
+            if (lane == j) { id = static_cast<int>(winner); chosen = m; }
+            if ((winner & 31u) == static_cast<uint32_t>(lane)) {
+                best = 0;
+#pragma unroll
+                for (int r = 0; r < V; ++r) {
+                    if (winner == static_cast<uint32_t>(r * 32 + lane)) key[r] = 0;
+                    best = max(best, key[r]);
+                }
             }
         }
     }
