@@ -55,10 +55,16 @@ int workspace_pool(int dev, cudaMemPool_t* out)
         props.handleTypes = cudaMemHandleTypeNone;
         props.location.type = cudaMemLocationTypeDevice;
         props.location.id = dev;
+        // The first call of a process may be one that is being captured.  A pool of its own touches nothing of the capture, but
+        // is refused while one is on unless this thread says so.
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        NVFP4_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
         cudaMemPool_t pool = nullptr;
-        NVFP4_CUDA_CHECK(cudaMemPoolCreate(&pool, &props));
         uint64_t keep = UINT64_MAX;
-        NVFP4_CUDA_CHECK(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep));
+        cudaError_t err = cudaMemPoolCreate(&pool, &props);
+        if (err == cudaSuccess) err = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep);
+        NVFP4_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+        if (err != cudaSuccess) return fail(NVFP4_E_CUDA, "no memory pool for workspaces: %s", cudaGetErrorString(err));
         pools[dev] = pool;
     }
     *out = pools[dev];

@@ -826,7 +826,7 @@ struct Operands {
 };
 
 // CTAs that find an SM of their own: clusters of four and eight do not divide the SMs of every GPC.
-int ctas_at_once(uint32_t splits_log2, int num_sms) { return splits_log2 < 2 ? num_sms : num_sms * 13 / 15; }
+int ctas_at_once(uint32_t splits_log2, int num_sms) { return splits_log2 < 2 || num_sms < 2 ? num_sms : num_sms * 13 / 15; }
 
 template <typename T, typename D, uint32_t BN, bool kSwap>
 int launch_tiles(const Operands& o, Epilogue e, uint32_t splits_log2, int num_sms, cudaStream_t stream)
@@ -1064,6 +1064,7 @@ int launch_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const 
                   cudaStream_t stream)
 {
     const Operands o{x, ldx, false, static_cast<uint32_t>(M), w, ldw, false, static_cast<uint32_t>(N), static_cast<uint32_t>(K), status};
+    if (activation == NVFP4_ACTIVATION_NONE) slopes = nullptr;
     const Epilogue e{d, ldd, slopes, lds, bias, residual, ldr, static_cast<uint32_t>(M), static_cast<uint32_t>(N), activation, false};
     return bf16 ? product<__nv_bfloat16>(o, e, out32, num_sms, stream) : product<__half>(o, e, out32, num_sms, stream);
 }

@@ -291,6 +291,51 @@ def test_repeated_calls_streams_and_graphs_give_the_same_bits(m, n, k):
 
 
 @gpu
+@pytest.mark.parametrize("sms", [1, 2, 3, 296])
+def test_any_number_of_sms(sms):
+    """set_num_sms sizes the persistent grids, and the choice of the form goes by it."""
+    before = _C.get_num_sms()
+    try:
+        _C.set_num_sms(sms)
+        for m, n, k in ((1, 300, 512), (130, 200, 1024), (700, 600, 64), (1300, 1288, 128)):
+            x, w, bias, residual = make(m, n, k, torch.bfloat16, 2)
+            check_forward(linear(x.cuda(), w.cuda(), bias.cuda(), residual.cuda(), activation="silu"), x, w, bias, residual, "silu", torch.bfloat16)
+    finally:
+        _C.set_num_sms(before)
+
+
+@gpu
+def test_slopes_are_left_alone_without_an_activation():
+    for n in (40, 41):
+        x, w, _, _ = make(600, n, 64, torch.float16, 1)
+        x, w = x.cuda(), w.cuda()
+        d, slopes = torch.empty(600, n, dtype=torch.float16, device="cuda"), torch.full((600, 48), 7, dtype=torch.int16, device="cuda")
+        rc = _C.lib().nvfp4_linear(x.data_ptr(), 64, w.data_ptr(), 64, None, None, 0, d.data_ptr(), n, slopes.data_ptr(), 48, 600, n, 64, 2, 2, 0, None,
+                                   torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert rc == 0 and (slopes == 7).all()
+        rc = _C.lib().nvfp4_linear(x.data_ptr(), 64, w.data_ptr(), 64, None, None, 0, d.data_ptr(), n, slopes.data_ptr(), 48, 600, n, 64, 2, 2, 1, None,
+                                   torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        want = (x.double() @ w.double().t() > 0).to(torch.int16) << 14
+        sure = (x.double() @ w.double().t()).abs() > 1e-4
+        assert rc == 0 and (slopes[:, :n] == want)[sure].all() and (slopes[:, n:] == 7).all()
+
+
+@gpu
+def test_outputs_beyond_32_bits():
+    """More output elements than 32 bits count; the last rows and columns against 64-bit products, and the gradient of the weight's last rows."""
+    m, n, k = 530000, 8200, 16
+    x = torch.randn(m, k, generator=torch.Generator("cuda").manual_seed(1), device="cuda").bfloat16()
+    w = (torch.randn(n, k, generator=torch.Generator("cuda").manual_seed(2), device="cuda") * 0.25).bfloat16()
+    for columns in (n, n - 1):                                            # through TMA, and the odd stride's way
+        d = linear(x, w[:columns], activation="silu")
+        at = torch.tensor([0, 1, 200000, 262143, 262144, m - 130, m - 2, m - 1], device="cuda")
+        check_forward(d[at], x[at].cpu(), w[:columns].cpu(), None, None, "silu", torch.bfloat16)
+        del d
+
+
+@gpu
 def test_a_captured_training_step():
     x, w, bias, residual = (t.cuda() for t in make(200, 136, 264, torch.bfloat16, 4))
     leaves = [t.requires_grad_() for t in (x, w, bias, residual)]

@@ -395,6 +395,58 @@ def test_places_outside_the_rows_are_not_read():
     assert torch.equal(y[0], rows[0]) and torch.equal(y[1], rows[5]) and (y[2] == 0).all()
 
 
+@gpu
+def test_offsets_beyond_32_bits():
+    """More elements in the sorted buffer than 32 bits count: forward and backward, checked on the device."""
+    tokens, k, experts, hidden = 66000, 8, 16, 8192
+    g = torch.Generator("cuda").manual_seed(3)
+    x = torch.randint(-8, 8, (tokens, hidden), generator=g, device="cuda").to(torch.bfloat16).requires_grad_()
+    ids = torch.randint(0, experts, (tokens, k), generator=g, device="cuda")
+    rows, order = sort_tokens(x, ids, experts, alignment=16)
+    assert rows.numel() > 1 << 32
+    assert (order.place >= 0).all() and order.place.max() > (1 << 32) // hidden
+    for lo in range(0, tokens, 4096):
+        assert torch.equal(rows.detach()[order.place[lo:lo + 4096]], x.detach()[lo:lo + 4096, None].expand(-1, k, -1))
+    assert (rows.detach()[order.source < 0] == 0).all()
+    w = torch.randint(1, 4, (tokens, k), generator=g, device="cuda").float().requires_grad_()
+    y = unsort_tokens(rows, order, w)                                     # small whole numbers: exact in FP32, rounded once
+    assert torch.equal(y.detach(), (x.detach().float() * w.detach().sum(dim=1, keepdim=True)).to(torch.bfloat16))
+    dy = torch.zeros(tokens, hidden, dtype=torch.bfloat16, device="cuda")
+    dy[:, ::97] = 1
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    assert torch.equal(dx.float(), dy.float() * w.detach().sum(dim=1, keepdim=True))
+    assert torch.equal(dw, (x.detach()[:, ::97].float().sum(dim=1, keepdim=True)).expand(-1, k))
+
+
+FIRST_CALL_IN_A_CAPTURE = """
+import torch, nvfp4_gemm
+from nvfp4_gemm import linear, route_tokens, sort_tokens, unsort_tokens
+x = torch.randn(600, 64, device="cuda").to(torch.bfloat16)
+gate = torch.randn(16, 64, device="cuda").to(torch.bfloat16)
+torch.cuda.synchronize()
+def step():
+    ids, w = route_tokens(linear(x, gate, out_dtype=torch.float32), 4)
+    rows, order = sort_tokens(x, ids, 16)
+    return unsort_tokens(rows, order, w)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = step()
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(y, step())
+"""
+
+
+@gpu
+def test_the_first_call_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_IN_A_CAPTURE], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
+
+
 # ---- streams, graphs, and a run of them ----------------------------------------------------------------------------
 
 
