@@ -372,8 +372,9 @@ NVFP4_API int nvfp4_unsort_tokens_backward(const void* dy, int64_t ldy_elems, co
  * and residual have any alignment and stride.
  * nvfp4_linear: d[M,N] = activation(x[M,K] w[N,K]^T + bias[N]) + residual[M,N].  d and residual have out_dtype, `dtype` or
  *   NVFP4_DTYPE_F32; bias (of type `dtype`) and residual may be NULL.  slopes (may be NULL; not written for NVFP4_ACTIVATION_NONE) receives
- *   activation'(x w^T + bias) for the backward pass, in multiples of 2^-14; -32768 stands for NaN.
- * nvfp4_linear_dz: dz[M,N] = dd * slopes, rounded to `dtype` for the products below, and db[N], the sums of its columns taken before
+ *   s = activation'(x w^T + bias) for the backward pass, as 8192 + s * 2^14 rounded; -1 stands for NaN.
+ *   The FP32 activations are off by a few units in the last place, those of 16-bit outputs by some 2^-20 of their value.
+ * nvfp4_linear_dz: dz[M,N] = dd * s (from its slopes), rounded to `dtype` for the products below, and db[N], the sums of its columns taken before
  *   that rounding.  dd has out_dtype, any alignment and stride; slopes NULL: 1.  slopes and dz start on 16 bytes and have row strides
  *   that are multiples of 8, N rounded up to 8 at least; what lies behind column N of dz's rows up to there is overwritten.  dz or db
  *   may be NULL.

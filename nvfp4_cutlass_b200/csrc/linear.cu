@@ -45,33 +45,14 @@ template <> __device__ __forceinline__ __half from_float<__half>(float v) { retu
 // ---- activations -----------------------------------------------------------------------------------------------------
 // gelu(z) = z Phi(z); its tanh form 0.5 z (1 + tanh u), u = c (z + 0.044715 z^3), is z sigmoid(2 u) as silu is z sigmoid(z): none of
 // them loses the digits of small values to a sum near zero.
-// kExact, for FP32 outputs: CUDA's full-precision functions.  For 16-bit outputs the epilogue would be bound by them (an IEEE division alone
-// takes more instructions than the rest; 16384 x 1024 x 1024 with silu took 86 us, 37 without): hardware exponential and
-// reciprocal, off by 2^-21 or so of the value, and erfc by the rational Chebyshev fit of Press et al., Numerical Recipes,
-// 6.2, off by 1.2e-7 of its value everywhere.
+// Two forms.  For FP32 outputs CUDA's full-precision functions (activate).  For 16-bit outputs the epilogue would be bound by them (an IEEE
+// division alone takes more instructions than the rest; 16384 x 1024 x 1024 with silu took 86 us, 37 without): there (activate2) two values to
+// an instruction, the hardware's base-2 exponential and reciprocal, off by 2^-21 or so of the value, and erfc by the Chebyshev fit of Press et
+// al., Numerical Recipes, 6.2, erfc(x) = t exp(-x^2 + P(t)), t = 1 / (1 + x / 2), off by 1.2e-7 of its value everywhere.
 constexpr float kGeluC = 0.7978845608028654f;        // sqrt(2 / pi)
-template <bool kExact> __device__ __forceinline__ float exponential(float x) { return kExact ? expf(x) : __expf(x); }
-template <bool kExact> __device__ __forceinline__ float reciprocal(float x) { return kExact ? 1.0f / x : __fdividef(1.0f, x); }
-template <bool kExact>
-__device__ __forceinline__ float normal_cdf(float z)
-{
-    if constexpr (kExact) return normcdff(z);
-    const float x = fabsf(z) * 0.7071067811865476f, t = reciprocal<false>(fmaf(0.5f, x, 1.0f));
-    float p = 0.17087277f;
-    p = fmaf(p, t, -0.82215223f);
-    p = fmaf(p, t, 1.48851587f);
-    p = fmaf(p, t, -1.13520398f);
-    p = fmaf(p, t, 0.27886807f);
-    p = fmaf(p, t, -0.18628806f);
-    p = fmaf(p, t, 0.09678418f);
-    p = fmaf(p, t, 0.37409196f);
-    p = fmaf(p, t, 1.00002368f);
-    p = fmaf(p, t, -1.26551223f);
-    const float half_erfc = 0.5f * t * exponential<false>(fmaf(-x, x, p));
-    return z < 0.0f ? half_erfc : 1.0f - half_erfc;
-}
+constexpr float kLog2e = 1.4426950408889634f;
 // y = activation(z) and, with kSlope, its derivative there.
-template <int kAct, bool kExact, bool kSlope>
+template <int kAct, bool kSlope>
 __device__ __forceinline__ void activate(float z, float& y, float& slope)
 {
     if constexpr (kAct == NVFP4_ACTIVATION_RELU) {
@@ -83,13 +64,13 @@ __device__ __forceinline__ void activate(float z, float& y, float& slope)
     } else {
         const float bounded = fminf(fmaxf(z, -40.0f), 40.0f);                 // beyond, the slope is constant: no infinity times zero
         if constexpr (kAct == NVFP4_ACTIVATION_GELU) {
-            const float cdf = normal_cdf<kExact>(z);
+            const float cdf = normcdff(z);
             y = z * cdf;
-            if constexpr (kSlope) slope = fmaf(bounded, 0.3989422804014327f * exponential<kExact>(-0.5f * bounded * bounded), cdf);
+            if constexpr (kSlope) slope = fmaf(bounded, 0.3989422804014327f * expf(-0.5f * bounded * bounded), cdf);
         } else {
             constexpr bool kSilu = kAct == NVFP4_ACTIVATION_SILU;
             const float u2 = kSilu ? z : 2.0f * kGeluC * z * fmaf(0.044715f * z, z, 1.0f);
-            const float e = exponential<kExact>(-fabsf(u2)), near = reciprocal<kExact>(1.0f + e), far = e * near;
+            const float e = expf(-fabsf(u2)), near = 1.0f / (1.0f + e), far = e * near;
             const float sigmoid = u2 >= 0.0f ? near : far;                    // the larger of sigmoid(u2) and 1 - sigmoid(u2), or the smaller
             y = z * sigmoid;
             if constexpr (kSlope) {
@@ -99,11 +80,63 @@ __device__ __forceinline__ void activate(float z, float& y, float& slope)
         }
     }
 }
-// For the backward pass a slope, all of which lie in (-0.2, 1.2), is kept as a multiple of 2^-14 in 16 bits: off by 2^-15 at most, less
-// than the rounding of the gradient that it multiplies, where z kept in BF16 would cost as much as that rounding again.
-constexpr int kSlopeNan = -32768;
-__device__ __forceinline__ int16_t pack_slope(float s) { return static_cast<int16_t>(s != s ? kSlopeNan : __float2int_rn(s * 16384.0f)); }
-__device__ __forceinline__ float unpack_slope(int16_t c) { return c == kSlopeNan ? __uint_as_float(0x7fc00000u) : c * (1.0f / 16384.0f); }
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 exp2_of(float2 v) { return make_float2(ptx::ex2_approx(v.x), ptx::ex2_approx(v.y)); }
+__device__ __forceinline__ float2 reciprocal_of(float2 v) { return make_float2(ptx::rcp_approx(v.x), ptx::rcp_approx(v.y)); }
+// min(|z|, 40), NaN for NaN: slopes are constant beyond
+__device__ __forceinline__ float2 bounded_size(float2 z) { return make_float2(ptx::min_nan(fabsf(z.x), 40.0f), ptx::min_nan(fabsf(z.y), 40.0f)); }
+__device__ __forceinline__ float2 with_sign(float2 size, float2 z) { return make_float2(copysignf(size.x, z.x), copysignf(size.y, z.y)); }
+template <int kAct, bool kSlope>
+__device__ __forceinline__ void activate2(float2 z, float2& y, float2& slope)
+{
+    using ptx::fma_f32x2;
+    using ptx::mul_f32x2;
+    if constexpr (kAct == NVFP4_ACTIVATION_RELU || kAct == NVFP4_ACTIVATION_NONE) {
+        activate<kAct, kSlope>(z.x, y.x, slope.x);
+        activate<kAct, kSlope>(z.y, y.y, slope.y);
+    } else if constexpr (kAct == NVFP4_ACTIVATION_GELU) {
+        const float2 size = bounded_size(z), t = reciprocal_of(fma_f32x2(size, both(0.35355339f), both(1.0f)));
+        // -x^2 + P(t) in base 2, less one for the half of Phi(-|z|) = erfc(|z| / sqrt 2) / 2
+        float2 p = both(0.17087277f * kLog2e);
+        p = fma_f32x2(p, t, both(-0.82215223f * kLog2e));
+        p = fma_f32x2(p, t, both(1.48851587f * kLog2e));
+        p = fma_f32x2(p, t, both(-1.13520398f * kLog2e));
+        p = fma_f32x2(p, t, both(0.27886807f * kLog2e));
+        p = fma_f32x2(p, t, both(-0.18628806f * kLog2e));
+        p = fma_f32x2(p, t, both(0.09678418f * kLog2e));
+        p = fma_f32x2(p, t, both(0.37409196f * kLog2e));
+        p = fma_f32x2(p, t, both(1.00002368f * kLog2e));
+        p = fma_f32x2(p, t, both(-1.26551223f * kLog2e - 1.0f));
+        const float2 square = mul_f32x2(mul_f32x2(size, both(-0.5f * kLog2e)), size);
+        const float2 tail = mul_f32x2(t, exp2_of(fma_f32x2(square, both(1.0f), p))), body = fma_f32x2(tail, both(-1.0f), both(1.0f));
+        const float2 cdf = make_float2(z.x < 0.0f ? tail.x : body.x, z.y < 0.0f ? tail.y : body.y);
+        y = mul_f32x2(z, cdf);
+        if constexpr (kSlope) slope = fma_f32x2(mul_f32x2(with_sign(size, z), both(0.3989422804014327f)), exp2_of(square), cdf);
+    } else {
+        constexpr bool kSilu = kAct == NVFP4_ACTIVATION_SILU;
+        const float2 u2 = kSilu ? z : mul_f32x2(mul_f32x2(z, both(2.0f * kGeluC)), fma_f32x2(mul_f32x2(z, both(0.044715f)), z, both(1.0f)));
+        const float2 e = exp2_of(mul_f32x2(make_float2(fabsf(u2.x), fabsf(u2.y)), both(-kLog2e)));
+        const float2 near = reciprocal_of(fma_f32x2(e, both(1.0f), both(1.0f))), far = mul_f32x2(e, near);
+        const float2 sigmoid = make_float2(u2.x >= 0.0f ? near.x : far.x, u2.y >= 0.0f ? near.y : far.y);
+        y = mul_f32x2(z, sigmoid);
+        if constexpr (kSlope) {
+            float2 inner = with_sign(bounded_size(z), z);
+            if constexpr (!kSilu) inner = mul_f32x2(mul_f32x2(inner, both(2.0f * kGeluC)), fma_f32x2(mul_f32x2(inner, both(3.0f * 0.044715f)), inner, both(1.0f)));
+            slope = fma_f32x2(inner, mul_f32x2(near, far), sigmoid);
+        }
+    }
+}
+// For the backward pass a slope, all of which lie in (-0.2, 1.2), is kept in 16 bits as 8192 + slope * 2^14: off by 2^-15 at most, less than the
+// rounding of the gradient that it multiplies, where z kept in BF16 would cost as much as that rounding again.  Adding 2^23 + 2^22 + 8192 puts
+// the rounded number into a float's lower bits; of a NaN those are all ones, -1, which no slope has.
+constexpr float kSlopeScale = 16384.0f, kSlopeShift = 12582912.0f + 8192.0f;
+__device__ __forceinline__ uint32_t slope_code(float s) { return __float_as_uint(fmaf(s, kSlopeScale, kSlopeShift)); }
+__device__ __forceinline__ uint32_t slope_codes(float2 s)
+{
+    const float2 c = ptx::fma_f32x2(s, both(kSlopeScale), both(kSlopeShift));
+    return __byte_perm(__float_as_uint(c.x), __float_as_uint(c.y), 0x5410);
+}
+__device__ __forceinline__ float unpack_slope(int16_t c) { return c == -1 ? __uint_as_float(0x7fc00000u) : (c - 8192) * (1.0f / 16384.0f); }
 
 // Calls f(std::integral_constant<int, activation>) for a code: one switch around a loop of elements.
 template <typename F>
@@ -155,18 +188,30 @@ __device__ __forceinline__ void finish(float (&v)[kN], uint32_t row0, uint32_t c
     if (e.activation != NVFP4_ACTIVATION_NONE)
         with_activation(e.activation, [&](auto act) {
             constexpr int kAct = decltype(act)::value;
-            constexpr bool kExact = std::is_same<D, float>::value;
-            float slope;
+            auto two = [&](uint32_t i, float2& slope, auto with_slope) {
+                constexpr bool kSlope = decltype(with_slope)::value;
+                if constexpr (std::is_same<D, float>::value) {
+                    activate<kAct, kSlope>(v[i], v[i], slope.x);
+                    activate<kAct, kSlope>(v[i + 1], v[i + 1], slope.y);
+                } else {
+                    float2 y;
+                    activate2<kAct, kSlope>(make_float2(v[i], v[i + 1]), y, slope);
+                    v[i] = y.x;
+                    v[i + 1] = y.y;
+                }
+            };
+            float2 slope = make_float2(0.0f, 0.0f);
             if (e.slopes != nullptr) {
                 int16_t* to = e.slopes + static_cast<int64_t>(row0) * e.lds + at;
 #pragma unroll
-                for (uint32_t i = 0; i < kN; ++i) {
-                    activate<kAct, kExact, true>(v[i], v[i], slope);
-                    if (i < rows && mine) to[i * e.lds] = pack_slope(slope);
+                for (uint32_t i = 0; i < kN; i += 2) {
+                    two(i, slope, std::true_type{});
+                    if (i < rows && mine) to[i * e.lds] = static_cast<int16_t>(slope_code(slope.x));
+                    if (i + 1 < rows && mine) to[(i + 1) * e.lds] = static_cast<int16_t>(slope_code(slope.y));
                 }
             } else {
 #pragma unroll
-                for (uint32_t i = 0; i < kN; ++i) activate<kAct, kExact, false>(v[i], v[i], slope);
+                for (uint32_t i = 0; i < kN; i += 2) two(i, slope, std::false_type{});
             }
         });
     if (e.residual != nullptr) {
@@ -312,22 +357,28 @@ struct Stage {
             if (e.activation != NVFP4_ACTIVATION_NONE)
                 with_activation(e.activation, [&](auto act) {
                     constexpr int kAct = decltype(act)::value;
-                    float slope[2];
+                    float2 y, slope;
                     if (e.slopes != nullptr) {
 #pragma unroll
                         for (uint32_t q = 0; q < 4; ++q) {
                             uint32_t w[4];
 #pragma unroll
                             for (uint32_t i = 0; i < 4; ++i) {
-#pragma unroll
-                                for (uint32_t j = 0; j < 2; ++j) activate<kAct, false, true>(v[8 * q + 2 * i + j], v[8 * q + 2 * i + j], slope[j]);
-                                w[i] = static_cast<uint16_t>(pack_slope(slope[0])) | static_cast<uint32_t>(static_cast<uint16_t>(pack_slope(slope[1]))) << 16;
+                                const uint32_t at = 8 * q + 2 * i;
+                                activate2<kAct, true>(make_float2(v[at], v[at + 1]), y, slope);
+                                v[at] = y.x;
+                                v[at + 1] = y.y;
+                                w[i] = slope_codes(slope);
                             }
                             ptx::sts128(piece(slopes + box * slopes_step, q), w[0], w[1], w[2], w[3]);
                         }
                     } else {
 #pragma unroll
-                        for (uint32_t i = 0; i < 32; ++i) activate<kAct, false, false>(v[i], v[i], slope[0]);
+                        for (uint32_t i = 0; i < 32; i += 2) {
+                            activate2<kAct, false>(make_float2(v[i], v[i + 1]), y, slope);
+                            v[i] = y.x;
+                            v[i + 1] = y.y;
+                        }
                     }
                 });
 #pragma unroll

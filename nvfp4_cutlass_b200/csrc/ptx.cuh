@@ -455,6 +455,19 @@ NVFP4_DEVICE uint32_t max_abs_bf16x2(uint32_t a, uint32_t b)
     asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
+NVFP4_DEVICE float ex2_approx(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// The smaller one, NaN if either is NaN.
+NVFP4_DEVICE float min_nan(float a, float b)
+{
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 NVFP4_DEVICE float rcp_approx(float x)
 {
     float r;

@@ -317,9 +317,47 @@ def test_slopes_are_left_alone_without_an_activation():
         rc = _C.lib().nvfp4_linear(x.data_ptr(), 64, w.data_ptr(), 64, None, None, 0, d.data_ptr(), n, slopes.data_ptr(), 48, 600, n, 64, 2, 2, 1, None,
                                    torch.cuda.current_stream().cuda_stream)
         torch.cuda.synchronize()
-        want = (x.double() @ w.double().t() > 0).to(torch.int16) << 14
+        want = ((x.double() @ w.double().t() > 0).to(torch.int16) << 14) + 8192
         sure = (x.double() @ w.double().t()).abs() > 1e-4
         assert rc == 0 and (slopes[:, :n] == want)[sure].all() and (slopes[:, n:] == 7).all()
+
+
+@gpu
+@pytest.mark.parametrize("activation", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_activations_and_slopes_of_extreme_values(activation):
+    """z from a sweep over all of FP16, infinities and NaN, in each of the epilogue's ways: K = 8 with one nonzero product gives z exactly."""
+    z = torch.arange(-32768, 32768, dtype=torch.int32).to(torch.int16).view(torch.float16)
+    z = torch.cat([z, torch.tensor([-0.0, 65504.0, -65504.0], dtype=torch.float16)])
+    finite = torch.isfinite(z)
+    n = 8
+    w = torch.zeros(n, 8, dtype=torch.float16)
+    w[:, 0] = 1
+    for rows in (z[-9000:], z, z[20000:20100]):                            # tiles, pairs, few rows
+        x = torch.zeros(rows.numel(), 8, dtype=torch.float16)
+        x[:, 0] = rows
+        for columns in (8, 7):
+            for out in (torch.float16, torch.float32):
+                leaf = x.cuda().requires_grad_()
+                y = linear(leaf, w[:columns].cuda(), activation=activation, out_dtype=out)
+                d = torch.zeros(rows.numel(), columns, dtype=out)
+                d[:, 0] = 1
+                (dx,) = torch.autograd.grad(y, leaf, d.cuda())
+                v = rows.double()
+                real = torch.isfinite(rows)
+                want = act64(v, activation)[:, None].expand(-1, columns)
+                got = y.detach().cpu().double()
+                argument = {"gelu": v * v / 2 + 2, "gelu_tanh": 1.6 * (v.abs() + 0.044715 * v.abs() ** 3)}.get(activation, v.abs()).clamp(max=200)[:, None]
+                floor = 2.0 ** -24 if out == torch.float16 else 1e-37
+                assert (got - want)[real].abs().le((want.abs() * ((16 + 4 * argument) * 2.0 ** -23 + 1.01 * HALF_STEP[out]) + floor)[real]).all()
+                assert torch.isnan(got[torch.isnan(rows)]).all() and (got[rows == math.inf] == math.inf).all()
+                leaf64 = torch.where(real, v, 0.0).requires_grad_()
+                (slope,) = torch.autograd.grad(act64(leaf64, activation).sum(), leaf64)
+                slope = torch.where(torch.isnan(slope), 0.0, slope) if activation == "gelu_tanh" else slope     # 0 * inf of the formula far out
+                far = v.abs() > 30                                         # there the formulas meet their limits
+                slope = torch.where(far, (v > 0).double(), slope)
+                sx = dx[:, 0].cpu().double()
+                assert (sx - slope)[real].abs().le(2.0 ** -15 + 64 * 2.0 ** -23 + 1.1 * 2.0 ** -11).all()
+                assert torch.isnan(sx[torch.isnan(rows)]).all() and (sx[rows == math.inf] == 1).all()
 
 
 @gpu
