@@ -231,10 +231,19 @@ sort_place_kernel(const int64_t* __restrict__ ids, int64_t n, int64_t chunk, int
     for (int i = 0; i < 2; ++i) {
         const int e = column + i * width;
         if (e >= experts || slice >= slices) continue;
-        for (unsigned c = slice; c < gridDim.x; c += slices) {
-            const uint32_t v = counts[static_cast<int64_t>(c) * experts + e];
-            all[i] += v;
-            if (c < blockIdx.x) before[i] += v;
+        // eight loads under way (one at a time, 128 chunks of 65536 pairs took 20 us)
+        for (unsigned c0 = slice; c0 < gridDim.x; c0 += 8 * slices) {
+            uint32_t v[8];
+#pragma unroll
+            for (unsigned u = 0; u < 8; ++u) {
+                const unsigned c = c0 + u * slices;
+                v[u] = c < gridDim.x ? counts[static_cast<int64_t>(c) * experts + e] : 0u;
+            }
+#pragma unroll
+            for (unsigned u = 0; u < 8; ++u) {
+                all[i] += v[u];
+                if (c0 + u * slices < blockIdx.x) before[i] += v[u];
+            }
         }
     }
     auto add_up = [&](const uint32_t (&part)[2], auto&& store) {
