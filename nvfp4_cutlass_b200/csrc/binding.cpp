@@ -21,6 +21,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <algorithm>
+#include <optional>
 
 #include "../../include/nvfp4_b200.h"
 
@@ -204,6 +205,8 @@ template <typename T>
 T* pointer(const at::Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
 // The gradient of an output in rows that the kernels can read
 at::Tensor in_rows(const at::Tensor& t) { return t.size(0) > 0 && t.size(1) > 0 && t.stride(1) == 1 && t.stride(0) >= t.size(1) ? t : t.contiguous(); }
+// An argument of a node that may be missing: nodes take no undefined tensors
+std::optional<at::Tensor> present(const at::Tensor& t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; }
 // Gradients that were computed without being recorded: whoever differentiates them again gets an error instead of nothing.
 variable_list once(variable_list grads)
 {
@@ -328,8 +331,10 @@ PyObject* sort(PyObject*, PyObject* const* args, Py_ssize_t count)
 }
 
 struct UnsortNode : torch::autograd::Function<UnsortNode> {
-    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& rows, const at::Tensor& weights, const at::Tensor& place, const at::Tensor& source)
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& rows, const std::optional<at::Tensor>& given, const at::Tensor& place,
+                              const at::Tensor& source)
     {
+        const at::Tensor weights = given.value_or(at::Tensor());
         const bool want_rows = rows.requires_grad(), want_weights = weights.defined() && weights.requires_grad();
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({want_weights ? rows : at::Tensor(), weights, place, source});
@@ -370,7 +375,7 @@ PyObject* unsort(PyObject*, PyObject* const* args, Py_ssize_t count)
             if (weights == nullptr || weights->sizes() != place->sizes()) Py_RETURN_NONE;
         }
         const at::Tensor w = weights != nullptr ? *weights : at::Tensor();
-        return THPVariable_Wrap(at::GradMode::is_enabled() && (wants_gradient(rows) || wants_gradient(weights)) ? UnsortNode::apply(*rows, w, *place, *source)
+        return THPVariable_Wrap(at::GradMode::is_enabled() && (wants_gradient(rows) || wants_gradient(weights)) ? UnsortNode::apply(*rows, present(w), *place, *source)
                                                                                                                 : sum_rows(*rows, *place, w, true));
     } catch (const std::exception&) {
         Py_RETURN_NONE;
@@ -393,9 +398,10 @@ at::Tensor linear_forward(const at::Tensor& x, const at::Tensor& w, const at::Te
     return d;
 }
 struct LinearNode : torch::autograd::Function<LinearNode> {
-    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias, const at::Tensor& residual,
-                              int64_t activation, bool out32)
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& given_bias,
+                              const std::optional<at::Tensor>& given_residual, int64_t activation, bool out32)
     {
+        const at::Tensor bias = given_bias.value_or(at::Tensor()), residual = given_residual.value_or(at::Tensor());
         const bool want_x = x.requires_grad(), want_w = w.requires_grad(), want_bias = bias.defined() && bias.requires_grad();
         at::Tensor slopes;
         if (activation != NVFP4_ACTIVATION_NONE && (want_x || want_w || want_bias)) slopes = fresh(x, at::kShort, {x.size(0), (w.size(0) + 7) / 8 * 8});
@@ -465,7 +471,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count)
         }
         const bool record = at::GradMode::is_enabled() && (wants_gradient(x) || wants_gradient(w) || (bias.defined() && bias.requires_grad()) ||
                                                            (residual.defined() && residual.requires_grad()));
-        return THPVariable_Wrap(record ? LinearNode::apply(*x, *w, bias, residual, activation, out32 != 0)
+        return THPVariable_Wrap(record ? LinearNode::apply(*x, *w, present(bias), present(residual), activation, out32 != 0)
                                        : linear_forward(*x, *w, bias, residual, activation, out32 != 0, at::Tensor()));
     } catch (const std::exception&) {
         Py_RETURN_NONE;

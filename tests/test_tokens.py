@@ -615,6 +615,23 @@ def test_the_binding_s_gradients_are_the_general_way_s(monkeypatch):
 
 
 @gpu
+def test_the_binding_records_calls_with_and_without_their_optional_arguments():
+    _C.lib()
+    b = _C._binding
+    x = torch.randn(20, 64, generator=gen(1)).half().cuda().requires_grad_()
+    w, bias, residual = x.detach()[:16].clone(), x.detach()[0, :16].clone(), torch.zeros(20, 16, dtype=torch.float16, device="cuda")
+    for args in ((None, None), (bias, None), (None, residual), (bias, residual)):
+        d = b.linear(x, w, *args, 4, 0)
+        assert d is not None and torch.autograd.grad(d.sum(), x)[0].shape == x.shape
+    rows, place, source, _ = b.sort(x, some_ids(20, 2, 4, 1, "uniform").cuda(), 4, 16)
+    for weights in (None, torch.rand(20, 2, device="cuda")):
+        y = b.unsort(rows, place, source, weights)
+        assert y is not None and torch.autograd.grad(y.sum(), x, retain_graph=True)[0].shape == x.shape
+    ids, weights = b.route(x, 4, 0, 1)
+    assert torch.autograd.grad(weights.sum(), x)[0].shape == x.shape
+
+
+@gpu
 def test_what_is_not_differentiated_costs_nothing():
     x = torch.randn(6, 8, generator=gen(1)).cuda().requires_grad_()
     rows, order = sort_tokens(x, some_ids(6, 2, 4, 1, "uniform").cuda(), 4, alignment=16)
