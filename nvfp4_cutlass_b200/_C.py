@@ -124,7 +124,6 @@ def _bind(library):
     except (ImportError, OSError) as e:
         if torch.version.cuda is not None:
             warnings.warn(f"{_BINDING_PATH} does not load ({e}): GEMM calls take some 6 us more on the host", RuntimeWarning, stacklevel=3)
-        _binding = None
         return _no_binding
     address = lambda entry: ctypes.cast(entry, ctypes.c_void_p).value
     binding.bind(address(library.nvfp4_grouped_gemm_contiguous))

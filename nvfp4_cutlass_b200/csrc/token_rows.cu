@@ -155,8 +155,9 @@ __device__ __forceinline__ int group_of(const uint32_t* start, int experts, uint
 }
 
 // Rows move as words W of 16, 4 or 2 bytes: the widest that both buffers' starts, strides and the row's length are multiples of.
-// A warp's piece of a row: kPieceWords words a lane.
-constexpr int kPieceWords = 4;
+// A warp's piece of a row: so many words a lane.
+template <typename W>
+constexpr int kPieceWords = sizeof(W) == 16 ? 4 : sizeof(W) == 4 ? 8 : 16;
 
 template <typename W>
 __global__ void __launch_bounds__(kThreads)
@@ -165,7 +166,7 @@ sort_one_kernel(const W* __restrict__ x, int64_t ldx, const int64_t* __restrict_
 {
     extern __shared__ uint32_t smem[];
     const Plan s(smem, experts);
-    const uint32_t lane = threadIdx.x & 31, pieces = (row_words + 32 * kPieceWords - 1) / (32 * kPieceWords);
+    const uint32_t lane = threadIdx.x & 31, pieces = (row_words + 32 * kPieceWords<W> - 1) / (32 * kPieceWords<W>);
     const uint64_t units = static_cast<uint64_t>(m) * pieces, step = static_cast<uint64_t>(gridDim.x) * kWarps;
     const uint64_t mine = static_cast<uint64_t>(threadIdx.x >> 5) * gridDim.x + blockIdx.x;      // consecutive units to different blocks
     uint16_t* order = reinterpret_cast<uint16_t*>(smem + plan_words(experts));      // pairs in the order of the experts
@@ -189,15 +190,15 @@ sort_one_kernel(const W* __restrict__ x, int64_t ldx, const int64_t* __restrict_
         }
         const W* from = x + static_cast<int64_t>(pair / k) * ldx;
         W* to = rows + static_cast<int64_t>(r) * row_words;
-        W v[kPieceWords];
-        const uint32_t c0 = piece * 32 * kPieceWords + lane;
+        W v[kPieceWords<W>];
+        const uint32_t c0 = piece * 32 * kPieceWords<W> + lane;
 #pragma unroll
-        for (int i = 0; i < kPieceWords; ++i) {
+        for (int i = 0; i < kPieceWords<W>; ++i) {
             v[i] = W{};
             if (live && c0 + i * 32 < row_words) v[i] = from[c0 + i * 32];
         }
 #pragma unroll
-        for (int i = 0; i < kPieceWords; ++i)
+        for (int i = 0; i < kPieceWords<W>; ++i)
             if (c0 + i * 32 < row_words) to[c0 + i * 32] = v[i];
     }
 }
@@ -283,16 +284,16 @@ sort_move_kernel(const W* __restrict__ x, int64_t ldx, uint32_t tokens, int k, i
                  const uint32_t* __restrict__ groups, const int64_t* __restrict__ place, W* __restrict__ rows, int32_t* __restrict__ source,
                  int32_t* __restrict__ m_indices)
 {
-    const uint32_t lane = threadIdx.x & 31, pieces = (row_words + 32 * kPieceWords - 1) / (32 * kPieceWords);
+    const uint32_t lane = threadIdx.x & 31, pieces = (row_words + 32 * kPieceWords<W> - 1) / (32 * kPieceWords<W>);
     const uint64_t token_units = static_cast<uint64_t>(tokens) * pieces, units = token_units + (m + kRowsPerUnit - 1) / kRowsPerUnit;
     ptx::grid_dependency_wait();
     for (uint64_t unit = static_cast<uint64_t>(threadIdx.x >> 5) * gridDim.x + blockIdx.x; unit < units; unit += static_cast<uint64_t>(gridDim.x) * kWarps) {
         if (unit < token_units) {
-            const uint32_t t = static_cast<uint32_t>(unit / pieces), c0 = static_cast<uint32_t>(unit % pieces) * 32 * kPieceWords + lane;
+            const uint32_t t = static_cast<uint32_t>(unit / pieces), c0 = static_cast<uint32_t>(unit % pieces) * 32 * kPieceWords<W> + lane;
             const W* from = x + static_cast<int64_t>(t) * ldx;
-            W v[kPieceWords];
+            W v[kPieceWords<W>];
 #pragma unroll
-            for (int i = 0; i < kPieceWords; ++i)
+            for (int i = 0; i < kPieceWords<W>; ++i)
                 if (c0 + i * 32 < row_words) v[i] = from[c0 + i * 32];
             for (int j0 = 0; j0 < k; j0 += 32) {
                 const int64_t mine = j0 + static_cast<int>(lane) < k ? place[static_cast<int64_t>(t) * k + j0 + lane] : -1;
@@ -302,7 +303,7 @@ sort_move_kernel(const W* __restrict__ x, int64_t ldx, uint32_t tokens, int k, i
                     if (r < 0) continue;
                     W* to = rows + r * row_words;
 #pragma unroll
-                    for (int i = 0; i < kPieceWords; ++i)
+                    for (int i = 0; i < kPieceWords<W>; ++i)
                         if (c0 + i * 32 < row_words) to[c0 + i * 32] = v[i];
                 }
             }
@@ -326,12 +327,12 @@ sort_move_kernel(const W* __restrict__ x, int64_t ldx, uint32_t tokens, int k, i
 
 // ---- back: y[t] = sum_j w[t, j] * rows[place[t, j]] ------------------------------------------------------------------------------------
 
-// What a lane moves at a time: 16 bytes of elements of T, or one of them, as bits.  (Arrays of the 16-bit types' classes end up in local
+// What a lane moves at a time: 16 or 4 bytes of elements of T, or one of them, as bits.  (Arrays of the 16-bit types' classes end up in local
 // memory.)  Loads are plain here as elsewhere in this file: __ldg, an asm statement, may be moved ahead of the test that guards it.
-template <typename T, bool kWide>
+template <typename T, int kBytes>
 struct Pack {
-    using Bits = std::conditional_t<kWide, uint4, std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>>;
-    static constexpr int kN = kWide ? 16 / static_cast<int>(sizeof(T)) : 1;
+    using Bits = std::conditional_t<kBytes == 16, uint4, std::conditional_t<kBytes == 4, uint32_t, uint16_t>>;
+    static constexpr int kN = kBytes / static_cast<int>(sizeof(T)), kSize = kBytes;
     static __device__ __forceinline__ float2 two(uint32_t w)
     {
         if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
@@ -349,13 +350,14 @@ struct Pack {
     }
     static __device__ __forceinline__ void unpack(const Bits& bits, float (&f)[kN])
     {
-        if constexpr (!kWide) {
-            if constexpr (sizeof(T) == 4) f[0] = __uint_as_float(bits);
-            else f[0] = two(bits).x;
+        if constexpr (kBytes == 2) {
+            f[0] = two(bits).x;
         } else {
-            const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
+            uint32_t w[kBytes / 4];
+            if constexpr (kBytes == 16) { w[0] = bits.x; w[1] = bits.y; w[2] = bits.z; w[3] = bits.w; }
+            else w[0] = bits;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < kBytes / 4; ++i) {
                 if constexpr (sizeof(T) == 4) {
                     f[i] = __uint_as_float(w[i]);
                 } else {
@@ -368,38 +370,40 @@ struct Pack {
     }
     static __device__ __forceinline__ Bits pack(const float (&f)[kN])
     {
-        if constexpr (!kWide) {
-            if constexpr (sizeof(T) == 4) return __float_as_uint(f[0]);
-            else return static_cast<uint16_t>(one_word(f[0], 0.0f));
+        if constexpr (kBytes == 2) {
+            return static_cast<uint16_t>(one_word(f[0], 0.0f));
         } else {
-            uint32_t w[4];
+            uint32_t w[kBytes / 4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < kBytes / 4; ++i) {
                 if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(f[i]);
                 else w[i] = one_word(f[2 * i], f[2 * i + 1]);
             }
-            return make_uint4(w[0], w[1], w[2], w[3]);
+            if constexpr (kBytes == 16) return make_uint4(w[0], w[1], w[2], w[3]);
+            else return w[0];
         }
     }
 };
 
 // A warp takes a piece of a token, kPer packs a lane; the rows of up to four choices are under way together.  FP32, ascending j.
 // The gradient of the sort is the same sum without weights.
-constexpr int kPer = 2, kFlight = 4;
+template <typename P>
+constexpr int kPer = P::kSize == 16 ? 2 : P::kSize == 4 ? 4 : 8;              // packs of a lane: of narrow ones more
+constexpr int kFlight = 4;
 template <typename P>
 __global__ void __launch_bounds__(256, 3)
 unsort_kernel(const typename P::Bits* __restrict__ rows, int64_t ld, const int64_t* __restrict__ place, const float* __restrict__ w, uint32_t tokens,
               int k, int64_t m, uint32_t row_packs, typename P::Bits* __restrict__ y)
 {
     constexpr int kN = P::kN;
-    const uint32_t lane = threadIdx.x & 31, pieces = (row_packs + 32 * kPer - 1) / (32 * kPer);
+    const uint32_t lane = threadIdx.x & 31, pieces = (row_packs + 32 * kPer<P> - 1) / (32 * kPer<P>);
     const uint64_t units = static_cast<uint64_t>(tokens) * pieces;
     ptx::grid_dependency_wait();
     for (uint64_t unit = static_cast<uint64_t>(threadIdx.x >> 5) * gridDim.x + blockIdx.x; unit < units; unit += static_cast<uint64_t>(gridDim.x) * 8) {
-        const uint32_t t = static_cast<uint32_t>(unit / pieces), c0 = static_cast<uint32_t>(unit % pieces) * 32 * kPer + lane;
-        float acc[kPer][kN];
+        const uint32_t t = static_cast<uint32_t>(unit / pieces), c0 = static_cast<uint32_t>(unit % pieces) * 32 * kPer<P> + lane;
+        float acc[kPer<P>][kN];
 #pragma unroll
-        for (int i = 0; i < kPer; ++i)
+        for (int i = 0; i < kPer<P>; ++i)
 #pragma unroll
             for (int q = 0; q < kN; ++q) acc[i][q] = 0.0f;
         for (int j0 = 0; j0 < k; j0 += 32) {
@@ -412,7 +416,7 @@ unsort_kernel(const typename P::Bits* __restrict__ rows, int64_t ld, const int64
             }
             const int here = min(32, k - j0);
             for (int j1 = 0; j1 < here; j1 += kFlight) {
-                typename P::Bits v[kFlight][kPer];
+                typename P::Bits v[kFlight][kPer<P>];
                 bool live[kFlight];
                 float wj[kFlight];
 #pragma unroll
@@ -422,7 +426,7 @@ unsort_kernel(const typename P::Bits* __restrict__ rows, int64_t ld, const int64
                     live[u] = j1 + u < here && r >= 0;
                     if (live[u]) {
 #pragma unroll
-                        for (int i = 0; i < kPer; ++i)
+                        for (int i = 0; i < kPer<P>; ++i)
                             if (c0 + i * 32 < row_packs) v[u][i] = rows[r * ld + c0 + i * 32];
                     }
                 }
@@ -430,7 +434,7 @@ unsort_kernel(const typename P::Bits* __restrict__ rows, int64_t ld, const int64
                 for (int u = 0; u < kFlight; ++u) {
                     if (!live[u]) continue;
 #pragma unroll
-                    for (int i = 0; i < kPer; ++i) {
+                    for (int i = 0; i < kPer<P>; ++i) {
                         float f[kN];
                         P::unpack(v[u][i], f);
 #pragma unroll
@@ -440,7 +444,7 @@ unsort_kernel(const typename P::Bits* __restrict__ rows, int64_t ld, const int64
             }
         }
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
+        for (int i = 0; i < kPer<P>; ++i) {
             if (c0 + i * 32 >= row_packs) continue;
             y[static_cast<int64_t>(t) * row_packs + c0 + i * 32] = P::pack(acc[i]);
         }
@@ -575,7 +579,7 @@ RingShape ring_shape(int64_t tokens, int k, int64_t row_bytes)
 // at a time in few registers.  The pairs of a token are neighbouring warps', which read dy from L1 behind the first.  (A block to a token,
 // eight rows at a time to a thread, took 138 registers and ran at an eighth of the warps: 455 us for 8192 x 8 rows of 8 KB.)
 // Behind the pairs: warps that zero the rows whose source is -1.  drows or dw may be NULL; rows is read for dw alone.
-constexpr int kBackThreads = 256, kBackWarps = kBackThreads / 32, kBackPer = 4;
+constexpr int kBackThreads = 256, kBackWarps = kBackThreads / 32;
 template <typename P>
 __global__ void __launch_bounds__(kBackThreads, 4)
 unsort_backward_kernel(const typename P::Bits* __restrict__ dy, int64_t ldy, const typename P::Bits* __restrict__ rows, int64_t ld,
@@ -583,7 +587,7 @@ unsort_backward_kernel(const typename P::Bits* __restrict__ dy, int64_t ldy, con
                        uint32_t m, uint32_t row_packs, typename P::Bits* __restrict__ drows, float* __restrict__ dw)
 {
     using Bits = typename P::Bits;
-    constexpr int kN = P::kN;
+    constexpr int kN = P::kN, kBackPer = P::kSize == 16 ? 4 : 8;
     const uint32_t lane = threadIdx.x & 31;
     const uint64_t units = static_cast<uint64_t>(pairs) + (drows != nullptr ? m : 0);
     ptx::grid_dependency_wait();
@@ -639,13 +643,17 @@ unsort_backward_kernel(const typename P::Bits* __restrict__ dy, int64_t ldy, con
     }
 }
 
-// Calls f(Pack<type, wide>*) for a type code.
+// Calls f(Pack<type, bytes>*) for a type code and the widest pack that everything in `bits` (addresses, strides and lengths in bytes) is a
+// multiple of.
 template <typename F>
-int with_pack(int dtype, bool wide, F&& f)
+int with_pack(int dtype, uintptr_t bits, F&& f)
 {
     auto packs = [&](auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;
-        return wide ? f(static_cast<Pack<T, true>*>(nullptr)) : f(static_cast<Pack<T, false>*>(nullptr));
+        if ((bits & 15u) == 0) return f(static_cast<Pack<T, 16>*>(nullptr));
+        if constexpr (sizeof(T) == 2)
+            if ((bits & 3u) != 0) return f(static_cast<Pack<T, 2>*>(nullptr));
+        return f(static_cast<Pack<T, 4>*>(nullptr));
     };
     switch (dtype) {
         case NVFP4_DTYPE_BF16: return packs(static_cast<__nv_bfloat16*>(nullptr));
@@ -671,7 +679,7 @@ int sort_with(const void* x, int64_t ldx_bytes, int64_t tokens, int k, int64_t r
 {
     const int64_t n = tokens * k, ldx = ldx_bytes / static_cast<int64_t>(sizeof(W));
     const uint32_t row_words = static_cast<uint32_t>(row_bytes / static_cast<int64_t>(sizeof(W)));
-    const uint64_t pieces = (row_words + 32 * kPieceWords - 1) / (32 * kPieceWords);
+    const uint64_t pieces = (row_words + 32 * kPieceWords<W> - 1) / (32 * kPieceWords<W>);
     const size_t plan_bytes = plan_words(experts) * sizeof(uint32_t);
     int dev = 0;
     NVFP4_CUDA_CHECK(cudaGetDevice(&dev));
@@ -724,12 +732,12 @@ int launch_unsort_tokens(const void* rows, int64_t ld, int dtype, int64_t m, con
                          void* y, int num_sms, cudaStream_t stream)
 {
     const size_t size = elem_bytes(dtype);
-    const bool wide = ((reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(y) | static_cast<uintptr_t>(ld * size) | hidden * size) & 15u) == 0;
-    return with_pack(dtype, wide, [&](auto* type) {
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(y) | static_cast<uintptr_t>(ld * size) | hidden * size;
+    return with_pack(dtype, bits, [&](auto* type) {
         using P = std::remove_pointer_t<decltype(type)>;
         using Bits = typename P::Bits;
         constexpr int kN = P::kN;
-        if constexpr (kN > 1) {
+        if constexpr (P::kSize == 16) {
             const RingShape shape = ring_shape(tokens, k, static_cast<int64_t>(hidden * size));
             if (shape.depth >= 2 && shape.units >= kRingLeast * static_cast<uint32_t>(num_sms)) {
                 static bool attr_set[host::kMaxDevices] = {};
@@ -745,7 +753,7 @@ int launch_unsort_tokens(const void* rows, int64_t ld, int dtype, int64_t m, con
             }
         }
         const uint32_t packs = static_cast<uint32_t>(hidden / kN);
-        const uint64_t units = static_cast<uint64_t>(tokens) * ((packs + 32 * kPer - 1) / (32 * kPer));
+        const uint64_t units = static_cast<uint64_t>(tokens) * ((packs + 32 * kPer<P> - 1) / (32 * kPer<P>));
         return host::launch_kernel(unsort_kernel<P>, dim3(blocks_for(units, 8, num_sms, 8)), dim3(256), 0, stream, true,
                                    static_cast<const Bits*>(rows), ld / kN, place, w, static_cast<uint32_t>(tokens), k, m, packs,
                                    static_cast<Bits*>(y));
@@ -757,9 +765,9 @@ int launch_unsort_tokens_backward(const void* dy, int64_t ldy, const void* rows,
                                   cudaStream_t stream)
 {
     const size_t size = elem_bytes(dtype);
-    const bool wide = ((reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(drows) |
-                        static_cast<uintptr_t>(ldy * size) | static_cast<uintptr_t>(ld * size) | hidden * size) & 15u) == 0;
-    return with_pack(dtype, wide, [&](auto* type) {
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(drows) |
+                           static_cast<uintptr_t>(ldy * size) | static_cast<uintptr_t>(ld * size) | hidden * size;
+    return with_pack(dtype, bits, [&](auto* type) {
         using P = std::remove_pointer_t<decltype(type)>;
         using Bits = typename P::Bits;
         constexpr int kN = P::kN;
