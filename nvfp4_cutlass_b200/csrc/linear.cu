@@ -5,12 +5,13 @@
 //
 // Each product is D[r, c] = sum_k A[r, k] B[c, k] with an operand's memory running along k (K-major: x and w in the forward product) or
 // along its own rows (MN-major: w in dx, both in dw); TMA brings 64 of k either way and the instruction descriptor says which, so
-// nothing is transposed in memory.  Two kernels:
+// nothing is transposed in memory.  Three kernels:
 //   product_kernel       one 128 x BN tile to a CTA; up to eight CTAs of a cluster share the contraction of a tile where there are few
 //                        tiles, and add their partial sums through distributed shared memory in a fixed order
 //   product_pair_kernel  persistent CTA pairs, 256 x 256 tiles, two accumulators in turn: the epilogue of a tile runs under the
 //                        products of the next
-// Sums are FP32 in tensor memory from the first product to the epilogue, which rounds once.
+//   token_kernel         one or two rows of x and a small weight: no tensor cores
+// Sums are FP32 from the first product to the epilogue, which rounds once.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -683,6 +684,70 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     }
 }
 
+// ---- one or two tokens ---------------------------------------------------------------------------------------------------
+
+// A product of one or two rows is a pass over the weight and nothing else.  While the weight is small, what counts is how soon the loads go
+// out, not how many are under way: no tensor memory, barriers or clusters; some warps (a power of two) take a row of w, a lane eight
+// 16-byte loads at a time, FP32 sums in a fixed order, and one lane a token finishes the element.
+// This / the tensor cores, one token, BF16, in a graph: 512 x 512 1.8 / 3.6 us, 1024 x 4096 3.6 / 4.9, 4096 x 1024 3.6 / 5.2, 3000 x 2048 6.2 / 6.0,
+// 2048 x 4096 6.5 / 6.3, 4096 x 4096 11.3 / 9.1: taken up to kTokenMostWeights elements of w.
+constexpr uint64_t kTokenMostWeights = 5u << 20;
+constexpr int kTokenThreads = 256, kTokenWarps = kTokenThreads / 32, kTokenLoads = 8;
+template <typename T, typename D, int kTokens>
+__global__ void __launch_bounds__(kTokenThreads)
+token_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw, uint32_t k, uint32_t warps_log2, const Epilogue e)
+{
+    __shared__ float part[kTokenWarps][kTokens];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = 1u << warps_log2, share = warp & (warps - 1);
+    const uint32_t n = blockIdx.x * (kTokenWarps >> warps_log2) + (warp >> warps_log2);
+    const bool mine = n < e.cols;
+    ptx::grid_dependency_wait();
+    float sum[kTokens];
+#pragma unroll
+    for (int t = 0; t < kTokens; ++t) sum[t] = 0.0f;
+    if (mine) {
+        const uint4* row = reinterpret_cast<const uint4*>(w + static_cast<int64_t>(n) * ldw);
+        const uint32_t words = k / 8, step = 32 * warps;
+        for (uint32_t c0 = share * 32 + lane; c0 < words; c0 += step * kTokenLoads) {
+            uint4 v[kTokenLoads];
+#pragma unroll
+            for (int i = 0; i < kTokenLoads; ++i) v[i] = c0 + i * step < words ? row[c0 + i * step] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int i = 0; i < kTokenLoads; ++i) {
+                if (c0 + i * step >= words) break;
+                const uint32_t vw[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+                for (int t = 0; t < kTokens; ++t) {
+                    const uint4 q = reinterpret_cast<const uint4*>(x + t * ldx)[c0 + i * step];
+                    const uint32_t xw[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 a = unpack2<T>(vw[j]), b = unpack2<T>(xw[j]);
+                        sum[t] = fmaf(a.x, b.x, sum[t]);
+                        sum[t] = fmaf(a.y, b.y, sum[t]);
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < kTokens; ++t) {
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum[t] += __shfl_xor_sync(kAll, sum[t], d);
+        if (lane == 0) part[warp][t] = sum[t];
+    }
+    __syncthreads();
+    if (!mine || share != 0 || lane >= kTokens) return;
+    float z = 0.0f;
+    for (uint32_t i = 0; i < warps; ++i) z += part[warp + i][lane];
+    if (e.bias != nullptr) z += to_float(static_cast<const T*>(e.bias)[n]);
+    float y = z, slope = 1.0f;
+    with_activation(e.activation, [&](auto act) { activate<decltype(act)::value, true>(z, y, slope); });
+    if (e.slopes != nullptr) e.slopes[lane * e.lds + n] = static_cast<int16_t>(slope_code(slope));
+    if (e.residual != nullptr) y += to_float(static_cast<const D*>(e.residual)[lane * e.ldr + n]);
+    static_cast<D*>(e.d)[lane * e.ldd + n] = from_float<D>(y);
+}
+
 // ---- persistent CTA pairs ----------------------------------------------------------------------------------------------
 
 constexpr int kPairThreads = 320;                    // warp 0: TMA, warp 1: products (even CTA), warps 2-9: epilogue
@@ -988,10 +1053,23 @@ Form choose_form(const Operands& o, bool wide, int num_sms)
     return best;
 }
 
+template <typename T, typename D>
+int launch_tokens(const Operands& o, const Epilogue& e, int num_sms, cudaStream_t stream)
+{
+    // warps to a row: until there are sixteen to an SM, each with a batch of loads at least
+    uint32_t warps_log2 = 0;
+    while (warps_log2 < 3 && (static_cast<uint64_t>(o.rows_b) << warps_log2) < 16 * static_cast<uint64_t>(num_sms) && (o.k / 8 >> (warps_log2 + 1)) >= 32) ++warps_log2;
+    const uint32_t rows = kTokenWarps >> warps_log2;
+    auto kernel = o.rows_a == 1 ? token_kernel<T, D, 1> : token_kernel<T, D, 2>;
+    return host::launch_kernel(kernel, dim3((o.rows_b + rows - 1) / rows), dim3(kTokenThreads), 0, stream, true, static_cast<const T*>(o.a), o.lda,
+                               static_cast<const T*>(o.b), o.ldb, o.k, warps_log2, e);
+}
+
 // The output (rows_a, rows_b), of type D.
 template <typename T, typename D>
 int launch_product(const Operands& o, const Epilogue& e, int num_sms, cudaStream_t stream)
 {
+    if (o.rows_a <= 2 && !o.a_mn && !o.b_mn && static_cast<uint64_t>(o.rows_b) * o.k <= kTokenMostWeights) return launch_tokens<T, D>(o, e, num_sms, stream);
     const Form f = choose_form(o, !std::is_same<D, T>::value, num_sms);
     if (f.kind == Form::kSwap) {                     // the weight's rows on the tensor memory's lanes
         const Operands s{o.b, o.ldb, false, o.rows_b, o.a, o.lda, false, o.rows_a, o.k, o.status};

@@ -106,7 +106,7 @@ def test_host_tensors_are_refused():
 
 # tokens to the tiles of the few-row form (16, 32, 64, 128), contractions that split over clusters or not, narrow, odd and wide outputs,
 # left-over pieces of every tile, enough tiles for the pairs
-SIZES = [(1, 1, 8), (1, 4096, 4096), (3, 25, 3768), (16, 128, 64), (17, 513, 2048), (33, 1411, 2048), (64, 96, 520), (65, 31, 72), (128, 1000, 1024),
+SIZES = [(1, 1, 8), (1, 4096, 4096), (2, 4096, 2048), (1, 700, 4104), (2, 513, 2048), (1, 130, 20000), (2, 9, 1000), (3, 25, 3768), (16, 128, 64), (17, 513, 2048), (33, 1411, 2048), (64, 96, 520), (65, 31, 72), (128, 1000, 1024),
          (129, 64, 200), (300, 33, 1032), (257, 129, 8), (500, 256, 4096), (1000, 65, 136), (2049, 128, 4096), (777, 3001, 264), (4099, 2050, 72), (2500, 4104, 392)]
 
 
@@ -178,7 +178,7 @@ def test_python_refusals():
 
 # ---- backward --------------------------------------------------------------------------------------------------------
 
-TRAIN_SIZES = [(1, 1, 8), (1, 300, 64), (7, 33, 72), (130, 64, 200), (33, 1411, 520), (300, 129, 1032), (1000, 128, 2048), (513, 2050, 264), (2600, 2056, 3080)]
+TRAIN_SIZES = [(1, 1, 8), (1, 300, 64), (2, 41, 264), (7, 33, 72), (130, 64, 200), (33, 1411, 520), (300, 129, 1032), (1000, 128, 2048), (513, 2050, 264), (2600, 2056, 3080)]
 
 
 @gpu
