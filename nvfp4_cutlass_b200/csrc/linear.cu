@@ -1032,7 +1032,7 @@ Form choose_form(const Operands& o, bool wide, int num_sms)
     Form best{Form::kNormal, 128, 0};
     double least = 1e30;
     auto consider = [&](Form::Kind kind, uint64_t tiles, const TileCost& c, double start, uint32_t most_log2) {
-        for (uint32_t s = 0; s <= most_log2 && (k_blocks >> s) >= 2; ++s) {
+        for (uint32_t s = 0; s <= most_log2 && (s == 0 || k_blocks >> s >= 2); ++s) {
             const uint64_t at_once = ctas_at_once(s, num_sms);
             const double resident = static_cast<double>(((tiles << s) + at_once - 1) / at_once);
             const double loop = ((k_blocks + (1u << s) - 1) >> s) * c.block * resident;
