@@ -282,17 +282,20 @@ __device__ __forceinline__ void load_accumulators(uint32_t taddr, float (&v)[kN]
     for (uint32_t i = 0; i < kN; ++i) v[i] = __uint_as_float(raw[i]);
 }
 
-// An epilogue warp's way out through shared memory, where TMA can address the output: 32 rows x 64 columns at a time, a row (128 bytes,
-// 128-byte swizzle) to a lane as tensor memory gives them, so that nothing has to be transposed and every line of the output is
+// An epilogue warp's way out through shared memory, where TMA can address the output: 32 rows x 64 columns (32 of FP32) at a time, a row (128
+// bytes, 128-byte swizzle) to a lane as tensor memory gives them, so that nothing has to be transposed and every line of the output is
 // written whole.  The residual comes into the same buffer by TMA beforehand and is replaced by the result in place.
-constexpr uint32_t kBox = 64, kBoxBytes = 32 * kBox * 2;
+// Slopes go the same way beside a 16-bit output.
+template <typename D>
+constexpr uint32_t kBox = 128 / sizeof(D);
+constexpr uint32_t kBoxBytes = 32 * 128;
 struct Maps {
-    CUtensorMap d, residual, slopes;                 // boxes of 32 rows x 64 columns
+    CUtensorMap d, residual, slopes;                 // boxes of 32 rows x 128 bytes
 };
-template <typename T>
+template <typename T, typename D>
 struct Stage {
-    uint32_t out, out_step, slopes, slopes_step;     // shared memory: buffers of the output (and residual) and of the slopes, of box 0 and from there to box 1's
-    uint64_t* landed;                                // [2] residual of a box is there
+    uint32_t out, out_step, slopes, slopes_step;     // shared memory: buffers of the output (and residual) and of the slopes, of box 0 and from one to the next
+    uint64_t* landed;                                // per box: its residual is there
     uint32_t phase = 0;
     const Maps* maps;
 
@@ -332,7 +335,7 @@ struct Stage {
                 b[i] = bits[min(col + 2 * i, e.cols - 1)] | static_cast<uint32_t>(bits[min(col + 2 * i + 1, e.cols - 1)]) << 16;
         }
     }
-    // One box: accumulators at taddr, columns [col, col + 64).  False: the residual never came.
+    // One box: accumulators at taddr, columns [col, col + kBox<D>).  False: the residual never came.
     __device__ __forceinline__ bool finish(uint32_t taddr, uint32_t box, uint32_t col, uint32_t row0, uint32_t lane, const Epilogue& e,
                                            volatile uint32_t* abort_flag)
     {
@@ -341,7 +344,7 @@ struct Stage {
             phase ^= 1u << box;
         }
 #pragma unroll
-        for (uint32_t half = 0; half < 2; ++half) {
+        for (uint32_t half = 0; half < kBox<D> / 32; ++half) {
             float v[32];
             uint32_t b[16];
             if (e.bias != nullptr) load_bias(e, col + half * 32, b);
@@ -355,48 +358,69 @@ struct Stage {
                 }
             }
             auto piece = [&](uint32_t buffer, uint32_t q) { return buffer + lane * 128 + (((half * 4 + q) ^ (lane & 7u)) << 4); };
-            if (e.activation != NVFP4_ACTIVATION_NONE)
-                with_activation(e.activation, [&](auto act) {
-                    constexpr int kAct = decltype(act)::value;
-                    float2 y, slope;
-                    if (e.slopes != nullptr) {
+            if constexpr (std::is_same<D, float>::value) {
+                if (e.activation != NVFP4_ACTIVATION_NONE)
+                    with_activation(e.activation, [&](auto act) {
+                        float slope;
 #pragma unroll
-                        for (uint32_t q = 0; q < 4; ++q) {
-                            uint32_t w[4];
+                        for (uint32_t i = 0; i < 32; ++i) activate<decltype(act)::value, false>(v[i], v[i], slope);
+                    });
 #pragma unroll
-                            for (uint32_t i = 0; i < 4; ++i) {
-                                const uint32_t at = 8 * q + 2 * i;
-                                activate2<kAct, true>(make_float2(v[at], v[at + 1]), y, slope);
-                                v[at] = y.x;
-                                v[at + 1] = y.y;
-                                w[i] = slope_codes(slope);
-                            }
-                            ptx::sts128(piece(slopes + box * slopes_step, q), w[0], w[1], w[2], w[3]);
-                        }
-                    } else {
-#pragma unroll
-                        for (uint32_t i = 0; i < 32; i += 2) {
-                            activate2<kAct, false>(make_float2(v[i], v[i + 1]), y, slope);
-                            v[i] = y.x;
-                            v[i + 1] = y.y;
-                        }
+                for (uint32_t q = 0; q < 8; ++q) {
+                    const uint32_t to = piece(out + box * out_step, q);
+                    if (e.residual != nullptr) {
+                        const uint4 r = ptx::lds128(to);
+                        v[4 * q] += __uint_as_float(r.x);
+                        v[4 * q + 1] += __uint_as_float(r.y);
+                        v[4 * q + 2] += __uint_as_float(r.z);
+                        v[4 * q + 3] += __uint_as_float(r.w);
                     }
-                });
-#pragma unroll
-            for (uint32_t q = 0; q < 4; ++q) {
-                const uint32_t to = piece(out + box * out_step, q);
-                if (e.residual != nullptr) {
-                    const uint4 r = ptx::lds128(to);
-                    const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-                        const float2 f = unpack2<T>(rw[i]);
-                        v[8 * q + 2 * i] += f.x;
-                        v[8 * q + 2 * i + 1] += f.y;
-                    }
+                    ptx::sts128(to, __float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]), __float_as_uint(v[4 * q + 3]));
                 }
-                ptx::sts128(to, pack2<T>(v[8 * q], v[8 * q + 1]), pack2<T>(v[8 * q + 2], v[8 * q + 3]), pack2<T>(v[8 * q + 4], v[8 * q + 5]),
-                            pack2<T>(v[8 * q + 6], v[8 * q + 7]));
+            } else {
+                if (e.activation != NVFP4_ACTIVATION_NONE)
+                    with_activation(e.activation, [&](auto act) {
+                        constexpr int kAct = decltype(act)::value;
+                        float2 y, slope;
+                        if (e.slopes != nullptr) {
+#pragma unroll
+                            for (uint32_t q = 0; q < 4; ++q) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (uint32_t i = 0; i < 4; ++i) {
+                                    const uint32_t at = 8 * q + 2 * i;
+                                    activate2<kAct, true>(make_float2(v[at], v[at + 1]), y, slope);
+                                    v[at] = y.x;
+                                    v[at + 1] = y.y;
+                                    w[i] = slope_codes(slope);
+                                }
+                                ptx::sts128(piece(slopes + box * slopes_step, q), w[0], w[1], w[2], w[3]);
+                            }
+                        } else {
+#pragma unroll
+                            for (uint32_t i = 0; i < 32; i += 2) {
+                                activate2<kAct, false>(make_float2(v[i], v[i + 1]), y, slope);
+                                v[i] = y.x;
+                                v[i + 1] = y.y;
+                            }
+                        }
+                    });
+#pragma unroll
+                for (uint32_t q = 0; q < 4; ++q) {
+                    const uint32_t to = piece(out + box * out_step, q);
+                    if (e.residual != nullptr) {
+                        const uint4 r = ptx::lds128(to);
+                        const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            const float2 f = unpack2<T>(rw[i]);
+                            v[8 * q + 2 * i] += f.x;
+                            v[8 * q + 2 * i + 1] += f.y;
+                        }
+                    }
+                    ptx::sts128(to, pack2<T>(v[8 * q], v[8 * q + 1]), pack2<T>(v[8 * q + 2], v[8 * q + 3]), pack2<T>(v[8 * q + 4], v[8 * q + 5]),
+                                pack2<T>(v[8 * q + 6], v[8 * q + 7]));
+                }
             }
         }
         ptx::fence_proxy_async_smem();
@@ -451,7 +475,7 @@ __host__ __device__ constexpr uint32_t partial_pad(uint32_t bn, uint32_t splits)
 __host__ __device__ constexpr uint32_t partial_bytes(uint32_t bn, uint32_t splits) { return splits > 1 ? (bn + splits * partial_pad(bn, splits)) * BM * 4 : 0; }
 constexpr uint32_t tile_smem(uint32_t bn, uint32_t depth, uint32_t splits)
 {
-    return 1024 + depth * tile_stage(bn) + partial_bytes(bn, splits) + (2 * kMaxDepth + 4) * 8 + 16 + kTileEpiWarps * 16;
+    return 1024 + depth * tile_stage(bn) + partial_bytes(bn, splits) + (2 * kMaxDepth + 4) * 8 + 16 + kTileEpiWarps * 32;
 }
 // For an FP32 output the epilogue warps take the accumulators over every four K blocks and add them up in registers, two accumulators in
 // turn: the tensor core cuts what it adds to a long sum (K = 4096 in one accumulator: off by 4.3e-6 of the result, FP32 sums by 6e-7).
@@ -475,8 +499,8 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     uint64_t* drained = full + kMaxDepth;
     uint64_t* tmem_full = drained + kMaxDepth;       // per accumulator
     uint64_t* tmem_empty = tmem_full + 2;
-    uint64_t* landed = tmem_empty + 2;               // [epilogue warp][2]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(landed + 2 * kTileEpiWarps);
+    uint64_t* landed = tmem_empty + 2;               // [epilogue warp][4] residual of a box
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(landed + 4 * kTileEpiWarps);
     volatile uint32_t* abort_flag = tmem_slot + 1;
 
     const uint32_t warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -484,7 +508,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < depth; ++i) { ptx::mbar_init(full + i, 1); ptx::mbar_init(drained + i, 1); }
         for (uint32_t i = 0; i < 2; ++i) { ptx::mbar_init(tmem_full + i, 1); ptx::mbar_init(tmem_empty + i, kTileEpiWarps); }
-        for (uint32_t i = 0; i < 2 * kTileEpiWarps; ++i) ptx::mbar_init(landed + i, 1);
+        for (uint32_t i = 0; i < 4 * kTileEpiWarps; ++i) ptx::mbar_init(landed + i, 1);
         *abort_flag = 0;
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&tm_a);
@@ -654,16 +678,18 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
             }
         }
     } else if (warp >= 2 && ok && e.staged) {
-        // the ring is at rest (the accumulators are complete): its memory takes the boxes, out and slopes of two for every warp
-        if constexpr (!kSwap && !kWide) {
+        // the ring is at rest (the accumulators are complete): its memory takes the boxes, four for every warp: of the output, or two of the
+        // output and two of the slopes
+        if constexpr (!kSwap) {
+            constexpr uint32_t kColumns = kBox<D>;
             const uint32_t at = smem + (warp - 2) * 4 * kBoxBytes, row0 = a0 + quad * 32;
-            Stage<T> stage{at, kBoxBytes, at + 2 * kBoxBytes, kBoxBytes, landed + 2 * (warp - 2), 0, &maps};
+            Stage<T, D> stage{at, kBoxBytes, at + 2 * kBoxBytes, kBoxBytes, landed + 4 * (warp - 2), 0, &maps};
             if (row0 < e.rows) {
                 if (e.residual != nullptr)
-                    for (uint32_t c = 0; c < live; c += kBox) stage.request(c / kBox, b0 + c, row0, lane);
+                    for (uint32_t c = 0; c < live; c += kColumns) stage.request(c / kColumns, b0 + c, row0, lane);
 #pragma unroll 1
-                for (uint32_t c = 0; c < live; c += kBox)
-                    if (!stage.finish(taddr + c, c / kBox, b0 + c, row0, lane, e, abort_flag)) { give_up(); break; }
+                for (uint32_t c = 0; c < live; c += kColumns)
+                    if (!stage.finish(taddr + c, c / kColumns, b0 + c, row0, lane, e, abort_flag)) { give_up(); break; }
                 if (lane == 0) ptx::bulk_wait();
             }
         }
@@ -850,19 +876,20 @@ product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         const uint32_t tmem_empty_even = ptx::map_to_cta(ptx::smem_u32(tmem_empty), 0);
         const uint32_t boxes = smem + kOffBoxes + (warp - kPairFirstEpi) * 2 * kBoxBytes;
         const bool both = e.slopes != nullptr;       // the second buffer takes the slopes
-        Stage<T> stage{boxes, both ? 0u : kBoxBytes, boxes + kBoxBytes, 0u, landed + 2 * (warp - kPairFirstEpi), 0, &maps};
+        constexpr uint32_t kBoxColumns = kBox<T>;
+        Stage<T, T> stage{boxes, both ? 0u : kBoxBytes, boxes + kBoxBytes, 0u, landed + 2 * (warp - kPairFirstEpi), 0, &maps};
         uint32_t n = 0;
         for (uint32_t tile = pair_id; ok && tile < tiles; tile += num_pairs, ++n) {
             const uint32_t acc = n & 1;
             uint32_t a_blk, b_blk;
             gemm::tile_coords(tile, p.tiles_a, p.tiles_b, 8, a_blk, b_blk);
             const uint32_t row0 = (a_blk * 2 + rank) * BM + quad * 32, col0 = b_blk * kPairBN + half * 128;
-            const bool wanted = row0 < e.rows && col0 < e.cols, second = col0 + kBox < e.cols;
+            const bool wanted = row0 < e.rows && col0 < e.cols, second = col0 + kBoxColumns < e.cols;
             if (e.staged && wanted) {
                 stage.reclaim(lane);
                 if (e.residual != nullptr) {
                     stage.request(0, col0, row0, lane);
-                    if (second && !both) stage.request(1, col0 + kBox, row0, lane);
+                    if (second && !both) stage.request(1, col0 + kBoxColumns, row0, lane);
                 }
             }
             if (!ptx::all_lanes(ptx::mbar_wait_relaxed(tmem_full + acc, (n >> 1) & 1, abort_flag, 50))) { give_up(); break; }
@@ -873,9 +900,9 @@ product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                 for (uint32_t box = 0; wanted && ok && box < (second ? 2u : 1u); ++box) {
                     if (box == 1 && both) {
                         stage.reclaim(lane);
-                        if (e.residual != nullptr) stage.request(1, col0 + kBox, row0, lane);
+                        if (e.residual != nullptr) stage.request(1, col0 + kBoxColumns, row0, lane);
                     }
-                    if (!stage.finish(taddr + box * kBox, box, col0 + box * kBox, row0, lane, e, abort_flag)) give_up();
+                    if (!stage.finish(taddr + box * kBoxColumns, box, col0 + box * kBoxColumns, row0, lane, e, abort_flag)) give_up();
                 }
             } else if (wanted) {
 #pragma unroll 1
@@ -915,20 +942,24 @@ int operand_map(CUtensorMap* map, const void* base, int64_t ld, bool mn_major, u
                                       mn_major ? 64 : tile, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Maps of what the epilogue moves by TMA, if it can; T has 16 bits, as the slopes have.
-template <typename T>
+// Maps of what the epilogue moves by TMA, if it can.
+template <typename T, typename D>
 int output_maps(Maps* maps, Epilogue* e)
 {
-    auto aligned = [](const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0; };
+    constexpr bool kFloat = std::is_same<D, float>::value;
+    auto aligned = [](const void* p, int64_t ld, int64_t size) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld * size % 16 == 0; };
     *maps = Maps{};
-    e->staged = aligned(e->d, e->ldd) && (e->residual == nullptr || aligned(e->residual, e->ldr)) && (e->slopes == nullptr || aligned(e->slopes, e->lds));
+    e->staged = aligned(e->d, e->ldd, sizeof(D)) && (e->residual == nullptr || aligned(e->residual, e->ldr, sizeof(D))) &&
+                (e->slopes == nullptr || (!kFloat && aligned(e->slopes, e->lds, 2)));
     if (!e->staged) return NVFP4_OK;
     auto map = [&](CUtensorMap* m, CUtensorMapDataType type, const void* base, int64_t ld) {
-        return host::encode_tensor_map_2d(m, type, 2, base, e->cols, e->rows, static_cast<uint64_t>(ld) * 2, kBox, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+        return host::encode_tensor_map_2d(m, type, sizeof(D), base, e->cols, e->rows, static_cast<uint64_t>(ld) * sizeof(D), kBox<D>, 32,
+                                          CU_TENSOR_MAP_SWIZZLE_128B);
     };
-    if (int rc = map(&maps->d, kMapType<T>, e->d, e->ldd)) return rc;
+    constexpr CUtensorMapDataType kType = kFloat ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : kMapType<T>;
+    if (int rc = map(&maps->d, kType, e->d, e->ldd)) return rc;
     if (e->residual != nullptr)
-        if (int rc = map(&maps->residual, kMapType<T>, e->residual, e->ldr)) return rc;
+        if (int rc = map(&maps->residual, kType, e->residual, e->ldr)) return rc;
     if (e->slopes != nullptr)
         if (int rc = map(&maps->slopes, CU_TENSOR_MAP_DATA_TYPE_UINT16, e->slopes, e->lds)) return rc;
     return NVFP4_OK;
@@ -949,9 +980,9 @@ int launch_tiles(const Operands& o, Epilogue e, uint32_t splits_log2, int num_sm
 {
     CUtensorMap tm_a, tm_b;
     Maps maps{};
-    if constexpr (!kSwap && std::is_same<D, T>::value)
+    if constexpr (!kSwap)
         if (splits_log2 == 0)
-            if (int rc = output_maps<T>(&maps, &e)) return rc;
+            if (int rc = output_maps<T, D>(&maps, &e)) return rc;
     if (int rc = operand_map<T>(&tm_a, o.a, o.lda, o.a_mn, o.rows_a, o.k, BM)) return rc;
     if (int rc = operand_map<T>(&tm_b, o.b, o.ldb, o.b_mn, o.rows_b, o.k, BN)) return rc;
     Product p{};
@@ -985,7 +1016,7 @@ int launch_pairs(const Operands& o, Epilogue e, int num_sms, cudaStream_t stream
 {
     CUtensorMap tm_a, tm_b;
     Maps maps;
-    if (int rc = output_maps<T>(&maps, &e)) return rc;
+    if (int rc = output_maps<T, T>(&maps, &e)) return rc;
     if (int rc = operand_map<T>(&tm_a, o.a, o.lda, o.a_mn, o.rows_a, o.k, BM)) return rc;
     if (int rc = operand_map<T>(&tm_b, o.b, o.ldb, o.b_mn, o.rows_b, o.k, BM)) return rc;
     Product p{};
@@ -1015,6 +1046,8 @@ int launch_pairs(const Operands& o, Epilogue e, int num_sms, cudaStream_t stream
 // cluster costs by the tile's columns.  Estimates are within a tenth or so of what was measured: 64 x 4096 x 4096 (swap 64 / 4) 10.4 for
 // 11.1, 256 x 1024 x 4096 (swap 64 / 4) 7.9 for 9.9, 512 x 4096 x 4096 (normal 128) 18 for 19, 1024 x 4096 x 4096 (pairs) 24 for 26.  Against the
 // best of all forms by measurement the choice loses up to 8 % over 1 to 2048 rows, 128 to 4096 columns, K 1024 and 4096.
+// Tiles of 128 columns with an FP32 output have an SM to themselves (the sums in their registers): of several, nobody's products run under
+// another's sums and stores, and a block costs 0.41 us.  8192 x 4096 on swapped tiles of 64 / tiles of 128: K = 64 47 / 63 us, 1024 110 / 124, 4096 321 / 354.
 struct Form {
     enum Kind { kSwap, kNormal, kPairs } kind;
     uint32_t bn, splits_log2;
@@ -1035,8 +1068,9 @@ Form choose_form(const Operands& o, bool wide, int num_sms)
         for (uint32_t s = 0; s <= most_log2 && (s == 0 || k_blocks >> s >= 2); ++s) {
             const uint64_t at_once = ctas_at_once(s, num_sms);
             const double resident = static_cast<double>(((tiles << s) + at_once - 1) / at_once);
-            const double loop = ((k_blocks + (1u << s) - 1) >> s) * c.block * resident;
-            const double t = start * (resident > 2 ? resident / 2 : 1) + (s ? c.split : 0) + std::sqrt(loop * loop + hbm * hbm);
+            const bool alone = wide && c.bn == 128 && resident > 1;
+            const double loop = ((k_blocks + (1u << s) - 1) >> s) * (alone ? 0.41 : c.block) * resident;
+            const double t = start * (alone ? resident : resident > 2 ? resident / 2 : 1) + (s ? c.split : 0) + std::sqrt(loop * loop + hbm * hbm);
             if (t < least) { least = t; best = Form{kind, c.bn, s}; }
             if (tiles << (s + 1) > 2 * static_cast<uint64_t>(num_sms)) break;
         }
