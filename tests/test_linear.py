@@ -121,6 +121,18 @@ def test_products_against_64_bits(m, n, k):
         check_forward(linear(x.cuda(), w.cuda(), bias.cuda(), out_dtype=torch.float32, activation=act), x, w, bias, None, act, torch.float32)
 
 
+# One wave of wide tiles and several waves of them, columns and rows left over, rows that are whole 16 bytes and rows that are not
+@gpu
+@pytest.mark.parametrize("m, n, k", [(16283, 128, 264), (4000, 500, 392), (3900, 500, 64), (2500, 4104, 392), (1000, 1001, 72), (9000, 36, 8)])
+def test_fp32_outputs_with_a_residual(m, n, k):
+    x, w, bias, residual = make(m, n, k, torch.bfloat16, m + n, torch.float32)
+    check_forward(linear(x.cuda(), w.cuda(), bias.cuda(), residual.cuda(), activation="gelu", out_dtype=torch.float32), x, w, bias, residual, "gelu",
+                  torch.float32)
+    wide = torch.full((m, n + 4), 7.0, device="cuda")                       # a residual of longer rows
+    wide[:, :n] = residual.cuda()
+    check_forward(linear(x.cuda(), w.cuda(), None, wide[:, :n], out_dtype=torch.float32), x, w, None, residual, "none", torch.float32)
+
+
 @gpu
 @pytest.mark.parametrize("activation", ACTIVATIONS)
 @pytest.mark.parametrize("m, n, k", [(5, 200, 512), (200, 200, 64), (3000, 1536, 128)])
