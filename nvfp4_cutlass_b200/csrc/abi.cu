@@ -856,7 +856,7 @@ int nvfp4_unsort_tokens_backward(const void* dy, int64_t ldy_elems, const void* 
     NVFP4_REQUIRE(on_elements(dy, dtype) && on_elements(rows, dtype) && on_elements(drows, dtype), "rows are not aligned to their type");
     host::DeviceInfo* dev;
     if (int rc = host::device_info(-1, &dev)) return rc;
-    return launch_unsort_tokens_backward(dy, ldy_elems, rows, ld_elems, dtype, M, place, source, w, tokens, k, hidden, drows, dw, dev->hw_sms,
+    return launch_unsort_tokens_backward(dy, ldy_elems, rows, ld_elems, dtype, M, place, w, tokens, k, hidden, drows, dw, dev->hw_sms,
                                          static_cast<cudaStream_t>(stream));
 }
 

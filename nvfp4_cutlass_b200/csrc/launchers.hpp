@@ -65,8 +65,7 @@ int launch_sort_tokens(const void* x, int64_t ldx_bytes, int64_t tokens, int k, 
 int launch_unsort_tokens(const void* rows, int64_t ld, int dtype, int64_t m, const int64_t* place, const float* w, int64_t tokens, int k, int hidden,
                          void* y, int num_sms, cudaStream_t stream);
 int launch_unsort_tokens_backward(const void* dy, int64_t ldy, const void* rows, int64_t ld, int dtype, int64_t m, const int64_t* place,
-                                  const int32_t* source, const float* w, int64_t tokens, int k, int hidden, void* drows, float* dw, int num_sms,
-                                  cudaStream_t stream);
+                                  const float* w, int64_t tokens, int k, int hidden, void* drows, float* dw, int num_sms, cudaStream_t stream);
 
 int launch_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual, int64_t ldr, void* d, int64_t ldd,
                   int16_t* slopes, int64_t lds, int M, int N, int K, bool bf16, bool out32, int activation, int32_t* status, int num_sms,

@@ -574,16 +574,31 @@ RingShape ring_shape(int64_t tokens, int k, int64_t row_bytes)
     return r;
 }
 
-// Gradients of that sum: drows[place[t, j]] = w[t, j] * dy[t], zero for rows without a pair, dw[t, j] = <dy[t], rows[place[t, j]]>.
+// Gradients of that sum: drows[r] = sum of w[t, j] * dy[t] over the pairs that name row r, dw[t, j] = <dy[t], rows[place[t, j]]>.
+// The sum takes any order that names rows, not the sort's alone: a part of its tokens, pairs dropped afterwards, one row for several
+// pairs.  So every row's pairs are counted first (a count does not depend on the atomics' order; 8192 x 8 pairs: with the clearing
+// of the counts 4 us of the 214).
 // A warp takes a pair: its dot product stays inside the warp, in a fixed order, and four packs a lane of the row and of dy are under way
 // at a time in few registers.  The pairs of a token are neighbouring warps', which read dy from L1 behind the first.  (A block to a token,
-// eight rows at a time to a thread, took 138 registers and ran at an eighth of the warps: 455 us for 8192 x 8 rows of 8 KB.)
-// Behind the pairs: warps that zero the rows whose source is -1.  drows or dw may be NULL; rows is read for dw alone.
+// eight rows at a time to a thread, took 138 registers and ran at an eighth of the warps: 455 us for 8192 x 8 rows of 8 KB.)  A row that
+// this pair alone names is written on the way.
+// Behind the pairs: warps for the rows that none names (zero) or several do: those look their pairs up among all, in ascending order, FP32,
+// rounded once.  drows or dw may be NULL; rows is read for dw alone, named for drows.
 constexpr int kBackThreads = 256, kBackWarps = kBackThreads / 32;
+__global__ void __launch_bounds__(kBackThreads)
+count_names_kernel(const int64_t* __restrict__ place, uint32_t pairs, uint32_t m, uint32_t* __restrict__ named)
+{
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
+    for (uint64_t p = static_cast<uint64_t>(blockIdx.x) * kBackThreads + threadIdx.x; p < pairs; p += static_cast<uint64_t>(gridDim.x) * kBackThreads) {
+        const int64_t r = place[p];
+        if (r >= 0 && r < m) atomicAdd(named + r, 1u);
+    }
+}
 template <typename P>
 __global__ void __launch_bounds__(kBackThreads, 4)
 unsort_backward_kernel(const typename P::Bits* __restrict__ dy, int64_t ldy, const typename P::Bits* __restrict__ rows, int64_t ld,
-                       const int64_t* __restrict__ place, const int32_t* __restrict__ source, const float* __restrict__ w, uint32_t pairs, uint32_t k,
+                       const int64_t* __restrict__ place, const uint32_t* __restrict__ named, const float* __restrict__ w, uint32_t pairs, uint32_t k,
                        uint32_t m, uint32_t row_packs, typename P::Bits* __restrict__ drows, float* __restrict__ dw)
 {
     using Bits = typename P::Bits;
@@ -593,9 +608,30 @@ unsort_backward_kernel(const typename P::Bits* __restrict__ dy, int64_t ldy, con
     ptx::grid_dependency_wait();
     for (uint64_t unit = static_cast<uint64_t>(blockIdx.x) * kBackWarps + (threadIdx.x >> 5); unit < units; unit += static_cast<uint64_t>(gridDim.x) * kBackWarps) {
         if (unit >= pairs) {
-            const uint32_t r = static_cast<uint32_t>(unit - pairs);
-            if (source[r] >= 0) continue;
-            for (uint32_t c = lane; c < row_packs; c += 32) drows[static_cast<int64_t>(r) * row_packs + c] = Bits{};
+            const uint32_t r = static_cast<uint32_t>(unit - pairs), names = named[r];
+            if (names == 1) continue;
+            Bits* to = drows + static_cast<int64_t>(r) * row_packs;
+            for (uint32_t c0 = 0; c0 < row_packs; c0 += 32) {
+                const uint32_t c = c0 + lane;
+                float acc[kN];
+#pragma unroll
+                for (int q = 0; q < kN; ++q) acc[q] = 0.0f;
+                uint32_t left = names;
+                for (uint32_t p0 = 0; left != 0 && p0 < pairs; p0 += 32) {
+                    unsigned mine = __ballot_sync(kAll, p0 + lane < pairs && place[p0 + lane] == r);
+                    left -= __popc(mine);
+                    for (; mine != 0; mine &= mine - 1) {
+                        const uint32_t p = p0 + __ffs(mine) - 1;
+                        const float weight = w != nullptr ? w[p] : 1.0f;
+                        if (c >= row_packs) continue;
+                        float f[kN];
+                        P::unpack(dy[static_cast<int64_t>(p / k) * ldy + c], f);
+#pragma unroll
+                        for (int q = 0; q < kN; ++q) acc[q] = fmaf(weight, f[q], acc[q]);
+                    }
+                }
+                if (c < row_packs) to[c] = P::pack(acc);
+            }
             continue;
         }
         const uint32_t p = static_cast<uint32_t>(unit);
@@ -604,6 +640,8 @@ unsort_backward_kernel(const typename P::Bits* __restrict__ dy, int64_t ldy, con
             if (dw != nullptr && lane == 0) dw[p] = 0.0f;
             continue;
         }
+        const bool write = drows != nullptr && named[r] == 1;
+        if (dw == nullptr && !write) continue;
         const float weight = w != nullptr ? w[p] : 1.0f;
         const Bits* from = dy + static_cast<int64_t>(p / k) * ldy;
         const Bits* row = rows + r * ld;
@@ -629,7 +667,7 @@ unsort_backward_kernel(const typename P::Bits* __restrict__ dy, int64_t ldy, con
 #pragma unroll
                     for (int q = 0; q < kN; ++q) dot = fmaf(gf[q], f[q], dot);
                 }
-                if (drows != nullptr) {
+                if (write) {
 #pragma unroll
                     for (int q = 0; q < kN; ++q) f[q] = weight * gf[q];
                     to[c0 + i * 32] = P::pack(f);
@@ -761,22 +799,41 @@ int launch_unsort_tokens(const void* rows, int64_t ld, int dtype, int64_t m, con
 }
 
 int launch_unsort_tokens_backward(const void* dy, int64_t ldy, const void* rows, int64_t ld, int dtype, int64_t m, const int64_t* place,
-                                  const int32_t* source, const float* w, int64_t tokens, int k, int hidden, void* drows, float* dw, int num_sms,
-                                  cudaStream_t stream)
+                                  const float* w, int64_t tokens, int k, int hidden, void* drows, float* dw, int num_sms, cudaStream_t stream)
 {
     const size_t size = elem_bytes(dtype);
     const uintptr_t bits = reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(drows) |
                            static_cast<uintptr_t>(ldy * size) | static_cast<uintptr_t>(ld * size) | hidden * size;
-    return with_pack(dtype, bits, [&](auto* type) {
+    const uint64_t pairs = static_cast<uint64_t>(tokens) * k, units = pairs + (drows != nullptr ? m : 0);
+    uint32_t* named = nullptr;                       // pairs to a row
+    if (drows != nullptr && m > 0) {
+        int dev = 0;
+        NVFP4_CUDA_CHECK(cudaGetDevice(&dev));
+        cudaMemPool_t pool;
+        if (int rc = host::workspace_pool(dev, &pool)) return rc;
+        const size_t bytes = static_cast<size_t>(m) * sizeof(uint32_t);
+        NVFP4_CUDA_CHECK(cudaMallocFromPoolAsync(reinterpret_cast<void**>(&named), bytes, pool, stream));
+        int rc = NVFP4_OK;
+        if (cudaError_t err = cudaMemsetAsync(named, 0, bytes, stream); err != cudaSuccess) rc = host::fail(NVFP4_E_CUDA, "clearing the counts failed: %s", cudaGetErrorString(err));
+        if (rc == NVFP4_OK && pairs > 0)
+            rc = host::launch_kernel(count_names_kernel, dim3(blocks_for((pairs + 31) / 32, kBackWarps, num_sms, 8)), dim3(kBackThreads), 0, stream, true, place,
+                                     static_cast<uint32_t>(pairs), static_cast<uint32_t>(m), named);
+        if (rc != NVFP4_OK) {
+            cudaFreeAsync(named, stream);
+            return rc;
+        }
+    }
+    const int rc = with_pack(dtype, bits, [&](auto* type) {
         using P = std::remove_pointer_t<decltype(type)>;
         using Bits = typename P::Bits;
         constexpr int kN = P::kN;
-        const uint64_t pairs = static_cast<uint64_t>(tokens) * k, units = pairs + (drows != nullptr ? m : 0);
         return host::launch_kernel(unsort_backward_kernel<P>, dim3(blocks_for(units, kBackWarps, num_sms, 8)), dim3(kBackThreads), 0, stream, true,
-                                   static_cast<const Bits*>(dy), ldy / kN, static_cast<const Bits*>(rows), ld / kN, place, source, w,
+                                   static_cast<const Bits*>(dy), ldy / kN, static_cast<const Bits*>(rows), ld / kN, place, named, w,
                                    static_cast<uint32_t>(pairs), static_cast<uint32_t>(k), static_cast<uint32_t>(m), static_cast<uint32_t>(hidden / kN),
                                    static_cast<Bits*>(drows), dw);
     });
+    if (named != nullptr) cudaFreeAsync(named, stream);
+    return rc;
 }
 
 }  // namespace nvfp4

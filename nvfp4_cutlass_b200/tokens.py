@@ -120,8 +120,10 @@ def unsort_tokens(rows: torch.Tensor, order: TokenOrder, weights: Optional[torch
     """y[t] = sum over the choices j of weights[t, j] * rows[order.place[t, j]], (tokens, hidden) of the rows' type.
 
     ``rows`` (M, hidden) in the order that sort_tokens gave, ``weights`` float32 (tokens, k), or None for a plain sum.  Sums are FP32 in
-    ascending j, rounded once.  A pair without a row contributes nothing, and its weight's gradient is 0.  Differentiable in ``rows`` and
-    ``weights``; the gradient of rows without a pair is zero."""
+    ascending j, rounded once.  A pair without a row (a place outside [0, M)) contributes nothing, and its weight's gradient is 0.
+    Differentiable in ``rows`` and ``weights``; the gradient of rows that no pair names is zero.  ``order.place`` may also be a part of the
+    sort's, have pairs masked out, or name a row more than once (whose gradient is then the sum over its pairs): forward and backward follow
+    it alone."""
     place, source = order.place, order.source
     if _C._binding is not None:
         result = _C._binding.unsort(rows, place, source, weights)

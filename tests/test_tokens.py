@@ -640,3 +640,67 @@ def test_what_is_not_differentiated_costs_nothing():
     assert weights.requires_grad and not ids.requires_grad
     with torch.no_grad():
         assert not sort_tokens(x, ids, 8)[0].requires_grad and not route_tokens(x, 2)[1].requires_grad
+
+
+# Orders that the caller has changed or made: what the forward sum takes from a row is what its gradient gets, whoever made the order
+def hand_made(kind, ids, experts, alignment):
+    place, source, m_indices = order_by_loops(ids, experts, alignment)
+    h = len(ids) // 2
+    if kind == "first half":
+        place = place[:h]
+    elif kind == "second half":
+        place = place[h:]
+    elif kind == "dropped late":
+        place = place.masked_fill(torch.rand(place.shape, generator=gen(8)) < 0.4, -1)
+    elif kind == "dropped all":
+        place = torch.full_like(place, -1)
+    elif kind == "one row for many":                                     # every third pair names one of three rows, some names are no rows
+        place.view(-1)[::3] = torch.tensor([2, 5, len(source) - 1]).repeat(place.numel())[:place.view(-1)[::3].numel()]
+        place.view(-1)[1::7] = len(source) + 3
+    elif kind == "twice in a token":
+        place[:, 1] = place[:, 0]
+    elif kind == "shuffled":
+        place = place[torch.randperm(len(place), generator=gen(9))]
+    return TokenOrder(place, source, m_indices)
+
+
+HAND_MADE = ["first half", "second half", "dropped late", "dropped all", "one row for many", "twice in a token", "shuffled"]
+
+
+@gpu
+@pytest.mark.parametrize("binding", [True, False])
+@pytest.mark.parametrize("kind", HAND_MADE)
+@pytest.mark.parametrize("tokens, k, experts, hidden", [(5, 2, 3, 8), (40, 4, 8, 70), (301, 6, 64, 520), (3000, 3, 16, 33)])
+def test_gradients_of_orders_made_by_hand(tokens, k, experts, hidden, kind, binding, monkeypatch):
+    _C.lib()
+    if not binding:
+        monkeypatch.setattr(_C, "_binding", None)
+    order = hand_made(kind, some_ids(tokens, k, experts, 4, "uniform"), experts, 16)
+    place, m = order.place, len(order.source)
+    on_gpu = TokenOrder(*(t.cuda() for t in order))
+    for dtype in ALL_TYPES:
+        rows, w = torch.randn(m, hidden, generator=gen(1)).to(dtype), torch.randn(place.shape, generator=gen(2))
+        dy = torch.randn(len(place), hidden, generator=gen(3)).to(dtype)
+        for weights in (w, None):
+            leaves = [rows.cuda().requires_grad_()] + ([weights.cuda().requires_grad_()] if weights is not None else [])
+            y = unsort_tokens(leaves[0], on_gpu, *leaves[1:])
+            live = (place >= 0) & (place < m)
+            named = torch.where(live, place, -1)
+            assert (y.detach().cpu().double() - sum_by_loops(rows, named, weights)).abs().le(sum_bound(rows, named, weights, dtype)).all()
+            for again in range(2):
+                stale = torch.full((m, hidden), float("nan"), dtype=dtype, device="cuda")      # what the next allocation of that size finds
+                del stale
+                grads = torch.autograd.grad(y, leaves, dy.cuda(), retain_graph=True)
+                # drows[r]: the sum over the pairs that name r, in FP32, rounded once
+                scale = (weights if weights is not None else torch.ones(place.shape)).double()
+                terms = (scale[..., None] * dy.double()[:, None, :])[live]
+                want = torch.zeros(m, hidden, dtype=torch.float64).index_add_(0, place[live], terms)
+                size = torch.zeros(m, hidden, dtype=torch.float64).index_add_(0, place[live], terms.abs())
+                count = torch.zeros(m, dtype=torch.float64).index_add_(0, place[live], torch.ones(int(live.sum()), dtype=torch.float64))
+                tolerance = size * (count[:, None] * 2.0 ** -24 + 1.01 * HALF_STEP[dtype]) + (2.0 ** -25 if dtype == torch.float16 else 1e-40)
+                assert (grads[0].cpu().double() - want).abs().le(tolerance).all()
+                first = grads[0] if again == 0 else first
+                assert torch.equal(grads[0], first)
+                if weights is not None:
+                    dots = torch.where(live[..., None], rows.double()[place.clamp(0, m - 1)], 0.0) * dy.double()[:, None, :]
+                    assert (grads[1].cpu().double() - dots.sum(dim=2)).abs().le(dots.abs().sum(dim=2) * (hidden + 16) * 2.0 ** -24 + 1e-40).all()
