@@ -142,6 +142,8 @@ int dtype_code(at::ScalarType type)
 {
     return type == at::kBFloat16 ? NVFP4_DTYPE_BF16 : type == at::kHalf ? NVFP4_DTYPE_F16 : type == at::kFloat ? NVFP4_DTYPE_F32 : -1;
 }
+// A tangent of forward mode: the general way refuses it.
+bool has_tangent(const at::Tensor& t) { return t._fw_grad(0).defined(); }
 // A 2-D tensor of one of the three types on the current device with contiguous rows that do not overlap, at least a row and a column.
 const at::Tensor* matrix(PyObject* o)
 {
@@ -149,7 +151,8 @@ const at::Tensor* matrix(PyObject* o)
     const at::Tensor& t = THPVariable_Unpack(o);
     return t.is_cuda() && t.layout() == at::kStrided && t.has_storage() && t.dim() == 2 && dtype_code(t.scalar_type()) >= 0 && t.size(0) >= 1 &&
                    t.size(1) >= 1 && t.size(0) <= INT32_MAX && t.size(1) <= INT32_MAX && (t.size(1) == 1 || t.stride(1) == 1) &&
-                   (t.size(0) == 1 || t.stride(0) >= t.size(1)) && t.get_device() == c10::cuda::current_device() && !t.is_conj() && !t.is_neg()
+                   (t.size(0) == 1 || t.stride(0) >= t.size(1)) && t.get_device() == c10::cuda::current_device() && !t.is_conj() && !t.is_neg() &&
+                   !has_tangent(t)
                ? &t
                : nullptr;
 }
@@ -159,7 +162,7 @@ int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t
 const at::Tensor* beside(PyObject* o, at::ScalarType type, int64_t dim, const at::Tensor& like)
 {
     const at::Tensor* t = plain(o, type, dim);
-    return t != nullptr && t->get_device() == like.get_device() && t->is_contiguous() ? t : nullptr;
+    return t != nullptr && t->get_device() == like.get_device() && t->is_contiguous() && !has_tangent(*t) ? t : nullptr;
 }
 bool wants_gradient(const at::Tensor* t) { return t != nullptr && t->requires_grad(); }
 // A small int argument; false where it is none.

@@ -2,7 +2,7 @@
 
 The router's projection (FP32 logits out of BF16 rows), shared experts and the projections of an attention block: what a model keeps in
 BF16 or FP16 beside the quantised experts.  Operands are read where they lie, whichever way a product needs them; sums are FP32.  CUDA
-kernels of the library throughout; CPU tensors are refused.  The reference project has the grouped quantised product alone.
+kernels of the library throughout; CPU tensors are refused, and tensors with tangents of forward mode.  The reference project has the grouped quantised product alone.
 """
 from __future__ import annotations
 
@@ -11,7 +11,7 @@ from typing import Optional
 import torch
 
 from . import _C
-from .tokens import _differentiable
+from .tokens import _differentiable, _refuse_tangents
 
 
 class _Linear(torch.autograd.Function):
@@ -49,6 +49,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
         result = _C._binding.linear(x, w, bias, residual, _C.ACTIVATION_CODES[activation], 1 if out_dtype is torch.float32 else 0)
         if result is not None:
             return result
+    _refuse_tangents(x, w, bias, residual)
     if not _differentiable(x, w, bias, residual):
         return _C.linear(x, w, bias, residual, activation, out_dtype, device_status=device_status)[0]
     return _Linear.apply(x, w, bias, residual, activation, out_dtype, device_status)

@@ -8,13 +8,14 @@ gradients.
 
 Nothing comes back to the host: the sorted buffer has as many rows as any routing of so many pairs can need, so the calls can be
 captured in a CUDA graph whose replays see other routings.  All of it is CUDA kernels of the library; CPU tensors are refused.  Gradients are
-computed once (no second derivatives).  The reference project begins at rows that are grouped already.
+computed once (no second derivatives) and backwards: tensors with tangents of forward mode are refused.  The reference project begins at rows that are grouped already.
 """
 from __future__ import annotations
 
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _C
 
@@ -22,6 +23,12 @@ from . import _C
 def _differentiable(*tensors) -> bool:
     """Whether a call has to be recorded: outside of training the autograd layer costs a launch-bound call as much as its kernel."""
     return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+
+
+def _refuse_tangents(*tensors) -> None:
+    """The operators have no forward-mode derivatives: an output without a tangent would pass for a constant."""
+    if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("this operator has no derivative in forward mode: its inputs must not carry tangents")
 
 
 class _Route(torch.autograd.Function):
@@ -54,6 +61,7 @@ def route_tokens(logits: torch.Tensor, k: int, *, scores: str = "softmax", renor
         result = _C._binding.route(logits, k, _C.SCORE_CODES[scores], 1 if renormalize else 0)
         if result is not None:
             return result
+    _refuse_tangents(logits)
     if not _differentiable(logits):
         return _C.route_tokens(logits, int(k), scores, bool(renormalize))
     return _Route.apply(logits, int(k), scores, bool(renormalize))
@@ -95,6 +103,7 @@ def sort_tokens(x: torch.Tensor, ids: torch.Tensor, num_experts: int, *, alignme
         result = _C._binding.sort(x, ids, num_experts, alignment)
         if result is not None:
             return result[0], TokenOrder(*result[1:])
+    _refuse_tangents(x)
     call = _Sort.apply if _differentiable(x) else _C.sort_tokens
     rows, place, source, m_indices = call(x, ids, int(num_experts), int(alignment))
     return rows, TokenOrder(place, source, m_indices)
@@ -129,6 +138,7 @@ def unsort_tokens(rows: torch.Tensor, order: TokenOrder, weights: Optional[torch
         result = _C._binding.unsort(rows, place, source, weights)
         if result is not None:
             return result
+    _refuse_tangents(rows, weights)
     _C._require(isinstance(rows, torch.Tensor) and source.dtype == torch.int32 and source.dim() == 1 and source.is_contiguous() and
                 rows.dim() == 2 and rows.shape[0] == source.shape[0], "rows has the rows of the order")
     _C._one_device(rows, weights, place, source)

@@ -5,9 +5,10 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import nvfp4_gemm
-from nvfp4_gemm import _C, TokenOrder, route_tokens, sort_tokens, unsort_tokens
+from nvfp4_gemm import _C, TokenOrder, linear, route_tokens, sort_tokens, unsort_tokens
 
 gpu = pytest.mark.gpu
 HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
@@ -704,3 +705,70 @@ def test_gradients_of_orders_made_by_hand(tokens, k, experts, hidden, kind, bind
                 if weights is not None:
                     dots = torch.where(live[..., None], rows.double()[place.clamp(0, m - 1)], 0.0) * dy.double()[:, None, :]
                     assert (grads[1].cpu().double() - dots.sum(dim=2)).abs().le(dots.abs().sum(dim=2) * (hidden + 16) * 2.0 ** -24 + 1e-40).all()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("binding", [True, False])
+def test_tangents_of_forward_mode_are_refused_not_lost(device, binding, monkeypatch):
+    _C.lib()
+    if not binding:
+        monkeypatch.setattr(_C, "_binding", None)
+    m = 16
+    x, w = torch.randn(m, 8, device=device).to(torch.bfloat16), torch.rand(m, 2, device=device)
+    order = TokenOrder(torch.zeros(m, 2, dtype=torch.int64, device=device), torch.zeros(m, dtype=torch.int32, device=device),
+                       torch.zeros(m, dtype=torch.int32, device=device))
+    bias, residual = torch.zeros(m, device=device, dtype=torch.bfloat16), torch.zeros(m, m, device=device, dtype=torch.bfloat16)
+    calls = [(lambda t: route_tokens(t, 2), x), (lambda t: sort_tokens(t, order.place, 4, alignment=8), x), (lambda t: unsort_tokens(t, order), x),
+             (lambda t: unsort_tokens(x, order, t), w), (lambda t: linear(t, x), x), (lambda t: linear(x, t), x), (lambda t: linear(x, x, t), bias),
+             (lambda t: linear(x, x, None, t), residual)]
+    for call, primal in calls:
+        for recorded in (False, True):
+            with forward_ad.dual_level():
+                dual = forward_ad.make_dual(primal.clone().requires_grad_(recorded), torch.ones_like(primal))
+                with pytest.raises(RuntimeError, match="forward mode"):
+                    call(dual)
+            if device == "cuda":
+                with forward_ad.dual_level():                             # a tensor without a tangent is an ordinary one
+                    call(primal)
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (primal,), (torch.ones_like(primal),))
+
+
+@gpu
+@pytest.mark.parametrize("binding", [True, False])
+def test_saved_tensors_may_be_kept_on_the_host(binding, monkeypatch):
+    """What the nodes keep goes through the hooks on saved tensors, and comes back with strides of its own."""
+    _C.lib()
+    if not binding:
+        monkeypatch.setattr(_C, "_binding", None)
+    wide = torch.randn(40, 88, generator=gen(1)).to(torch.bfloat16).cuda().requires_grad_()
+    logits, w = torch.randn(40, 9, generator=gen(2)).cuda().requires_grad_(), torch.randn(24, 72, generator=gen(3)).to(torch.bfloat16).cuda().requires_grad_()
+
+    def step():
+        x = wide[:, 8:80]
+        ids, weights = route_tokens(logits[:, 1:], 3)
+        rows, order = sort_tokens(x, ids, 8, alignment=16)
+        y = linear(unsort_tokens(rows, order, weights), w, activation="gelu") + linear(x, w, activation="none")
+        return torch.autograd.grad(y.float().square().sum(), [wide, logits, w])
+
+    want = step()
+    with torch.autograd.graph.save_on_cpu():
+        got = step()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@gpu
+@pytest.mark.parametrize("binding", [True, False])
+def test_function_transforms_are_refused(binding, monkeypatch):
+    _C.lib()
+    if not binding:
+        monkeypatch.setattr(_C, "_binding", None)
+    x = torch.randn(3, 16, 8, generator=gen(1)).to(torch.bfloat16).cuda()
+    ids = torch.zeros(16, 2, dtype=torch.int64, device="cuda")
+    rows, order = sort_tokens(x[0], ids, 4, alignment=8)
+    for call in (lambda t: route_tokens(t, 2)[1], lambda t: sort_tokens(t, ids, 4, alignment=8)[0], lambda t: linear(t, x[0]),
+                 lambda t: unsort_tokens(t[:1].expand(len(rows), -1).contiguous(), order)):
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(x)
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: call(t).float().sum())(x[0])
