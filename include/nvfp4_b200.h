@@ -374,7 +374,8 @@ NVFP4_API int nvfp4_unsort_tokens_backward(const void* dy, int64_t ldy_elems, co
  * and residual have any alignment and stride.
  * nvfp4_linear: d[M,N] = activation(x[M,K] w[N,K]^T + bias[N]) + residual[M,N].  d and residual have out_dtype, `dtype` or
  *   NVFP4_DTYPE_F32; bias (of type `dtype`) and residual may be NULL.  slopes (may be NULL; not written for NVFP4_ACTIVATION_NONE) receives
- *   s = activation'(x w^T + bias) for the backward pass, as 8192 + s * 2^14 rounded; -1 stands for NaN.
+ *   s = activation'(x w^T + bias) for the backward pass: s in (-0.0622, 0) as the bits of FP16(s * 2^20), other s as 8192 + s * 2^14
+ *   rounded, NaN as -1.  Off by 2^-15 at most, and in the negative tails by 2^-11 of s (down to 2^-34).
  *   The FP32 activations are off by a few units in the last place, those of 16-bit outputs by some 2^-20 of their value.
  * nvfp4_linear_dz: dz[M,N] = dd * s (from its slopes), rounded to `dtype` for the products below, and db[N], the sums of its columns taken before
  *   that rounding.  dd has out_dtype, any alignment and stride; slopes NULL: 1.  slopes and dz start on 16 bytes and have row strides

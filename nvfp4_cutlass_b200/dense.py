@@ -43,8 +43,9 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     ``out_dtype``: the operands' type, or float32.  ``activation``: none, relu, gelu, gelu_tanh or silu.  Sums, bias, activation and residual
     are FP32, rounded once.  ``device_status``: int32 on the device that receives bit 0 should a bounded wait in the kernels expire.
 
-    Differentiable in x, w, bias and residual.  The backward pass keeps the activation's slope, off by 2^-15 at most, and rounds the
-    gradient in front of the activation to the operands' type: the tensor cores take no wider operands."""
+    Differentiable in x, w, bias and residual.  The backward pass keeps the activation's slope in 16 bits, off by 2^-15 at most and in the
+    negative tails of gelu and silu by 2^-11 of itself, and rounds the gradient in front of the activation to the operands' type: the
+    tensor cores take no wider operands."""
     if _C._binding is not None and device_status is None and activation in _C.ACTIVATION_CODES and (out_dtype is None or out_dtype is torch.float32 or out_dtype is x.dtype):
         result = _C._binding.linear(x, w, bias, residual, _C.ACTIVATION_CODES[activation], 1 if out_dtype is torch.float32 else 0)
         if result is not None:

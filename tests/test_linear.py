@@ -436,3 +436,34 @@ def test_router_sorted_experts_and_shared_expert_train_together():
     # every value passes at most six roundings to FP16 on its way (rows, hidden products, dz, sums): relative to the largest of its kind
     for a, b in zip([y.detach(), *got], [want_y.detach(), *want]):
         assert (a.cpu().double() - b).abs().max() <= 6 * 2.0 ** -11 * 4 * b.abs().max()
+
+
+@gpu
+@pytest.mark.parametrize("activation, lo, hi", [("silu", -20.0, -5.0), ("gelu", -7.0, -3.5), ("gelu_tanh", -6.0, -3.5)])
+def test_gradients_keep_their_digits_where_slopes_are_small(activation, lo, hi):
+    """Units deep in the negative tail: z is the bias, exact in its type, and one row's bias gradient is dz."""
+    for dtype in (torch.bfloat16, torch.float16):
+        for m, n in ((1, 513), (1, 512), (70, 512), (300, 2048), (2600, 4096), (2600, 4097)):      # token kernel, few rows, tiles, pairs, odd widths
+            for out in (dtype, torch.float32):
+                x, w = torch.zeros(m, 8, dtype=dtype), torch.zeros(n, 8, dtype=dtype)
+                x[:, 0], w[:, 0] = 1, 1
+                bias = torch.linspace(lo, hi, n).to(dtype)
+                z = bias.double() + 1
+                at = (torch.arange(n) * 7) % m                            # a row of its own to every column, or few: the others are zero
+                scale = 2.0 ** (torch.floor(-torch.log2(z.abs() * torch.exp(-0.5 * z * z if activation != "silu" else z))).clamp(max=14))
+                dd = torch.zeros(m, n, dtype=out)
+                dd[at, torch.arange(n)] = scale.to(out)                   # brings what FP16 could not hold into its range
+                leaves = [t.cuda().requires_grad_() for t in (x, w, bias)]
+                y = linear(*leaves, activation=activation, out_dtype=out)
+                dw, db = torch.autograd.grad(y, leaves[1:], dd.cuda())
+                leaf = z.clone().requires_grad_()
+                (slope,) = torch.autograd.grad(act64(leaf, activation).sum(), leaf)
+                want = slope * scale
+                # the slope's code is off by 2^-11 of it; exp of an argument of up to 30 with three roundings, twice over where slope and
+                # value nearly cancel; then the rounding of db, or of dz and dw
+                argument = {"gelu": z * z / 2 + 2, "gelu_tanh": 1.6 * (z.abs() + 0.044715 * z.abs() ** 3)}.get(activation, z.abs())
+                error = want.abs() * (2.0 ** -11 + 2 * (16 + 4 * argument) * 2.0 ** -23)
+                tiny = 2.0 ** -25 if dtype == torch.float16 else 1e-40
+                for got, roundings in ((db, 1), (dw[:, 0], 2)):
+                    off = (got.cpu().double() - want).abs()
+                    assert off.le(error * 1.01 + roundings * (want.abs() * 1.02 * HALF_STEP[dtype] + tiny)).all(), float((off / want.abs()).max())
