@@ -156,16 +156,17 @@ route_kernel(const T* __restrict__ logits, int64_t ld, int64_t tokens, int exper
 }
 
 // dlogits from the gradient g of the weights.  p are the softmax's scores, s the sigmoid's, w the weights, sums over a token's choices:
-//   softmax                 p_i (g_i - sum g p)           every expert of the row; g_i = 0 for one that was not chosen
+//   softmax                 p_j (sum_i p_i (g_j - g_i) + g_j (1 - sum_i p_i)) of a chosen one, -p_i sum g p of the others
 //   softmax, renormalised   w_j sum_i w_i (g_j - g_i)     the chosen alone: the others' share falls out of the ratio
 //   sigmoid                 g_j s_j (1 - s_j)
 //   sigmoid, renormalised   (1 - s_j) w_j sum_i w_i (g_j - g_i)
-// The sums of differences keep their digits where one weight is near 1 and g - sum(g w) would cancel.
+// The sums of differences keep their digits where one weight is near 1 and g - sum(g w) would cancel; 1 - sum p is the sum of the others' scores.
 template <typename T, bool kSigmoid>
 __global__ void __launch_bounds__(kRouteWarps * 32)
 route_backward_kernel(const T* __restrict__ logits, int64_t ld, int64_t tokens, int experts, int k, bool renormalize,
                       const int64_t* __restrict__ ids, const float* __restrict__ grad, T* __restrict__ dlogits)
 {
+    __shared__ uint32_t chosen[kRouteWarps][32];
     const int lane = threadIdx.x & 31;
     const int64_t t = static_cast<int64_t>(blockIdx.x) * kRouteWarps + (threadIdx.x >> 5);
     ptx::grid_dependency_wait();
@@ -178,21 +179,36 @@ route_backward_kernel(const T* __restrict__ logits, int64_t ld, int64_t tokens, 
     const bool live = id >= 0 && id < experts;
     const float l = live ? to_float(row[id]) : __uint_as_float(0xff800000u);
     if (!live) g = 0.0f;
+    // sum over the choices of a_i (g - g_i), by every lane for its own g
+    auto weighted_differences = [&](float a) {
+        float sum = 0.0f;
+        for (int j = 0; j < k; ++j) sum += __shfl_sync(kAll, a, j) * (g - __shfl_sync(kAll, g, j));
+        return sum;
+    };
     float d, share = 0.0f, biggest = 0.0f;
     const bool dense = !kSigmoid && !renormalize;
     if (dense) {
+        uint32_t* mine = chosen[threadIdx.x >> 5];                            // bit i % 32 of word i / 32: expert i was chosen
+        mine[lane] = 0;
+        __syncwarp();
+        if (live) atomicOr(mine + (id >> 5), 1u << (id & 31));
         uint32_t best = 0;
         for (int i = lane; i < experts; i += 32) best = max(best, key_of(to_float(row[i])));
         biggest = value_of(__reduce_max_sync(kAll, best));
-        float total = 0.0f;
+        __syncwarp();
+        float picked = 0.0f, rest = 0.0f;                                     // scores times their total: of the chosen, of the others
         if (biggest != __uint_as_float(0xff800000u)) {
-            for (int i = lane; i < experts; i += 32) total += expf(to_float(row[i]) - biggest);
-            total = warp_sum(total);
-            share = 1.0f / total;
+            for (int i = lane; i < experts; i += 32) {
+                const float e = expf(to_float(row[i]) - biggest);
+                if (mine[i >> 5] >> lane & 1u) picked += e;
+                else rest += e;
+            }
+            rest = warp_sum(rest);
+            share = 1.0f / (warp_sum(picked) + rest);
         }
         const float p = live ? expf(l - biggest) * share : 0.0f;
         const float sum = warp_sum(g * p);
-        d = p * (g - sum);
+        d = p * (weighted_differences(p) + g * (rest * share));
         for (int i = lane; i < experts; i += 32) {
             // a masked expert's score is 0, also in a row that has no other
             const float v = to_float(row[i]);
@@ -203,9 +219,7 @@ route_backward_kernel(const T* __restrict__ logits, int64_t ld, int64_t tokens, 
         const float rest = 1.0f / (1.0f + expf(l));                           // 1 - sigmoid(l)
         if (renormalize) {
             const float w = choice_weight<kSigmoid>(l, live, top, 0.0f, true);
-            float spread = 0.0f;
-            for (int j = 0; j < k; ++j) spread += __shfl_sync(kAll, w, j) * (g - __shfl_sync(kAll, g, j));
-            d = w * spread;
+            d = w * weighted_differences(w);
             if (kSigmoid) d *= rest;
         } else {
             d = g * choice_weight<kSigmoid>(l, live, top, 0.0f, false) * rest;

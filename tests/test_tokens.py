@@ -772,3 +772,34 @@ def test_function_transforms_are_refused(binding, monkeypatch):
             torch.func.vmap(call)(x)
         with pytest.raises(RuntimeError):
             torch.func.grad(lambda t: call(t).float().sum())(x[0])
+
+
+@gpu
+@pytest.mark.parametrize("k", [1, 2, 6])
+@pytest.mark.parametrize("ahead", [0.0, 6.0, 12.0, 16.0, 18.0, 24.0, 30.0])
+def test_routing_gradient_of_a_confident_token(ahead, k):
+    """One logit far above the rest: the chosen expert's gradient is what the others leave of its score, and keeps its digits."""
+    for experts in (8, 33, 128, 1000):
+        for dtype in ALL_TYPES:
+            logits = (torch.randn(6, experts, generator=gen(experts)) * 0.5).to(dtype).float()
+            logits[torch.arange(6), torch.arange(6) % experts] = 3.0 + ahead
+            logits[5, 7] = -math.inf
+            logits = logits.to(dtype)
+            for grad in (torch.ones(6, k), torch.rand(6, k, generator=gen(k)) + 0.5, torch.randn(6, k, generator=gen(k + 1))):
+                leaf = logits.cuda().requires_grad_()
+                ids, weights = route_tokens(leaf, k, renormalize=False)
+                (got,) = torch.autograd.grad(weights, leaf, grad.cuda())
+                p = torch.softmax(logits.double(), dim=1)
+                chosen = torch.zeros(6, experts, dtype=torch.float64).scatter_(1, ids.cpu(), 1.0)
+                g = torch.zeros(6, experts, dtype=torch.float64).scatter_(1, ids.cpu(), grad.double())
+                left = (p * (1 - chosen)).sum(dim=1, keepdim=True)
+                # g_j - sum g p over the chosen i = sum p_i (g_j - g_i) + g_j * (what the others have of p); its terms may cancel, each is
+                # off by its scores' bound
+                differences = (p * chosen)[:, None, :] * (g[:, :, None] - g[:, None, :])
+                want = p * torch.where(chosen > 0, differences.sum(dim=2) + g * left, -(g * p).sum(dim=1, keepdim=True))
+                size = p * torch.where(chosen > 0, differences.abs().sum(dim=2) + (g * left).abs(), (g * p).abs().sum(dim=1, keepdim=True))
+                # three scores to a product, FP32 differences of g, sums of up to k + 1 terms, one rounding
+                bound = 3 * weight_bound(logits.double(), k) + (k + 8) * 2.0 ** -24
+                tolerance = size * bound + want.abs() * 1.01 * HALF_STEP[dtype] + (2.0 ** -25 if dtype == torch.float16 else 1e-38)
+                off = (got.cpu().double() - want).abs()
+                assert off.le(tolerance).all(), float((off / tolerance).max())
