@@ -383,7 +383,8 @@ NVFP4_API int nvfp4_unsort_tokens_backward(const void* dy, int64_t ldy_elems, co
  *   may be NULL.
  * nvfp4_linear_dx: dx[M,K] = dz w.      nvfp4_linear_dw: dw[N,K] = dz^T x.      Rounded to `dtype`.
  * An FP32 output takes partial sums of 256 products out of the tensor cores and adds them as FP32; others stay in their accumulator.
- * device_status (may be NULL) receives bit 0 if a bounded wait expired.  No counterparts in the reference project. */
+ * device_status (may be NULL) receives bit 0 if a bounded wait expired; what was not finished then is NaN.  No counterparts in the
+ * reference project. */
 NVFP4_API int nvfp4_linear(const void* x, int64_t ldx_elems, const void* w, int64_t ldw_elems, const void* bias, const void* residual,
                            int64_t ldr_elems, void* d, int64_t ldd_elems, int16_t* slopes, int64_t lds_elems, int M, int N, int K, int dtype,
                            int out_dtype, int activation, int32_t* device_status, void* stream);
@@ -421,6 +422,14 @@ NVFP4_API int nvfp4_debug_wait_timeout(int64_t budget_cycles, int32_t* device_st
  * cycles (at most 2e9).  The kernel ends by itself; every gw is NaN. */
 NVFP4_API int nvfp4_debug_quantize_weight_expired(const void* w, int w_dtype, int E, int N, int K, void* b, void* sfb, float* gw,
                                                   int64_t budget_cycles, void* stream);
+
+/* Test hook: nvfp4_linear whose waits can only run out, after budget_cycles clock cycles (at most 2e9): no product is issued, or, with
+ * withhold_residuals, no residual is fetched (by the kernels that fetch it by TMA; others finish).  The kernel ends by itself, with NaN in
+ * d and in the slopes and bit 0 in *device_status.  One or two rows with a small weight take no such wait and finish. */
+NVFP4_API int nvfp4_debug_linear_expired(const void* x, int64_t ldx_elems, const void* w, int64_t ldw_elems, const void* bias, const void* residual,
+                                         int64_t ldr_elems, void* d, int64_t ldd_elems, int16_t* slopes, int64_t lds_elems, int M, int N, int K,
+                                         int dtype, int out_dtype, int activation, int withhold_residuals, int64_t budget_cycles,
+                                         int32_t* device_status, void* stream);
 
 /* Measurement hook: issues `iters` rounds of resident-operand block-scaled FP4 MMAs
  * (128 x 256 x 64 each) per SM with no memory traffic and returns through

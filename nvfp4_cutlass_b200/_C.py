@@ -48,7 +48,7 @@ EXPORTS = ("nvfp4_last_error", "nvfp4_version", "nvfp4_get_num_sms", "nvfp4_set_
            "nvfp4_grouped_gemm_swiglu_contiguous", "nvfp4_grouped_gemm_masked", "nvfp4_load_checkpoint_weights",
            "nvfp4_read_status", "nvfp4_debug_split_workspace", "nvfp4_debug_wait_timeout", "nvfp4_debug_quantize_weight_expired", "nvfp4_plan_peer_masked", "nvfp4_plan_one_rank",
            "nvfp4_peer_barrier", "nvfp4_route_tokens", "nvfp4_route_tokens_backward", "nvfp4_sort_tokens", "nvfp4_unsort_tokens",
-           "nvfp4_unsort_tokens_backward", "nvfp4_linear", "nvfp4_linear_dz", "nvfp4_linear_dx", "nvfp4_linear_dw")
+           "nvfp4_unsort_tokens_backward", "nvfp4_linear", "nvfp4_linear_dz", "nvfp4_linear_dx", "nvfp4_linear_dw", "nvfp4_debug_linear_expired")
 
 
 def library_path() -> str:
@@ -105,6 +105,7 @@ def lib() -> ctypes.CDLL:
         L.nvfp4_unsort_tokens.argtypes = [vp, i64, i32, i64, vp, vp, i64, i32, i32, vp, vp]
         L.nvfp4_unsort_tokens_backward.argtypes = [vp, i64, vp, i64, i32, i64, vp, vp, vp, i64, i32, i32, vp, vp, vp]
         L.nvfp4_linear.argtypes = [vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, i32, i32, vp, vp]
+        L.nvfp4_debug_linear_expired.argtypes = [vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, i32, i32, i32, i64, vp, vp]
         L.nvfp4_linear_dz.argtypes = [vp, i64, vp, i64, vp, i64, vp, i32, i32, i32, i32, vp]
         L.nvfp4_linear_dx.argtypes = [vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp]
         L.nvfp4_linear_dw.argtypes = [vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp]
@@ -846,6 +847,20 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias, residual, activation: str, ou
                                   slopes.data_ptr() if keep else None, slopes.shape[1] if keep else 0, m, n, k, DTYPE_CODES[x.dtype],
                                   DTYPE_CODES[out_dtype], ACTIVATION_CODES[activation],
                                   device_status.data_ptr() if device_status is not None else None, _stream()))
+    return d, slopes
+
+
+def debug_linear_expired(x: torch.Tensor, w: torch.Tensor, bias, residual, activation: str, out_dtype, budget_cycles: int, device_status,
+                         withhold_residuals: bool = False):
+    """linear(..., keep=True) whose waits run out after `budget_cycles` (test hook): (d, slopes), NaN (-1) throughout."""
+    (m, k), n, dev = x.shape, w.shape[0], _one_device(x, w, bias, residual, device_status)
+    _require(all(t is None or t.is_contiguous() for t in (x, w, bias, residual)), "contiguous tensors")
+    d, slopes = torch.zeros(m, n, dtype=out_dtype, device=dev), torch.zeros(m, (n + 7) // 8 * 8, dtype=torch.int16, device=dev)
+    pointer = lambda t: t.data_ptr() if t is not None else None
+    with _on(dev):
+        _check(lib().nvfp4_debug_linear_expired(x.data_ptr(), k, w.data_ptr(), k, pointer(bias), pointer(residual), n, d.data_ptr(), n, slopes.data_ptr(),
+                                                slopes.shape[1], m, n, k, DTYPE_CODES[x.dtype], DTYPE_CODES[out_dtype], ACTIVATION_CODES[activation],
+                                                1 if withhold_residuals else 0, int(budget_cycles), pointer(device_status), _stream()))
     return d, slopes
 
 

@@ -882,11 +882,10 @@ static int tensor_core_device(host::DeviceInfo** dev)
     return NVFP4_OK;
 }
 
-int nvfp4_linear(const void* x, int64_t ldx_elems, const void* w, int64_t ldw_elems, const void* bias, const void* residual, int64_t ldr_elems, void* d,
-                 int64_t ldd_elems, int16_t* slopes, int64_t lds_elems, int M, int N, int K, int dtype, int out_dtype, int activation,
-                 int32_t* device_status, void* stream)
+static int linear(const void* x, int64_t ldx_elems, const void* w, int64_t ldw_elems, const void* bias, const void* residual, int64_t ldr_elems, void* d,
+                  int64_t ldd_elems, int16_t* slopes, int64_t lds_elems, int M, int N, int K, int dtype, int out_dtype, int activation,
+                  int32_t* device_status, void* stream, int64_t budget, bool withhold_residuals)
 {
-    host::clear_error();
     if (int rc = check_linear(M, N, K, dtype)) return rc;
     NVFP4_REQUIRE(out_dtype == dtype || out_dtype == NVFP4_DTYPE_F32, "the output has the operands' type or FP32 (type codes %d, %d)", out_dtype, dtype);
     NVFP4_REQUIRE(activation >= NVFP4_ACTIVATION_NONE && activation <= NVFP4_ACTIVATION_SILU, "unknown activation %d", activation);
@@ -900,7 +899,27 @@ int nvfp4_linear(const void* x, int64_t ldx_elems, const void* w, int64_t ldw_el
     host::DeviceInfo* dev;
     if (int rc = tensor_core_device(&dev)) return rc;
     return launch_linear(x, ldx_elems, w, ldw_elems, bias, residual, ldr_elems, d, ldd_elems, slopes, lds_elems, M, N, K, dtype == NVFP4_DTYPE_BF16,
-                         out_dtype == NVFP4_DTYPE_F32, activation, device_status, dev->num_sms, static_cast<cudaStream_t>(stream));
+                         out_dtype == NVFP4_DTYPE_F32, activation, device_status, dev->num_sms, static_cast<cudaStream_t>(stream), budget,
+                         withhold_residuals);
+}
+
+int nvfp4_linear(const void* x, int64_t ldx_elems, const void* w, int64_t ldw_elems, const void* bias, const void* residual, int64_t ldr_elems, void* d,
+                 int64_t ldd_elems, int16_t* slopes, int64_t lds_elems, int M, int N, int K, int dtype, int out_dtype, int activation,
+                 int32_t* device_status, void* stream)
+{
+    host::clear_error();
+    return linear(x, ldx_elems, w, ldw_elems, bias, residual, ldr_elems, d, ldd_elems, slopes, lds_elems, M, N, K, dtype, out_dtype, activation,
+                  device_status, stream, 0, false);
+}
+
+int nvfp4_debug_linear_expired(const void* x, int64_t ldx_elems, const void* w, int64_t ldw_elems, const void* bias, const void* residual,
+                               int64_t ldr_elems, void* d, int64_t ldd_elems, int16_t* slopes, int64_t lds_elems, int M, int N, int K, int dtype,
+                               int out_dtype, int activation, int withhold_residuals, int64_t budget_cycles, int32_t* device_status, void* stream)
+{
+    host::clear_error();
+    NVFP4_REQUIRE(budget_cycles > 0 && budget_cycles <= 2000000000ll, "budget_cycles outside (0, 2e9]");
+    return linear(x, ldx_elems, w, ldw_elems, bias, residual, ldr_elems, d, ldd_elems, slopes, lds_elems, M, N, K, dtype, out_dtype, activation,
+                  device_status, stream, budget_cycles, withhold_residuals != 0);
 }
 
 int nvfp4_linear_dz(const void* dd, int64_t ldd_elems, const int16_t* slopes, int64_t lds_elems, void* dz, int64_t lddz_elems, void* db, int M, int N,

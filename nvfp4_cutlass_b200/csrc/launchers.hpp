@@ -69,7 +69,7 @@ int launch_unsort_tokens_backward(const void* dy, int64_t ldy, const void* rows,
 
 int launch_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual, int64_t ldr, void* d, int64_t ldd,
                   int16_t* slopes, int64_t lds, int M, int N, int K, bool bf16, bool out32, int activation, int32_t* status, int num_sms,
-                  cudaStream_t stream);
+                  cudaStream_t stream, int64_t budget = 0, bool withhold_residuals = false);
 int launch_linear_dz(const void* dd, int64_t ldd, bool dd32, const int16_t* slopes, int64_t lds, void* dz, int64_t lddz, void* db, int M, int N,
                      bool bf16, int num_sms, cudaStream_t stream);
 int launch_linear_dx(const void* dz, int64_t lddz, const void* w, int64_t ldw, void* dx, int64_t lddx, int M, int N, int K, bool bf16, int32_t* status,

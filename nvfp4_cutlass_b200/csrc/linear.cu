@@ -12,6 +12,9 @@
 //                        products of the next
 //   token_kernel         one or two rows of x and a small weight: no tensor cores
 // Sums are FP32 from the first product to the epilogue, which rounds once.
+// Every wait is bounded.  One that runs out sets the status bit, where there is a status word, and leaves NaN in what its block did not
+// finish (in split form in what the cluster did not), so that nothing that was never computed passes for a result; the block leaves when its
+// copies and products in flight have ended, within the same bound.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -320,6 +323,9 @@ struct Stage {
     uint64_t* landed;                                // per box: its residual is there
     uint32_t phase = 0;
     const Maps* maps;
+    long long budget;                                // of a wait, in cycles
+    uint32_t requested = 0;                          // boxes whose residual is under way
+    bool withhold = false;                           // test of the expired wait: residuals are not asked for
 
     // Everything that the warp has given to TMA has been read: the buffers may be written.
     __device__ __forceinline__ void reclaim(uint32_t lane) const
@@ -327,12 +333,24 @@ struct Stage {
         if (lane == 0) ptx::bulk_wait_read();
         __syncwarp();
     }
-    __device__ __forceinline__ void request(uint32_t box, uint32_t col, uint32_t row0, uint32_t lane) const
+    __device__ __forceinline__ void request(uint32_t box, uint32_t col, uint32_t row0, uint32_t lane)
     {
+        if (withhold) return;
+        requested |= 1u << box;
         if (lane == 0) {
             ptx::mbar_arrive_expect_tx(landed + box, kBoxBytes);
             tma_load(out + box * out_step, &maps->residual, landed + box, col, row0);
         }
+    }
+    // After a wait that expired
+    __device__ __forceinline__ void settle()
+    {
+        const long long until = clock64() + budget;
+#pragma unroll
+        for (uint32_t box = 0; box < 4; ++box)
+            if (requested >> box & 1u) ptx::mbar_settle(landed + box, phase >> box & 1u, until);
+        requested = 0;
+        __syncwarp();
     }
     static __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int32_t c0, int32_t c1)
     {
@@ -362,8 +380,9 @@ struct Stage {
                                            volatile uint32_t* abort_flag)
     {
         if (e.residual != nullptr) {
-            if (!ptx::all_lanes(ptx::mbar_wait_impl(landed + box, phase >> box & 1u, abort_flag))) return false;
+            if (!ptx::all_lanes(ptx::mbar_wait_budget(landed + box, phase >> box & 1u, abort_flag, budget))) return false;
             phase ^= 1u << box;
+            requested &= ~(1u << box);
         }
 #pragma unroll
         for (uint32_t half = 0; half < kBox<D> / 32; ++half) {
@@ -483,7 +502,11 @@ struct Product {
     uint32_t splits_log2, depth;                     // product_kernel: CTAs to a tile, ring positions
     bool a_mn, b_mn;
     int32_t* status;
+    long long budget;                                // of every wait, in cycles
+    uint32_t withhold;                               // what a test of the expired waits keeps back: kProducts, kResiduals
 };
+enum Withhold : uint32_t { kNothing = 0, kProducts = 1, kResiduals = 2 };
+constexpr float kNan = NAN;
 
 // ---- one tile to a CTA or cluster --------------------------------------------------------------------------------------
 
@@ -497,7 +520,7 @@ __host__ __device__ constexpr uint32_t partial_pad(uint32_t bn, uint32_t splits)
 __host__ __device__ constexpr uint32_t partial_bytes(uint32_t bn, uint32_t splits) { return splits > 1 ? (bn + splits * partial_pad(bn, splits)) * BM * 4 : 0; }
 constexpr uint32_t tile_smem(uint32_t bn, uint32_t depth, uint32_t splits)
 {
-    return 1024 + depth * tile_stage(bn) + partial_bytes(bn, splits) + (2 * kMaxDepth + 4) * 8 + 16 + kTileEpiWarps * 32;
+    return 1024 + depth * tile_stage(bn) + partial_bytes(bn, splits) + (2 * kMaxDepth + 5) * 8 + 16 + kTileEpiWarps * 32;
 }
 // For an FP32 output the epilogue warps take the accumulators over every four K blocks and add them up in registers, two accumulators in
 // turn: the tensor core cuts what it adds to a long sum (K = 4096 in one accumulator: off by 4.3e-6 of the result, FP32 sums by 6e-7).
@@ -522,7 +545,8 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     uint64_t* tmem_full = drained + kMaxDepth;       // per accumulator
     uint64_t* tmem_empty = tmem_full + 2;
     uint64_t* landed = tmem_empty + 2;               // [epilogue warp][4] residual of a box
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(landed + 4 * kTileEpiWarps);
+    uint64_t* settled = landed + 4 * kTileEpiWarps;  // the products have ended, after a wait that expired
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(settled + 1);
     volatile uint32_t* abort_flag = tmem_slot + 1;
 
     const uint32_t warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -530,7 +554,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < depth; ++i) { ptx::mbar_init(full + i, 1); ptx::mbar_init(drained + i, 1); }
         for (uint32_t i = 0; i < 2; ++i) { ptx::mbar_init(tmem_full + i, 1); ptx::mbar_init(tmem_empty + i, kTileEpiWarps); }
-        for (uint32_t i = 0; i < 4 * kTileEpiWarps; ++i) ptx::mbar_init(landed + i, 1);
+        for (uint32_t i = 0; i < 4 * kTileEpiWarps + 1; ++i) ptx::mbar_init(landed + i, 1);
         *abort_flag = 0;
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&tm_a);
@@ -564,8 +588,9 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     if (warp == 0) {
         const uint32_t issue = ptx::elect_one();
         Ring r;
-        for (uint32_t kb = kb0; kb < kb1; ++kb) {
-            if (!ptx::all_lanes(ptx::mbar_wait_impl(drained + r.slot, r.phase ^ 1, abort_flag))) { give_up(); break; }
+        uint32_t loaded = 0;
+        for (uint32_t kb = kb0; kb < kb1; ++kb, ++loaded) {
+            if (!ptx::all_lanes(ptx::mbar_wait_budget(drained + r.slot, r.phase ^ 1, abort_flag, p.budget))) { give_up(); break; }
             uint8_t* to = gen + r.slot * kStage;
             uint64_t* bar = full + r.slot;
             ptx::mbar_arrive_expect_tx(bar, kStage, issue);
@@ -576,18 +601,23 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         ptx::grid_launch_dependents();
         // the last commits arrive before the block may leave
         for (uint32_t i = 0; ok && i < depth; ++i) {
-            if (!ptx::all_lanes(ptx::mbar_wait_impl(drained + r.slot, r.phase ^ 1, abort_flag))) give_up();
+            if (!ptx::all_lanes(ptx::mbar_wait_budget(drained + r.slot, r.phase ^ 1, abort_flag, p.budget))) give_up();
             next(r);
+        }
+        if (!ok) {
+            const long long until = clock64() + p.budget;
+            for (uint32_t n = loaded > depth ? loaded - depth : 0; n < loaded; ++n) ptx::mbar_settle(full + n % depth, n / depth & 1u, until);
+            __syncwarp();
         }
     } else if (warp == 1) {
         const uint32_t issue = ptx::elect_one();
         const uint32_t idesc = ptx::make_idesc_f16(BM, BN, std::is_same<T, __nv_bfloat16>::value, p.a_mn, p.b_mn);
         Ring r;
-        for (uint32_t kb = kb0; kb < kb1; ++kb) {
+        for (uint32_t kb = kb0; kb < kb1 && p.withhold != kProducts; ++kb) {
             const uint32_t n = kb - kb0, c = kWide ? n / kChunkBlocks : 0, acc = c & 1;
             const bool first = kWide ? n % kChunkBlocks == 0 : n == 0;
-            if (kWide && first && !ptx::all_lanes(ptx::mbar_wait_impl(tmem_empty + acc, ((c >> 1) & 1) ^ 1, abort_flag))) { give_up(); break; }
-            if (!ptx::all_lanes(ptx::mbar_wait_impl(full + r.slot, r.phase, abort_flag))) { give_up(); break; }
+            if (kWide && first && !ptx::all_lanes(ptx::mbar_wait_budget(tmem_empty + acc, ((c >> 1) & 1) ^ 1, abort_flag, p.budget))) { give_up(); break; }
+            if (!ptx::all_lanes(ptx::mbar_wait_budget(full + r.slot, r.phase, abort_flag, p.budget))) { give_up(); break; }
             ptx::tcgen05_fence_after_sync();
             const uint32_t at = smem + r.slot * kStage;
 #pragma unroll
@@ -597,6 +627,11 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
             if (kb + 1 == kb1 || (kWide && n % kChunkBlocks == kChunkBlocks - 1)) ptx::tcgen05_commit(tmem_full + acc, issue);
             next(r);
         }
+        if (!ok || !ptx::all_lanes(*abort_flag == 0)) {
+            ptx::tcgen05_commit(settled, issue);
+            ptx::mbar_settle(settled, 0, clock64() + p.budget);
+            __syncwarp();
+        }
     } else {
         [[maybe_unused]] float sum[kWide ? BN : 1];
         if constexpr (kWide) {
@@ -605,7 +640,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         }
         for (uint32_t c = 0; c < chunks; ++c) {
             const uint32_t acc = c & 1;
-            if (!ptx::all_lanes(ptx::mbar_wait_relaxed(tmem_full + acc, (c >> 1) & 1, abort_flag, 20))) { give_up(); break; }
+            if (!ptx::all_lanes(ptx::mbar_wait_relaxed(tmem_full + acc, (c >> 1) & 1, abort_flag, 20, p.budget))) { give_up(); break; }
             ptx::tcgen05_fence_after_sync();
             if constexpr (kWide) {
 #pragma unroll
@@ -646,12 +681,16 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         const uint32_t width_log2 = __popc(BN - 1) - p.splits_log2, width = 1u << width_log2;          // columns that a CTA finishes
         constexpr uint32_t kWords = partial_words(BN);
         const uint32_t pitch = (width + partial_pad(BN, splits)) * 4, block = BM * pitch;                       // of a row, of a source's rows
-        if (warp >= 2 && ok) {
+        if (warp >= 2) {
             const uint32_t mine = partial + rank * block + row * pitch;
 #pragma unroll 1
             for (uint32_t c0 = 0; c0 < live; c0 += kChunk) {
                 float v[kChunk];
                 load_accumulators(taddr + c0, v);
+                if (!ok) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kChunk; ++i) v[i] = kNan;
+                }
 #pragma unroll
                 for (uint32_t i = 0; i < kChunk; i += kWords) {
                     const uint32_t c = c0 + i;               // columns that nobody wants included: they have their place, too
@@ -662,7 +701,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
             }
         }
         ptx::cluster_sync();                         // partial sums have arrived; nobody touches another CTA's memory from here on
-        if (warp >= 2 && ok) {
+        if (warp >= 2) {
             const float* mine = reinterpret_cast<const float*>(gen + (partial - smem) + row * pitch);
 #pragma unroll 1
             for (uint32_t c0 = 0; c0 < width; c0 += kChunk) {
@@ -699,28 +738,38 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                 give(v, first, kSwap ? count : 32);
             }
         }
-    } else if (warp >= 2 && ok && e.staged) {
-        // the ring is at rest (the accumulators are complete): its memory takes the boxes, four for every warp: of the output, or two of the
-        // output and two of the slopes
+    } else if (warp >= 2) {
+        uint32_t done = 0;                           // columns of the tile that have left
         if constexpr (!kSwap) {
-            constexpr uint32_t kColumns = kBox<D>;
-            const uint32_t at = smem + (warp - 2) * 4 * kBoxBytes, row0 = a0 + quad * 32;
-            Stage<T, D> stage{at, kBoxBytes, at + 2 * kBoxBytes, kBoxBytes, landed + 4 * (warp - 2), 0, &maps};
-            if (row0 < e.rows) {
-                if (e.residual != nullptr)
-                    for (uint32_t c = 0; c < live; c += kColumns) stage.request(c / kColumns, b0 + c, row0, lane);
+            if (e.staged && ok) {
+                // the ring is at rest (the accumulators are complete): its memory takes the boxes, four for every warp: of the output, or
+                // two of the output and two of the slopes
+                constexpr uint32_t kColumns = kBox<D>;
+                const uint32_t at = smem + (warp - 2) * 4 * kBoxBytes, row0 = a0 + quad * 32;
+                Stage<T, D> stage{at, kBoxBytes, at + 2 * kBoxBytes, kBoxBytes, landed + 4 * (warp - 2), 0, &maps, p.budget, 0, p.withhold == kResiduals};
+                if (row0 < e.rows) {
+                    if (e.residual != nullptr)
+                        for (uint32_t c = 0; c < live; c += kColumns) stage.request(c / kColumns, b0 + c, row0, lane);
 #pragma unroll 1
-                for (uint32_t c = 0; c < live; c += kColumns)
-                    if (!stage.finish(taddr + c, c / kColumns, b0 + c, row0, lane, e, abort_flag)) { give_up(); break; }
-                if (lane == 0) ptx::bulk_wait();
+                    for (; done < live; done += kColumns)
+                        if (!stage.finish(taddr + done, done / kColumns, b0 + done, row0, lane, e, abort_flag)) { give_up(); break; }
+                    if (!ok) stage.settle();
+                    if (lane == 0) ptx::bulk_wait();
+                    __syncwarp();
+                } else {
+                    done = live;
+                }
             }
         }
-    } else if (warp >= 2 && ok) {
         // (unrolled, a cold call spent 3 us a chunk fetching instructions: 13 us of a router's 41)
 #pragma unroll 1
-        for (uint32_t c0 = 0; c0 < live; c0 += kChunk) {
+        for (uint32_t c0 = done; c0 < live; c0 += kChunk) {
             float v[kChunk];
             load_accumulators(taddr + c0, v);
+            if (!ok) {
+#pragma unroll
+                for (uint32_t i = 0; i < kChunk; ++i) v[i] = kNan;
+            }
             give(v, c0, kSwap ? min(kChunk, live - c0) : 32);
         }
     }
@@ -806,7 +855,7 @@ constexpr int kPairThreads = 320;                    // warp 0: TMA, warp 1: pro
 constexpr uint32_t kPairFirstEpi = 2;
 constexpr uint32_t kPairDepth = 5, kPairStage = 2 * kSlotA, kPairBN = 256, kPairEpiWarps = 8;
 // behind the ring: two boxes for every epilogue warp (of the output, or of the output and the slopes), barriers
-constexpr uint32_t kPairSmem = 1024 + kPairDepth * kPairStage + kPairEpiWarps * 2 * kBoxBytes + (2 * kPairDepth + 4 + 2 * kPairEpiWarps) * 8 + 16;
+constexpr uint32_t kPairSmem = 1024 + kPairDepth * kPairStage + kPairEpiWarps * 2 * kBoxBytes + (2 * kPairDepth + 5 + 2 * kPairEpiWarps) * 8 + 16;
 static_assert(kPairSmem <= 232448, "shared memory of an SM");
 
 template <typename T>
@@ -823,7 +872,8 @@ product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     uint64_t* tmem_full = drained + kPairDepth;      // each CTA, per accumulator: complete
     uint64_t* tmem_empty = tmem_full + 2;            // even CTA, per accumulator: read by the epilogue warps of both
     uint64_t* landed = tmem_empty + 2;               // [epilogue warp][2] residual of a box
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(landed + 2 * kPairEpiWarps);
+    uint64_t* settled = landed + 2 * kPairEpiWarps;  // even CTA: the products have ended, after a wait that expired
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(settled + 1);
     volatile uint32_t* abort_flag = tmem_slot + 1;
 
     const uint32_t warp = ptx::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -831,7 +881,7 @@ product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kPairDepth; ++i) { ptx::mbar_init(full + i, 1); ptx::mbar_init(drained + i, 1); }
         for (uint32_t i = 0; i < 2; ++i) { ptx::mbar_init(tmem_full + i, 1); ptx::mbar_init(tmem_empty + i, 2 * kPairEpiWarps); }
-        for (uint32_t i = 0; i < 2 * kPairEpiWarps; ++i) ptx::mbar_init(landed + i, 1);
+        for (uint32_t i = 0; i < 2 * kPairEpiWarps + 1; ++i) ptx::mbar_init(landed + i, 1);
         *abort_flag = 0;
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&tm_a);
@@ -855,12 +905,13 @@ product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         const uint32_t issue = ptx::elect_one();
         const uint32_t full_even = ptx::map_to_cta(ptx::smem_u32(full), 0);
         Ring r;
+        uint32_t loaded = 0;                         // ring positions with copies in them
         for (uint32_t tile = pair_id; ok && tile < tiles; tile += num_pairs) {
             uint32_t a_blk, b_blk;
             gemm::tile_coords(tile, p.tiles_a, p.tiles_b, 8, a_blk, b_blk);
             const uint32_t a0 = (a_blk * 2 + rank) * BM, b0 = b_blk * kPairBN + rank * (kPairBN / 2);
             for (uint32_t kb = 0; kb < p.k_blocks; ++kb) {
-                if (!ptx::all_lanes(ptx::mbar_wait_impl(drained + r.slot, r.phase ^ 1, abort_flag))) { give_up(); break; }
+                if (!ptx::all_lanes(ptx::mbar_wait_budget(drained + r.slot, r.phase ^ 1, abort_flag, p.budget))) { give_up(); break; }
                 // the even CTA announces the bytes of both; the odd CTA's complete on its barrier
                 if (rank == 0) ptx::mbar_arrive_expect_tx(full + r.slot, 2 * kPairStage, issue);
                 uint8_t* to = gen + r.slot * kPairStage;
@@ -868,11 +919,23 @@ product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                 load_tile<BM>(to, p.a_mn, a0, kb, [&](uint8_t* dst, uint32_t c0, uint32_t c1) { ptx::tma_load_2d_pair(dst, &tm_a, bar, c0, c1, issue); });
                 load_tile<BM>(to + kSlotA, p.b_mn, b0, kb, [&](uint8_t* dst, uint32_t c0, uint32_t c1) { ptx::tma_load_2d_pair(dst, &tm_b, bar, c0, c1, issue); });
                 r.advance<kPairDepth>();
+                loaded = min(loaded + 1, kPairDepth);
             }
         }
         ptx::grid_launch_dependents();
         if (ok && !gemm::drain_ring<kPairDepth>(r, [&](uint32_t i, uint32_t parity) {
-                return ptx::all_lanes(ptx::mbar_wait_impl(drained + i, parity, abort_flag)); })) give_up();
+                return ptx::all_lanes(ptx::mbar_wait_budget(drained + i, parity, abort_flag, p.budget)); })) give_up();
+        // (the odd CTA's copies complete on the even one's barriers, and it cannot leave before that one; any that the even CTA has not
+        // announced are as old as the wait that ran out in the odd one)
+        if (!ok && rank == 0) {
+            const long long until = clock64() + p.budget;
+            for (uint32_t i = 0; i < loaded; ++i) {  // backwards from the next position: the last use of each
+                if (r.slot == 0) { r.slot = kPairDepth; r.phase ^= 1; }
+                --r.slot;
+                ptx::mbar_settle(full + r.slot, r.phase, until);
+            }
+            __syncwarp();
+        }
     } else if (warp == 1) {
         if (rank == 0) {
             const uint32_t issue = ptx::elect_one();
@@ -880,12 +943,12 @@ product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
             constexpr uint16_t kBoth = 3;
             Ring r;
             uint32_t n = 0;
-            for (uint32_t tile = pair_id; ok && tile < tiles; tile += num_pairs, ++n) {
+            for (uint32_t tile = pair_id; ok && tile < tiles && p.withhold != kProducts; tile += num_pairs, ++n) {
                 const uint32_t acc = n & 1;
-                if (!ptx::all_lanes(ptx::mbar_wait_impl(tmem_empty + acc, ((n >> 1) & 1) ^ 1, abort_flag))) { give_up(); break; }
+                if (!ptx::all_lanes(ptx::mbar_wait_budget(tmem_empty + acc, ((n >> 1) & 1) ^ 1, abort_flag, p.budget))) { give_up(); break; }
                 ptx::tcgen05_fence_after_sync();
                 for (uint32_t kb = 0; kb < p.k_blocks; ++kb) {
-                    if (!ptx::all_lanes(ptx::mbar_wait_impl(full + r.slot, r.phase, abort_flag))) { give_up(); break; }
+                    if (!ptx::all_lanes(ptx::mbar_wait_budget(full + r.slot, r.phase, abort_flag, p.budget))) { give_up(); break; }
                     ptx::tcgen05_fence_after_sync();
                     const uint32_t at = smem + r.slot * kPairStage;
 #pragma unroll
@@ -896,6 +959,11 @@ product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                 }
                 if (ok) ptx::tcgen05_commit_pair(tmem_full + acc, kBoth, issue);
             }
+            if (!ok || !ptx::all_lanes(*abort_flag == 0)) {
+                ptx::tcgen05_commit_pair(settled, 1, issue);
+                ptx::mbar_settle(settled, 0, clock64() + p.budget);
+                __syncwarp();
+            }
         }
     } else {
         const uint32_t quad = warp & 3, half = (warp - kPairFirstEpi) >> 2;   // its lanes; columns [128 half, 128 half + 128) of the tile
@@ -903,24 +971,25 @@ product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         const uint32_t boxes = smem + kOffBoxes + (warp - kPairFirstEpi) * 2 * kBoxBytes;
         const bool both = e.slopes != nullptr;       // the second buffer takes the slopes
         constexpr uint32_t kBoxColumns = kBox<T>;
-        Stage<T, T> stage{boxes, both ? 0u : kBoxBytes, boxes + kBoxBytes, 0u, landed + 2 * (warp - kPairFirstEpi), 0, &maps};
+        Stage<T, T> stage{boxes, both ? 0u : kBoxBytes, boxes + kBoxBytes, 0u, landed + 2 * (warp - kPairFirstEpi), 0, &maps, p.budget, 0, p.withhold == kResiduals};
         uint32_t n = 0;
-        for (uint32_t tile = pair_id; ok && tile < tiles; tile += num_pairs, ++n) {
+        for (uint32_t tile = pair_id; tile < tiles; tile += num_pairs, ++n) {
             const uint32_t acc = n & 1;
             uint32_t a_blk, b_blk;
             gemm::tile_coords(tile, p.tiles_a, p.tiles_b, 8, a_blk, b_blk);
             const uint32_t row0 = (a_blk * 2 + rank) * BM + quad * 32, col0 = b_blk * kPairBN + half * 128;
             const bool wanted = row0 < e.rows && col0 < e.cols, second = col0 + kBoxColumns < e.cols;
-            if (e.staged && wanted) {
+            if (e.staged && wanted && ok) {
                 stage.reclaim(lane);
                 if (e.residual != nullptr) {
                     stage.request(0, col0, row0, lane);
                     if (second && !both) stage.request(1, col0 + kBoxColumns, row0, lane);
                 }
             }
-            if (!ptx::all_lanes(ptx::mbar_wait_relaxed(tmem_full + acc, (n >> 1) & 1, abort_flag, 50))) { give_up(); break; }
+            if (ok && !ptx::all_lanes(ptx::mbar_wait_relaxed(tmem_full + acc, (n >> 1) & 1, abort_flag, 50, p.budget))) give_up();
             ptx::tcgen05_fence_after_sync();
             const uint32_t taddr = tmem + ((quad * 32) << 16) + acc * kPairBN + half * 128;
+            uint32_t done = 0;                       // of the 128 columns, those that have left
             if (e.staged) {
 #pragma unroll 1
                 for (uint32_t box = 0; wanted && ok && box < (second ? 2u : 1u); ++box) {
@@ -929,17 +998,25 @@ product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                         if (e.residual != nullptr) stage.request(1, col0 + kBoxColumns, row0, lane);
                     }
                     if (!stage.finish(taddr + box * kBoxColumns, box, col0 + box * kBoxColumns, row0, lane, e, abort_flag)) give_up();
+                    else done += kBoxColumns;
                 }
-            } else if (wanted) {
+                if (!ok) stage.settle();
+            }
+            if (wanted && (!e.staged || !ok)) {
 #pragma unroll 1
-                for (uint32_t c = 0; c < 128; c += 32) {
+                for (uint32_t c = done; c < 128; c += 32) {
                     if (col0 + c >= e.cols) break;
                     float v[32];
                     load_accumulators(taddr + c, v);
+                    if (!ok) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; ++i) v[i] = kNan;
+                    }
                     transpose(v, lane);
                     finish<T, T>(v, row0, 32, col0 + c + lane, e);
                 }
             }
+            if (!ok) continue;
             ptx::tcgen05_fence_before_sync();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive_remote(tmem_empty_even + acc * 8);
@@ -996,6 +1073,8 @@ struct Operands {
     const void* b; int64_t ldb; bool b_mn; uint32_t rows_b;
     uint32_t k;
     int32_t* status;
+    long long budget = ptx::kWaitBudgetCycles;
+    uint32_t withhold = kNothing;
 };
 
 // CTAs that find an SM of their own: clusters of four and eight do not divide the SMs of every GPC.
@@ -1019,6 +1098,8 @@ int launch_tiles(const Operands& o, Epilogue e, uint32_t splits_log2, int num_sm
     p.a_mn = o.a_mn;
     p.b_mn = o.b_mn;
     p.status = o.status;
+    p.budget = o.budget;
+    p.withhold = o.withhold;
     const uint64_t ctas = static_cast<uint64_t>(p.tiles_a) * p.tiles_b << splits_log2;
     // One CTA to an SM: its ring may fill the shared memory; more: two share it.  Clusters of eight, too, leave room for a second CTA: of
     // those that fill their SMs not even sixteen run at once (256 x 128 x 4096, 16 of them: 8.9 us, a second wave; 5.7 so).
@@ -1052,6 +1133,8 @@ int launch_pairs(const Operands& o, Epilogue e, int num_sms, cudaStream_t stream
     p.a_mn = o.a_mn;
     p.b_mn = o.b_mn;
     p.status = o.status;
+    p.budget = o.budget;
+    p.withhold = o.withhold;
     int dev = 0;
     NVFP4_CUDA_CHECK(cudaGetDevice(&dev));
     static bool attr_set[host::kMaxDevices] = {};
@@ -1132,7 +1215,7 @@ int launch_product(const Operands& o, const Epilogue& e, int num_sms, cudaStream
     if (o.rows_a <= 2 && !o.a_mn && !o.b_mn && static_cast<uint64_t>(o.rows_b) * o.k <= kTokenMostWeights) return launch_tokens<T, D>(o, e, num_sms, stream);
     const Form f = choose_form(o, !std::is_same<D, T>::value, num_sms);
     if (f.kind == Form::kSwap) {                     // the weight's rows on the tensor memory's lanes
-        const Operands s{o.b, o.ldb, false, o.rows_b, o.a, o.lda, false, o.rows_a, o.k, o.status};
+        const Operands s{o.b, o.ldb, false, o.rows_b, o.a, o.lda, false, o.rows_a, o.k, o.status, o.budget, o.withhold};
         switch (f.bn) {
             case 16: return launch_tiles<T, D, 16, true>(s, e, f.splits_log2, num_sms, stream);
             case 32: return launch_tiles<T, D, 32, true>(s, e, f.splits_log2, num_sms, stream);
@@ -1250,9 +1333,13 @@ static int product(const Operands& o, const Epilogue& e, bool out32, int num_sms
 
 int launch_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual, int64_t ldr, void* d, int64_t ldd,
                   int16_t* slopes, int64_t lds, int M, int N, int K, bool bf16, bool out32, int activation, int32_t* status, int num_sms,
-                  cudaStream_t stream)
+                  cudaStream_t stream, int64_t budget, bool withhold_residuals)
 {
-    const Operands o{x, ldx, false, static_cast<uint32_t>(M), w, ldw, false, static_cast<uint32_t>(N), static_cast<uint32_t>(K), status};
+    Operands o{x, ldx, false, static_cast<uint32_t>(M), w, ldw, false, static_cast<uint32_t>(N), static_cast<uint32_t>(K), status};
+    if (budget > 0) {                                // the test of waits that run out
+        o.budget = budget;
+        o.withhold = withhold_residuals ? kResiduals : kProducts;
+    }
     if (activation == NVFP4_ACTIVATION_NONE) slopes = nullptr;
     const Epilogue e{d, ldd, slopes, lds, bias, residual, ldr, static_cast<uint32_t>(M), static_cast<uint32_t>(N), activation, false};
     return bf16 ? product<__nv_bfloat16>(o, e, out32, num_sms, stream) : product<__half>(o, e, out32, num_sms, stream);

@@ -70,7 +70,8 @@ NVFP4_DEVICE bool mbar_wait_impl(uint64_t* bar, uint32_t parity, volatile uint32
 
 // The same bounded wait for roles that wait long and need not react within cycles (an epilogue warp waiting
 // for a whole tile): it sleeps between polls, which leaves issue slots and power to the warps that work.
-NVFP4_DEVICE bool mbar_wait_relaxed(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t sleep_ns)
+NVFP4_DEVICE bool mbar_wait_relaxed(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t sleep_ns,
+                                    long long budget = kWaitBudgetCycles)
 {
     if (mbar_try_wait(bar, parity)) return true;
     const long long t0 = clock64();
@@ -80,8 +81,15 @@ NVFP4_DEVICE bool mbar_wait_relaxed(uint64_t* bar, uint32_t parity, volatile uin
             __nanosleep(sleep_ns);
             if (mbar_try_wait(bar, parity)) return true;
         }
-        if (*abort_flag != 0 || clock64() - t0 > kWaitBudgetCycles) return false;
+        if (*abort_flag != 0 || clock64() - t0 > budget) return false;
     }
+}
+
+// On the way out after a wait that expired: what was asked of this barrier (copies into the block's shared memory, products) comes to its
+// end, or the clock reaches `until`; whoever leaves earlier leaves copies behind that land in the next block's memory.
+NVFP4_DEVICE void mbar_settle(uint64_t* bar, uint32_t parity, long long until)
+{
+    while (!mbar_try_wait(bar, parity) && clock64() < until) {}
 }
 
 // The outcome of a wait that all 32 lanes of a warp made, the same for every lane.  Each lane polls on its own and may

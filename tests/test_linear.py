@@ -467,3 +467,37 @@ def test_gradients_keep_their_digits_where_slopes_are_small(activation, lo, hi):
                 for got, roundings in ((db, 1), (dw[:, 0], 2)):
                     off = (got.cpu().double() - want).abs()
                     assert off.le(error * 1.01 + roundings * (want.abs() * 1.02 * HALF_STEP[dtype] + tiny)).all(), float((off / want.abs()).max())
+
+
+# ---- waits that run out ----------------------------------------------------------------------------------------------
+
+
+def test_expired_waits_need_a_bound():
+    for budget in (0, -1, 2000000001):
+        assert "budget" in error_of(_C.lib().nvfp4_debug_linear_expired(1024, 64, 1024, 64, None, None, 0, 1024, 32, None, 0, 4, 32, 64, 0, 0, 0, 0, budget, None, None))
+
+
+# the swapped tiles, split over clusters and not, the other ones, pairs; rows that TMA addresses and rows that it does not
+@gpu
+@pytest.mark.parametrize("m, n, k", [(1, 4096, 4096), (33, 1411, 2048), (256, 4096, 1024), (400, 200, 1024), (200, 2049, 64), (3000, 2056, 128), (3000, 2057, 128), (3000, 128, 4096),
+                                     (2500, 4104, 392), (16384, 128, 264)])
+def test_what_an_expired_wait_leaves_is_nan(m, n, k):
+    """Products that are never issued, residuals that are never fetched: the kernels end after half a millisecond, with the status bit and NaN
+    in place of results, also for callers without a status word, and the next call is an ordinary one."""
+    seen = 0
+    for out in (torch.bfloat16, torch.float32):
+        x, w, bias, residual = (t.cuda() for t in make(m, n, k, torch.bfloat16, 3, out))
+        want, _ = _C.linear(x, w, bias, residual, "gelu", out, keep=True)
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        for word in (status, None):
+            for r in (residual, None):
+                d, slopes = _C.debug_linear_expired(x, w, bias, r, "gelu", out, 1_000_000, word)
+                assert torch.isnan(d).all() and (slopes[:, :n] == -1).all() and (slopes[:, n:] == 0).all()
+        with pytest.raises(RuntimeError, match="error 4"):
+            _C.read_status(status)
+        d, _ = _C.debug_linear_expired(x, w, bias, residual, "gelu", out, 1_000_000, status, withhold_residuals=True)
+        expired = int(status.item())
+        assert torch.isnan(d).all() if expired else torch.equal(d, want)     # forms that read it themselves finish
+        seen += expired
+        assert torch.equal(_C.linear(x, w, bias, residual, "gelu", out, keep=True)[0], want)
+    assert seen or (m, n, k) != (3000, 2056, 128)
