@@ -423,6 +423,11 @@ NVFP4_API int nvfp4_debug_wait_timeout(int64_t budget_cycles, int32_t* device_st
 NVFP4_API int nvfp4_debug_quantize_weight_expired(const void* w, int w_dtype, int E, int N, int K, void* b, void* sfb, float* gw,
                                                   int64_t budget_cycles, void* stream);
 
+/* Test hook: nvfp4_unsort_tokens whose waits can only run out, after budget_cycles clock cycles (at most 2e9), where it takes the ring of bulk
+ * copies (many tokens, rows of whole 16-byte words): no row is requested, y is NaN.  Other sizes finish. */
+NVFP4_API int nvfp4_debug_unsort_expired(const void* rows, int64_t ld_elems, int dtype, int64_t M, const int64_t* place, const float* w, int64_t tokens,
+                                         int k, int hidden, void* y, int64_t budget_cycles, void* stream);
+
 /* Test hook: nvfp4_linear whose waits can only run out, after budget_cycles clock cycles (at most 2e9): no product is issued, or, with
  * withhold_residuals, no residual is fetched (by the kernels that fetch it by TMA; others finish).  The kernel ends by itself, with NaN in
  * d and in the slopes and bit 0 in *device_status.  One or two rows with a small weight take no such wait and finish. */

@@ -48,7 +48,7 @@ EXPORTS = ("nvfp4_last_error", "nvfp4_version", "nvfp4_get_num_sms", "nvfp4_set_
            "nvfp4_grouped_gemm_swiglu_contiguous", "nvfp4_grouped_gemm_masked", "nvfp4_load_checkpoint_weights",
            "nvfp4_read_status", "nvfp4_debug_split_workspace", "nvfp4_debug_wait_timeout", "nvfp4_debug_quantize_weight_expired", "nvfp4_plan_peer_masked", "nvfp4_plan_one_rank",
            "nvfp4_peer_barrier", "nvfp4_route_tokens", "nvfp4_route_tokens_backward", "nvfp4_sort_tokens", "nvfp4_unsort_tokens",
-           "nvfp4_unsort_tokens_backward", "nvfp4_linear", "nvfp4_linear_dz", "nvfp4_linear_dx", "nvfp4_linear_dw", "nvfp4_debug_linear_expired")
+           "nvfp4_unsort_tokens_backward", "nvfp4_linear", "nvfp4_linear_dz", "nvfp4_linear_dx", "nvfp4_linear_dw", "nvfp4_debug_linear_expired", "nvfp4_debug_unsort_expired")
 
 
 def library_path() -> str:
@@ -105,6 +105,7 @@ def lib() -> ctypes.CDLL:
         L.nvfp4_unsort_tokens.argtypes = [vp, i64, i32, i64, vp, vp, i64, i32, i32, vp, vp]
         L.nvfp4_unsort_tokens_backward.argtypes = [vp, i64, vp, i64, i32, i64, vp, vp, vp, i64, i32, i32, vp, vp, vp]
         L.nvfp4_linear.argtypes = [vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, i32, i32, vp, vp]
+        L.nvfp4_debug_unsort_expired.argtypes = [vp, i64, i32, i64, vp, vp, i64, i32, i32, vp, i64, vp]
         L.nvfp4_debug_linear_expired.argtypes = [vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, i32, i32, i32, i64, vp, vp]
         L.nvfp4_linear_dz.argtypes = [vp, i64, vp, i64, vp, i64, vp, i32, i32, i32, i32, vp]
         L.nvfp4_linear_dx.argtypes = [vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp]
@@ -791,6 +792,16 @@ def unsort_tokens(rows: torch.Tensor, place: torch.Tensor, weights) -> torch.Ten
     with _on(dev):
         _check(lib().nvfp4_unsort_tokens(rows.data_ptr(), ld, DTYPE_CODES[rows.dtype], m, place.data_ptr(),
                                          weights.data_ptr() if weights is not None else None, tokens, k, hidden, y.data_ptr(), _stream()))
+    return y
+
+
+def debug_unsort_expired(rows: torch.Tensor, place: torch.Tensor, weights: torch.Tensor, budget_cycles: int) -> torch.Tensor:
+    """unsort_tokens whose waits run out after `budget_cycles` (test hook): NaN throughout, where it takes the ring."""
+    _require(all(t.is_contiguous() for t in (rows, place, weights)), "contiguous tensors")
+    y = torch.zeros(place.shape[0], rows.shape[1], dtype=rows.dtype, device=_one_device(rows, place, weights))
+    with _on(rows.device):
+        _check(lib().nvfp4_debug_unsort_expired(rows.data_ptr(), rows.shape[1], DTYPE_CODES[rows.dtype], rows.shape[0], place.data_ptr(), weights.data_ptr(),
+                                                place.shape[0], place.shape[1], rows.shape[1], y.data_ptr(), int(budget_cycles), _stream()))
     return y
 
 

@@ -830,17 +830,31 @@ int nvfp4_sort_tokens(const void* x, int64_t ldx_elems, int dtype, int64_t token
                               static_cast<cudaStream_t>(stream));
 }
 
-int nvfp4_unsort_tokens(const void* rows, int64_t ld_elems, int dtype, int64_t M, const int64_t* place, const float* w, int64_t tokens, int k,
-                        int hidden, void* y, void* stream)
+static int unsort_tokens(const void* rows, int64_t ld_elems, int dtype, int64_t M, const int64_t* place, const float* w, int64_t tokens, int k,
+                         int hidden, void* y, void* stream, int64_t budget)
 {
-    host::clear_error();
     if (int rc = check_token_rows(dtype, M, tokens, k, hidden, ld_elems)) return rc;
     if (tokens == 0) return NVFP4_OK;
     NVFP4_REQUIRE((rows || M == 0) && place && y, "null pointer argument");
     NVFP4_REQUIRE(on_elements(rows, dtype) && on_elements(y, dtype), "rows are not aligned to their type");
     host::DeviceInfo* dev;
     if (int rc = host::device_info(-1, &dev)) return rc;
-    return launch_unsort_tokens(rows, ld_elems, dtype, M, place, w, tokens, k, hidden, y, dev->hw_sms, static_cast<cudaStream_t>(stream));
+    return launch_unsort_tokens(rows, ld_elems, dtype, M, place, w, tokens, k, hidden, y, dev->hw_sms, static_cast<cudaStream_t>(stream), budget);
+}
+
+int nvfp4_unsort_tokens(const void* rows, int64_t ld_elems, int dtype, int64_t M, const int64_t* place, const float* w, int64_t tokens, int k,
+                        int hidden, void* y, void* stream)
+{
+    host::clear_error();
+    return unsort_tokens(rows, ld_elems, dtype, M, place, w, tokens, k, hidden, y, stream, 0);
+}
+
+int nvfp4_debug_unsort_expired(const void* rows, int64_t ld_elems, int dtype, int64_t M, const int64_t* place, const float* w, int64_t tokens, int k,
+                               int hidden, void* y, int64_t budget_cycles, void* stream)
+{
+    host::clear_error();
+    NVFP4_REQUIRE(budget_cycles > 0 && budget_cycles <= 2000000000ll, "budget_cycles outside (0, 2e9]");
+    return unsort_tokens(rows, ld_elems, dtype, M, place, w, tokens, k, hidden, y, stream, budget_cycles);
 }
 
 int nvfp4_unsort_tokens_backward(const void* dy, int64_t ldy_elems, const void* rows, int64_t ld_elems, int dtype, int64_t M, const int64_t* place,

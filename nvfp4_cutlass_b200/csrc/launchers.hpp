@@ -63,7 +63,7 @@ int launch_route_backward(const void* logits, int64_t ld, int dtype, int64_t tok
 int launch_sort_tokens(const void* x, int64_t ldx_bytes, int64_t tokens, int k, int64_t row_bytes, const int64_t* ids, int experts, int alignment,
                        int64_t m, void* rows, int64_t* place, int32_t* source, int32_t* m_indices, int num_sms, cudaStream_t stream);
 int launch_unsort_tokens(const void* rows, int64_t ld, int dtype, int64_t m, const int64_t* place, const float* w, int64_t tokens, int k, int hidden,
-                         void* y, int num_sms, cudaStream_t stream);
+                         void* y, int num_sms, cudaStream_t stream, int64_t budget = 0);
 int launch_unsort_tokens_backward(const void* dy, int64_t ldy, const void* rows, int64_t ld, int dtype, int64_t m, const int64_t* place,
                                   const float* w, int64_t tokens, int k, int hidden, void* drows, float* dw, int num_sms, cudaStream_t stream);
 

@@ -457,7 +457,8 @@ unsort_kernel(const typename P::Bits* __restrict__ rows, int64_t ld, const int64
 // A unit is a piece of one token's rows, or `group` whole tokens whose rows are short; a slot of the ring takes a unit's pairs (at most
 // 32), `stride` bytes each.  Warp 0 looks up a pair per lane, one unit ahead, leaves the weights and the mask of pairs with a row beside
 // the slot and requests the rows; the other warps add them up in FP32 in ascending j, the order of the kernel above: the same bits.
-// Every wait is bounded; a block whose wait ran out leaves NaN in what it did not finish.
+// Every wait is bounded; a block whose wait ran out leaves NaN in what it did not finish, and leaves when its copies in flight have landed,
+// within the same bound.
 constexpr int kRingWorkers = 16, kRingThreads = 32 * (1 + kRingWorkers), kRingPairs = 32, kRingMaxDepth = 12;
 struct RingSlot {
     float w[kRingPairs];
@@ -467,6 +468,8 @@ struct RingSlot {
 constexpr uint32_t kRingLeast = 2;
 struct RingShape {
     uint32_t tokens, k, group, units, pieces, row_bytes, stride, depth;
+    long long budget = ptx::kWaitBudgetCycles;       // of every wait, in cycles
+    bool withhold = false;                           // test of the expired wait: no row is requested
 };
 template <typename P>
 __global__ void __launch_bounds__(kRingThreads, 1)
@@ -505,8 +508,10 @@ unsort_ring_kernel(const uint8_t* __restrict__ rows, int64_t ld_bytes, const int
             weight = w != nullptr ? w[at] : 1.0f;
         };
         look_up(blockIdx.x);
-        for (uint32_t unit = blockIdx.x; unit < shape.units; unit += gridDim.x) {
-            if (!ptx::all_lanes(ptx::mbar_wait_impl(freed + slot, phase ^ 1, abort_flag))) { *abort_flag = 1; break; }
+        uint32_t loaded = 0;
+        bool ok = true;
+        for (uint32_t unit = blockIdx.x; unit < shape.units && !shape.withhold; unit += gridDim.x, ++loaded) {
+            if (!ptx::all_lanes(ptx::mbar_wait_budget(freed + slot, phase ^ 1, abort_flag, shape.budget))) { *abort_flag = 1; ok = false; break; }
             const uint32_t from = unit % shape.pieces * shape.stride, bytes = min(shape.stride, shape.row_bytes - from);
             const unsigned live = __ballot_sync(kAll, row >= 0);
             if (lane < pairs) info[slot].w[lane] = weight;
@@ -518,11 +523,15 @@ unsort_ring_kernel(const uint8_t* __restrict__ rows, int64_t ld_bytes, const int
             look_up(unit + gridDim.x);
             next();
         }
+        if (!ok || !ptx::all_lanes(*abort_flag == 0)) {
+            const long long until = clock64() + shape.budget;
+            for (uint32_t n = loaded > shape.depth ? loaded - shape.depth : 0; n < loaded; ++n) ptx::mbar_settle(full + n % shape.depth, n / shape.depth & 1u, until);
+        }
         return;
     }
     bool ok = true;
     for (uint32_t unit = blockIdx.x; unit < shape.units; unit += gridDim.x) {
-        if (ok && !ptx::all_lanes(ptx::mbar_wait_impl(full + slot, phase, abort_flag))) { *abort_flag = 1; ok = false; }
+        if (ok && !ptx::all_lanes(ptx::mbar_wait_budget(full + slot, phase, abort_flag, shape.budget))) { *abort_flag = 1; ok = false; }
         const uint32_t base = smem + slot * slot_bytes, live = ok ? info[slot].live : 0u;
         const uint32_t t0 = unit / shape.pieces * shape.group, here = min(shape.group, shape.tokens - t0);
         const uint32_t from = unit % shape.pieces * shape.stride, words = min(shape.stride, shape.row_bytes - from) / 16;
@@ -767,7 +776,7 @@ int launch_sort_tokens(const void* x, int64_t ldx_bytes, int64_t tokens, int k, 
 }
 
 int launch_unsort_tokens(const void* rows, int64_t ld, int dtype, int64_t m, const int64_t* place, const float* w, int64_t tokens, int k, int hidden,
-                         void* y, int num_sms, cudaStream_t stream)
+                         void* y, int num_sms, cudaStream_t stream, int64_t budget)
 {
     const size_t size = elem_bytes(dtype);
     const uintptr_t bits = reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(y) | static_cast<uintptr_t>(ld * size) | hidden * size;
@@ -776,7 +785,8 @@ int launch_unsort_tokens(const void* rows, int64_t ld, int dtype, int64_t m, con
         using Bits = typename P::Bits;
         constexpr int kN = P::kN;
         if constexpr (P::kSize == 16) {
-            const RingShape shape = ring_shape(tokens, k, static_cast<int64_t>(hidden * size));
+            RingShape shape = ring_shape(tokens, k, static_cast<int64_t>(hidden * size));
+            if (budget > 0) { shape.budget = budget; shape.withhold = true; }
             if (shape.depth >= 2 && shape.units >= kRingLeast * static_cast<uint32_t>(num_sms)) {
                 static bool attr_set[host::kMaxDevices] = {};
                 int dev = 0;

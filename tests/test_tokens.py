@@ -803,3 +803,22 @@ def test_routing_gradient_of_a_confident_token(ahead, k):
                 tolerance = size * bound + want.abs() * 1.01 * HALF_STEP[dtype] + (2.0 ** -25 if dtype == torch.float16 else 1e-38)
                 off = (got.cpu().double() - want).abs()
                 assert off.le(tolerance).all(), float((off / tolerance).max())
+
+
+def test_expired_waits_of_the_sum_need_a_bound():
+    for budget in (0, -1, 2000000001):
+        assert "budget" in error_of(_C.lib().nvfp4_debug_unsort_expired(16, 8, 0, 64, 16, 16, 4, 1, 8, 16, budget, None))
+
+
+@gpu
+@pytest.mark.parametrize("tokens, k, hidden", [(1000, 8, 4096), (5000, 2, 64), (3000, 32, 1024), (3000, 6, 520)])
+def test_what_an_expired_wait_of_the_sum_leaves_is_nan(tokens, k, hidden):
+    """Rows that are never fetched: the kernel ends after half a millisecond, with NaN in place of sums, and the next call is an ordinary one."""
+    ids = some_ids(tokens, k, 64, 1, "holes").cuda()
+    w = torch.rand(tokens, k, generator=gen(2)).cuda()
+    for dtype in ALL_TYPES:
+        rows, order = sort_tokens(torch.randn(tokens, hidden, generator=gen(1)).to(dtype).cuda(), ids, 64, alignment=16)
+        want = unsort_tokens(rows, order, w)
+        y = _C.debug_unsort_expired(rows, order.place, w, 1_000_000)
+        assert torch.isnan(y).all()
+        assert torch.equal(unsort_tokens(rows, order, w), want)
