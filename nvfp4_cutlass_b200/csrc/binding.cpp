@@ -208,6 +208,9 @@ template <typename T>
 T* pointer(const at::Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
 // The gradient of an output in rows that the kernels can read
 at::Tensor in_rows(const at::Tensor& t) { return t.size(0) > 0 && t.size(1) > 0 && t.stride(1) == 1 && t.stride(0) >= t.size(1) ? t : t.contiguous(); }
+// Whether this backward pass asks for a gradient (autograd.grad names some; an argument may require one that it does not): `edge` counts the
+// tensors among the node's arguments, of which missing ones are none.
+bool wanted(AutogradContext* ctx, size_t edge, bool there = true) { return there && ctx->needs_input_grad(edge); }
 // An argument of a node that may be missing: nodes take no undefined tensors
 std::optional<at::Tensor> present(const at::Tensor& t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; }
 // Gradients that were computed without being recorded: whoever differentiates them again gets an error instead of nothing.
@@ -338,11 +341,9 @@ struct UnsortNode : torch::autograd::Function<UnsortNode> {
                               const at::Tensor& source)
     {
         const at::Tensor weights = given.value_or(at::Tensor());
-        const bool want_rows = rows.requires_grad(), want_weights = weights.defined() && weights.requires_grad();
+        const bool want_weights = weights.defined() && weights.requires_grad();
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({want_weights ? rows : at::Tensor(), weights, place, source});
-        ctx->saved_data["rows"] = want_rows;
-        ctx->saved_data["weights"] = want_weights;
         return sum_rows(rows, place, weights, true);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads)
@@ -352,8 +353,8 @@ struct UnsortNode : torch::autograd::Function<UnsortNode> {
         const variable_list saved = ctx->get_saved_variables();
         const at::Tensor &rows = saved[0], &weights = saved[1], &place = saved[2], &source = saved[3], dy = in_rows(grads[0]);
         const c10::cuda::CUDAGuard guard(dy.device());
-        const bool want_weights = ctx->saved_data["weights"].toBool();
-        if (ctx->saved_data["rows"].toBool()) out[0] = fresh(dy, dy.scalar_type(), {source.size(0), dy.size(1)});
+        const bool want_weights = wanted(ctx, 1, weights.defined());
+        if (wanted(ctx, 0)) out[0] = fresh(dy, dy.scalar_type(), {source.size(0), dy.size(1)});
         if (want_weights) out[1] = fresh(dy, at::kFloat, place.sizes());
         check(g_entry.unsort_backward(dy.data_ptr(), row_stride(dy), want_weights ? rows.data_ptr() : nullptr, want_weights ? row_stride(rows) : dy.size(1),
                                       dtype_code(dy.scalar_type()), source.size(0), pointer<int64_t>(place), pointer<int32_t>(source),
@@ -410,8 +411,8 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
         if (activation != NVFP4_ACTIVATION_NONE && (want_x || want_w || want_bias)) slopes = fresh(x, at::kShort, {x.size(0), (w.size(0) + 7) / 8 * 8});
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({want_w ? x : at::Tensor(), want_x ? w : at::Tensor(), slopes});
-        ctx->saved_data["bias"] = want_bias;
-        ctx->saved_data["residual"] = residual.defined() && residual.requires_grad();
+        ctx->saved_data["bias"] = bias.defined();
+        ctx->saved_data["residual"] = residual.defined();
         ctx->saved_data["type"] = static_cast<int64_t>(x.scalar_type());
         return linear_forward(x, w, bias, residual, static_cast<int>(activation), out32, slopes);
     }
@@ -421,8 +422,9 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
         if (!grads[0].defined()) return out;
         const variable_list saved = ctx->get_saved_variables();
         const at::Tensor &x = saved[0], &w = saved[1], &slopes = saved[2];
-        const bool want_bias = ctx->saved_data["bias"].toBool(), products = x.defined() || w.defined();
-        if (ctx->saved_data["residual"].toBool()) out[3] = grads[0];
+        const bool has_bias = ctx->saved_data["bias"].toBool(), want_x = wanted(ctx, 0), want_w = wanted(ctx, 1), want_bias = wanted(ctx, 2, has_bias),
+                   products = want_x || want_w;
+        if (wanted(ctx, has_bias ? 3 : 2, ctx->saved_data["residual"].toBool())) out[3] = grads[0];
         if (products || want_bias) {
             const at::Tensor dd = in_rows(grads[0]);
             const c10::cuda::CUDAGuard guard(dd.device());
@@ -436,12 +438,12 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
             if (want_bias || (products && !as_it_is))
                 check(g_entry.linear_dz(dd.data_ptr(), row_stride(dd), pointer<int16_t>(slopes), slopes.defined() ? slopes.size(1) : 0,
                                         as_it_is ? nullptr : pointer<void>(dz), ldz, pointer<void>(out[2]), m, n, code, dtype_code(dd.scalar_type()), stream()));
-            if (w.defined()) {
+            if (want_x) {
                 out[0] = fresh(dd, type, {m, w.size(1)});
                 check(g_entry.linear_dx(dz.data_ptr(), ldz, w.data_ptr(), row_stride(w), out[0].data_ptr(), w.size(1), m, n, static_cast<int>(w.size(1)), code,
                                         nullptr, stream()));
             }
-            if (x.defined()) {
+            if (want_w) {
                 out[1] = fresh(dd, type, {n, x.size(1)});
                 check(g_entry.linear_dw(dz.data_ptr(), ldz, x.data_ptr(), row_stride(x), out[1].data_ptr(), x.size(1), m, n, static_cast<int>(x.size(1)), code,
                                         nullptr, stream()));

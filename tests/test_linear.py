@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from nvfp4_gemm import _C, linear, route_tokens, sort_tokens, unsort_tokens
+from nvfp4_gemm import _C, TokenOrder, linear, route_tokens, sort_tokens, unsort_tokens
 
 gpu = pytest.mark.gpu
 HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
@@ -501,3 +501,37 @@ def test_what_an_expired_wait_leaves_is_nan(m, n, k):
         seen += expired
         assert torch.equal(_C.linear(x, w, bias, residual, "gelu", out, keep=True)[0], want)
     assert seen or (m, n, k) != (3000, 2056, 128)
+
+
+@gpu
+def test_gradients_that_nobody_asks_for_are_not_computed():
+    """x from a layer before needs a gradient, this call of autograd.grad does not: no memory is taken for it."""
+    m, n, k = 4096, 64, 4096
+
+    def memory(y, wanted, dd):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        grads = torch.autograd.grad(y, wanted, dd, retain_graph=True)
+        torch.cuda.synchronize()
+        return torch.cuda.max_memory_allocated() - before, grads
+
+    x, w, bias, residual = (t.cuda().requires_grad_() for t in make(m, n, k, torch.bfloat16, 1))
+    dd = torch.randn(m, n, generator=gen(2)).bfloat16().cuda()
+    leaves = [x, w, bias, residual]
+    for activation in ("none", "silu"):
+        y = linear(*leaves, activation=activation)
+        _, full = memory(y, leaves, dd)
+        for i, most in ((1, 4 << 20), (2, 4 << 20), (3, 1 << 20)):       # dx alone is 32 MB
+            taken, (grad,) = memory(y, [leaves[i]], dd)
+            assert taken < most and torch.equal(grad, full[i]), (activation, i, taken)
+    rows = torch.randn(4096, 4096, generator=gen(3)).bfloat16().cuda().requires_grad_()
+    place = torch.randperm(4096, generator=gen(4)).view(2048, 2).cuda()
+    order = TokenOrder(place, torch.zeros(4096, dtype=torch.int32, device="cuda"), torch.zeros(4096, dtype=torch.int32, device="cuda"))
+    weights = torch.rand(2048, 2, generator=gen(5)).cuda().requires_grad_()
+    y = unsort_tokens(rows, order, weights)
+    dy = torch.randn(2048, 4096, generator=gen(6)).bfloat16().cuda()
+    _, full = memory(y, [rows, weights], dy)
+    taken, (grad,) = memory(y, [weights], dy)
+    assert taken < 4 << 20 and torch.equal(grad, full[1])
+    assert torch.equal(memory(y, [rows], dy)[1][0], full[0])
