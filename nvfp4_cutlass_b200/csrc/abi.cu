@@ -123,9 +123,19 @@ int encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t e
     const cuuint32_t box[2] = {box0, box1};
     const cuuint32_t elem_strides[2] = {1, 1};
     (void)elem_bytes;
-    const CUresult r = encode(map, dtype, 2, const_cast<void*>(base), dims, strides, box, elem_strides,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto encode_it = [&] {
+        return encode(map, dtype, 2, const_cast<void*>(base), dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode_it();
+    if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+        // A thread that has called nothing of the runtime yet which needs the device (autograd's, in a backward pass that begins with a
+        // product; a thread of the caller's) has no context of its own; the driver's functions do not look for one.
+        int dev = 0;
+        NVFP4_CUDA_CHECK(cudaGetDevice(&dev));
+        NVFP4_CUDA_CHECK(cudaSetDevice(dev));
+        r = encode_it();
+    }
     if (r != CUDA_SUCCESS)
         return fail(NVFP4_E_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (dims %llu x %llu, box %u x %u)",
                     static_cast<int>(r), static_cast<unsigned long long>(dim0),

@@ -1,0 +1,54 @@
+"""First calls from threads that have not used the device yet: autograd's in a backward pass, threads of the caller's."""
+import subprocess
+import sys
+
+import pytest
+
+from conftest import ROOT
+
+pytestmark = pytest.mark.gpu
+
+SETUP = """
+import threading
+import torch, nvfp4_gemm
+x = torch.randn(384, 512, device="cuda").to(torch.bfloat16)
+w = torch.randn(256, 512, device="cuda").to(torch.bfloat16)
+weights = nvfp4_gemm.quantize_weight_nvfp4(w[None].contiguous())
+m_indices = nvfp4_gemm.make_m_indices([384]).cuda()
+d = torch.empty(384, 256, device="cuda", dtype=torch.bfloat16)
+ids = torch.zeros(384, 4, dtype=torch.int64, device="cuda")
+logits = torch.randn(384, 16, device="cuda")
+def gemm(**kw):
+    nvfp4_gemm.m_grouped_bf16_dual_nvfp4_gemm_contiguous(x, *weights, d, m_indices, **kw)
+    return d
+def moved():
+    rows, order = nvfp4_gemm.sort_tokens(x, ids, 4)
+    return nvfp4_gemm.unsort_tokens(rows, order)
+torch.cuda.synchronize()
+def backward():                  # without an activation or a bias the first kernel is a product
+    leaf = x.clone().requires_grad_()
+    y = nvfp4_gemm.linear(leaf, w)
+    return torch.autograd.grad(y, leaf, torch.ones_like(y))[0]
+def in_a_thread(call):
+    out = []
+    t = threading.Thread(target=lambda: (out.append(call()), torch.cuda.synchronize()))
+    t.start(); t.join()
+    assert out, "the thread's call failed"
+    return out[0].clone()
+"""
+BACKWARD = """
+got = backward()
+want = torch.ones(384, 256, device="cuda").bfloat16() @ w
+assert (got.float() - want.float()).abs().max() <= 2 * 2.0 ** -8 * want.float().abs().max()      # two roundings of one sum
+"""
+CALLS = """
+for call in (lambda: nvfp4_gemm.linear(x, w), gemm, lambda: gemm(tune_split_transform=2), lambda: gemm(tune_split_transform=2, tune_cluster=1),
+             lambda: gemm(tune_swap_ab=1, m_alignment=128), moved, lambda: nvfp4_gemm.route_tokens(logits, 3)[1]):
+    assert torch.equal(in_a_thread(call), call())
+"""
+
+
+@pytest.mark.parametrize("calls", [BACKWARD, CALLS], ids=["backward", "calls"])
+def test_the_first_call_of_a_thread(calls):
+    r = subprocess.run([sys.executable, "-c", SETUP + calls], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
