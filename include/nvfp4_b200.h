@@ -382,7 +382,8 @@ NVFP4_API int nvfp4_unsort_tokens_backward(const void* dy, int64_t ldy_elems, co
  *   that are multiples of 8, N rounded up to 8 at least; what lies behind column N of dz's rows up to there is overwritten.  dz or db
  *   may be NULL.
  * nvfp4_linear_dx: dx[M,K] = dz w.      nvfp4_linear_dw: dw[N,K] = dz^T x.      Rounded to `dtype`.
- * An FP32 output takes partial sums of 256 products out of the tensor cores and adds them as FP32; others stay in their accumulator.
+ * An FP32 output takes partial sums of 256 products out of the tensor cores and adds them as FP32; a 16-bit output does so every 1024
+ * products where there are more than 16384 (FP16) or 262144 (BF16) to a sum of a thread block; fewer stay in their accumulator.
  * device_status (may be NULL) receives bit 0 if a bounded wait expired; what was not finished then is NaN.  No counterparts in the
  * reference project. */
 NVFP4_API int nvfp4_linear(const void* x, int64_t ldx_elems, const void* w, int64_t ldw_elems, const void* bias, const void* residual,

@@ -524,16 +524,23 @@ constexpr uint32_t tile_smem(uint32_t bn, uint32_t depth, uint32_t splits)
 }
 // For an FP32 output the epilogue warps take the accumulators over every four K blocks and add them up in registers, two accumulators in
 // turn: the tensor core cuts what it adds to a long sum (K = 4096 in one accumulator: off by 4.3e-6 of the result, FP32 sums by 6e-7).
-constexpr uint32_t kChunkBlocks = 4;
+// The cut goes one way and grows with the sum: over operands of one sign by 6e-9 of it for every product of FP16, 1.9e-9 of BF16 (37500 to 275000
+// tokens to an accumulator).  A 16-bit output stays in its accumulator while that is less than half of the half step of its rounding, 2^-12
+// and 2^-9; longer sums (a weight's gradient over very many tokens) are taken out every sixteen K blocks (kLong; dw of 65536 FP16 tokens, 4096 x
+// 2048: some 1.5 ms, 0.9 on CTA pairs).
+constexpr uint32_t kChunkBlocks = 4, kLongChunkBlocks = 16;
+template <typename T>
+constexpr uint32_t kLongestSum = std::is_same<T, __half>::value ? 16384 : 262144;
 
 // kSwap: A is the weight and the output's columns lie on the tensor memory's lanes; else A is x and a warp's 32 x 32 accumulators are
 // transposed first.  D: type of the output.
-template <typename T, typename D, uint32_t BN, bool kSwap>
-__global__ void __launch_bounds__(kTileThreads, std::is_same<D, float>::value && BN > 64 ? 1 : 2)
+template <typename T, typename D, uint32_t BN, bool kSwap, bool kLong>
+__global__ void __launch_bounds__(kTileThreads, (std::is_same<D, float>::value || kLong) && BN > 64 ? 1 : 2)
 product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ Maps maps, const Product p,
                const Epilogue e)
 {
-    constexpr bool kWide = std::is_same<D, float>::value;
+    constexpr bool kWide = std::is_same<D, float>::value || kLong;
+    constexpr uint32_t kTaken = kLong ? kLongChunkBlocks : kChunkBlocks;     // K blocks after which accumulators are taken out
     constexpr uint32_t kChunk = BN < 32 ? BN : 32, kStage = tile_stage(BN), kCols = (kWide ? 2 : 1) * BN < 32 ? 32 : (kWide ? 2 : 1) * BN;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -573,7 +580,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     const uint32_t a0 = a_blk * BM, b0 = b_blk * BN;
     const uint32_t kb0 = static_cast<uint32_t>(static_cast<uint64_t>(p.k_blocks) * rank >> p.splits_log2);
     const uint32_t kb1 = static_cast<uint32_t>(static_cast<uint64_t>(p.k_blocks) * (rank + 1) >> p.splits_log2);
-    const uint32_t chunks = kWide ? (kb1 - kb0 + kChunkBlocks - 1) / kChunkBlocks : 1;
+    const uint32_t chunks = kWide ? (kb1 - kb0 + kTaken - 1) / kTaken : 1;
     bool ok = true;
     auto give_up = [&] {
         *abort_flag = 1;
@@ -614,8 +621,8 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         const uint32_t idesc = ptx::make_idesc_f16(BM, BN, std::is_same<T, __nv_bfloat16>::value, p.a_mn, p.b_mn);
         Ring r;
         for (uint32_t kb = kb0; kb < kb1 && p.withhold != kProducts; ++kb) {
-            const uint32_t n = kb - kb0, c = kWide ? n / kChunkBlocks : 0, acc = c & 1;
-            const bool first = kWide ? n % kChunkBlocks == 0 : n == 0;
+            const uint32_t n = kb - kb0, c = kWide ? n / kTaken : 0, acc = c & 1;
+            const bool first = kWide ? n % kTaken == 0 : n == 0;
             if (kWide && first && !ptx::all_lanes(ptx::mbar_wait_budget(tmem_empty + acc, ((c >> 1) & 1) ^ 1, abort_flag, p.budget))) { give_up(); break; }
             if (!ptx::all_lanes(ptx::mbar_wait_budget(full + r.slot, r.phase, abort_flag, p.budget))) { give_up(); break; }
             ptx::tcgen05_fence_after_sync();
@@ -624,7 +631,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
             for (uint32_t s = 0; s < BK / 16; ++s)
                 ptx::tcgen05_mma_f16(tmem + acc * BN, operand_desc(at, p.a_mn, s), operand_desc(at + kSlotA, p.b_mn, s), idesc, first && s == 0 ? 0u : 1u, issue);
             ptx::tcgen05_commit(drained + r.slot, issue);
-            if (kb + 1 == kb1 || (kWide && n % kChunkBlocks == kChunkBlocks - 1)) ptx::tcgen05_commit(tmem_full + acc, issue);
+            if (kb + 1 == kb1 || (kWide && n % kTaken == kTaken - 1)) ptx::tcgen05_commit(tmem_full + acc, issue);
             next(r);
         }
         if (!ok || !ptx::all_lanes(*abort_flag == 0)) {
@@ -1080,7 +1087,7 @@ struct Operands {
 // CTAs that find an SM of their own: clusters of four and eight do not divide the SMs of every GPC.
 int ctas_at_once(uint32_t splits_log2, int num_sms) { return splits_log2 < 2 || num_sms < 2 ? num_sms : num_sms * 13 / 15; }
 
-template <typename T, typename D, uint32_t BN, bool kSwap>
+template <typename T, typename D, uint32_t BN, bool kSwap, bool kLong = false>
 int launch_tiles(const Operands& o, Epilogue e, uint32_t splits_log2, int num_sms, cudaStream_t stream)
 {
     CUtensorMap tm_a, tm_b;
@@ -1110,11 +1117,11 @@ int launch_tiles(const Operands& o, Epilogue e, uint32_t splits_log2, int num_sm
     NVFP4_CUDA_CHECK(cudaGetDevice(&dev));
     static bool attr_set[host::kMaxDevices] = {};
     if (!attr_set[dev]) {
-        NVFP4_CUDA_CHECK(cudaFuncSetAttribute(product_kernel<T, D, BN, kSwap>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmem));
+        NVFP4_CUDA_CHECK(cudaFuncSetAttribute(product_kernel<T, D, BN, kSwap, kLong>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmem));
         attr_set[dev] = true;
     }
     NVFP4_REQUIRE(ctas <= INT32_MAX, "too many tiles (%llu)", static_cast<unsigned long long>(ctas));
-    return host::launch_kernel_cluster(product_kernel<T, D, BN, kSwap>, dim3(static_cast<unsigned>(ctas)), dim3(kTileThreads),
+    return host::launch_kernel_cluster(product_kernel<T, D, BN, kSwap, kLong>, dim3(static_cast<unsigned>(ctas)), dim3(kTileThreads),
                                        tile_smem(BN, p.depth, 1u << splits_log2), stream, true, 1u << splits_log2, tm_a, tm_b, maps, p, e);
 }
 
@@ -1214,6 +1221,14 @@ int launch_product(const Operands& o, const Epilogue& e, int num_sms, cudaStream
 {
     if (o.rows_a <= 2 && !o.a_mn && !o.b_mn && static_cast<uint64_t>(o.rows_b) * o.k <= kTokenMostWeights) return launch_tokens<T, D>(o, e, num_sms, stream);
     const Form f = choose_form(o, !std::is_same<D, T>::value, num_sms);
+    if constexpr (std::is_same<D, T>::value) {
+        if (o.k >> f.splits_log2 > kLongestSum<T>) {         // CTAs of a cluster have sums of their own
+            const uint64_t tiles = static_cast<uint64_t>((o.rows_a + BM - 1) / BM) * ((o.rows_b + 127) / 128);
+            uint32_t splits_log2 = 0;
+            while (splits_log2 < 2 && tiles << (splits_log2 + 1) <= static_cast<uint64_t>(ctas_at_once(splits_log2 + 1, num_sms))) ++splits_log2;
+            return launch_tiles<T, D, 128, false, true>(o, e, splits_log2, num_sms, stream);
+        }
+    }
     if (f.kind == Form::kSwap) {                     // the weight's rows on the tensor memory's lanes
         const Operands s{o.b, o.ldb, false, o.rows_b, o.a, o.lda, false, o.rows_a, o.k, o.status, o.budget, o.withhold};
         switch (f.bn) {

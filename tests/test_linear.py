@@ -535,3 +535,22 @@ def test_gradients_that_nobody_asks_for_are_not_computed():
     taken, (grad,) = memory(y, [weights], dy)
     assert taken < 4 << 20 and torch.equal(grad, full[1])
     assert torch.equal(memory(y, [rows], dy)[1][0], full[0])
+
+
+@gpu
+@pytest.mark.parametrize("dtype, tokens, n, k", [(torch.float16, 70001, 1300, 1032), (torch.float16, 150000, 40, 64), (torch.float16, 500000, 300, 264),
+                                                 (torch.bfloat16, 1100000, 40, 64), (torch.bfloat16, 2300001, 9, 8), (torch.bfloat16, 300000, 1100, 2056)])
+def test_sums_over_very_many_tokens(dtype, tokens, n, k):
+    """Operands of one sign: a cut at every step of the sum shows, and in FP16 it would be more than the rounding of the result."""
+    g = torch.Generator("cuda").manual_seed(5)
+    x = (torch.rand(tokens, k, generator=g, device="cuda") + 0.5).to(dtype)
+    dd = ((torch.rand(tokens, n, generator=g, device="cuda") + 0.5) * (8.0 / tokens)).to(dtype)
+    w = torch.zeros(n, k, dtype=dtype, device="cuda").requires_grad_()
+    (dw,) = torch.autograd.grad(linear(x, w), w, dd)
+    want = sum(dd[i:i + 100000].double().t() @ x[i:i + 100000].double() for i in range(0, tokens, 100000))
+    # sums of 1024 products leave the tensor core, which may cut at each of its 64 steps (2^-22 of the sum so far, on average half of the
+    # last), and are added in FP32, where a rounding is of the sum so far, too
+    error = want * ((tokens / 1024 / 2 + 4) * 2.0 ** -24 + 32 * 2.0 ** -22)
+    step = 2.0 ** (torch.floor(torch.log2(want)) - {torch.float16: 10, torch.bfloat16: 7}[dtype])
+    worst = ((dw.double() - want).abs() - (0.5 * step + error))
+    assert worst.max() <= 0
