@@ -162,7 +162,7 @@ int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t
 const at::Tensor* beside(PyObject* o, at::ScalarType type, int64_t dim, const at::Tensor& like)
 {
     const at::Tensor* t = plain(o, type, dim);
-    return t != nullptr && t->get_device() == like.get_device() && t->is_contiguous() && !has_tangent(*t) ? t : nullptr;
+    return t != nullptr && t->get_device() == like.get_device() && t->is_contiguous() && !t->is_neg() && !has_tangent(*t) ? t : nullptr;
 }
 bool wants_gradient(const at::Tensor* t) { return t != nullptr && t->requires_grad(); }
 // A small int argument; false where it is none.
@@ -207,7 +207,11 @@ void forward(F&& launch)                 // holding the interpreter's lock
 template <typename T>
 T* pointer(const at::Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
 // The gradient of an output in rows that the kernels can read
-at::Tensor in_rows(const at::Tensor& t) { return t.size(0) > 0 && t.size(1) > 0 && t.stride(1) == 1 && t.stride(0) >= t.size(1) ? t : t.contiguous(); }
+at::Tensor in_rows(const at::Tensor& given)
+{
+    const at::Tensor t = given.is_neg() ? given.resolve_neg() : given;      // the memory holds the values with the other sign
+    return t.size(0) > 0 && t.size(1) > 0 && t.stride(1) == 1 && t.stride(0) >= t.size(1) ? t : t.contiguous();
+}
 // Whether this backward pass asks for a gradient (autograd.grad names some; an argument may require one that it does not): `edge` counts the
 // tensors among the node's arguments, of which missing ones are none.
 bool wanted(AutogradContext* ctx, size_t edge, bool there = true) { return there && ctx->needs_input_grad(edge); }
@@ -249,7 +253,7 @@ struct RouteNode : torch::autograd::Function<RouteNode> {
     {
         if (!grads[1].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
         const variable_list saved = ctx->get_saved_variables();
-        const at::Tensor &logits = saved[0], &ids = saved[1], g = grads[1].contiguous();
+        const at::Tensor &logits = saved[0], &ids = saved[1], g = grads[1].resolve_neg().contiguous();
         const c10::cuda::CUDAGuard guard(logits.device());
         at::Tensor dlogits = fresh(logits, logits.scalar_type(), logits.sizes());
         check(g_entry.route_backward(logits.data_ptr(), row_stride(logits), dtype_code(logits.scalar_type()), logits.size(0), static_cast<int>(logits.size(1)),

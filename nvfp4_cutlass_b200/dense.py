@@ -11,7 +11,7 @@ from typing import Optional
 import torch
 
 from . import _C
-from .tokens import _differentiable, _refuse_tangents
+from .tokens import _differentiable, _own_signs, _refuse_tangents
 
 
 class _Linear(torch.autograd.Function):
@@ -29,7 +29,8 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, dd):
         dx = dw = db = None
         if any(ctx.needs_input_grad[:3]):
-            rows = dd if dd.stride(-1) == 1 and dd.stride(0) >= dd.shape[1] else dd.contiguous()
+            rows = _own_signs(dd)
+            rows = rows if rows.stride(-1) == 1 and rows.stride(0) >= rows.shape[1] else rows.contiguous()
             dx, dw, db = _C.linear_backward(rows, *ctx.saved_tensors, *ctx.form)
         return dx, dw, db, dd if ctx.needs_input_grad[3] else None, None, None, None
 
@@ -51,6 +52,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
         if result is not None:
             return result
     _refuse_tangents(x, w, bias, residual)
+    x, w, bias, residual = (_own_signs(t) for t in (x, w, bias, residual))
     if not _differentiable(x, w, bias, residual):
         return _C.linear(x, w, bias, residual, activation, out_dtype, device_status=device_status)[0]
     return _Linear.apply(x, w, bias, residual, activation, out_dtype, device_status)

@@ -31,6 +31,11 @@ def _refuse_tangents(*tensors) -> None:
         raise RuntimeError("this operator has no derivative in forward mode: its inputs must not carry tangents")
 
 
+def _own_signs(t):
+    """A tensor whose memory holds its values: torch may keep a negated view as the memory of what it negates."""
+    return t.resolve_neg() if isinstance(t, torch.Tensor) else t
+
+
 class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, k, scores, renormalize):
@@ -47,7 +52,7 @@ class _Route(torch.autograd.Function):
         if dweights is None:
             return None, None, None, None
         logits, ids = ctx.saved_tensors
-        return _C.route_tokens_backward(logits, ids, dweights, *ctx.form), None, None, None
+        return _C.route_tokens_backward(logits, ids, _own_signs(dweights), *ctx.form), None, None, None
 
 
 def route_tokens(logits: torch.Tensor, k: int, *, scores: str = "softmax", renormalize: bool = True):
@@ -62,6 +67,7 @@ def route_tokens(logits: torch.Tensor, k: int, *, scores: str = "softmax", renor
         if result is not None:
             return result
     _refuse_tangents(logits)
+    logits = _own_signs(logits)
     if not _differentiable(logits):
         return _C.route_tokens(logits, int(k), scores, bool(renormalize))
     return _Route.apply(logits, int(k), scores, bool(renormalize))
@@ -88,7 +94,7 @@ class _Sort(torch.autograd.Function):
     def backward(ctx, drows, *_):
         if drows is None:
             return None, None, None, None
-        return _C.unsort_tokens(drows.contiguous(), ctx.saved_tensors[0], None), None, None, None
+        return _C.unsort_tokens(_own_signs(drows).contiguous(), ctx.saved_tensors[0], None), None, None, None
 
 
 def sort_tokens(x: torch.Tensor, ids: torch.Tensor, num_experts: int, *, alignment: int = 128):
@@ -104,6 +110,7 @@ def sort_tokens(x: torch.Tensor, ids: torch.Tensor, num_experts: int, *, alignme
         if result is not None:
             return result[0], TokenOrder(*result[1:])
     _refuse_tangents(x)
+    x = _own_signs(x)
     call = _Sort.apply if _differentiable(x) else _C.sort_tokens
     rows, place, source, m_indices = call(x, ids, int(num_experts), int(alignment))
     return rows, TokenOrder(place, source, m_indices)
@@ -121,7 +128,7 @@ class _Unsort(torch.autograd.Function):
     def backward(ctx, dy):
         rows, weights, place, source = ctx.saved_tensors
         want_rows, want_weights = ctx.needs_input_grad[:2]
-        drows, dweights = _C.unsort_tokens_backward(dy.contiguous(), rows, place, source, weights, want_rows, want_weights)
+        drows, dweights = _C.unsort_tokens_backward(_own_signs(dy).contiguous(), rows, place, source, weights, want_rows, want_weights)
         return drows, dweights, None, None
 
 
@@ -139,6 +146,7 @@ def unsort_tokens(rows: torch.Tensor, order: TokenOrder, weights: Optional[torch
         if result is not None:
             return result
     _refuse_tangents(rows, weights)
+    rows, weights = _own_signs(rows), _own_signs(weights)
     _C._require(isinstance(rows, torch.Tensor) and source.dtype == torch.int32 and source.dim() == 1 and source.is_contiguous() and
                 rows.dim() == 2 and rows.shape[0] == source.shape[0], "rows has the rows of the order")
     _C._one_device(rows, weights, place, source)

@@ -822,3 +822,28 @@ def test_what_an_expired_wait_of_the_sum_leaves_is_nan(tokens, k, hidden):
         y = _C.debug_unsort_expired(rows, order.place, w, 1_000_000)
         assert torch.isnan(y).all()
         assert torch.equal(unsort_tokens(rows, order, w), want)
+
+
+@gpu
+@pytest.mark.parametrize("binding", [True, False])
+def test_tensors_that_stand_for_their_negatives(binding, monkeypatch):
+    _C.lib()
+    if not binding:
+        monkeypatch.setattr(_C, "_binding", None)
+    x = torch.randn(40, 16, generator=gen(1)).cuda()
+    negative = torch._neg_view(x)
+    assert torch.equal(route_tokens(negative, 3)[0], route_tokens(-x, 3)[0])
+    ids = torch.zeros(40, 2, dtype=torch.int64, device="cuda")
+    rows, order = sort_tokens(negative, ids, 2, alignment=16)
+    assert torch.equal(rows, sort_tokens(-x, ids, 2, alignment=16)[0])
+    w = torch.rand(40, 2, generator=gen(2)).cuda()
+    assert torch.equal(unsort_tokens(torch._neg_view(rows), order, w), unsort_tokens(-rows, order, w))
+    assert torch.equal(unsort_tokens(rows, order, torch._neg_view(w)), unsort_tokens(rows, order, -w))
+    h = x.half()
+    b = torch.randn(40, generator=gen(3)).half().cuda()
+    r = torch.randn(40, 40, generator=gen(3)).half().cuda()
+    n = torch._neg_view
+    assert torch.equal(linear(n(h), h, n(b), n(r)), linear(-h, h, -b, -r)) and torch.equal(linear(h, n(h)), linear(h, -h))
+    leaf = h.clone().requires_grad_()
+    y = linear(leaf, h)
+    assert torch.equal(torch.autograd.grad(y, leaf, n(r), retain_graph=True)[0], torch.autograd.grad(y, leaf, -r)[0])
