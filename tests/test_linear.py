@@ -554,3 +554,19 @@ def test_sums_over_very_many_tokens(dtype, tokens, n, k):
     step = 2.0 ** (torch.floor(torch.log2(want)) - {torch.float16: 10, torch.bfloat16: 7}[dtype])
     worst = ((dw.double() - want).abs() - (0.5 * step + error))
     assert worst.max() <= 0
+
+
+@gpu
+@pytest.mark.parametrize("m, n, k", [(1, 300, 4096), (2, 64, 20000), (1, 1000, 20000), (5, 200, 4096), (40, 500, 20000), (300, 128, 4096), (700, 1024, 4096), (3000, 128, 20000),
+                                     (3000, 3001, 4096), (16384, 128, 4096)])
+def test_fp32_outputs_are_sums_of_short_sums(m, n, k):
+    """Operands of one sign: nothing cancels, and a sum that stayed in the tensor core's accumulator, or lost a part, would show (BF16 products are
+    cut by 1.9e-9 of the sum each, FP16 ones by 6e-9: 8e-6 and more for K = 4096)."""
+    g = torch.Generator("cuda").manual_seed(m)
+    few = m <= 2 and n * k <= 5 << 20                                     # without tensor cores: a lane's chain of K / 32 products at most
+    error = (k / 64 + 16) * 2.0 ** -24 if few else 8 * 2.0 ** -22 + (k / 512 + 12) * 2.0 ** -24      # 16 steps of 16, K / 256 sums, up to eight CTAs' sums
+    for dtype in (torch.bfloat16, torch.float16):
+        x = (torch.rand(m, k, generator=g, device="cuda") + 0.5).to(dtype)
+        w = (torch.rand(n, k, generator=g, device="cuda") + 0.5).to(dtype)
+        want = x.double() @ w.double().t()
+        assert ((linear(x, w, out_dtype=torch.float32).double() - want).abs() / want).max() <= error
