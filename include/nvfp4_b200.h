@@ -382,6 +382,9 @@ NVFP4_API int nvfp4_unsort_tokens_backward(const void* dy, int64_t ldy_elems, co
  *   that are multiples of 8, N rounded up to 8 at least; what lies behind column N of dz's rows up to there is overwritten.  dz or db
  *   may be NULL.
  * nvfp4_linear_dx: dx[M,K] = dz w.      nvfp4_linear_dw: dw[N,K] = dz^T x.      Rounded to `dtype`.
+ * ..._scaled: the same with a power of two between dz and the products, for FP32 gradients of FP16 operands, which may lie outside of FP16.
+ *   nvfp4_linear_dz_scaled writes that power to *scale, a float on the device, and dz over it: 1 where the largest finite |dz| is in
+ *   [1/4, 65504], else what brings it to [2^14, 2^15); the products take `scale` and multiply their sums by *scale.  NULL: as without.
  * An FP32 output takes partial sums of 256 products out of the tensor cores and adds them as FP32; a 16-bit output does so every 1024
  * products where there are more than 16384 (FP16) or 262144 (BF16) to a sum of a thread block; fewer stay in their accumulator.
  * device_status (may be NULL) receives bit 0 if a bounded wait expired; what was not finished then is NaN.  No counterparts in the
@@ -395,6 +398,12 @@ NVFP4_API int nvfp4_linear_dx(const void* dz, int64_t lddz_elems, const void* w,
                               int K, int dtype, int32_t* device_status, void* stream);
 NVFP4_API int nvfp4_linear_dw(const void* dz, int64_t lddz_elems, const void* x, int64_t ldx_elems, void* dw, int64_t lddw_elems, int M, int N,
                               int K, int dtype, int32_t* device_status, void* stream);
+NVFP4_API int nvfp4_linear_dz_scaled(const void* dd, int64_t ldd_elems, const int16_t* slopes, int64_t lds_elems, void* dz, int64_t lddz_elems, void* db,
+                                     int M, int N, int dtype, int out_dtype, float* scale, void* stream);
+NVFP4_API int nvfp4_linear_dx_scaled(const void* dz, int64_t lddz_elems, const void* w, int64_t ldw_elems, void* dx, int64_t lddx_elems, int M, int N,
+                                     int K, int dtype, const float* scale, int32_t* device_status, void* stream);
+NVFP4_API int nvfp4_linear_dw_scaled(const void* dz, int64_t lddz_elems, const void* x, int64_t ldx_elems, void* dw, int64_t lddw_elems, int M, int N,
+                                     int K, int dtype, const float* scale, int32_t* device_status, void* stream);
 
 /* Test hook: Algorithm 1 exactly as the GEMM's transform warps run it (same device
  * code, same shared-memory layouts), with the codes copied out instead of being fed to

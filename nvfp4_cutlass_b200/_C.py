@@ -48,7 +48,8 @@ EXPORTS = ("nvfp4_last_error", "nvfp4_version", "nvfp4_get_num_sms", "nvfp4_set_
            "nvfp4_grouped_gemm_swiglu_contiguous", "nvfp4_grouped_gemm_masked", "nvfp4_load_checkpoint_weights",
            "nvfp4_read_status", "nvfp4_debug_split_workspace", "nvfp4_debug_wait_timeout", "nvfp4_debug_quantize_weight_expired", "nvfp4_plan_peer_masked", "nvfp4_plan_one_rank",
            "nvfp4_peer_barrier", "nvfp4_route_tokens", "nvfp4_route_tokens_backward", "nvfp4_sort_tokens", "nvfp4_unsort_tokens",
-           "nvfp4_unsort_tokens_backward", "nvfp4_linear", "nvfp4_linear_dz", "nvfp4_linear_dx", "nvfp4_linear_dw", "nvfp4_debug_linear_expired", "nvfp4_debug_unsort_expired")
+           "nvfp4_unsort_tokens_backward", "nvfp4_linear", "nvfp4_linear_dz", "nvfp4_linear_dx", "nvfp4_linear_dw", "nvfp4_linear_dz_scaled", "nvfp4_linear_dx_scaled", "nvfp4_linear_dw_scaled",
+           "nvfp4_debug_linear_expired", "nvfp4_debug_unsort_expired")
 
 
 def library_path() -> str:
@@ -110,6 +111,9 @@ def lib() -> ctypes.CDLL:
         L.nvfp4_linear_dz.argtypes = [vp, i64, vp, i64, vp, i64, vp, i32, i32, i32, i32, vp]
         L.nvfp4_linear_dx.argtypes = [vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp]
         L.nvfp4_linear_dw.argtypes = [vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp]
+        L.nvfp4_linear_dz_scaled.argtypes = [vp, i64, vp, i64, vp, i64, vp, i32, i32, i32, i32, vp, vp]
+        L.nvfp4_linear_dx_scaled.argtypes = [vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp, vp]
+        L.nvfp4_linear_dw_scaled.argtypes = [vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp, vp]
         _contiguous_call = _bind(L)
         _lib = L                                     # last: another thread that finds it set makes its call at once
     return _lib
@@ -130,8 +134,8 @@ def _bind(library):
     address = lambda entry: ctypes.cast(entry, ctypes.c_void_p).value
     binding.bind(address(library.nvfp4_grouped_gemm_contiguous))
     binding.bind_operators(*(address(getattr(library, "nvfp4_" + name)) for name in (
-        "last_error", "route_tokens", "route_tokens_backward", "sort_tokens", "unsort_tokens", "unsort_tokens_backward", "linear", "linear_dz",
-        "linear_dx", "linear_dw")))
+        "last_error", "route_tokens", "route_tokens_backward", "sort_tokens", "unsort_tokens", "unsort_tokens_backward", "linear", "linear_dz_scaled",
+        "linear_dx_scaled", "linear_dw_scaled")))
     _binding = binding
     return binding.contiguous
 
@@ -895,17 +899,20 @@ def linear_backward(dd: torch.Tensor, x, w, slopes, dtype: torch.dtype, want_bia
     if products and not as_it_is:
         dz = _padded(m, n, dtype, dev)
         ldz = dz.shape[1]
+    # an FP32 gradient may lie outside of FP16
+    scale = torch.empty(1, dtype=torch.float32, device=dev) if products and dtype == torch.float16 and dd.dtype == torch.float32 else None
+    factor = scale.data_ptr() if scale is not None else None
     with _on(dev):
         if want_bias or (products and not as_it_is):
-            _check(lib().nvfp4_linear_dz(dd.data_ptr(), ldd, slopes.data_ptr() if slopes is not None else None, slopes.shape[1] if slopes is not None else 0,
-                                         None if as_it_is or not products else dz.data_ptr(), ldz, db.data_ptr() if want_bias else None, m, n,
-                                         code, DTYPE_CODES[dd.dtype], _stream()))
+            _check(lib().nvfp4_linear_dz_scaled(dd.data_ptr(), ldd, slopes.data_ptr() if slopes is not None else None, slopes.shape[1] if slopes is not None else 0,
+                                                None if as_it_is or not products else dz.data_ptr(), ldz, db.data_ptr() if want_bias else None, m, n,
+                                                code, DTYPE_CODES[dd.dtype], factor, _stream()))
         if w is not None:
-            _check(lib().nvfp4_linear_dx(dz.data_ptr(), ldz, w.data_ptr(), _operand(w, "w"), dx.data_ptr(), dx.shape[1], m, n, dx.shape[1], code, status,
-                                         _stream()))
+            _check(lib().nvfp4_linear_dx_scaled(dz.data_ptr(), ldz, w.data_ptr(), _operand(w, "w"), dx.data_ptr(), dx.shape[1], m, n, dx.shape[1], code,
+                                                factor, status, _stream()))
         if x is not None:
-            _check(lib().nvfp4_linear_dw(dz.data_ptr(), ldz, x.data_ptr(), _operand(x, "x"), dw.data_ptr(), dw.shape[1], m, n, dw.shape[1], code, status,
-                                         _stream()))
+            _check(lib().nvfp4_linear_dw_scaled(dz.data_ptr(), ldz, x.data_ptr(), _operand(x, "x"), dw.data_ptr(), dw.shape[1], m, n, dw.shape[1], code,
+                                                factor, status, _stream()))
     return dx, dw, db
 
 

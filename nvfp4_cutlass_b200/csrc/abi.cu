@@ -946,13 +946,16 @@ int nvfp4_debug_linear_expired(const void* x, int64_t ldx_elems, const void* w, 
                   device_status, stream, budget_cycles, withhold_residuals != 0);
 }
 
-int nvfp4_linear_dz(const void* dd, int64_t ldd_elems, const int16_t* slopes, int64_t lds_elems, void* dz, int64_t lddz_elems, void* db, int M, int N,
-                    int dtype, int out_dtype, void* stream)
+int nvfp4_linear_dz_scaled(const void* dd, int64_t ldd_elems, const int16_t* slopes, int64_t lds_elems, void* dz, int64_t lddz_elems, void* db, int M, int N,
+                           int dtype, int out_dtype, float* scale, void* stream)
 {
     host::clear_error();
     if (int rc = check_linear(M, N, 8, dtype)) return rc;
     NVFP4_REQUIRE(out_dtype == dtype || out_dtype == NVFP4_DTYPE_F32, "the output has the operands' type or FP32 (type codes %d, %d)", out_dtype, dtype);
+    NVFP4_REQUIRE(scale == nullptr || (dtype == NVFP4_DTYPE_F16 && out_dtype == NVFP4_DTYPE_F32), "a scale goes with FP16 operands and an FP32 gradient");
     if (M == 0 || N == 0 || (dz == nullptr && db == nullptr)) return NVFP4_OK;
+    NVFP4_REQUIRE(on_elements(scale, NVFP4_DTYPE_F32), "scale is not aligned to its type");
+    NVFP4_REQUIRE(scale == nullptr || dz != nullptr, "a scale goes with dz");
     const int64_t padded = (static_cast<int64_t>(N) + 7) / 8 * 8;
     NVFP4_REQUIRE(dd != nullptr && ldd_elems >= N && on_elements(dd, out_dtype), "dd is null, not aligned to its type, or its rows overlap");
     NVFP4_REQUIRE(on_elements(db, dtype), "db is not aligned to its type");
@@ -962,12 +965,17 @@ int nvfp4_linear_dz(const void* dd, int64_t ldd_elems, const int16_t* slopes, in
         if (int rc = check_operand("dz", dz, lddz_elems, padded)) return rc;
     host::DeviceInfo* dev;
     if (int rc = tensor_core_device(&dev)) return rc;
-    return launch_linear_dz(dd, ldd_elems, out_dtype == NVFP4_DTYPE_F32, slopes, lds_elems, dz, lddz_elems, db, M, N, dtype == NVFP4_DTYPE_BF16, dev->hw_sms,
+    return launch_linear_dz(dd, ldd_elems, out_dtype == NVFP4_DTYPE_F32, slopes, lds_elems, dz, lddz_elems, db, M, N, dtype == NVFP4_DTYPE_BF16, scale, dev->hw_sms,
                             static_cast<cudaStream_t>(stream));
 }
+int nvfp4_linear_dz(const void* dd, int64_t ldd_elems, const int16_t* slopes, int64_t lds_elems, void* dz, int64_t lddz_elems, void* db, int M, int N,
+                    int dtype, int out_dtype, void* stream)
+{
+    return nvfp4_linear_dz_scaled(dd, ldd_elems, slopes, lds_elems, dz, lddz_elems, db, M, N, dtype, out_dtype, nullptr, stream);
+}
 
-int nvfp4_linear_dx(const void* dz, int64_t lddz_elems, const void* w, int64_t ldw_elems, void* dx, int64_t lddx_elems, int M, int N, int K, int dtype,
-                    int32_t* device_status, void* stream)
+int nvfp4_linear_dx_scaled(const void* dz, int64_t lddz_elems, const void* w, int64_t ldw_elems, void* dx, int64_t lddx_elems, int M, int N, int K, int dtype,
+                           const float* scale, int32_t* device_status, void* stream)
 {
     host::clear_error();
     if (int rc = check_linear(M, N, K, dtype)) return rc;
@@ -978,12 +986,17 @@ int nvfp4_linear_dx(const void* dz, int64_t lddz_elems, const void* w, int64_t l
     NVFP4_REQUIRE(dx != nullptr && lddx_elems >= K && on_elements(dx, dtype), "dx is null, not aligned to its type, or its rows overlap");
     host::DeviceInfo* dev;
     if (int rc = tensor_core_device(&dev)) return rc;
-    return launch_linear_dx(dz, lddz_elems, w, ldw_elems, dx, lddx_elems, M, N, K, dtype == NVFP4_DTYPE_BF16, device_status, dev->num_sms,
+    return launch_linear_dx(dz, lddz_elems, w, ldw_elems, dx, lddx_elems, M, N, K, dtype == NVFP4_DTYPE_BF16, scale, device_status, dev->num_sms,
                             static_cast<cudaStream_t>(stream));
 }
-
-int nvfp4_linear_dw(const void* dz, int64_t lddz_elems, const void* x, int64_t ldx_elems, void* dw, int64_t lddw_elems, int M, int N, int K, int dtype,
+int nvfp4_linear_dx(const void* dz, int64_t lddz_elems, const void* w, int64_t ldw_elems, void* dx, int64_t lddx_elems, int M, int N, int K, int dtype,
                     int32_t* device_status, void* stream)
+{
+    return nvfp4_linear_dx_scaled(dz, lddz_elems, w, ldw_elems, dx, lddx_elems, M, N, K, dtype, nullptr, device_status, stream);
+}
+
+int nvfp4_linear_dw_scaled(const void* dz, int64_t lddz_elems, const void* x, int64_t ldx_elems, void* dw, int64_t lddw_elems, int M, int N, int K, int dtype,
+                           const float* scale, int32_t* device_status, void* stream)
 {
     host::clear_error();
     if (int rc = check_linear(M, N, K, dtype)) return rc;
@@ -994,8 +1007,13 @@ int nvfp4_linear_dw(const void* dz, int64_t lddz_elems, const void* x, int64_t l
     NVFP4_REQUIRE(dw != nullptr && lddw_elems >= K && on_elements(dw, dtype), "dw is null, not aligned to its type, or its rows overlap");
     host::DeviceInfo* dev;
     if (int rc = tensor_core_device(&dev)) return rc;
-    return launch_linear_dw(dz, lddz_elems, x, ldx_elems, dw, lddw_elems, M, N, K, dtype == NVFP4_DTYPE_BF16, device_status, dev->num_sms,
+    return launch_linear_dw(dz, lddz_elems, x, ldx_elems, dw, lddw_elems, M, N, K, dtype == NVFP4_DTYPE_BF16, scale, device_status, dev->num_sms,
                             static_cast<cudaStream_t>(stream));
+}
+int nvfp4_linear_dw(const void* dz, int64_t lddz_elems, const void* x, int64_t ldx_elems, void* dw, int64_t lddw_elems, int M, int N, int K, int dtype,
+                    int32_t* device_status, void* stream)
+{
+    return nvfp4_linear_dw_scaled(dz, lddz_elems, x, ldx_elems, dw, lddw_elems, M, N, K, dtype, nullptr, device_status, stream);
 }
 
 int nvfp4_debug_decompose(const void* a, int64_t lda_elems, int M, int K, int scale_policy, void* q0, void* q1,

@@ -111,9 +111,9 @@ struct Entries {
     decltype(&nvfp4_unsort_tokens) unsort;
     decltype(&nvfp4_unsort_tokens_backward) unsort_backward;
     decltype(&nvfp4_linear) linear;
-    decltype(&nvfp4_linear_dz) linear_dz;
-    decltype(&nvfp4_linear_dx) linear_dx;
-    decltype(&nvfp4_linear_dw) linear_dw;
+    decltype(&nvfp4_linear_dz_scaled) linear_dz;
+    decltype(&nvfp4_linear_dx_scaled) linear_dx;
+    decltype(&nvfp4_linear_dw_scaled) linear_dw;
 } g_entry = {};
 
 // bind_operators(addresses of the entries in the order of Entries)
@@ -438,19 +438,22 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
             const bool as_it_is = !slopes.defined() && dd.scalar_type() == type && row_stride(dd) % 8 == 0 && reinterpret_cast<uintptr_t>(dd.data_ptr()) % 16 == 0;
             at::Tensor dz = as_it_is ? dd : products ? fresh(dd, type, {m, (n + 7) / 8 * 8}) : at::Tensor();
             const int64_t ldz = dz.defined() ? row_stride(dz) : 0;
+            // an FP32 gradient may lie outside of FP16
+            const at::Tensor scale = products && type == at::kHalf && dd.scalar_type() == at::kFloat ? fresh(dd, at::kFloat, {1}) : at::Tensor();
             if (want_bias) out[2] = fresh(dd, type, {n});
             if (want_bias || (products && !as_it_is))
                 check(g_entry.linear_dz(dd.data_ptr(), row_stride(dd), pointer<int16_t>(slopes), slopes.defined() ? slopes.size(1) : 0,
-                                        as_it_is ? nullptr : pointer<void>(dz), ldz, pointer<void>(out[2]), m, n, code, dtype_code(dd.scalar_type()), stream()));
+                                        as_it_is ? nullptr : pointer<void>(dz), ldz, pointer<void>(out[2]), m, n, code, dtype_code(dd.scalar_type()),
+                                        pointer<float>(scale), stream()));
             if (want_x) {
                 out[0] = fresh(dd, type, {m, w.size(1)});
                 check(g_entry.linear_dx(dz.data_ptr(), ldz, w.data_ptr(), row_stride(w), out[0].data_ptr(), w.size(1), m, n, static_cast<int>(w.size(1)), code,
-                                        nullptr, stream()));
+                                        pointer<float>(scale), nullptr, stream()));
             }
             if (want_w) {
                 out[1] = fresh(dd, type, {n, x.size(1)});
                 check(g_entry.linear_dw(dz.data_ptr(), ldz, x.data_ptr(), row_stride(x), out[1].data_ptr(), x.size(1), m, n, static_cast<int>(x.size(1)), code,
-                                        nullptr, stream()));
+                                        pointer<float>(scale), nullptr, stream()));
             }
         }
         return once(std::move(out));

@@ -71,11 +71,11 @@ int launch_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const 
                   int16_t* slopes, int64_t lds, int M, int N, int K, bool bf16, bool out32, int activation, int32_t* status, int num_sms,
                   cudaStream_t stream, int64_t budget = 0, bool withhold_residuals = false);
 int launch_linear_dz(const void* dd, int64_t ldd, bool dd32, const int16_t* slopes, int64_t lds, void* dz, int64_t lddz, void* db, int M, int N,
-                     bool bf16, int num_sms, cudaStream_t stream);
-int launch_linear_dx(const void* dz, int64_t lddz, const void* w, int64_t ldw, void* dx, int64_t lddx, int M, int N, int K, bool bf16, int32_t* status,
-                     int num_sms, cudaStream_t stream);
-int launch_linear_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, void* dw, int64_t lddw, int M, int N, int K, bool bf16, int32_t* status,
-                     int num_sms, cudaStream_t stream);
+                     bool bf16, float* scale, int num_sms, cudaStream_t stream);
+int launch_linear_dx(const void* dz, int64_t lddz, const void* w, int64_t ldw, void* dx, int64_t lddx, int M, int N, int K, bool bf16,
+                     const float* scale, int32_t* status, int num_sms, cudaStream_t stream);
+int launch_linear_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, void* dw, int64_t lddw, int M, int N, int K, bool bf16,
+                     const float* scale, int32_t* status, int num_sms, cudaStream_t stream);
 
 int launch_gemm_swap(const void* a, int64_t lda, const void* b, const void* sfb, const float* gw, void* d,
                      int64_t ldd, const int32_t* m_indices, int M, int N, int K, int E, bool residual,

@@ -138,15 +138,7 @@ __device__ __forceinline__ void activate2(float2 z, float2& y, float2& slope)
 //          FP16(slope * 2^20), off by 2^-11 of the slope down to 2^-34 and by 2^-45 below.
 // Small positive slopes lie beside the one zero of the slope, where z's own rounding counts as much, and stay in the first form.
 constexpr float kSlopeScale = 16384.0f, kSlopeShift = 12582912.0f + 8192.0f, kTailScale = 1048576.0f, kTailLimit = -65216.0f;
-template <int kAct>
-__device__ __forceinline__ int16_t slope_code(float s)
-{
-    const __half tail = __float2half_rn(s * kTailScale);
-    if (kAct != NVFP4_ACTIVATION_RELU && __hlt(tail, __float2half_rn(0.0f)) && __hgt(tail, __float2half_rn(kTailLimit)))
-        return static_cast<int16_t>(__half_as_ushort(tail));
-    return static_cast<int16_t>(__float_as_uint(fmaf(s, kSlopeScale, kSlopeShift)));
-}
-// Two of them, with masks from comparisons of two halves at once: a training step of 8192 x 4096 x 512 with silu takes 178 us in a graph (183
+// Codes of two slopes, by masks from comparisons of two halves at once: a training step of 8192 x 4096 x 512 with silu takes 178 us in a graph (183
 // with values compared and selected one by one, 170 without the second form).
 template <int kAct>
 __device__ __forceinline__ uint32_t slope_codes(float2 s)
@@ -186,6 +178,7 @@ struct Epilogue {
     const void* residual; int64_t ldr;               // of d's type, or NULL
     uint32_t rows, cols;
     int activation;
+    const float* scale;                              // what the sums are multiplied by, or NULL: see linear_dz_kernel
     bool staged;                                     // rows of d, residual and slopes are multiples of 16 bytes: see Stage
 };
 
@@ -195,7 +188,7 @@ struct Epilogue {
 // 4096 x 4096 took 465 us in place of the 184 without a residual).  All of them are plain loads: __ldg is an asm statement that the
 // compiler may move, and it was moved ahead of the test for a NULL bias, out of the loop over a tile's columns.
 template <typename T, typename D, uint32_t kN>
-__device__ __forceinline__ void finish(float (&v)[kN], uint32_t row0, uint32_t count, uint32_t col, const Epilogue& e)
+__device__ __forceinline__ void finish(float (&v)[kN], uint32_t row0, uint32_t count, uint32_t col, const Epilogue& e, float factor)
 {
     if (row0 >= e.rows || count == 0) return;
     const uint32_t rows = min(count, e.rows - row0), last = rows - 1, at = min(col, e.cols - 1);
@@ -205,6 +198,10 @@ __device__ __forceinline__ void finish(float (&v)[kN], uint32_t row0, uint32_t c
         const D* from = static_cast<const D*>(e.residual) + static_cast<int64_t>(row0) * e.ldr + at;
 #pragma unroll
         for (uint32_t i = 0; i < kN; ++i) r[i] = from[static_cast<int64_t>(min(i, last)) * e.ldr];
+    }
+    if (factor != 1.0f) {
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i) v[i] *= factor;
     }
     if (e.bias != nullptr) {
         const float b = to_float(static_cast<const T*>(e.bias)[at]);
@@ -232,8 +229,9 @@ __device__ __forceinline__ void finish(float (&v)[kN], uint32_t row0, uint32_t c
 #pragma unroll
                 for (uint32_t i = 0; i < kN; i += 2) {
                     two(i, slope, std::true_type{});
-                    if (i < rows && mine) to[i * e.lds] = slope_code<kAct>(slope.x);
-                    if (i + 1 < rows && mine) to[(i + 1) * e.lds] = slope_code<kAct>(slope.y);
+                    const uint32_t codes = slope_codes<kAct>(slope);
+                    if (i < rows && mine) to[i * e.lds] = static_cast<int16_t>(codes);
+                    if (i + 1 < rows && mine) to[(i + 1) * e.lds] = static_cast<int16_t>(codes >> 16);
                 }
             } else {
 #pragma unroll
@@ -324,6 +322,7 @@ struct Stage {
     uint32_t phase = 0;
     const Maps* maps;
     long long budget;                                // of a wait, in cycles
+    float factor;                                    // *e.scale, where there is one (read in front of every box it took 5 of a call's 28 us)
     uint32_t requested = 0;                          // boxes whose residual is under way
     bool withhold = false;                           // test of the expired wait: residuals are not asked for
 
@@ -390,6 +389,14 @@ struct Stage {
             uint32_t b[16];
             if (e.bias != nullptr) load_bias(e, col + half * 32, b);
             load_accumulators(taddr + half * 32, v);
+            if (factor != 1.0f) {
+#pragma unroll
+                for (uint32_t i = 0; i < 32; i += 2) {
+                    const float2 f = ptx::mul_f32x2(make_float2(v[i], v[i + 1]), both(factor));
+                    v[i] = f.x;
+                    v[i + 1] = f.y;
+                }
+            }
             if (e.bias != nullptr) {
 #pragma unroll
                 for (uint32_t i = 0; i < 16; ++i) {
@@ -591,6 +598,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         if (++r.slot == depth) { r.slot = 0; r.phase ^= 1; }
     };
     const uint32_t quad = warp & 3, row = quad * 32 + lane;                   // epilogue: the warp's quarter of the lanes
+    const float factor = e.scale != nullptr ? *e.scale : 1.0f;
     const uint32_t taddr = tmem + ((quad * 32) << 16);
     if (warp == 0) {
         const uint32_t issue = ptx::elect_one();
@@ -678,10 +686,10 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     const uint32_t live = kSwap ? min(BN, e.rows - b0) : min(BN, e.cols - b0);          // columns of the tile that anybody wants
     auto give = [&](float (&v)[kChunk], uint32_t column, uint32_t count) {    // columns [column, column + count) of the tile
         if constexpr (kSwap) {
-            finish<T, D>(v, b0 + column, count, a0 + row, e);
+            finish<T, D>(v, b0 + column, count, a0 + row, e, factor);
         } else {
             transpose(v, lane);
-            finish<T, D>(v, a0 + quad * 32, 32, b0 + column + lane, e);
+            finish<T, D>(v, a0 + quad * 32, 32, b0 + column + lane, e, factor);
         }
     };
     if (splits > 1) {
@@ -753,7 +761,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                 // two of the output and two of the slopes
                 constexpr uint32_t kColumns = kBox<D>;
                 const uint32_t at = smem + (warp - 2) * 4 * kBoxBytes, row0 = a0 + quad * 32;
-                Stage<T, D> stage{at, kBoxBytes, at + 2 * kBoxBytes, kBoxBytes, landed + 4 * (warp - 2), 0, &maps, p.budget, 0, p.withhold == kResiduals};
+                Stage<T, D> stage{at, kBoxBytes, at + 2 * kBoxBytes, kBoxBytes, landed + 4 * (warp - 2), 0, &maps, p.budget, factor, 0, p.withhold == kResiduals};
                 if (row0 < e.rows) {
                     if (e.residual != nullptr)
                         for (uint32_t c = 0; c < live; c += kColumns) stage.request(c / kColumns, b0 + c, row0, lane);
@@ -844,13 +852,14 @@ token_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int6
     if (!mine || share != 0 || lane >= kTokens) return;
     float z = 0.0f;
     for (uint32_t i = 0; i < warps; ++i) z += part[warp + i][lane];
+    if (e.scale != nullptr) z *= *e.scale;
     if (e.bias != nullptr) z += to_float(static_cast<const T*>(e.bias)[n]);
     float y = z;
     with_activation(e.activation, [&](auto act) {
         constexpr int kAct = decltype(act)::value;
         float slope = 1.0f;
         activate<kAct, true>(z, y, slope);
-        if (e.slopes != nullptr) e.slopes[lane * e.lds + n] = slope_code<kAct>(slope);
+        if (e.slopes != nullptr) e.slopes[lane * e.lds + n] = static_cast<int16_t>(slope_codes<kAct>(both(slope)));
     });
     if (e.residual != nullptr) y += to_float(static_cast<const D*>(e.residual)[lane * e.ldr + n]);
     static_cast<D*>(e.d)[lane * e.ldd + n] = from_float<D>(y);
@@ -977,8 +986,9 @@ product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         const uint32_t tmem_empty_even = ptx::map_to_cta(ptx::smem_u32(tmem_empty), 0);
         const uint32_t boxes = smem + kOffBoxes + (warp - kPairFirstEpi) * 2 * kBoxBytes;
         const bool both = e.slopes != nullptr;       // the second buffer takes the slopes
+        const float factor = e.scale != nullptr ? *e.scale : 1.0f;
         constexpr uint32_t kBoxColumns = kBox<T>;
-        Stage<T, T> stage{boxes, both ? 0u : kBoxBytes, boxes + kBoxBytes, 0u, landed + 2 * (warp - kPairFirstEpi), 0, &maps, p.budget, 0, p.withhold == kResiduals};
+        Stage<T, T> stage{boxes, both ? 0u : kBoxBytes, boxes + kBoxBytes, 0u, landed + 2 * (warp - kPairFirstEpi), 0, &maps, p.budget, factor, 0, p.withhold == kResiduals};
         uint32_t n = 0;
         for (uint32_t tile = pair_id; tile < tiles; tile += num_pairs, ++n) {
             const uint32_t acc = n & 1;
@@ -1020,7 +1030,7 @@ product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                         for (uint32_t i = 0; i < 32; ++i) v[i] = kNan;
                     }
                     transpose(v, lane);
-                    finish<T, T>(v, row0, 32, col0 + c + lane, e);
+                    finish<T, T>(v, row0, 32, col0 + c + lane, e, factor);
                 }
             }
             if (!ok) continue;
@@ -1248,17 +1258,44 @@ int launch_product(const Operands& o, const Epilogue& e, int num_sms, cudaStream
 // dz = dd * activation'(z), rounded once for the tensor cores, and per block of rows the sums of its columns before that rounding.
 // A thread takes eight columns (16 bytes of the slopes and of dz, whose rows are padded to that) of every eighth row of its block's; a
 // block 256 columns.  One pass over dd and the slopes, bound by their bytes.
+// FP32 gradients of FP16 operands may lie outside of FP16: those of a mean over many tokens below its smallest number, where dz would be
+// zero, others above its largest.  So every block leaves its largest finite |dz| in `peaks`, and a second pass, which is over at once if the
+// largest of all is in [1/4, 65504], writes dz times a power of two that brings that to [2^14, 2^15), so that what is lost is 2^-39 of the
+// largest; the products multiply their sums by that power's inverse, *scale.  (Training step of 4096 x 2048 x 2048 with silu in a graph: 158 -> 165 us
+// with gradients that FP16 holds.)
+__device__ __forceinline__ float dz_factor(float most)
+{
+    if (most == 0.0f || (most >= 0.25f && most <= 65504.0f)) return 1.0f;
+    const int exponent = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -112);      // at most 2^126: its inverse is no subnormal number
+    return __uint_as_float(static_cast<uint32_t>(127 + 14 - exponent) << 23);
+}
 constexpr int kGradThreads = 256, kGradColumns = 256, kGradRowLanes = 8;
-template <typename T, typename D>
+// kAgain: the second pass.
+template <typename T, typename D, bool kAgain>
 __global__ void __launch_bounds__(kGradThreads)
 linear_dz_kernel(const D* __restrict__ dd, int64_t ldd, bool wide, const int16_t* __restrict__ slopes, int64_t lds, T* __restrict__ dz, int64_t lddz, uint32_t rows,
-                 uint32_t cols, uint32_t rows_each, float* __restrict__ sums)
+                 uint32_t cols, uint32_t rows_each, float* __restrict__ sums, float* __restrict__ peaks, float* __restrict__ scale)
 {
     __shared__ float part[kGradRowLanes][kGradColumns];
     const uint32_t group = threadIdx.x % 32, row_lane = threadIdx.x / 32;
     const uint32_t col0 = blockIdx.x * kGradColumns + group * 8;
     const uint32_t first = blockIdx.y * rows_each, last = min(rows, first + rows_each);
     ptx::grid_dependency_wait();
+    float factor = 1.0f, most = 0.0f;
+    __shared__ uint32_t largest[kGradRowLanes];
+    // the largest of the block's numbers, none of them negative: their bits are in their order
+    auto largest_of_block = [&](float v) {
+        const uint32_t bits = __reduce_max_sync(kAll, __float_as_uint(v));
+        if (threadIdx.x % 32 == 0) largest[row_lane] = bits;
+        __syncthreads();
+        return __uint_as_float(__reduce_max_sync(kAll, largest[threadIdx.x % kGradRowLanes]));
+    };
+    if constexpr (kAgain) {
+        for (uint32_t i = threadIdx.x; i < gridDim.x * gridDim.y; i += kGradThreads) most = fmaxf(most, peaks[i]);
+        factor = dz_factor(largest_of_block(most));
+        if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *scale = 1.0f / factor;
+        if (factor == 1.0f) return;
+    }
     float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (col0 < cols) {
         const uint32_t here = min(8u, cols - col0);
@@ -1280,12 +1317,18 @@ linear_dz_kernel(const D* __restrict__ dd, int64_t ldd, bool wide, const int16_t
                 float v = to_float(g[i]);
                 if (slopes != nullptr) v *= unpack_slope(code[i]);
                 sum[i] += v;
+                if constexpr (kAgain) v *= factor;
+                else if (fabsf(v) < INFINITY && i < here) most = fmaxf(most, fabsf(v));
                 out[i] = from_float<T>(v);
             }
             if (dz != nullptr) *reinterpret_cast<uint4*>(dz + static_cast<int64_t>(r) * lddz + col0) = *reinterpret_cast<const uint4*>(out);
         }
     }
-    if (sums == nullptr) return;
+    if (!kAgain && peaks != nullptr) {
+        const float top = largest_of_block(most);
+        if (threadIdx.x == 0) peaks[blockIdx.y * gridDim.x + blockIdx.x] = top;
+    }
+    if (kAgain || sums == nullptr) return;
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) part[row_lane][group * 8 + i] = sum[i];
     __syncthreads();
@@ -1309,8 +1352,8 @@ linear_db_kernel(const float* __restrict__ sums, uint32_t blocks, uint32_t cols,
 }
 
 template <typename T, typename D>
-int launch_dz(const void* dd, int64_t ldd, const int16_t* slopes, int64_t lds, void* dz, int64_t lddz, void* db, uint32_t rows, uint32_t cols, int num_sms,
-              cudaStream_t stream)
+int launch_dz(const void* dd, int64_t ldd, const int16_t* slopes, int64_t lds, void* dz, int64_t lddz, void* db, uint32_t rows, uint32_t cols, float* scale,
+              int num_sms, cudaStream_t stream)
 {
     const unsigned columns = (cols + kGradColumns - 1) / kGradColumns;
     // about four blocks to an SM, at least eight rows to a block
@@ -1319,22 +1362,28 @@ int launch_dz(const void* dd, int64_t ldd, const int16_t* slopes, int64_t lds, v
     rows_each = (rows_each + kGradRowLanes - 1) / kGradRowLanes * kGradRowLanes;
     blocks = (rows + rows_each - 1) / rows_each;
     const bool wide = ((reinterpret_cast<uintptr_t>(dd) | static_cast<uintptr_t>(ldd * sizeof(D))) & 15u) == 0 && cols % 8 == 0;
-    float* sums = nullptr;
-    if (db != nullptr) {
+    float *workspace = nullptr, *sums = nullptr, *peaks = nullptr;
+    const size_t sum_words = db != nullptr ? static_cast<size_t>(blocks) * cols : 0, peak_words = scale != nullptr ? static_cast<size_t>(blocks) * columns : 0;
+    if (sum_words + peak_words > 0) {
         int dev = 0;
         NVFP4_CUDA_CHECK(cudaGetDevice(&dev));
         cudaMemPool_t pool;
         if (int rc = host::workspace_pool(dev, &pool)) return rc;
-        NVFP4_CUDA_CHECK(cudaMallocFromPoolAsync(reinterpret_cast<void**>(&sums), static_cast<size_t>(blocks) * cols * sizeof(float), pool, stream));
+        NVFP4_CUDA_CHECK(cudaMallocFromPoolAsync(reinterpret_cast<void**>(&workspace), (sum_words + peak_words) * sizeof(float), pool, stream));
+        if (db != nullptr) sums = workspace;
+        if (scale != nullptr) peaks = workspace + sum_words;
     }
-    int rc = host::launch_kernel(linear_dz_kernel<T, D>, dim3(columns, blocks), dim3(kGradThreads), 0, stream, true, static_cast<const D*>(dd), ldd, wide,
-                                 slopes, lds, static_cast<T*>(dz), lddz, rows, cols, rows_each, sums);
-    if (db != nullptr) {
-        if (rc == NVFP4_OK)
-            rc = host::launch_kernel(linear_db_kernel<T>, dim3((cols + kGradThreads - 1) / kGradThreads), dim3(kGradThreads), 0, stream, true, sums,
-                                     blocks, cols, static_cast<T*>(db));
-        cudaFreeAsync(sums, stream);
-    }
+    const dim3 grid(columns, blocks);
+    int rc = host::launch_kernel(linear_dz_kernel<T, D, false>, grid, dim3(kGradThreads), 0, stream, true, static_cast<const D*>(dd), ldd, wide, slopes, lds,
+                                 static_cast<T*>(dz), lddz, rows, cols, rows_each, sums, peaks, scale);
+    if constexpr (std::is_same<T, __half>::value && std::is_same<D, float>::value)
+        if (rc == NVFP4_OK && scale != nullptr)
+            rc = host::launch_kernel(linear_dz_kernel<T, D, true>, grid, dim3(kGradThreads), 0, stream, true, static_cast<const D*>(dd), ldd, wide, slopes, lds,
+                                     static_cast<T*>(dz), lddz, rows, cols, rows_each, static_cast<float*>(nullptr), peaks, scale);
+    if (rc == NVFP4_OK && db != nullptr)
+        rc = host::launch_kernel(linear_db_kernel<T>, dim3((cols + kGradThreads - 1) / kGradThreads), dim3(kGradThreads), 0, stream, true, sums, blocks, cols,
+                                 static_cast<T*>(db));
+    if (workspace != nullptr) cudaFreeAsync(workspace, stream);
     return rc;
 }
 
@@ -1356,34 +1405,34 @@ int launch_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const 
         o.withhold = withhold_residuals ? kResiduals : kProducts;
     }
     if (activation == NVFP4_ACTIVATION_NONE) slopes = nullptr;
-    const Epilogue e{d, ldd, slopes, lds, bias, residual, ldr, static_cast<uint32_t>(M), static_cast<uint32_t>(N), activation, false};
+    const Epilogue e{d, ldd, slopes, lds, bias, residual, ldr, static_cast<uint32_t>(M), static_cast<uint32_t>(N), activation, nullptr, false};
     return bf16 ? product<__nv_bfloat16>(o, e, out32, num_sms, stream) : product<__half>(o, e, out32, num_sms, stream);
 }
 
 int launch_linear_dz(const void* dd, int64_t ldd, bool dd32, const int16_t* slopes, int64_t lds, void* dz, int64_t lddz, void* db, int M, int N,
-                     bool bf16, int num_sms, cudaStream_t stream)
+                     bool bf16, float* scale, int num_sms, cudaStream_t stream)
 {
     const uint32_t m = static_cast<uint32_t>(M), n = static_cast<uint32_t>(N);
     if (bf16)
-        return dd32 ? launch_dz<__nv_bfloat16, float>(dd, ldd, slopes, lds, dz, lddz, db, m, n, num_sms, stream)
-                    : launch_dz<__nv_bfloat16, __nv_bfloat16>(dd, ldd, slopes, lds, dz, lddz, db, m, n, num_sms, stream);
-    return dd32 ? launch_dz<__half, float>(dd, ldd, slopes, lds, dz, lddz, db, m, n, num_sms, stream)
-                : launch_dz<__half, __half>(dd, ldd, slopes, lds, dz, lddz, db, m, n, num_sms, stream);
+        return dd32 ? launch_dz<__nv_bfloat16, float>(dd, ldd, slopes, lds, dz, lddz, db, m, n, scale, num_sms, stream)
+                    : launch_dz<__nv_bfloat16, __nv_bfloat16>(dd, ldd, slopes, lds, dz, lddz, db, m, n, scale, num_sms, stream);
+    return dd32 ? launch_dz<__half, float>(dd, ldd, slopes, lds, dz, lddz, db, m, n, scale, num_sms, stream)
+                : launch_dz<__half, __half>(dd, ldd, slopes, lds, dz, lddz, db, m, n, scale, num_sms, stream);
 }
 
-int launch_linear_dx(const void* dz, int64_t lddz, const void* w, int64_t ldw, void* dx, int64_t lddx, int M, int N, int K, bool bf16, int32_t* status,
-                     int num_sms, cudaStream_t stream)
+int launch_linear_dx(const void* dz, int64_t lddz, const void* w, int64_t ldw, void* dx, int64_t lddx, int M, int N, int K, bool bf16,
+                     const float* scale, int32_t* status, int num_sms, cudaStream_t stream)
 {
     const Operands o{dz, lddz, false, static_cast<uint32_t>(M), w, ldw, true, static_cast<uint32_t>(K), static_cast<uint32_t>(N), status};
-    const Epilogue e{dx, lddx, nullptr, 0, nullptr, nullptr, 0, static_cast<uint32_t>(M), static_cast<uint32_t>(K), NVFP4_ACTIVATION_NONE, false};
+    const Epilogue e{dx, lddx, nullptr, 0, nullptr, nullptr, 0, static_cast<uint32_t>(M), static_cast<uint32_t>(K), NVFP4_ACTIVATION_NONE, scale, false};
     return bf16 ? product<__nv_bfloat16>(o, e, false, num_sms, stream) : product<__half>(o, e, false, num_sms, stream);
 }
 
-int launch_linear_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, void* dw, int64_t lddw, int M, int N, int K, bool bf16, int32_t* status,
-                     int num_sms, cudaStream_t stream)
+int launch_linear_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, void* dw, int64_t lddw, int M, int N, int K, bool bf16,
+                     const float* scale, int32_t* status, int num_sms, cudaStream_t stream)
 {
     const Operands o{dz, lddz, true, static_cast<uint32_t>(N), x, ldx, true, static_cast<uint32_t>(K), static_cast<uint32_t>(M), status};
-    const Epilogue e{dw, lddw, nullptr, 0, nullptr, nullptr, 0, static_cast<uint32_t>(N), static_cast<uint32_t>(K), NVFP4_ACTIVATION_NONE, false};
+    const Epilogue e{dw, lddw, nullptr, 0, nullptr, nullptr, 0, static_cast<uint32_t>(N), static_cast<uint32_t>(K), NVFP4_ACTIVATION_NONE, scale, false};
     return bf16 ? product<__nv_bfloat16>(o, e, false, num_sms, stream) : product<__half>(o, e, false, num_sms, stream);
 }
 

@@ -46,7 +46,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
 
     Differentiable in x, w, bias and residual.  The backward pass keeps the activation's slope in 16 bits, off by 2^-15 at most and in the
     negative tails of gelu and silu by 2^-11 of itself, and rounds the gradient in front of the activation to the operands' type: the
-    tensor cores take no wider operands."""
+    tensor cores take no wider operands.  An FP32 gradient that FP16 operands cannot hold is brought into their range by a power of two
+    for the products, whose sums are multiplied by its inverse."""
     if _C._binding is not None and device_status is None and activation in _C.ACTIVATION_CODES and (out_dtype is None or out_dtype is torch.float32 or out_dtype is x.dtype):
         result = _C._binding.linear(x, w, bias, residual, _C.ACTIVATION_CODES[activation], 1 if out_dtype is torch.float32 else 0)
         if result is not None:

@@ -570,3 +570,68 @@ def test_fp32_outputs_are_sums_of_short_sums(m, n, k):
         w = (torch.rand(n, k, generator=g, device="cuda") + 0.5).to(dtype)
         want = x.double() @ w.double().t()
         assert ((linear(x, w, out_dtype=torch.float32).double() - want).abs() / want).max() <= error
+
+
+@gpu
+@pytest.mark.parametrize("binding", [True, False])
+@pytest.mark.parametrize("scale", [1e-9, 3e-20, 0.1, 1.0, 1e6, 1e9])
+@pytest.mark.parametrize("m, n, k", [(5, 24, 16), (300, 40, 64), (3000, 33, 72), (2700, 2056, 264)])
+def test_fp32_gradients_outside_of_fp16(m, n, k, scale, binding, monkeypatch):
+    """FP16 operands, an FP32 output and FP32 gradients that FP16 does not hold, while their sums times x or w are ordinary numbers."""
+    _C.lib()
+    if not binding:
+        monkeypatch.setattr(_C, "_binding", None)
+    g = gen(9)
+    dd = torch.randn(m, n, generator=g) * scale
+    big = min(max(2.0 / scale, 2.0 ** -10), 2.0 ** 9)                       # brings the terms of a sum towards 1
+    for activation in ("none", "silu"):
+        for which in ("dx", "dw"):
+            # the operand that the gradient meets is large (or small), the other one makes up for it in z
+            x, w = torch.randn(m, k, generator=g), torch.randn(n, k, generator=g)
+            x, w = (x / (big * k ** 0.5), w * big) if which == "dx" else (x * big, w / (big * k ** 0.5))
+            x, w, bias = x.half(), w.half(), torch.randn(n, generator=g).half()
+            leaves = [t.cuda().requires_grad_() for t in (x, w, bias)]
+            y = linear(*leaves, activation=activation, out_dtype=torch.float32)
+            dx, dw, db = torch.autograd.grad(y, leaves, dd.cuda())
+            z = (x.double() @ w.double().t() + bias.double()).requires_grad_()
+            (dz,) = torch.autograd.grad(act64(z, activation), z, dd.double())
+            z = z.detach()
+            slope = 0.0 if activation == "none" else 2.0 ** -15 + CURVATURE * (sum_error(x, w.t()) + z.abs() * 2.0 ** -23) + 64 * 2.0 ** -23
+            dz_error = dd.double().abs() * slope
+            # dz rounded to FP16 of a multiple whose largest is 1/4 at least: smaller than 2^-14 of that it loses up to 2^-25
+            rounded = dz_error + (dz.abs() + dz_error) * 1.01 * 2.0 ** -11 + 4 * 2.0 ** -25 * float(dz.abs().max())
+            for name, got, want, size, spread, terms in (("db", db, dz.sum(dim=0), dz.abs().sum(dim=0), dz_error.sum(dim=0), m),
+                                                         ("dx", dx, dz @ w.double(), dz.abs() @ w.double().abs(), rounded @ w.double().abs(), n),
+                                                         ("dw", dw, dz.t() @ x.double(), dz.abs().t() @ x.double().abs(), rounded.t() @ x.double().abs(), m)):
+                error = spread + size * (terms + 4) * 2.0 ** -23
+                ok = (got.cpu().double() - want).abs().le(error + (want.abs() + error) * 1.01 * 2.0 ** -11 + 2.0 ** -25)
+                held = want.abs() + error < 65000                         # a result beyond FP16 is an infinity, or its largest number
+                assert ok[held].all(), (name, activation, which)
+                assert (got.cpu().abs()[want.abs() - error > 65536] == math.inf).all()
+
+
+@gpu
+def test_infinite_gradients_stay_in_their_rows():
+    x, w, bias, _ = make(40, 24, 64, torch.float16, 3)
+    for scale in (1e-9, 1.0):
+        dd = torch.randn(40, 24, generator=gen(1)) * scale
+        clean = dd.clone()
+        dd[3, 5], dd[7, 2] = math.inf, math.nan
+        clean[3, 5] = clean[7, 2] = 0
+        leaves = [t.cuda().requires_grad_() for t in (x, w)]
+        y = linear(*leaves, out_dtype=torch.float32)
+        dx, dw = torch.autograd.grad(y, leaves, dd.cuda(), retain_graph=True)
+        want_x, want_w = torch.autograd.grad(y, leaves, clean.cuda())
+        rows, columns = torch.ones(40, dtype=torch.bool), torch.ones(24, dtype=torch.bool)
+        rows[[3, 7]] = False
+        columns[[5, 2]] = False
+        assert torch.equal(dx[rows], want_x[rows]) and torch.equal(dw[columns], want_w[columns])
+        assert torch.isnan(dx[7]).all() and not torch.isfinite(dx[3]).any() and not torch.isfinite(dw[2]).any()
+
+
+def test_scales_refuse():
+    lib = _C.lib()
+    assert "FP16 operands" in error_of(lib.nvfp4_linear_dz_scaled(1024, 32, 1024, 32, 1024, 32, None, 4, 32, 0, 1, 1024, None))
+    assert "FP16 operands" in error_of(lib.nvfp4_linear_dz_scaled(1024, 32, 1024, 32, 1024, 32, None, 4, 32, 2, 2, 1024, None))
+    assert "goes with dz" in error_of(lib.nvfp4_linear_dz_scaled(1024, 32, 1024, 32, None, 32, 1024, 4, 32, 2, 1, 1024, None))
+    assert "scale is not aligned" in error_of(lib.nvfp4_linear_dz_scaled(1024, 32, 1024, 32, 1024, 32, None, 4, 32, 2, 1, 1026, None))
