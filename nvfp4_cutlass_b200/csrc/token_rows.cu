@@ -585,61 +585,100 @@ RingShape ring_shape(int64_t tokens, int k, int64_t row_bytes)
 
 // Gradients of that sum: drows[r] = sum of w[t, j] * dy[t] over the pairs that name row r, dw[t, j] = <dy[t], rows[place[t, j]]>.
 // The sum takes any order that names rows, not the sort's alone: a part of its tokens, pairs dropped afterwards, one row for several
-// pairs.  So every row's pairs are counted first (a count does not depend on the atomics' order; 8192 x 8 pairs: with the clearing
-// of the counts 4 us of the 214).
+// pairs.  So a kernel in front makes a list of every row's pairs, in any order: head[r] is one of them, next[p] the one behind p, kNobody
+// ends it (8192 x 8 pairs: with the clearing of the heads 4 us of the 214).
 // A warp takes a pair: its dot product stays inside the warp, in a fixed order, and four packs a lane of the row and of dy are under way
 // at a time in few registers.  The pairs of a token are neighbouring warps', which read dy from L1 behind the first.  (A block to a token,
 // eight rows at a time to a thread, took 138 registers and ran at an eighth of the warps: 455 us for 8192 x 8 rows of 8 KB.)  A row that
 // this pair alone names is written on the way.
-// Behind the pairs: warps for the rows that none names (zero) or several do: those look their pairs up among all, in ascending order, FP32,
-// rounded once.  drows or dw may be NULL; rows is read for dw alone, named for drows.
+// Behind the pairs: warps for pieces of rows, four rows at a time (forward and backward of 8192 x 8 rows in a graph: 305 us; one row 338, eight
+// 306).  Those that nobody names are zeroed; those of several pairs get the sum in ascending pairs, FP32, rounded once: up to 32 pairs from
+// the list, more of them looked up among all pairs (every row named eight times: 0.28 ms in place of 0.21; a hundred times: 19 ms).
+// drows or dw may be NULL; rows is read for dw alone, head and next for drows.
 constexpr int kBackThreads = 256, kBackWarps = kBackThreads / 32;
+constexpr uint32_t kNobody = 0xffffffffu, kBackRows = 4;
+template <typename P>
+constexpr int kBackPer = P::kSize == 16 ? 4 : 8;                              // packs of a lane under way, or of a piece of a row
 __global__ void __launch_bounds__(kBackThreads)
-count_names_kernel(const int64_t* __restrict__ place, uint32_t pairs, uint32_t m, uint32_t* __restrict__ named)
+list_names_kernel(const int64_t* __restrict__ place, uint32_t pairs, uint32_t m, uint32_t* __restrict__ head, uint32_t* __restrict__ next)
 {
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
     for (uint64_t p = static_cast<uint64_t>(blockIdx.x) * kBackThreads + threadIdx.x; p < pairs; p += static_cast<uint64_t>(gridDim.x) * kBackThreads) {
         const int64_t r = place[p];
-        if (r >= 0 && r < m) atomicAdd(named + r, 1u);
+        if (r >= 0 && r < m) next[p] = atomicExch(head + r, static_cast<uint32_t>(p));
     }
+}
+// The gradient of row r, named by several pairs, in pack c of the lane (all lanes run this together, whether they have a pack or not).
+template <typename P>
+__device__ __forceinline__ typename P::Bits sum_of_names(const typename P::Bits* __restrict__ dy, int64_t ldy, const int64_t* __restrict__ place,
+                                                         const uint32_t* __restrict__ next, uint32_t first, const float* __restrict__ w, uint32_t pairs,
+                                                         uint32_t k, int64_t r, uint32_t c, bool there)
+{
+    constexpr int kN = P::kN;
+    const uint32_t lane = threadIdx.x & 31;
+    float acc[kN];
+#pragma unroll
+    for (int q = 0; q < kN; ++q) acc[q] = 0.0f;
+    auto add = [&](uint32_t p) {
+        if (!there) return;
+        const float weight = w != nullptr ? w[p] : 1.0f;
+        float f[kN];
+        P::unpack(dy[static_cast<int64_t>(p / k) * ldy + c], f);
+#pragma unroll
+        for (int q = 0; q < kN; ++q) acc[q] = fmaf(weight, f[q], acc[q]);
+    };
+    uint32_t mine = kNobody, count = 0, at = first;                           // lane i holds the i-th of the list
+    for (; at != kNobody && count < 32; ++count) {
+        if (lane == count) mine = at;
+        at = next[at];
+    }
+    if (at == kNobody) {
+        uint32_t rank = 0;
+        for (uint32_t i = 0; i < count; ++i) rank += __shfl_sync(kAll, mine, i) < mine;
+        for (uint32_t i = 0; i < count; ++i) add(__shfl_sync(kAll, mine, __ffs(__ballot_sync(kAll, lane < count && rank == i)) - 1));
+    } else {
+        for (uint32_t p0 = 0; p0 < pairs; p0 += 32)
+            for (unsigned here = __ballot_sync(kAll, p0 + lane < pairs && place[p0 + lane] == r); here != 0; here &= here - 1) add(p0 + __ffs(here) - 1);
+    }
+    return P::pack(acc);
 }
 template <typename P>
 __global__ void __launch_bounds__(kBackThreads, 4)
 unsort_backward_kernel(const typename P::Bits* __restrict__ dy, int64_t ldy, const typename P::Bits* __restrict__ rows, int64_t ld,
-                       const int64_t* __restrict__ place, const uint32_t* __restrict__ named, const float* __restrict__ w, uint32_t pairs, uint32_t k,
-                       uint32_t m, uint32_t row_packs, typename P::Bits* __restrict__ drows, float* __restrict__ dw)
+                       const int64_t* __restrict__ place, const uint32_t* __restrict__ head, const uint32_t* __restrict__ next, const float* __restrict__ w,
+                       uint32_t pairs, uint32_t k, uint32_t m, uint32_t row_packs, typename P::Bits* __restrict__ drows, float* __restrict__ dw)
 {
     using Bits = typename P::Bits;
-    constexpr int kN = P::kN, kBackPer = P::kSize == 16 ? 4 : 8;
-    const uint32_t lane = threadIdx.x & 31;
-    const uint64_t units = static_cast<uint64_t>(pairs) + (drows != nullptr ? m : 0);
+    constexpr int kN = P::kN, kPer = kBackPer<P>;
+    const uint32_t lane = threadIdx.x & 31, pieces = (row_packs + 32 * kPer - 1) / (32 * kPer);
+    const uint64_t units = static_cast<uint64_t>(pairs) + (drows != nullptr ? static_cast<uint64_t>((m + kBackRows - 1) / kBackRows) * pieces : 0);
     ptx::grid_dependency_wait();
     for (uint64_t unit = static_cast<uint64_t>(blockIdx.x) * kBackWarps + (threadIdx.x >> 5); unit < units; unit += static_cast<uint64_t>(gridDim.x) * kBackWarps) {
         if (unit >= pairs) {
-            const uint32_t r = static_cast<uint32_t>(unit - pairs), names = named[r];
-            if (names == 1) continue;
-            Bits* to = drows + static_cast<int64_t>(r) * row_packs;
-            for (uint32_t c0 = 0; c0 < row_packs; c0 += 32) {
-                const uint32_t c = c0 + lane;
-                float acc[kN];
+            const uint64_t u = unit - pairs;
+            const uint32_t r0 = static_cast<uint32_t>(u / pieces) * kBackRows, c0 = static_cast<uint32_t>(u % pieces) * 32 * kPer + lane;
+            uint32_t first = kNobody;
+            bool mine = false;                                                // the lane's row has no pair or several
+            if (lane < kBackRows && r0 + lane < m) {
+                first = head[r0 + lane];
+                mine = first == kNobody || next[first] != kNobody;
+            }
+            for (unsigned todo = __ballot_sync(kAll, mine); todo != 0; todo &= todo - 1) {
+                const int i = __ffs(todo) - 1;
+                const uint32_t r = r0 + i, of_row = __shfl_sync(kAll, first, i);
+                Bits* to = drows + static_cast<int64_t>(r) * row_packs;
+                if (of_row == kNobody) {
 #pragma unroll
-                for (int q = 0; q < kN; ++q) acc[q] = 0.0f;
-                uint32_t left = names;
-                for (uint32_t p0 = 0; left != 0 && p0 < pairs; p0 += 32) {
-                    unsigned mine = __ballot_sync(kAll, p0 + lane < pairs && place[p0 + lane] == r);
-                    left -= __popc(mine);
-                    for (; mine != 0; mine &= mine - 1) {
-                        const uint32_t p = p0 + __ffs(mine) - 1;
-                        const float weight = w != nullptr ? w[p] : 1.0f;
-                        if (c >= row_packs) continue;
-                        float f[kN];
-                        P::unpack(dy[static_cast<int64_t>(p / k) * ldy + c], f);
-#pragma unroll
-                        for (int q = 0; q < kN; ++q) acc[q] = fmaf(weight, f[q], acc[q]);
-                    }
+                    for (int j = 0; j < kPer; ++j)
+                        if (c0 + j * 32 < row_packs) to[c0 + j * 32] = Bits{};
+                    continue;
                 }
-                if (c < row_packs) to[c] = P::pack(acc);
+#pragma unroll 1
+                for (uint32_t c = c0; c - lane < row_packs && c < c0 + 32 * kPer; c += 32) {
+                    const Bits sum = sum_of_names<P>(dy, ldy, place, next, of_row, w, pairs, k, r, c, c < row_packs);
+                    if (c < row_packs) to[c] = sum;
+                }
             }
             continue;
         }
@@ -649,25 +688,25 @@ unsort_backward_kernel(const typename P::Bits* __restrict__ dy, int64_t ldy, con
             if (dw != nullptr && lane == 0) dw[p] = 0.0f;
             continue;
         }
-        const bool write = drows != nullptr && named[r] == 1;
+        const bool write = drows != nullptr && head[r] == p && next[p] == kNobody;
         if (dw == nullptr && !write) continue;
         const float weight = w != nullptr ? w[p] : 1.0f;
         const Bits* from = dy + static_cast<int64_t>(p / k) * ldy;
         const Bits* row = rows + r * ld;
         Bits* to = drows + r * row_packs;
         float dot = 0.0f;
-        for (uint32_t c0 = lane; c0 < row_packs; c0 += 32 * kBackPer) {
-            Bits g[kBackPer], v[kBackPer];
+        for (uint32_t c0 = lane; c0 < row_packs; c0 += 32 * kPer) {
+            Bits g[kPer], v[kPer];
 #pragma unroll
-            for (int i = 0; i < kBackPer; ++i)
+            for (int i = 0; i < kPer; ++i)
                 if (c0 + i * 32 < row_packs) g[i] = from[c0 + i * 32];
             if (dw != nullptr) {
 #pragma unroll
-                for (int i = 0; i < kBackPer; ++i)
+                for (int i = 0; i < kPer; ++i)
                     if (c0 + i * 32 < row_packs) v[i] = row[c0 + i * 32];
             }
 #pragma unroll
-            for (int i = 0; i < kBackPer; ++i) {
+            for (int i = 0; i < kPer; ++i) {
                 if (c0 + i * 32 >= row_packs) continue;
                 float gf[kN], f[kN];
                 P::unpack(g[i], gf);
@@ -814,22 +853,23 @@ int launch_unsort_tokens_backward(const void* dy, int64_t ldy, const void* rows,
     const size_t size = elem_bytes(dtype);
     const uintptr_t bits = reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(drows) |
                            static_cast<uintptr_t>(ldy * size) | static_cast<uintptr_t>(ld * size) | hidden * size;
-    const uint64_t pairs = static_cast<uint64_t>(tokens) * k, units = pairs + (drows != nullptr ? m : 0);
-    uint32_t* named = nullptr;                       // pairs to a row
+    const uint64_t pairs = static_cast<uint64_t>(tokens) * k, units = pairs + (drows != nullptr ? m : 0);       // (sizes the grid; the kernel has units of its own)
+    uint32_t *head = nullptr, *next = nullptr;
     if (drows != nullptr && m > 0) {
         int dev = 0;
         NVFP4_CUDA_CHECK(cudaGetDevice(&dev));
         cudaMemPool_t pool;
         if (int rc = host::workspace_pool(dev, &pool)) return rc;
-        const size_t bytes = static_cast<size_t>(m) * sizeof(uint32_t);
-        NVFP4_CUDA_CHECK(cudaMallocFromPoolAsync(reinterpret_cast<void**>(&named), bytes, pool, stream));
+        NVFP4_CUDA_CHECK(cudaMallocFromPoolAsync(reinterpret_cast<void**>(&head), (static_cast<size_t>(m) + pairs) * sizeof(uint32_t), pool, stream));
+        next = head + m;
         int rc = NVFP4_OK;
-        if (cudaError_t err = cudaMemsetAsync(named, 0, bytes, stream); err != cudaSuccess) rc = host::fail(NVFP4_E_CUDA, "clearing the counts failed: %s", cudaGetErrorString(err));
+        if (cudaError_t err = cudaMemsetAsync(head, 0xff, static_cast<size_t>(m) * sizeof(uint32_t), stream); err != cudaSuccess)
+            rc = host::fail(NVFP4_E_CUDA, "clearing the lists of pairs failed: %s", cudaGetErrorString(err));
         if (rc == NVFP4_OK && pairs > 0)
-            rc = host::launch_kernel(count_names_kernel, dim3(blocks_for((pairs + 31) / 32, kBackWarps, num_sms, 8)), dim3(kBackThreads), 0, stream, true, place,
-                                     static_cast<uint32_t>(pairs), static_cast<uint32_t>(m), named);
+            rc = host::launch_kernel(list_names_kernel, dim3(blocks_for((pairs + 31) / 32, kBackWarps, num_sms, 8)), dim3(kBackThreads), 0, stream, true, place,
+                                     static_cast<uint32_t>(pairs), static_cast<uint32_t>(m), head, next);
         if (rc != NVFP4_OK) {
-            cudaFreeAsync(named, stream);
+            cudaFreeAsync(head, stream);
             return rc;
         }
     }
@@ -838,11 +878,11 @@ int launch_unsort_tokens_backward(const void* dy, int64_t ldy, const void* rows,
         using Bits = typename P::Bits;
         constexpr int kN = P::kN;
         return host::launch_kernel(unsort_backward_kernel<P>, dim3(blocks_for(units, kBackWarps, num_sms, 8)), dim3(kBackThreads), 0, stream, true,
-                                   static_cast<const Bits*>(dy), ldy / kN, static_cast<const Bits*>(rows), ld / kN, place, named, w,
+                                   static_cast<const Bits*>(dy), ldy / kN, static_cast<const Bits*>(rows), ld / kN, place, head, next, w,
                                    static_cast<uint32_t>(pairs), static_cast<uint32_t>(k), static_cast<uint32_t>(m), static_cast<uint32_t>(hidden / kN),
                                    static_cast<Bits*>(drows), dw);
     });
-    if (named != nullptr) cudaFreeAsync(named, stream);
+    if (head != nullptr) cudaFreeAsync(head, stream);
     return rc;
 }
 
