@@ -635,3 +635,31 @@ def test_scales_refuse():
     assert "FP16 operands" in error_of(lib.nvfp4_linear_dz_scaled(1024, 32, 1024, 32, 1024, 32, None, 4, 32, 2, 2, 1024, None))
     assert "goes with dz" in error_of(lib.nvfp4_linear_dz_scaled(1024, 32, 1024, 32, None, 32, 1024, 4, 32, 2, 1, 1024, None))
     assert "scale is not aligned" in error_of(lib.nvfp4_linear_dz_scaled(1024, 32, 1024, 32, 1024, 32, None, 4, 32, 2, 1, 1026, None))
+
+
+@gpu
+def test_long_sums_with_everything_in_the_epilogue():
+    """FP16 sums of 20000 products of one sign that no cluster shares: forward with bias, activation, kept slopes and residual, and dx."""
+    g = torch.Generator("cuda").manual_seed(6)
+    some = lambda *s, scale=1.0: ((torch.rand(*s, generator=g, device="cuda") + 0.5) * scale).half()
+    dtype, k = torch.float16, 20000
+    cut = (k / 1024 / 2 + 4) * 2.0 ** -24 + 32 * 2.0 ** -22                  # sums of 1024 with 64 steps each, added in FP32
+    for n in (2056, 2057):                                                # through TMA, and the odd stride's way
+        x, w, bias, residual = some(2600, k), some(n, k, scale=1 / k), some(n), some(2600, n)
+        leaves = [t.requires_grad_() for t in (bias, residual)]
+        y = linear(x, w, *leaves, activation="silu")
+        z = x.double() @ w.double().t() + bias.detach().double()
+        want = act64(z, "silu") + residual.detach().double()
+        error = SLOPE * z * cut + want * 40 * 2.0 ** -23                  # z, silu and the sum, each with a few roundings
+        assert (y.detach().double() - want).abs().le(error + (want + error) * 1.01 * HALF_STEP[dtype]).all()
+        dd = some(2600, n, scale=1 / 2600)
+        db, dr = torch.autograd.grad(y, leaves, dd)
+        slope = torch.sigmoid(z) * (1 + z * (1 - torch.sigmoid(z)))
+        want = (dd.double() * slope).sum(dim=0)
+        assert torch.equal(dr, dd) and (db.double() - want).abs().le(want * (2.0 ** -13 + 1.01 * HALF_STEP[dtype])).all()      # slopes near 1.09: 2^-15 of them
+    x, w = torch.zeros(2600, 2056, dtype=dtype, device="cuda").requires_grad_(), some(k, 2056, scale=1 / k)
+    dd = some(2600, k)
+    (dx,) = torch.autograd.grad(linear(x, w), x, dd)
+    want = dd.double() @ w.double()
+    step = 2.0 ** (torch.floor(torch.log2(want)) - 10)
+    assert ((dx.double() - want).abs() <= 0.5 * step + want * cut).all()
