@@ -358,8 +358,9 @@ NVFP4_API int nvfp4_route_tokens_backward(const void* logits, int64_t ld_elems, 
  *   contiguous.  place outside [0, M) contributes nothing.  With w NULL it is the gradient of nvfp4_sort_tokens, too.
  * nvfp4_unsort_tokens_backward: drows[r] (M, hidden) contiguous = sum of w[t, j] * dy[t] over the pairs with place[t, j] == r (FP32, ascending
  *   pairs, rounded once), zero at rows that no pair names; dw[t, j] = <dy[t], rows[place[t, j]]> in FP32, 0 for a place outside [0, M).
- *   Any order, as in the forward call: a row may have no pair, one or several (more than 32 are slow: they are looked up among all pairs).  Either result may be NULL, and rows with dw NULL.  source stands beside place as nvfp4_sort_tokens gives it; what is
- *   computed follows from place alone. */
+ *   Any order, as in the forward call: a row may have no pair, one or several (more than 32 are slow: they are looked up among all pairs).
+ *   Either result may be NULL, and rows with dw NULL.  source stands beside place as nvfp4_sort_tokens gives it; what is computed
+ *   follows from place alone. */
 NVFP4_API int nvfp4_sort_tokens(const void* x, int64_t ldx_elems, int dtype, int64_t tokens, int k, int hidden, const int64_t* ids, int experts,
                                 int alignment, int64_t M, void* rows, int64_t* place, int32_t* source, int32_t* m_indices, void* stream);
 NVFP4_API int nvfp4_unsort_tokens(const void* rows, int64_t ld_elems, int dtype, int64_t M, const int64_t* place, const float* w, int64_t tokens,

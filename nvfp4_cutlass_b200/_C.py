@@ -48,8 +48,8 @@ EXPORTS = ("nvfp4_last_error", "nvfp4_version", "nvfp4_get_num_sms", "nvfp4_set_
            "nvfp4_grouped_gemm_swiglu_contiguous", "nvfp4_grouped_gemm_masked", "nvfp4_load_checkpoint_weights",
            "nvfp4_read_status", "nvfp4_debug_split_workspace", "nvfp4_debug_wait_timeout", "nvfp4_debug_quantize_weight_expired", "nvfp4_plan_peer_masked", "nvfp4_plan_one_rank",
            "nvfp4_peer_barrier", "nvfp4_route_tokens", "nvfp4_route_tokens_backward", "nvfp4_sort_tokens", "nvfp4_unsort_tokens",
-           "nvfp4_unsort_tokens_backward", "nvfp4_linear", "nvfp4_linear_dz", "nvfp4_linear_dx", "nvfp4_linear_dw", "nvfp4_linear_dz_scaled", "nvfp4_linear_dx_scaled", "nvfp4_linear_dw_scaled",
-           "nvfp4_debug_linear_expired", "nvfp4_debug_unsort_expired")
+           "nvfp4_unsort_tokens_backward", "nvfp4_linear", "nvfp4_linear_dz", "nvfp4_linear_dx", "nvfp4_linear_dw",
+           "nvfp4_linear_dz_scaled", "nvfp4_linear_dx_scaled", "nvfp4_linear_dw_scaled", "nvfp4_debug_linear_expired", "nvfp4_debug_unsort_expired")
 
 
 def library_path() -> str:

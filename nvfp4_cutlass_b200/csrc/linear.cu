@@ -988,7 +988,8 @@ product_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         const bool both = e.slopes != nullptr;       // the second buffer takes the slopes
         const float factor = e.scale != nullptr ? *e.scale : 1.0f;
         constexpr uint32_t kBoxColumns = kBox<T>;
-        Stage<T, T> stage{boxes, both ? 0u : kBoxBytes, boxes + kBoxBytes, 0u, landed + 2 * (warp - kPairFirstEpi), 0, &maps, p.budget, factor, 0, p.withhold == kResiduals};
+        Stage<T, T> stage{boxes, both ? 0u : kBoxBytes, boxes + kBoxBytes, 0u, landed + 2 * (warp - kPairFirstEpi), 0, &maps, p.budget, factor, 0,
+                          p.withhold == kResiduals};
         uint32_t n = 0;
         for (uint32_t tile = pair_id; tile < tiles; tile += num_pairs, ++n) {
             const uint32_t acc = n & 1;

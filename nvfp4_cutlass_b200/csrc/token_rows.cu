@@ -525,7 +525,8 @@ unsort_ring_kernel(const uint8_t* __restrict__ rows, int64_t ld_bytes, const int
         }
         if (!ok || !ptx::all_lanes(*abort_flag == 0)) {
             const long long until = clock64() + shape.budget;
-            for (uint32_t n = loaded > shape.depth ? loaded - shape.depth : 0; n < loaded; ++n) ptx::mbar_settle(full + n % shape.depth, n / shape.depth & 1u, until);
+            for (uint32_t n = loaded > shape.depth ? loaded - shape.depth : 0; n < loaded; ++n)
+                ptx::mbar_settle(full + n % shape.depth, n / shape.depth & 1u, until);
         }
         return;
     }

@@ -2,7 +2,8 @@
 
 The router's projection (FP32 logits out of BF16 rows), shared experts and the projections of an attention block: what a model keeps in
 BF16 or FP16 beside the quantised experts.  Operands are read where they lie, whichever way a product needs them; sums are FP32.  CUDA
-kernels of the library throughout; CPU tensors are refused, and tensors with tangents of forward mode.  The reference project has the grouped quantised product alone.
+kernels of the library throughout; CPU tensors are refused, and tensors with tangents of forward mode.  The reference project has the
+grouped quantised product alone.
 """
 from __future__ import annotations
 

@@ -8,7 +8,8 @@ gradients.
 
 Nothing comes back to the host: the sorted buffer has as many rows as any routing of so many pairs can need, so the calls can be
 captured in a CUDA graph whose replays see other routings.  All of it is CUDA kernels of the library; CPU tensors are refused.  Gradients are
-computed once (no second derivatives) and backwards: tensors with tangents of forward mode are refused.  The reference project begins at rows that are grouped already.
+computed once (no second derivatives) and backwards: tensors with tangents of forward mode are refused.  The reference project begins
+at rows that are grouped already.
 """
 from __future__ import annotations
 

@@ -52,3 +52,49 @@ for call in (lambda: nvfp4_gemm.linear(x, w), gemm, lambda: gemm(tune_split_tran
 def test_the_first_call_of_a_thread(calls):
     r = subprocess.run([sys.executable, "-c", SETUP + calls], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr
+
+
+def test_training_steps_of_several_threads_at_once():
+    """Every thread trains on a stream of its own, sizes that differ, workspaces out of one pool: the bits of the steps one after the other."""
+    import threading
+
+    import torch
+
+    from nvfp4_gemm import linear, route_tokens, sort_tokens, unsort_tokens
+
+    def case(i):
+        g = torch.Generator().manual_seed(i)
+        dtype = (torch.bfloat16, torch.float16)[i % 2]
+        tokens = 700 + 333 * i
+        leaf = lambda *s, scale: (torch.randn(*s, generator=g) * scale).to(dtype).cuda().requires_grad_()
+        leaves = [leaf(tokens, 256, scale=1.0), leaf(16, 256, scale=0.1), leaf(264, 256, scale=0.06), leaf(264, scale=0.1), leaf(256, 264, scale=0.06)]
+        dy = (torch.randn(tokens, 256, generator=g) * (1.0, 1e-6)[i % 2]).cuda()
+        return leaves, dy
+
+    def step(leaves, dy):
+        x, gate, w1, bias, w2 = leaves
+        ids, weights = route_tokens(linear(x, gate, out_dtype=torch.float32), 4, renormalize=False)
+        rows, order = sort_tokens(x, ids, 16, alignment=16)
+        d = linear(linear(rows, w1, bias, activation="silu"), w2)
+        y = linear(x, w2.detach()[:, :256].contiguous(), out_dtype=torch.float32) + unsort_tokens(d, order._replace(place=order.place.flip(1)), weights).float()
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    cases = [case(i) for i in range(4)]
+    want = [step(*c) for c in cases]
+    torch.cuda.synchronize()
+    same = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(15):
+                got = step(*cases[i])
+                stream.synchronize()
+                same.append(all(torch.equal(a, b) for a, b in zip(got, want[i])))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(same) == 4 * 15 and all(same)
