@@ -663,3 +663,45 @@ def test_long_sums_with_everything_in_the_epilogue():
     want = dd.double() @ w.double()
     step = 2.0 ** (torch.floor(torch.log2(want)) - 10)
     assert ((dx.double() - want).abs() <= 0.5 * step + want * cut).all()
+
+
+@gpu
+def test_captured_training_steps_side_by_side_see_new_data():
+    """Two captures of one step, replayed at the same time on streams of their own: lists of pairs, peaks of gradients and sums of columns live in
+    workspaces of each capture."""
+    tokens, experts, k, hidden = 700, 16, 4, 128
+    g = gen(7)
+    half = lambda *s, scale=1.0: (torch.randn(*s, generator=g) * scale).half().cuda().requires_grad_()
+    leaves = [half(tokens, hidden), half(experts, hidden, scale=0.2), half(264, hidden, scale=0.1), half(264, scale=0.1), half(hidden, 264, scale=0.06)]
+    dy = torch.randn(tokens, hidden, generator=g).cuda()
+
+    def step():
+        x, gate, w1, bias, w2 = leaves
+        ids, weights = route_tokens(linear(x, gate, out_dtype=torch.float32), k, renormalize=False)
+        rows, order = sort_tokens(x, ids, experts, alignment=16)
+        late = order._replace(place=order.place.masked_fill(weights.detach() < 0.05, -1))                    # pairs dropped afterwards
+        y = linear(linear(unsort_tokens(rows, late, weights), w1, bias, activation="gelu"), w2, out_dtype=torch.float32)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step())
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for scale in (1.0, 1e-7, 1e6):
+        with torch.no_grad():
+            leaves[0].copy_(torch.randn(tokens, hidden, generator=g))
+            dy.copy_(torch.randn(tokens, hidden, generator=g) * scale)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+                graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        torch.cuda.synchronize()
+        for out in outs:
+            assert all(torch.equal(a.nan_to_num(1.0, 2.0, 3.0), b.nan_to_num(1.0, 2.0, 3.0)) for a, b in zip(want, out))
