@@ -598,7 +598,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         if (++r.slot == depth) { r.slot = 0; r.phase ^= 1; }
     };
     const uint32_t quad = warp & 3, row = quad * 32 + lane;                   // epilogue: the warp's quarter of the lanes
-    const float factor = e.scale != nullptr ? *e.scale : 1.0f;
+    const float factor = !kSwap && e.scale != nullptr ? *e.scale : 1.0f;      // (swapped: forward products alone)
     const uint32_t taddr = tmem + ((quad * 32) << 16);
     if (warp == 0) {
         const uint32_t issue = ptx::elect_one();
@@ -1271,8 +1271,8 @@ __device__ __forceinline__ float dz_factor(float most)
     return __uint_as_float(static_cast<uint32_t>(127 + 14 - exponent) << 23);
 }
 constexpr int kGradThreads = 256, kGradColumns = 256, kGradRowLanes = 8;
-// kAgain: the second pass.
-template <typename T, typename D, bool kAgain>
+enum DzPass { kOnlyPass, kFirstPass, kSecondPass };                          // (a 4099 x 4096 pass that need not look for the largest: 16.7 us for 18.9)
+template <typename T, typename D, DzPass kPass>
 __global__ void __launch_bounds__(kGradThreads)
 linear_dz_kernel(const D* __restrict__ dd, int64_t ldd, bool wide, const int16_t* __restrict__ slopes, int64_t lds, T* __restrict__ dz, int64_t lddz, uint32_t rows,
                  uint32_t cols, uint32_t rows_each, float* __restrict__ sums, float* __restrict__ peaks, float* __restrict__ scale)
@@ -1291,7 +1291,7 @@ linear_dz_kernel(const D* __restrict__ dd, int64_t ldd, bool wide, const int16_t
         __syncthreads();
         return __uint_as_float(__reduce_max_sync(kAll, largest[threadIdx.x % kGradRowLanes]));
     };
-    if constexpr (kAgain) {
+    if constexpr (kPass == kSecondPass) {
         for (uint32_t i = threadIdx.x; i < gridDim.x * gridDim.y; i += kGradThreads) most = fmaxf(most, peaks[i]);
         factor = dz_factor(largest_of_block(most));
         if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *scale = 1.0f / factor;
@@ -1318,18 +1318,18 @@ linear_dz_kernel(const D* __restrict__ dd, int64_t ldd, bool wide, const int16_t
                 float v = to_float(g[i]);
                 if (slopes != nullptr) v *= unpack_slope(code[i]);
                 sum[i] += v;
-                if constexpr (kAgain) v *= factor;
-                else if (fabsf(v) < INFINITY && i < here) most = fmaxf(most, fabsf(v));
+                if constexpr (kPass == kSecondPass) v *= factor;
+                if (kPass == kFirstPass && fabsf(v) < INFINITY && i < here) most = fmaxf(most, fabsf(v));
                 out[i] = from_float<T>(v);
             }
             if (dz != nullptr) *reinterpret_cast<uint4*>(dz + static_cast<int64_t>(r) * lddz + col0) = *reinterpret_cast<const uint4*>(out);
         }
     }
-    if (!kAgain && peaks != nullptr) {
+    if constexpr (kPass == kFirstPass) {
         const float top = largest_of_block(most);
         if (threadIdx.x == 0) peaks[blockIdx.y * gridDim.x + blockIdx.x] = top;
     }
-    if (kAgain || sums == nullptr) return;
+    if (kPass == kSecondPass || sums == nullptr) return;
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) part[row_lane][group * 8 + i] = sum[i];
     __syncthreads();
@@ -1375,12 +1375,17 @@ int launch_dz(const void* dd, int64_t ldd, const int16_t* slopes, int64_t lds, v
         if (scale != nullptr) peaks = workspace + sum_words;
     }
     const dim3 grid(columns, blocks);
-    int rc = host::launch_kernel(linear_dz_kernel<T, D, false>, grid, dim3(kGradThreads), 0, stream, true, static_cast<const D*>(dd), ldd, wide, slopes, lds,
-                                 static_cast<T*>(dz), lddz, rows, cols, rows_each, sums, peaks, scale);
-    if constexpr (std::is_same<T, __half>::value && std::is_same<D, float>::value)
-        if (rc == NVFP4_OK && scale != nullptr)
-            rc = host::launch_kernel(linear_dz_kernel<T, D, true>, grid, dim3(kGradThreads), 0, stream, true, static_cast<const D*>(dd), ldd, wide, slopes, lds,
-                                     static_cast<T*>(dz), lddz, rows, cols, rows_each, static_cast<float*>(nullptr), peaks, scale);
+    auto pass = [&](auto kernel) {
+        return host::launch_kernel(kernel, grid, dim3(kGradThreads), 0, stream, true, static_cast<const D*>(dd), ldd, wide, slopes, lds, static_cast<T*>(dz), lddz,
+                                   rows, cols, rows_each, sums, peaks, scale);
+    };
+    int rc = NVFP4_OK;
+    if (scale == nullptr) {
+        rc = pass(linear_dz_kernel<T, D, kOnlyPass>);
+    } else if constexpr (std::is_same<T, __half>::value && std::is_same<D, float>::value) {
+        rc = pass(linear_dz_kernel<T, D, kFirstPass>);
+        if (rc == NVFP4_OK) rc = pass(linear_dz_kernel<T, D, kSecondPass>);
+    }
     if (rc == NVFP4_OK && db != nullptr)
         rc = host::launch_kernel(linear_db_kernel<T>, dim3((cols + kGradThreads - 1) / kGradThreads), dim3(kGradThreads), 0, stream, true, sums, blocks, cols,
                                  static_cast<T*>(db));
